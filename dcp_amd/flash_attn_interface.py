@@ -25,6 +25,10 @@ __all__ = [
     "forward_workspace",
     "_flash_attn_varlen_backward",
     "backward_workspace_bytes",
+    "paged_cache_attention",
+    "paged_cache_workspace_bytes",
+    "shared_prefix_attention",
+    "shared_prefix_workspace_bytes",
 ]
 
 
@@ -443,3 +447,165 @@ def _flash_attn_varlen_backward(
         *grouping, float(softmax_scale), dtype_code(q.dtype), _stream(),
     )
     return dq, dk, dv, None
+
+
+# ---------------------------------------------------------------------------
+# attention over a paged cache (no counterpart in the reference)
+# ---------------------------------------------------------------------------
+
+
+def paged_cache_workspace_bytes(n_tokens, batch, n_heads_q, n_heads_kv, head_dim, max_seqlen_q, max_seqlen_k) -> int:
+    """Scratch bytes ``paged_cache_attention`` needs for these sizes (0: none)."""
+    return _lib.load().dcp_paged_attn_workspace_bytes(n_tokens, batch, n_heads_q, n_heads_kv, head_dim, max_seqlen_q, max_seqlen_k)
+
+
+def shared_prefix_workspace_bytes(n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim, max_seqlen_q, max_seqlen_k, max_prefix_len) -> int:
+    """Scratch bytes ``shared_prefix_attention`` needs for these sizes."""
+    return _lib.load().dcp_shared_prefix_attn_workspace_bytes(n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim, max_seqlen_q,
+                                                             max_seqlen_k, max_prefix_len)
+
+
+def _paged_workspace(workspace, n_bytes: int, q) -> tuple:
+    if workspace is None:
+        if n_bytes == 0:
+            return None, 0, 0
+        workspace = torch.empty(n_bytes, dtype=torch.uint8, device=q.device)
+    elif not workspace.is_contiguous() or workspace.get_device() != q.get_device():
+        raise ValueError("workspace must be a contiguous tensor on q's device")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _paged_inputs(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, out, lse):
+    """Checks what both operators take; ``(out, lse, batch, strides of q, out and the cache)``."""
+    here = torch._C._cuda_getDevice()
+    if not (q.get_device() == here and k_cache.get_device() == here and v_cache.get_device() == here):
+        raise ValueError("q, k_cache and v_cache must be tensors of the current device")
+    if q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError(f"q must be [tokens, n_heads_q, D] with dense rows, got {list(q.shape)}")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1 \
+            or k_cache.shape[3] != q.shape[2]:
+        raise ValueError(f"k_cache and v_cache must be [n_pages, page_size, n_heads_kv, {q.shape[2]}] with the same strides and dense rows")
+    if not (q.dtype is k_cache.dtype is v_cache.dtype):
+        raise TypeError(f"q is {q.dtype}, the caches are {k_cache.dtype} and {v_cache.dtype}")
+    if block_table.dim() != 2 or (block_table.numel() > 0 and block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be [B, pages] with dense rows, got {list(block_table.shape)}")
+    batch = block_table.shape[0]
+    _table_here(block_table, "block_table", block_table.shape)
+    _table_here(seq_lens, "seq_lens", (batch,))
+    if cu_seqlens_q is not None:
+        _table_here(cu_seqlens_q, "cu_seqlens_q", (batch + 1,))
+    elif batch != q.shape[0]:
+        raise ValueError(f"without cu_seqlens_q every request has one token, got {q.shape[0]} for {batch}")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype is not q.dtype or out.stride(2) != 1 or out.get_device() != here:
+        raise ValueError(f"out must be like q, got {out.dtype} {list(out.shape)}")
+    if lse is None:
+        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+    elif tuple(lse.shape) != (q.shape[1], q.shape[0]) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != here:
+        raise ValueError(f"lse must be contiguous float32 [{q.shape[1]}, {q.shape[0]}]")
+    return out, lse, batch
+
+
+def _table_here(t, name: str, shape) -> None:
+    if t.dtype is not torch.int32 or t.get_device() != torch._C._cuda_getDevice() or tuple(t.shape) != tuple(shape) \
+            or (t.dim() == 1 and not t.is_contiguous()):
+        raise ValueError(f"{name} must be int32 {list(shape)} on the current device, got {t.dtype} {list(t.shape)} on {t.device}")
+
+
+def paged_cache_attention(
+    q,
+    k_cache,
+    v_cache,
+    block_table,
+    seq_lens,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    max_seqlen_q: Optional[int] = None,
+    max_seqlen_k: Optional[int] = None,
+    softmax_scale: Optional[float] = None,
+    window: Optional[int] = None,
+    n_starting: int = 0,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+):
+    """Attention of each request's last tokens over its keys in a paged cache; returns ``(out, lse)``.
+
+    q ``[tokens, H, D]``; caches ``[n_pages, page_size, Hkv, D]`` (any strides: the halves of a
+    ``[n_pages, page_size, 2, Hkv, D]`` buffer, say); ``block_table`` int32 ``[B, pages]``; ``seq_lens`` int32 ``[B]``, the
+    new tokens' keys among them.  ``cu_seqlens_q`` int32 ``[B + 1]``: the requests' tokens in q; without it, one each.
+    The query at position x sees the keys up to x: all of them, or with ``window`` the last ``window`` (itself among
+    them) and the first ``n_starting``, as ``lambda_mask_fn`` trains.  ``out`` like q, ``lse`` fp32 ``[H, tokens]``: 0 and
+    +inf where nothing is visible; tokens of no request are left as they were.
+    ``max_seqlen_q`` / ``max_seqlen_k``: the longest lengths as far as the host knows them (default: all tokens, a whole row of
+    pages); they decide how the work is split and change no result beyond its rounding.
+    ``workspace``: a tensor of ``paged_cache_workspace_bytes(...)`` bytes, for calls that may not allocate.
+    Page numbers outside of the cache name no page: nobody sees their keys.  Forward only.
+    """
+    out, lse, batch = _paged_inputs(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, out, lse)
+    n_tokens, n_heads_q, head_dim = q.shape
+    n_pages, page_size, n_heads_kv, _ = k_cache.shape
+    width = block_table.shape[1]
+    if window is not None and window < 1:
+        raise ValueError(f"window must be positive (None: no window), got {window}")
+    longest_q = (1 if cu_seqlens_q is None else max(n_tokens, 1)) if max_seqlen_q is None else int(max_seqlen_q)
+    longest_k = max(width * page_size, 1) if max_seqlen_k is None else int(max_seqlen_k)
+    scale = head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
+    n_bytes = paged_cache_workspace_bytes(n_tokens, batch, n_heads_q, n_heads_kv, head_dim, longest_q, longest_k)
+    workspace, address, size = _paged_workspace(workspace, n_bytes, q)
+    _lib.call("dcp_paged_attn", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(), block_table.data_ptr(),
+              seq_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), n_tokens, batch, n_heads_q, n_heads_kv, head_dim,
+              q.stride(0), q.stride(1), out.stride(0), out.stride(1), n_pages, page_size, k_cache.stride(0), k_cache.stride(1),
+              k_cache.stride(2), width, block_table.stride(0), longest_q, longest_k, 0 if window is None else int(window),
+              int(n_starting), scale, dtype_code(q.dtype), address, size, _stream())
+    return out, lse
+
+
+def shared_prefix_attention(
+    q,
+    k_cache,
+    v_cache,
+    prefix_table,
+    prefix_lens,
+    cu_groups,
+    block_table,
+    seq_lens,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    max_seqlen_q: Optional[int] = None,
+    max_seqlen_k: Optional[int] = None,
+    max_prefix_len: Optional[int] = None,
+    softmax_scale: Optional[float] = None,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+):
+    """``paged_cache_attention`` for requests that share long prefixes, each of which is read once for all of its requests.
+
+    Requests ``cu_groups[i]`` up to ``cu_groups[i + 1]`` (int32 ``[P + 1]``) share the ``prefix_lens[i]`` keys in the pages
+    ``prefix_table[i]`` (int32 ``[P, pages]``).  ``block_table`` and ``seq_lens`` are of the keys that follow, each request's own,
+    the new tokens' among them.  A query sees its whole prefix and its own keys up to itself, as ``shared_prefix_mask_fn``
+    trains: ``(out, lse)`` are those of the concatenation.  Requests outside of the groups have no prefix.
+    """
+    out, lse, batch = _paged_inputs(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, out, lse)
+    n_tokens, n_heads_q, head_dim = q.shape
+    n_pages, page_size, n_heads_kv, _ = k_cache.shape
+    width = block_table.shape[1]
+    if prefix_table.dim() != 2 or (prefix_table.numel() > 0 and prefix_table.shape[1] > 1 and prefix_table.stride(1) != 1):
+        raise ValueError(f"prefix_table must be [P, pages] with dense rows, got {list(prefix_table.shape)}")
+    n_prefixes, prefix_width = prefix_table.shape
+    _table_here(prefix_table, "prefix_table", prefix_table.shape)
+    _table_here(prefix_lens, "prefix_lens", (n_prefixes,))
+    _table_here(cu_groups, "cu_groups", (n_prefixes + 1,))
+    longest_q = (1 if cu_seqlens_q is None else max(n_tokens, 1)) if max_seqlen_q is None else int(max_seqlen_q)
+    longest_k = max(width * page_size, 1) if max_seqlen_k is None else int(max_seqlen_k)
+    longest_prefix = max(prefix_width * page_size, 1) if max_prefix_len is None else int(max_prefix_len)
+    scale = head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
+    n_bytes = shared_prefix_workspace_bytes(n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim, longest_q, longest_k, longest_prefix)
+    workspace, address, size = _paged_workspace(workspace, n_bytes, q)
+    _lib.call("dcp_shared_prefix_attn", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(),
+              prefix_table.data_ptr(), prefix_lens.data_ptr(), cu_groups.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+              0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim,
+              q.stride(0), q.stride(1), out.stride(0), out.stride(1), n_pages, page_size, k_cache.stride(0), k_cache.stride(1),
+              k_cache.stride(2), prefix_width, prefix_table.stride(0), width, block_table.stride(0),
+              longest_q, longest_k, longest_prefix, scale, dtype_code(q.dtype), address, size, _stream())
+    return out, lse

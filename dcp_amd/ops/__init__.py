@@ -15,3 +15,4 @@ from dcp_amd.ops.fused_ops import (  # noqa: F401
     fused_copy_fp32_varlen_lse,
     warmup_triton_ops,
 )
+from dcp_amd.ops.paged_cache import PagedCacheTables, paged_cache_tables, paged_cache_write  # noqa: F401

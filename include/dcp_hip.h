@@ -627,6 +627,120 @@ int dcp_greedy_stage_selection(
     int32_t* comm_src, int64_t comm_capacity, int64_t* n_comm,
     float* cross_node_load_out, float* intra_node_load_out);
 
+/*
+ * A paged K/V cache and the attention that answers over it (no counterpart in
+ * the reference, which trains with these masks and does not answer).
+ *
+ * The tables of one step, from the requests' lengths.  Request b has
+ * cached_lens[b] tokens in the cache and adds new_lens[b] (0 for one that
+ * rests); its row of block_table ([batch][table_width], rows table_stride
+ * entries apart) names the pages of what is cached.  In place, in the order of
+ * the requests, the pages that the new tokens need are taken from free_pages
+ * and appended to the rows; entries behind a row's last page are left as they
+ * were.  Token t of the step (the requests' new tokens one after another) gets
+ * positions[t] (in its request) and slot_mapping[t] = page * page_size + offset.
+ * cu_seqlens[batch + 1] are the sums of new_lens, seq_lens[b] = cached + new,
+ * *pages_taken the number of pages taken.
+ *  - A page that the free list has no more of is entered as -1, and *pages_taken
+ *    says how many it would have taken.  Tokens without a page (there, or past
+ *    table_width pages, or in a page that the table names -1) get slot -1.
+ *  - n_tokens: length of slot_mapping and positions.  Tokens past the last
+ *    request's have slot -1, position 0; those that do not fit are not entered.
+ *  - Negative lengths count as 0.
+ */
+int dcp_paged_cache_tables(const int32_t* cached_lens, const int32_t* new_lens,
+                           int32_t* block_table, int64_t table_stride,
+                           const int32_t* free_pages, int64_t* slot_mapping,
+                           int32_t* positions, int32_t* cu_seqlens,
+                           int32_t* seq_lens, int32_t* pages_taken, int batch,
+                           int table_width, int n_free, int page_size,
+                           int n_tokens, void* stream);
+
+/*
+ * Writes tokens' rows of K and V ([n_tokens][n_heads_kv][head_dim], token and
+ * head strides in elements of elem_size = 1, 2 or 4 bytes) into the cache
+ * ([n_pages][page_size][n_heads_kv][head_dim] with any strides, the same for
+ * both) at their slots.  A slot outside of the cache (such as -1) is skipped;
+ * the others have to differ from each other, and the inputs may not lie in the
+ * cache.
+ */
+int dcp_paged_cache_write(const void* k, const void* v,
+                          const int64_t* slot_mapping, void* k_cache,
+                          void* v_cache, int n_tokens, int n_heads_kv,
+                          int head_dim, int elem_size, int64_t token_stride,
+                          int64_t head_stride, int64_t n_pages, int page_size,
+                          int64_t cache_page_stride,
+                          int64_t cache_token_stride,
+                          int64_t cache_head_stride, void* stream);
+
+/*
+ * Attention over the cache.  Tokens [cu_seqlens_q[b], cu_seqlens_q[b+1]) of q
+ * ([n_tokens][n_heads_q][head_dim]; NULL cu_seqlens_q: one token a request) are
+ * the last ones of request b, whose seq_lens[b] keys are in the pages
+ * block_table[b * table_stride + i].  The query at position x sees the keys
+ * j <= x with j < n_starting or j > x - window (window 0: all j <= x), as the
+ * reference's lambda mask (dcp/runtime/flash_attention/utils.py:521-542).
+ * out[t][h] = softmax(softmax_scale q k^T) v, lse[h * n_tokens + t] its
+ * log-sum-exp; a query without a visible key (one before its request's first
+ * key among them) gets out = 0, lse = +inf.  Tokens of no request are left as
+ * they were.  q head h reads kv head h / (n_heads_q / n_heads_kv).
+ *  - Supported: bf16 and fp16, head_dim 64 or 128, page_size a multiple of 16,
+ *    softmax_scale > 0, any strides that are multiples of 8 elements (out: 4),
+ *    16-byte aligned tensors.
+ *  - Page numbers outside of [0, n_pages) name no page: nobody sees their keys.
+ *    Keys past the last entry of a row are not there.
+ *  - What the cache holds where no query of a request looks (behind its last key,
+ *    between its first tokens and its window) may be anything.  Queries of one
+ *    request are computed together: keys that any of them sees should be finite.
+ *  - max_seqlen_q, max_seqlen_k: the longest lengths, known on the host.  They
+ *    decide how the work is split, not what is computed: lengths past them give the same
+ *    results, slower.
+ *  - workspace: dcp_paged_attn_workspace_bytes(...) bytes (0: none needed),
+ *    16-byte aligned, for shares of the keys that are joined afterwards; contents
+ *    are overwritten.  Launches that may run at the same time need one each.
+ */
+size_t dcp_paged_attn_workspace_bytes(int n_tokens, int batch, int n_heads_q,
+                                      int n_heads_kv, int head_dim,
+                                      int max_seqlen_q, int max_seqlen_k);
+int dcp_paged_attn(const void* q, const void* k_cache, const void* v_cache,
+                   void* out, float* lse, const int32_t* block_table,
+                   const int32_t* seq_lens, const int32_t* cu_seqlens_q,
+                   int n_tokens, int batch, int n_heads_q, int n_heads_kv,
+                   int head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                   int64_t out_token_stride, int64_t out_head_stride,
+                   int n_pages, int page_size, int64_t page_stride,
+                   int64_t token_stride, int64_t head_stride, int table_width,
+                   int64_t table_stride, int max_seqlen_q, int max_seqlen_k,
+                   int window, int n_starting, float softmax_scale, int dtype,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The same for requests that share prefixes.  Requests [cu_groups[i],
+ * cu_groups[i+1]) share the prefix_lens[i] keys in the pages
+ * prefix_table[i * prefix_stride + j]; seq_lens and block_table are of the keys
+ * that follow, each request's own.  A query sees all of its prefix and its own
+ * keys up to itself: the result is that of the concatenation, the prefix is read
+ * once for all of its requests.  Requests outside of [cu_groups[0],
+ * cu_groups[n_prefixes]) have no prefix.  Everything else as above;
+ * the workspace is always needed.
+ */
+size_t dcp_shared_prefix_attn_workspace_bytes(
+    int n_tokens, int batch, int n_prefixes, int n_heads_q, int n_heads_kv,
+    int head_dim, int max_seqlen_q, int max_seqlen_k, int max_prefix_len);
+int dcp_shared_prefix_attn(
+    const void* q, const void* k_cache, const void* v_cache, void* out,
+    float* lse, const int32_t* prefix_table, const int32_t* prefix_lens,
+    const int32_t* cu_groups, const int32_t* block_table,
+    const int32_t* seq_lens, const int32_t* cu_seqlens_q, int n_tokens,
+    int batch, int n_prefixes, int n_heads_q, int n_heads_kv, int head_dim,
+    int64_t q_token_stride, int64_t q_head_stride, int64_t out_token_stride,
+    int64_t out_head_stride, int n_pages, int page_size, int64_t page_stride,
+    int64_t token_stride, int64_t head_stride, int prefix_width,
+    int64_t prefix_stride, int table_width, int64_t table_stride,
+    int max_seqlen_q, int max_seqlen_k, int max_prefix_len,
+    float softmax_scale, int dtype, void* workspace, size_t workspace_bytes,
+    void* stream);
+
 #ifdef __cplusplus
 }
 #endif
