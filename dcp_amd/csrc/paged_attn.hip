@@ -349,69 +349,496 @@ __global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const Paged
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(to + 16 * dt) = o[rt][dt];
       continue;
     }
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t token = out_row[rt] / p.n_heads_q, head = out_row[rt] % p.n_heads_q;
     uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + 4 * g;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
       *reinterpret_cast<u32x2*>(to + 16 * dt) = u32x2{pack2<DTYPE>(o[rt][dt][0] * inv, o[rt][dt][1] * inv),
                                                       pack2<DTYPE>(o[rt][dt][2] * inv, o[rt][dt][3] * inv)};
-    if (g == 0) p.lse[head * p.n_tokens + token] = l > 0.0f ? (m_run[rt] + log2f(l)) * kLn2 : INFINITY;
+    if (g == 0) p.lse[head * p.n_tokens + token] = l == 0.0f ? INFINITY : (m_run[rt] + log2f(l)) * kLn2;
   }
 }
 
-// Adds up a row's shares: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i, rounded once.  A wave takes a row.
+// ---------------------------------------------------------------------------
+// The kernel of few rows: answering token by token.  A request has few rows a kv head (tokens * group, at most 32), so the
+// keys' bytes bound it and what counts is how many of them are under way.  The waves of a workgroup share no tile:
+// each takes tiles of 32 keys of its own, every fourth, K straight into registers in the layout of the product, V into its own
+// part of LDS, both a tile ahead, and waits for nobody until its share of the keys is done.
+//
+// Work is cut by length, not by request: the tiles of all (request, rows, kv head) units are laid end to end and every
+// workgroup takes the same number of them, whatever the lengths are (they are known on the device only).  A unit inside one
+// workgroup's share is finished there; of one that is cut each piece goes to the workgroup's slot (0: the share begins in the
+// unit, 1: it ends in it) and the merge kernel joins them.
+// ---------------------------------------------------------------------------
+struct PagedFewParams {
+  PagedAttnParams a;
+  int64_t* starts;   // [0]: tiles of a workgroup; [1 + b]: tiles before request b
+  float* slot_out;   // [workgroup][2][rows][D]
+  f32x2* slot_sums;  // [workgroup][2][rows]
+};
+constexpr int kFewThreads = 256, kFewWaves = 4, kFewBN = 32;
+constexpr int kFewMaxBatch = 1 << 16;
+
+// What request b is to the kernel.
+struct FewRequest {
+  int first_tok, n_tok, n_keys, n_chunks, n_tiles;
+  template <typename P>
+  __device__ __forceinline__ FewRequest(const P& p, int b, int rows) {
+    const TokenRange tokens = tokens_of(p, b);
+    first_tok = tokens.begin;
+    n_tok = tokens.n;
+    n_keys = (int)min((int64_t)max(p.key_lens[b], 0), p.n_pages > 0 ? (int64_t)p.table_width * p.page_size : 0);
+    n_chunks = (n_tok * p.group + rows - 1) / rows;
+    const KeyGroups groups(p, max(n_keys - n_tok, 0), n_keys - 1);
+    n_tiles = max((groups.count() + 1) / 2, 1);  // (a request without keys has its rows written all the same)
+  }
+  __device__ __forceinline__ int64_t work(int n_heads_kv) const { return (int64_t)n_chunks * n_heads_kv * n_tiles; }
+};
+
+// Sum over the wave's lanes up to and with this one.
+__device__ __forceinline__ int64_t wave_scan(int64_t x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) {
+    const int64_t y = __shfl_up(x, off);
+    if (lane >= off) x += y;
+  }
+  return x;
+}
+__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+template <int DTYPE, int D, int RT>
+__global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFewParams params) {
+  const PagedAttnParams& p = params.a;
+  constexpr int KS = D / 32, DT = D / 16, ROWS = 16 * RT;
+  // V of 32 keys: load r of a tile brings rows r, r + LOADS, ... side by side (1 KiB), 32 bytes of padding between loads: eight
+  // consecutive rows then lie in eight different 32-byte bank windows for the transposing reads.
+  constexpr int LOADS = kFewBN * D * 2 / 1024, LOAD_BYTES = 1024 + 32, STAGE = LOADS * LOAD_BYTES;
+  constexpr int O_STRIDE = D + 4;  // floats: rows of the joined result, a wave's
+  constexpr int WAVE_BYTES = 2 * STAGE > ROWS * O_STRIDE * 4 ? 2 * STAGE : ROWS * O_STRIDE * 4;
+  __shared__ __attribute__((aligned(16))) char lds[kFewWaves][WAVE_BYTES];
+  __shared__ float sums_lds[kFewWaves][ROWS][2];
+  __shared__ int64_t chunk_lds[kFewMaxBatch / 64];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+  // ---- this workgroup's share of all tiles -----------------------------------------
+  auto work_of = [&](int b) -> int64_t { return b < p.batch ? FewRequest(p, b, ROWS).work(p.n_heads_kv) : 0; };
+  int64_t total, per, begin, end, before;  // before: tiles before the chunk of 64 requests in which the share begins
+  int chunk = 0;
+  const int n_chunks = (p.batch + 63) / 64;
+  int64_t scan = wave_scan(work_of(lane));
+  if (n_chunks == 1) {
+    total = lane_value(scan, 63);
+  } else {
+    for (int i = w; i < n_chunks; i += kFewWaves) {
+      const int64_t sum = wave_scan(work_of(i * 64 + lane));
+      if (lane == 63) chunk_lds[i] = sum;
+    }
+    __syncthreads();
+    total = 0;
+    for (int i = 0; i < n_chunks; i += 64) total += lane_value(wave_scan(i + lane < n_chunks ? chunk_lds[i + lane] : 0), 63);
+  }
+  per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kFewWaves);
+  begin = min((int64_t)blockIdx.x * per, total);
+  end = min(begin + per, total);
+  if (blockIdx.x == 0 && tid == 0) params.starts[0] = per;
+  if (begin >= end) return;
+  before = 0;
+  if (n_chunks > 1) {
+    for (int i = 0; i < n_chunks; i += 64) {
+      const int64_t sums = before + wave_scan(i + lane < n_chunks ? chunk_lds[i + lane] : 0);
+      const int passed = __popcll(__ballot(sums <= begin));
+      if (passed > 0) before = lane_value(sums, passed - 1);
+      chunk = i + passed;
+      if (passed < 64) break;
+    }
+    chunk = __builtin_amdgcn_readfirstlane(min(chunk, n_chunks - 1));
+    scan = wave_scan(work_of(chunk * 64 + lane));
+  }
+  const int passed = min(__popcll(__ballot(before + scan <= begin)), 63);
+  int b = __builtin_amdgcn_readfirstlane(chunk * 64 + passed);
+  int64_t b_start = before + (passed > 0 ? lane_value(scan, passed - 1) : 0);
+
+  const uint32_t v_at = lds_address(lds[w]);
+  int64_t at = begin;
+  while (at < end) {
+    const FewRequest request(p, b, ROWS);
+    const int64_t work = request.work(p.n_heads_kv);
+    if (at >= b_start + work) {  // (no rows, or done)
+      b_start += work;
+      if (++b >= p.batch) break;
+      continue;
+    }
+    if (at == b_start && tid == 0) params.starts[1 + b] = b_start;
+    const int unit = __builtin_amdgcn_readfirstlane((int)((at - b_start) / request.n_tiles));
+    const int t_begin = __builtin_amdgcn_readfirstlane((int)(at - b_start - (int64_t)unit * request.n_tiles));
+    const int t_end = __builtin_amdgcn_readfirstlane((int)min((int64_t)request.n_tiles, t_begin + (end - at)));
+    const int slot = at == begin ? 0 : 1;
+    at += t_end - t_begin;
+    const int kv_head = unit % p.n_heads_kv, row0 = unit / p.n_heads_kv * ROWS;
+    const KeyGroups groups(p, max(request.n_keys - request.n_tok, 0), request.n_keys - 1);
+    const int n_groups = request.n_keys > 0 ? groups.count() : 0;
+
+    // ---- this lane's rows --------------------------------------------------------------
+    int64_t out_row[RT];
+    int last_key[RT], first_key[RT];
+    bool live[RT];
+    int w_last = 0x7fffffff, w_first = 0;
+    u32x4 q[RT][KS];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = row0 + rt * 16 + n;
+      live[rt] = r < request.n_tok * p.group;
+      const int tok = r / p.group, head = kv_head * p.group + r % p.group;
+      out_row[rt] = (int64_t)(request.first_tok + tok) * p.n_heads_q + head;
+      last_key[rt] = live[rt] ? request.n_keys - request.n_tok + tok : 0x7fffffff;
+      first_key[rt] = live[rt] && p.window > 0 ? max(last_key[rt] - p.window + 1, 0) : 0;
+      const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (request.first_tok + tok) * p.q_token + head * p.q_head + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        q[rt][ks] = u32x4{0, 0, 0, 0};
+        if (live[rt]) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + 32 * ks);
+      }
+      w_last = min(w_last, wave_min(last_key[rt]));
+      w_first = max(w_first, wave_max(first_key[rt]));
+    }
+    f32x4 o[RT][DT];
+    float m_run[RT], l_run[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m_run[rt] = -INFINITY;
+      l_run[rt] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // ---- where the wave's next 32 tiles are: lane 2 i + j holds the 16-key group j of the i-th of them ------------
+    const int32_t* table = p.block_table + (int64_t)b * p.table_stride;
+    const uint16_t* k_base = reinterpret_cast<const uint16_t*>(p.k) + kv_head * p.head_stride;
+    const uint16_t* v_base = reinterpret_cast<const uint16_t*>(p.v) + kv_head * p.head_stride;
+    constexpr int kNoKey = 0x7fffff00;  // of a group that is not there: past every row's last key
+    int64_t lane_off = 0;
+    int lane_key = kNoKey;
+    auto look_up = [&](int step) {
+      const int group = 2 * (t_begin + w + kFewWaves * (step + (lane >> 1))) + (lane & 1);
+      lane_off = 0;
+      lane_key = kNoKey;
+      if (group < n_groups && group < 2 * t_end) {
+        const int key = groups.at(group) * 16, index = key / p.page_size;
+        const int page = table[index];
+        if ((unsigned)page < (unsigned)p.n_pages) {
+          lane_key = key;
+          lane_off = page * p.page_stride + (int64_t)(key - index * p.page_size) * p.token_stride;
+        }
+      }
+    };
+    // what a lane brings of a tile: K of key n of each group, 8 elements from 32 ks + 8 g; V rows of its half's group
+    constexpr int CH = D / 8;
+    const int64_t k_lane = n * p.token_stride + 8 * g;
+    const int v_row = lane / CH % (16 / LOADS) * LOADS;  // of load 0, in the group of the lane's half
+    const int64_t v_lane = v_row * p.token_stride + lane % CH * 8;
+    const int n_steps = n_groups > 0 && t_begin + w < t_end ? (t_end - t_begin - w + kFewWaves - 1) / kFewWaves : 0;
+    u32x4 k[2][KS];  // K of the tile at hand, and once its products are formed of the next one
+    int64_t off[2];  // where its two groups are
+    int next_key[2], tile_key[2];
+    auto place = [&](int step) {
+      if (step % 32 == 0) look_up(step);
+      const int src = 2 * (step % 32);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        off[kt] = lane_value(lane_off, src + kt);
+        next_key[kt] = __builtin_amdgcn_readlane(lane_key, src + kt);
+      }
+    };
+    auto issue_v = [&](int stage) {
+      const uint16_t* v = v_base + (lane >= 32 ? off[1] : off[0]) + v_lane;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
+#pragma unroll
+      for (int r = 0; r < LOADS; ++r) load_async_piece(v_at + stage * STAGE + r * LOAD_BYTES, v + r * p.token_stride);
+    };
+    auto issue_k = [&]() {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) k[kt][ks] = *reinterpret_cast<const u32x4*>(k_base + off[kt] + k_lane + 32 * ks);
+    };
+    const int v_rd = ((4 * g + (n >> 2)) % LOADS) * LOAD_BYTES + ((4 * g + (n >> 2)) / LOADS) * (D * 2) + 8 * (n & 3);
+    if (n_steps > 0) {
+      place(0);
+      issue_v(0);
+      issue_k();
+    }
+    for (int step = 0; step < n_steps; ++step) {
+      const int stage = step & 1;
+      wait_loads();
+      asm volatile("" ::: "memory");
+      tile_key[0] = next_key[0];
+      tile_key[1] = next_key[1];
+      const bool more = step + 1 < n_steps;
+      if (more) {
+        place(step + 1);
+        issue_v(stage ^ 1);
+      }
+      bool whole = true, full = true;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const int key = tile_key[kt];
+        whole = whole && key + 15 < groups.hull_end && (key + 15 < p.n_starting || key >= groups.window_begin);
+        full = full && key + 15 <= w_last && (key >= w_first || key + 15 < p.n_starting);
+      }
+      if (!whole) {  // V of keys that nobody sees may be anything: cleared by the lanes that brought it
+        const int key0 = lane >= 32 ? tile_key[1] : tile_key[0];
+#pragma unroll
+        for (int r = 0; r < LOADS; ++r)
+          if (!(key0 != kNoKey && groups.sees(p, key0 + v_row + r)))
+            *reinterpret_cast<u32x4*>(lds[w] + stage * STAGE + r * LOAD_BYTES + 16 * lane) = u32x4{0, 0, 0, 0};
+        asm volatile("" ::: "memory");
+      }
+      f32x4 s[RT][2];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          s[rt][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) s[rt][kt] = mfma_16x16x32<DTYPE>(k[kt][ks], q[rt][ks], s[rt][kt]);
+        }
+      if (more) issue_k();
+      if (!(whole & full)) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = tile_key[kt] + 4 * g + e;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              const bool visible = (key <= last_key[rt]) & ((key < p.n_starting) | (key >= first_key[rt])) & (tile_key[kt] != kNoKey);
+              s[rt][kt][e] = visible ? s[rt][kt][e] : -INFINITY;
+            }
+          }
+      }
+      u32x4 pb[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float mx = fmaxf(s[rt][0][0], s[rt][1][0]);
+#pragma unroll
+        for (int e = 1; e < 4; ++e) mx = fmaxf(mx, fmaxf(s[rt][0][e], s[rt][1][e]));
+        mx = rows_max(mx * p.scale_log2);
+        const float m_new = fmaxf(m_run[rt], mx);
+        if (__any(m_new != m_run[rt])) {
+          const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_run[rt] - m_new);
+          l_run[rt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[rt][dt][e] *= alpha;
+          m_run[rt] = m_new;
+        }
+        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          float x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = fast_exp2(fmaf(s[rt][kt][e], p.scale_log2, -m_use));
+            l_run[rt] += x[e];
+          }
+          pb[rt][2 * kt] = pack2<DTYPE>(x[0], x[1]);  // (rounded for the product, summed unrounded, as above)
+          pb[rt][2 * kt + 1] = pack2<DTYPE>(x[2], x[3]);
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const uint32_t from = v_at + stage * STAGE + v_rd + 32 * dt;
+        const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)from));
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(from + 512)));  // rows 16 further
+        const u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma_16x16x32<DTYPE>(a, pb[rt], o[rt][dt]);
+      }
+    }
+
+    // ---- the four waves' results joined --------------------------------------------------
+    asm volatile("" ::: "memory");
+    float* mine = reinterpret_cast<float*>(lds[w]);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float l = rows_sum(l_run[rt]);
+      if (g == 0) {
+        sums_lds[w][rt * 16 + n][0] = m_run[rt];
+        sums_lds[w][rt * 16 + n][1] = l;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mine + (rt * 16 + n) * O_STRIDE + 16 * dt + 4 * g) = o[rt][dt];
+    }
+    __syncthreads();
+    const bool cut = t_end - t_begin < request.n_tiles;
+    constexpr int PIECES = D / 4;  // of a row
+#pragma unroll
+    for (int i = tid; i < ROWS * PIECES; i += kFewThreads) {
+      const int row = i / PIECES, piece = i % PIECES, r = row0 + row;
+      if (r >= request.n_tok * p.group) continue;
+      float m = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kFewWaves; ++x) m = fmaxf(m, sums_lds[x][row][0]);
+      const float m_use = m == -INFINITY ? 0.0f : m;
+      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      float l = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kFewWaves; ++x) {
+        const float weight = fast_exp2(sums_lds[x][row][0] - m_use);
+        l += weight * sums_lds[x][row][1];
+        const f32x4 o4 = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[x]) + row * O_STRIDE + 4 * piece);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
+      }
+      const int64_t token = request.first_tok + r / p.group, head = kv_head * p.group + r % p.group;
+      if (cut || !p.direct) {
+        const int64_t to = cut ? ((int64_t)blockIdx.x * 2 + slot) * ROWS + row : (int64_t)p.first_share * p.n_tokens * p.n_heads_q + token * p.n_heads_q + head;
+        *reinterpret_cast<f32x4*>((cut ? params.slot_out : p.partial_out) + to * D + 4 * piece) = acc;
+        if (piece == 0) (cut ? params.slot_sums : p.partial_sums)[to] = f32x2{m, l};
+      } else {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + 4 * piece) =
+            u32x2{pack2<DTYPE>(acc[0] * inv, acc[1] * inv), pack2<DTYPE>(acc[2] * inv, acc[3] * inv)};
+        if (piece == 0) p.lse[head * p.n_tokens + token] = l == 0.0f ? INFINITY : (m + log2f(l)) * kLn2;
+      }
+    }
+    __syncthreads();  // nobody's part of LDS is filled again before all have read it
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The merge: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's parts, rounded once.  The parts are the pieces of a unit
+// that the kernel of few rows has cut, or the shares of the kernel of rows, or one or the other and the shares of a
+// prefix.  A workgroup takes a row: D / 4 lanes hold it in 16-byte pieces, and the 1024 / D sets of such lanes take parts in turn (a
+// wave that went through 128 parts alone took 17 us).
+// ---------------------------------------------------------------------------
 struct PagedMergeParams {
-  const float* partial_out;
-  const f32x2* partial_sums;
-  void* out;
-  float* lse;
-  const int32_t* cu_seqlens_q;
-  const int32_t* cu_groups;
-  int64_t out_token, out_head;
-  int n_tokens, n_heads_q, batch, n_prefixes;
-  int n_own, n_shares;  // shares of the requests' own keys; with those of the prefixes, which come behind them
+  PagedFewParams few;       // few.starts null: the kernel of rows has made the shares
+  const int32_t* cu_groups; // null: no prefixes
+  int n_prefixes, n_own, n_shares, rows;  // shares of the requests' own keys; with those of the prefixes, which come behind them; rows of a chunk
 };
 constexpr int kPagedMergeThreads = 256;
 template <int DTYPE, int D>
-__global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const PagedMergeParams p) {
-  const int lane = threadIdx.x & 63;
+__global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const PagedMergeParams params) {
+  const PagedAttnParams& p = params.few.a;
+  constexpr int PIECES = D / 4, SETS = kPagedMergeThreads / PIECES;
+  __shared__ f32x4 acc_lds[SETS][PIECES];
+  __shared__ f32x2 sums_lds[SETS];
+  const int row = blockIdx.x, tid = threadIdx.x, piece = tid % PIECES, set = tid / PIECES;
   const int64_t n_rows = p.n_tokens * p.n_heads_q;  // (fits 32 bits)
-  // (a wave has one row: said so, what follows from it is scalar, the branches too)
-  const int row = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * (kPagedMergeThreads / 64) + (threadIdx.x >> 6)));
-  if (row >= n_rows) return;
-  constexpr int PER = D / 64;
   // rows of no request are left as they were, and those of no prefix have no shares of one
   const int token = row / p.n_heads_q, head = row % p.n_heads_q;
-  auto first_token = [&](int r) { return p.cu_seqlens_q != nullptr ? p.cu_seqlens_q[min(max(r, 0), p.batch)] : r; };
-  if (token < first_token(0) || token >= first_token(p.batch)) return;
+  if ((token < first_token(p, 0)) | (token >= first_token(p, p.batch))) return;
   int first = 0, end = 0x7fffffff;
-  if (p.cu_groups != nullptr) {
-    first = first_token(p.cu_groups[0]);
-    end = first_token(p.cu_groups[p.n_prefixes]);
+  if (params.cu_groups != nullptr) {
+    PagedAttnParams of_prefix = p;
+    of_prefix.cu_groups = params.cu_groups;
+    first = first_token(of_prefix, 0);
+    end = first_token(of_prefix, params.n_prefixes);
   }
-  // (& on purpose: of the two conditions joined by && or ||, this compiler, clang 22, leaves the second one out)
-  const int n_shares = ((token >= first) & (token < end)) ? p.n_shares : p.n_own;
-  float m = -INFINITY;
-  for (int i = lane; i < n_shares; i += 64) m = fmaxf(m, p.partial_sums[i * n_rows + row][0]);
+  // (& on purpose: of two conditions joined by && or || here, this compiler, clang 22, left the second one out)
+  const int n_shares = ((token >= first) & (token < end)) ? params.n_shares : params.n_own;
+  // the pieces of a unit that was cut come first, in the place of the own share
+  int n_cut = 0, wg = 0, slot = 0, chunk_row = 0;
+  if (params.few.starts != nullptr) {
+    int b = token;
+    if (p.cu_seqlens_q != nullptr) {
+      int lo = 0, hi = p.batch;  // the last request that begins at or before the token
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 63) / 64, at = lo + (tid & 63) * step;
+        const int n = __popcll(__ballot((at < hi) & (first_token(p, min(at, p.batch)) <= token)));
+        if (n > 1) lo += (n - 1) * step;
+        hi = min(lo + step, hi);
+      }
+      b = __builtin_amdgcn_readfirstlane(lo);
+    }
+    const FewRequest request(p, b, params.rows);
+    const int r = (token - request.first_tok) * p.group + head % p.group;
+    chunk_row = r % params.rows;
+    const int64_t per = params.few.starts[0];
+    const int64_t start = params.few.starts[1 + b] + ((int64_t)(r / params.rows) * p.n_heads_kv + head / p.group) * request.n_tiles;
+    wg = (int)(start / per);
+    n_cut = (int)((start + request.n_tiles - 1) / per) - wg + 1;
+    slot = start == wg * per ? 0 : 1;
+    if (n_cut == 1) n_cut = 0;
+    if ((n_cut == 0) & (p.direct != 0)) return;  // done where it was computed
+  }
+  const int n_parts = n_cut > 0 ? n_cut + n_shares - 1 : n_shares;
+  // where part i is
+  auto part = [&](int i, const f32x2*& sums) -> const float* {
+    if (i < n_cut) {
+      const int64_t at = ((int64_t)(wg + i) * 2 + (i == 0 ? slot : 0)) * params.rows + chunk_row;
+      sums = params.few.slot_sums + at;
+      return params.few.slot_out + at * D;
+    }
+    const int64_t at = (i - n_cut + (n_cut > 0)) * n_rows + row;
+    sums = p.partial_sums + at;
+    return p.partial_out + at * D;
+  };
+  float m = -INFINITY, l = 0.0f;
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  constexpr int AT_ONCE = 4;
+  for (int i0 = set; i0 < n_parts; i0 += SETS * AT_ONCE) {
+    f32x2 ml[AT_ONCE];
+    f32x4 o4[AT_ONCE];
 #pragma unroll
-  for (int off = 32; off > 0; off /= 2) m = fmaxf(m, __shfl_xor(m, off));
+    for (int x = 0; x < AT_ONCE; ++x) {
+      const int i = min(i0 + x * SETS, n_parts - 1);
+      const f32x2* sums;
+      const float* from = part(i, sums);
+      ml[x] = *sums;
+      o4[x] = *reinterpret_cast<const f32x4*>(from + 4 * piece);
+    }
+    float m_new = m;
+#pragma unroll
+    for (int x = 0; x < AT_ONCE; ++x) {
+      if (i0 + x * SETS >= n_parts) ml[x] = f32x2{-INFINITY, 0.0f};
+      m_new = fmaxf(m_new, ml[x][0]);
+    }
+    const float m_use = m_new == -INFINITY ? 0.0f : m_new, old = fast_exp2(m - m_use);
+    l *= old;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= old;
+#pragma unroll
+    for (int x = 0; x < AT_ONCE; ++x) {
+      const float weight = fast_exp2(ml[x][0] - m_use);
+      l += weight * ml[x][1];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] += weight > 0.0f ? weight * o4[x][e] : 0.0f;  // (nothing is written of a share without weights)
+    }
+    m = m_new;
+  }
+  acc_lds[set][piece] = acc;
+  if (piece == 0) sums_lds[set] = f32x2{m, l};
+  __syncthreads();
+  if (tid >= PIECES) return;
+  m = -INFINITY;
+#pragma unroll
+  for (int x = 0; x < SETS; ++x) m = fmaxf(m, sums_lds[x][0]);
   const float m_use = m == -INFINITY ? 0.0f : m;
-  float acc[PER] = {}, l = 0.0f;
-  for (int i = 0; i < n_shares; ++i) {
-    const f32x2 ml = p.partial_sums[i * n_rows + row];
-    if (!(ml[1] != 0.0f)) continue;  // (no visible key, and nothing written)
-    const float weight = fast_exp2(ml[0] - m_use);
-    l += weight * ml[1];
-    const float* from = p.partial_out + (i * n_rows + row) * D + PER * lane;
+  l = 0.0f;
+  acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int e = 0; e < PER; ++e) acc[e] += weight * from[e];
+  for (int x = 0; x < SETS; ++x) {
+    const float weight = fast_exp2(sums_lds[x][0] - m_use);
+    l += weight * sums_lds[x][1];
+    const f32x4 o4 = acc_lds[x][tid];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + PER * lane;
-#pragma unroll
-  for (int e = 0; e < PER; ++e) to[e] = Elem<DTYPE>::store(acc[e] * inv);
-  if (lane == 0) p.lse[(int64_t)head * p.n_tokens + token] = l > 0.0f ? (m + log2f(l)) * kLn2 : INFINITY;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + 4 * tid) =
+      u32x2{pack2<DTYPE>(acc[0] * inv, acc[1] * inv), pack2<DTYPE>(acc[2] * inv, acc[3] * inv)};
+  if (tid == 0) p.lse[(int64_t)head * p.n_tokens + token] = l == 0.0f ? INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // ---- host ---------------------------------------------------------------------------
@@ -471,12 +898,69 @@ static int launch_rows(const PagedAttnParams& p, int head_dim, int dtype, void* 
   return check_launch("paged_rows_kernel");
 }
 
-static int launch_merge(const PagedAttnParams& p, const int32_t* cu_groups, int n_prefixes, int n_shares, int head_dim, int dtype, void* stream) {
-  const PagedMergeParams m = {p.partial_out, p.partial_sums, p.out, p.lse, p.cu_seqlens_q, cu_groups, p.out_token, p.out_head,
-                              p.n_tokens, p.n_heads_q, p.batch, n_prefixes, p.n_splits, n_shares};
-  const int64_t n_wg = ((int64_t)p.n_tokens * p.n_heads_q + kPagedMergeThreads / 64 - 1) / (kPagedMergeThreads / 64);
+// How a call is laid out: which kernel takes the requests' own keys, and what of the workspace is whose.
+struct PagedPlan {
+  int rows = 0;      // of a chunk of the kernel of few rows; 0: the kernel of rows takes them
+  int n_wg = 0;      // of the kernel of few rows
+  int n_own = 1, n_prefix = 0;  // shares
+  size_t starts = 0, slots = 0, shares = 0;  // bytes
+  size_t bytes() const { return starts + slots + shares; }
+};
+static size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+static PagedPlan plan_paged(const PagedShape& s, int64_t max_q, int64_t max_keys, int n_prefixes, int64_t max_prefix) {
+  PagedPlan plan;
+  const int64_t rows = max_q * (s.n_heads_q / s.n_heads_kv);
+  if (rows <= 32 && s.batch <= kFewMaxBatch) {
+    plan.rows = rows <= 16 ? 16 : 32;
+    plan.n_wg = 2 * device_cu_count();
+    plan.starts = up16((size_t)(s.batch + 1) * sizeof(int64_t));
+    plan.slots = (size_t)plan.n_wg * 2 * plan.rows * (s.head_dim + 2) * sizeof(float);
+  } else {
+    plan.n_own = row_shares(s, max_keys);
+  }
+  if (n_prefixes > 0) {
+    const PagedShape of_prefix = {s.n_tokens, n_prefixes, s.n_heads_q, s.n_heads_kv, s.head_dim};
+    plan.n_prefix = row_shares(of_prefix, max_prefix);
+  }
+  if (plan.n_own + plan.n_prefix > 1) plan.shares = shares_bytes(s, plan.n_own + plan.n_prefix);
+  return plan;
+}
+
+template <int RT>
+static void launch_few_rows(const PagedFewParams& f, const PagedPlan& plan, int head_dim, int dtype, void* stream) {
+  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)plan.n_wg), dim3(kFewThreads), 0, (hipStream_t)stream, f); };
+  if (dtype == DCP_DTYPE_BF16) {
+    if (head_dim == 128) launch(paged_few_kernel<DCP_DTYPE_BF16, 128, RT>);
+    else launch(paged_few_kernel<DCP_DTYPE_BF16, 64, RT>);
+  } else {
+    if (head_dim == 128) launch(paged_few_kernel<DCP_DTYPE_FP16, 128, RT>);
+    else launch(paged_few_kernel<DCP_DTYPE_FP16, 64, RT>);
+  }
+}
+
+// The requests' own keys, and the merge where there is something to join.
+static int launch_own(PagedAttnParams p, const PagedPlan& plan, const int32_t* cu_groups, int n_prefixes, int head_dim, int dtype, void* workspace,
+                      void* stream) {
+  PagedFewParams f = {};
+  if (plan.rows > 0) {
+    f.starts = reinterpret_cast<int64_t*>(workspace);
+    f.slot_out = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.starts);
+    f.slot_sums = reinterpret_cast<f32x2*>(f.slot_out + (size_t)plan.n_wg * 2 * plan.rows * head_dim);
+    f.a = p;
+    KernelTimer timer("paged_few_kernel", stream);
+    if (plan.rows == 16) launch_few_rows<1>(f, plan, head_dim, dtype, stream);
+    else launch_few_rows<2>(f, plan, head_dim, dtype, stream);
+    if (const int status = check_launch("paged_few_kernel")) return status;
+  } else {
+    if (const int status = launch_rows(p, head_dim, dtype, stream)) return status;
+    if (p.direct) return DCP_OK;
+    f.a = p;
+  }
+  const PagedMergeParams m = {f, cu_groups, n_prefixes, plan.n_own, plan.n_own + plan.n_prefix, plan.rows};
   KernelTimer timer("paged_merge_kernel", stream);
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(kPagedMergeThreads), 0, (hipStream_t)stream, m); };
+  auto launch = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.n_tokens * p.n_heads_q)), dim3(kPagedMergeThreads), 0, (hipStream_t)stream, m);
+  };
   if (dtype == DCP_DTYPE_BF16) {
     if (head_dim == 128) launch(paged_merge_kernel<DCP_DTYPE_BF16, 128>);
     else launch(paged_merge_kernel<DCP_DTYPE_BF16, 64>);
@@ -487,9 +971,9 @@ static int launch_merge(const PagedAttnParams& p, const int32_t* cu_groups, int 
   return check_launch("paged_merge_kernel");
 }
 
-static void place_shares(PagedAttnParams& p, void* workspace, int n_shares, int head_dim) {
-  p.partial_out = reinterpret_cast<float*>(workspace);
-  p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)n_shares * p.n_tokens * p.n_heads_q * head_dim);
+static void place_shares(PagedAttnParams& p, const PagedPlan& plan, void* workspace, int head_dim) {
+  p.partial_out = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.starts + plan.slots);
+  p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)(plan.n_own + plan.n_prefix) * p.n_tokens * p.n_heads_q * head_dim);
 }
 
 }  // namespace dcp
@@ -499,9 +983,8 @@ using namespace dcp;
 extern "C" size_t dcp_paged_attn_workspace_bytes(int n_tokens, int batch, int n_heads_q, int n_heads_kv, int head_dim, int max_seqlen_q,
                                                  int max_seqlen_k) {
   if (n_tokens <= 0 || batch <= 0 || n_heads_q <= 0 || n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0) return 0;
-  const PagedShape s = {n_tokens, batch, n_heads_q, n_heads_kv, head_dim};
-  const int n = row_shares(s, max_seqlen_k);
-  return n > 1 ? shares_bytes(s, n) : 0;
+  if (max_seqlen_q <= 0 || max_seqlen_k <= 0) return 0;
+  return plan_paged({n_tokens, batch, n_heads_q, n_heads_kv, head_dim}, max_seqlen_q, max_seqlen_k, 0, 0).bytes();
 }
 
 extern "C" int dcp_paged_attn(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse, const int32_t* block_table,
@@ -532,24 +1015,24 @@ extern "C" int dcp_paged_attn(const void* q, const void* k_cache, const void* v_
   if (n_tokens == 0 || batch == 0) return DCP_OK;
   DCP_REQUIRE(q && out && lse && block_table && seq_lens && (n_pages == 0 || (k_cache && v_cache)), "paged_attn: null argument");
   DCP_REQUIRE(max_seqlen_q > 0 && max_seqlen_k > 0, "paged_attn: the longest lengths must be positive");
-  p.n_splits = row_shares(s, max_seqlen_k);
+  const PagedPlan plan = plan_paged(s, max_seqlen_q, max_seqlen_k, 0, 0);
+  p.n_splits = plan.n_own;
   const int64_t tiles = row_tiles(s);
   DCP_REQUIRE(tiles < ((int64_t)1 << 31), "paged_attn: too many rows");
   p.n_tiles = (int)tiles;
-  p.direct = p.n_splits == 1;
-  const size_t needed = p.direct ? 0 : shares_bytes(s, p.n_splits);
+  p.direct = plan.n_own == 1;
+  const size_t needed = plan.bytes();
   DCP_REQUIRE(needed == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= needed),
               "paged_attn: workspace of %zu bytes is missing, not 16-byte aligned or smaller than the %zu needed", workspace_bytes, needed);
-  if (!p.direct) place_shares(p, workspace, p.n_splits, head_dim);
-  if (const int status = launch_rows(p, head_dim, dtype, stream)) return status;
-  return p.direct ? DCP_OK : launch_merge(p, nullptr, 0, p.n_splits, head_dim, dtype, stream);
+  if (!p.direct) place_shares(p, plan, workspace, head_dim);
+  return launch_own(p, plan, nullptr, 0, head_dim, dtype, workspace, stream);
 }
 
 extern "C" size_t dcp_shared_prefix_attn_workspace_bytes(int n_tokens, int batch, int n_prefixes, int n_heads_q, int n_heads_kv, int head_dim,
                                                          int max_seqlen_q, int max_seqlen_k, int max_prefix_len) {
   if (n_tokens <= 0 || batch <= 0 || n_prefixes <= 0 || n_heads_q <= 0 || n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0) return 0;
-  const PagedShape s = {n_tokens, batch, n_heads_q, n_heads_kv, head_dim}, of_prefix = {n_tokens, n_prefixes, n_heads_q, n_heads_kv, head_dim};
-  return shares_bytes(s, row_shares(s, max_seqlen_k) + row_shares(of_prefix, max_prefix_len));
+  if (max_seqlen_q <= 0 || max_seqlen_k <= 0 || max_prefix_len <= 0) return 0;
+  return plan_paged({n_tokens, batch, n_heads_q, n_heads_kv, head_dim}, max_seqlen_q, max_seqlen_k, n_prefixes, max_prefix_len).bytes();
 }
 
 extern "C" int dcp_shared_prefix_attn(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse,
@@ -588,20 +1071,19 @@ extern "C" int dcp_shared_prefix_attn(const void* q, const void* k_cache, const 
   DCP_REQUIRE(q && out && lse && prefix_table && prefix_lens && cu_groups && block_table && seq_lens && (n_pages == 0 || (k_cache && v_cache)),
               "shared_prefix_attn: null argument");
   DCP_REQUIRE(max_seqlen_q > 0 && max_seqlen_k > 0 && max_prefix_len > 0, "shared_prefix_attn: the longest lengths must be positive");
-  p.n_splits = row_shares(s, max_seqlen_k);
-  pre.n_splits = row_shares(of_prefix, max_prefix_len);
+  const PagedPlan plan = plan_paged(s, max_seqlen_q, max_seqlen_k, n_prefixes, max_prefix_len);
+  p.n_splits = plan.n_own;
+  pre.n_splits = plan.n_prefix;
   const int64_t tiles = row_tiles(s);
   DCP_REQUIRE(tiles < ((int64_t)1 << 31) - n_prefixes, "shared_prefix_attn: too many rows");
   p.n_tiles = (int)tiles;
   pre.n_tiles = (int)row_tiles(of_prefix);
-  const int n_shares = p.n_splits + pre.n_splits;
-  const size_t needed = shares_bytes(s, n_shares);
+  const size_t needed = plan.bytes();
   DCP_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= needed,
               "shared_prefix_attn: workspace of %zu bytes is missing, not 16-byte aligned or smaller than the %zu needed", workspace_bytes, needed);
-  place_shares(p, workspace, n_shares, head_dim);
-  place_shares(pre, workspace, n_shares, head_dim);
-  pre.first_share = p.n_splits;
+  place_shares(p, plan, workspace, head_dim);
+  place_shares(pre, plan, workspace, head_dim);
+  pre.first_share = plan.n_own;
   if (const int status = launch_rows(pre, head_dim, dtype, stream)) return status;
-  if (const int status = launch_rows(p, head_dim, dtype, stream)) return status;
-  return launch_merge(p, cu_groups, n_prefixes, n_shares, head_dim, dtype, stream);
+  return launch_own(p, plan, cu_groups, n_prefixes, head_dim, dtype, workspace, stream);
 }
