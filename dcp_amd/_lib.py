@@ -56,11 +56,8 @@ SIGNATURES = {
     "dcp_attn_bwd_select": [_I],
     "dcp_paged_cache_tables": [_P, _P, _P, _L] + [_P] * 6 + [_I] * 5 + [_P],
     "dcp_paged_cache_write": [_P] * 5 + [_I] * 4 + [_L] * 3 + [_I] + [_L] * 3 + [_P],
-    "dcp_paged_attn_workspace_bytes": [_I] * 7,
-    "dcp_paged_attn": [_P] * 8 + [_I] * 5 + [_L] * 4 + [_I] * 2 + [_L] * 3 + [_I, _L] + [_I] * 4 + [_F, _I, _P, c_size_t, _P],
-    "dcp_shared_prefix_attn_workspace_bytes": [_I] * 9,
-    "dcp_shared_prefix_attn": [_P] * 11 + [_I] * 6 + [_L] * 4 + [_I] * 2 + [_L] * 3 + [_I, _L, _I, _L] + [_I] * 3
-                              + [_F, _I, _P, c_size_t, _P],
+    "dcp_paged_attn_workspace_bytes": [_P],
+    "dcp_paged_attn": [_P, _P, c_size_t, _P],
     "dcp_greedy_stage_selection": [_I, _P, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _L, _P, _P, _P],
 }
 
@@ -97,8 +94,7 @@ def load():
             fn.restype = {"dcp_last_error": c_char_p, "dcp_record_begin": c_void_p, "dcp_record_free": None, "dcp_attn_bwd_workspace_bytes": c_size_t,
                           "dcp_attn_fwd_workspace_bytes": c_size_t,
                           "dcp_attn_bwd_static_scratch_bytes": c_size_t,
-                          "dcp_attn_bwd_workspace_bytes_kv": c_size_t, "dcp_paged_attn_workspace_bytes": c_size_t,
-                          "dcp_shared_prefix_attn_workspace_bytes": c_size_t}.get(name, c_int)
+                          "dcp_attn_bwd_workspace_bytes_kv": c_size_t, "dcp_paged_attn_workspace_bytes": c_size_t}.get(name, c_int)
         _lib = lib
     return _lib
 

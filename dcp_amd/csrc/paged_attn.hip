@@ -128,6 +128,14 @@ __device__ __forceinline__ void load_async_piece(uint32_t lds_at, const uint16_t
                : "memory");
 }
 
+// The same for what is read once (it takes no room in the caches).
+__device__ __forceinline__ void load_async_piece_nt(uint32_t lds_at, const uint16_t* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds_at)), "v"(from)
+               : "memory");
+}
+
 template <int DTYPE, int D>
 __global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const PagedAttnParams p) {
   typedef KvTile<D> Tile;
@@ -373,10 +381,14 @@ __global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const Paged
 // ---------------------------------------------------------------------------
 struct PagedFewParams {
   PagedAttnParams a;
-  int64_t* starts;   // [0]: tiles of a workgroup; [1 + b]: tiles before request b
-  float* slot_out;   // [workgroup][2][rows][D]
-  f32x2* slot_sums;  // [workgroup][2][rows]
+  int2* cuts;        // [token][q head]: see cut_of
+  float* slot_out;   // [workgroup][2][head of the workgroup][rows][D]
+  f32x2* slot_sums;  // [workgroup][2][head of the workgroup][rows]
+  int heads;         // kv heads a workgroup takes at once: 1, 2 or 4, as many to each of which it has 4 / heads waves
 };
+// What the merge needs to know of a row: the workgroup that begins its unit, how many the unit is cut over, the slot of the first
+// piece (the others are in slot 0) and the row in the slots.
+__device__ __forceinline__ int2 cut_of(int wg, int n_pieces, int slot, int row) { return int2{wg, n_pieces | row << 20 | slot << 28}; }
 constexpr int kFewThreads = 256, kFewWaves = 4, kFewBN = 32;
 constexpr int kFewMaxBatch = 1 << 16;
 
@@ -393,7 +405,7 @@ struct FewRequest {
     const KeyGroups groups(p, max(n_keys - n_tok, 0), n_keys - 1);
     n_tiles = max((groups.count() + 1) / 2, 1);  // (a request without keys has its rows written all the same)
   }
-  __device__ __forceinline__ int64_t work(int n_heads_kv) const { return (int64_t)n_chunks * n_heads_kv * n_tiles; }
+  __device__ __forceinline__ int64_t work(int head_groups) const { return (int64_t)n_chunks * head_groups * n_tiles; }
 };
 
 // Sum over the wave's lanes up to and with this one.
@@ -426,8 +438,11 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
+  const int heads = params.heads, head_groups = p.n_heads_kv / heads, turns = kFewWaves / heads;
+  const int my_head = w % heads, my_turn = w / heads;  // of the workgroup's heads; of the waves that share its tiles
+
   // ---- this workgroup's share of all tiles -----------------------------------------
-  auto work_of = [&](int b) -> int64_t { return b < p.batch ? FewRequest(p, b, ROWS).work(p.n_heads_kv) : 0; };
+  auto work_of = [&](int b) -> int64_t { return b < p.batch ? FewRequest(p, b, ROWS).work(head_groups) : 0; };
   int64_t total, per, begin, end, before;  // before: tiles before the chunk of 64 requests in which the share begins
   int chunk = 0;
   const int n_chunks = (p.batch + 63) / 64;
@@ -443,10 +458,9 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
     total = 0;
     for (int i = 0; i < n_chunks; i += 64) total += lane_value(wave_scan(i + lane < n_chunks ? chunk_lds[i + lane] : 0), 63);
   }
-  per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kFewWaves);
+  per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)turns);
   begin = min((int64_t)blockIdx.x * per, total);
   end = min(begin + per, total);
-  if (blockIdx.x == 0 && tid == 0) params.starts[0] = per;
   if (begin >= end) return;
   before = 0;
   if (n_chunks > 1) {
@@ -468,19 +482,19 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
   int64_t at = begin;
   while (at < end) {
     const FewRequest request(p, b, ROWS);
-    const int64_t work = request.work(p.n_heads_kv);
+    const int64_t work = request.work(head_groups);
     if (at >= b_start + work) {  // (no rows, or done)
       b_start += work;
       if (++b >= p.batch) break;
       continue;
     }
-    if (at == b_start && tid == 0) params.starts[1 + b] = b_start;
     const int unit = __builtin_amdgcn_readfirstlane((int)((at - b_start) / request.n_tiles));
     const int t_begin = __builtin_amdgcn_readfirstlane((int)(at - b_start - (int64_t)unit * request.n_tiles));
     const int t_end = __builtin_amdgcn_readfirstlane((int)min((int64_t)request.n_tiles, t_begin + (end - at)));
     const int slot = at == begin ? 0 : 1;
+    const int n_cut = t_begin == 0 ? (int)((at + request.n_tiles - 1) / per) - (int)blockIdx.x + 1 : 0;
     at += t_end - t_begin;
-    const int kv_head = unit % p.n_heads_kv, row0 = unit / p.n_heads_kv * ROWS;
+    const int kv_head0 = unit % head_groups * heads, kv_head = kv_head0 + my_head, row0 = unit / head_groups * ROWS;
     const KeyGroups groups(p, max(request.n_keys - request.n_tok, 0), request.n_keys - 1);
     const int n_groups = request.n_keys > 0 ? groups.count() : 0;
 
@@ -525,7 +539,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
     int64_t lane_off = 0;
     int lane_key = kNoKey;
     auto look_up = [&](int step) {
-      const int group = 2 * (t_begin + w + kFewWaves * (step + (lane >> 1))) + (lane & 1);
+      const int group = 2 * (t_begin + my_turn + turns * (step + (lane >> 1))) + (lane & 1);
       lane_off = 0;
       lane_key = kNoKey;
       if (group < n_groups && group < 2 * t_end) {
@@ -542,7 +556,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
     const int64_t k_lane = n * p.token_stride + 8 * g;
     const int v_row = lane / CH % (16 / LOADS) * LOADS;  // of load 0, in the group of the lane's half
     const int64_t v_lane = v_row * p.token_stride + lane % CH * 8;
-    const int n_steps = n_groups > 0 && t_begin + w < t_end ? (t_end - t_begin - w + kFewWaves - 1) / kFewWaves : 0;
+    const int n_steps = n_groups > 0 && t_begin + my_turn < t_end ? (t_end - t_begin - my_turn + turns - 1) / turns : 0;
     u32x4 k[2][KS];  // K of the tile at hand, and once its products are formed of the next one
     int64_t off[2];  // where its two groups are
     int next_key[2], tile_key[2];
@@ -559,13 +573,13 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
       const uint16_t* v = v_base + (lane >= 32 ? off[1] : off[0]) + v_lane;
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
 #pragma unroll
-      for (int r = 0; r < LOADS; ++r) load_async_piece(v_at + stage * STAGE + r * LOAD_BYTES, v + r * p.token_stride);
+      for (int r = 0; r < LOADS; ++r) load_async_piece_nt(v_at + stage * STAGE + r * LOAD_BYTES, v + r * p.token_stride);
     };
     auto issue_k = [&]() {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) k[kt][ks] = *reinterpret_cast<const u32x4*>(k_base + off[kt] + k_lane + 32 * ks);
+        for (int ks = 0; ks < KS; ++ks) k[kt][ks] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_base + off[kt] + k_lane + 32 * ks));
     };
     const int v_rd = ((4 * g + (n >> 2)) % LOADS) * LOAD_BYTES + ((4 * g + (n >> 2)) / LOADS) * (D * 2) + 8 * (n & 3);
     if (n_steps > 0) {
@@ -681,27 +695,25 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
     __syncthreads();
     const bool cut = t_end - t_begin < request.n_tiles;
     constexpr int PIECES = D / 4;  // of a row
-#pragma unroll
-    for (int i = tid; i < ROWS * PIECES; i += kFewThreads) {
-      const int row = i / PIECES, piece = i % PIECES, r = row0 + row;
+    for (int i = tid; i < heads * ROWS * PIECES; i += kFewThreads) {
+      const int piece = i % PIECES, row = i / PIECES % ROWS, of = i / PIECES / ROWS, r = row0 + row;
       if (r >= request.n_tok * p.group) continue;
       float m = -INFINITY;
-#pragma unroll
-      for (int x = 0; x < kFewWaves; ++x) m = fmaxf(m, sums_lds[x][row][0]);
+      for (int x = of; x < kFewWaves; x += heads) m = fmaxf(m, sums_lds[x][row][0]);
       const float m_use = m == -INFINITY ? 0.0f : m;
       f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
       float l = 0.0f;
-#pragma unroll
-      for (int x = 0; x < kFewWaves; ++x) {
+      for (int x = of; x < kFewWaves; x += heads) {
         const float weight = fast_exp2(sums_lds[x][row][0] - m_use);
         l += weight * sums_lds[x][row][1];
         const f32x4 o4 = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[x]) + row * O_STRIDE + 4 * piece);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
       }
-      const int64_t token = request.first_tok + r / p.group, head = kv_head * p.group + r % p.group;
+      const int64_t token = request.first_tok + r / p.group, head = (kv_head0 + of) * p.group + r % p.group;
+      if (piece == 0 && t_begin == 0) params.cuts[token * p.n_heads_q + head] = cut_of((int)blockIdx.x, n_cut, slot, of * ROWS + row);
       if (cut || !p.direct) {
-        const int64_t to = cut ? ((int64_t)blockIdx.x * 2 + slot) * ROWS + row : (int64_t)p.first_share * p.n_tokens * p.n_heads_q + token * p.n_heads_q + head;
+        const int64_t to = cut ? (((int64_t)blockIdx.x * 2 + slot) * heads + of) * ROWS + row : (int64_t)p.first_share * p.n_tokens * p.n_heads_q + token * p.n_heads_q + head;
         *reinterpret_cast<f32x4*>((cut ? params.slot_out : p.partial_out) + to * D + 4 * piece) = acc;
         if (piece == 0) (cut ? params.slot_sums : p.partial_sums)[to] = f32x2{m, l};
       } else {
@@ -722,7 +734,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
 // wave that went through 128 parts alone took 17 us).
 // ---------------------------------------------------------------------------
 struct PagedMergeParams {
-  PagedFewParams few;       // few.starts null: the kernel of rows has made the shares
+  PagedFewParams few;       // few.cuts null: the kernel of rows has made the shares
   const int32_t* cu_groups; // null: no prefixes
   int n_prefixes, n_own, n_shares, rows;  // shares of the requests' own keys; with those of the prefixes, which come behind them; rows of a chunk
 };
@@ -748,27 +760,14 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   // (& on purpose: of two conditions joined by && or || here, this compiler, clang 22, left the second one out)
   const int n_shares = ((token >= first) & (token < end)) ? params.n_shares : params.n_own;
   // the pieces of a unit that was cut come first, in the place of the own share
-  int n_cut = 0, wg = 0, slot = 0, chunk_row = 0;
-  if (params.few.starts != nullptr) {
-    int b = token;
-    if (p.cu_seqlens_q != nullptr) {
-      int lo = 0, hi = p.batch;  // the last request that begins at or before the token
-      while (hi - lo > 1) {
-        const int step = (hi - lo + 63) / 64, at = lo + (tid & 63) * step;
-        const int n = __popcll(__ballot((at < hi) & (first_token(p, min(at, p.batch)) <= token)));
-        if (n > 1) lo += (n - 1) * step;
-        hi = min(lo + step, hi);
-      }
-      b = __builtin_amdgcn_readfirstlane(lo);
-    }
-    const FewRequest request(p, b, params.rows);
-    const int r = (token - request.first_tok) * p.group + head % p.group;
-    chunk_row = r % params.rows;
-    const int64_t per = params.few.starts[0];
-    const int64_t start = params.few.starts[1 + b] + ((int64_t)(r / params.rows) * p.n_heads_kv + head / p.group) * request.n_tiles;
-    wg = (int)(start / per);
-    n_cut = (int)((start + request.n_tiles - 1) / per) - wg + 1;
-    slot = start == wg * per ? 0 : 1;
+  int n_cut = 0, wg = 0, slot = 0, slot_row = 0;
+  const int slot_rows = params.few.heads * params.rows;
+  if (params.few.cuts != nullptr) {
+    const int2 at = params.few.cuts[row];
+    wg = at.x;
+    n_cut = at.y & 0xfffff;
+    slot_row = at.y >> 20 & 0xff;
+    slot = at.y >> 28;
     if (n_cut == 1) n_cut = 0;
     if ((n_cut == 0) & (p.direct != 0)) return;  // done where it was computed
   }
@@ -776,7 +775,7 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   // where part i is
   auto part = [&](int i, const f32x2*& sums) -> const float* {
     if (i < n_cut) {
-      const int64_t at = ((int64_t)(wg + i) * 2 + (i == 0 ? slot : 0)) * params.rows + chunk_row;
+      const int64_t at = ((int64_t)(wg + i) * 2 + (i == 0 ? slot : 0)) * slot_rows + slot_row;
       sums = params.few.slot_sums + at;
       return params.few.slot_out + at * D;
     }
@@ -851,6 +850,10 @@ static int64_t row_tiles(const PagedShape& s) {
   return (int64_t)s.n_tokens * (s.n_heads_q / s.n_heads_kv) / kRowsBM + s.batch;
 }
 // Shares of a tile's keys: enough for two rounds of the device's workgroups.
+// Keys that the queries of a request see, of all of them.
+static int64_t seen_keys(int64_t max_q, int64_t max_keys, int window, int n_starting) {
+  return window > 0 ? std::min(max_keys, max_q + window + n_starting) : max_keys;
+}
 static int row_shares(const PagedShape& s, int64_t max_keys) {
   const int64_t items = std::max<int64_t>(row_tiles(s) * s.n_heads_kv, 1);
   const int64_t wanted = (4 * (int64_t)device_cu_count() + items - 1) / items;
@@ -859,28 +862,6 @@ static int row_shares(const PagedShape& s, int64_t max_keys) {
 }
 static size_t shares_bytes(const PagedShape& s, int n_shares) {
   return (size_t)n_shares * s.n_tokens * s.n_heads_q * (s.head_dim + 2) * sizeof(float);
-}
-
-static int check_paged(const char* what, const PagedShape& s, const PagedAttnParams& p, float softmax_scale, int dtype) {
-  if (dtype != DCP_DTYPE_BF16 && dtype != DCP_DTYPE_FP16)
-    return fail(DCP_ERR_UNSUPPORTED, "%s: dtype %d unsupported (bf16 and fp16 only)", what, dtype);
-  if (s.head_dim != 64 && s.head_dim != 128) return fail(DCP_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (64 or 128)", what, s.head_dim);
-  DCP_REQUIRE(s.n_tokens >= 0 && s.batch >= 0 && p.n_pages >= 0, "%s: negative size", what);
-  DCP_REQUIRE(s.n_heads_q > 0 && s.n_heads_kv > 0 && s.n_heads_q % s.n_heads_kv == 0, "%s: n_heads_q %d must be a multiple of n_heads_kv %d",
-              what, s.n_heads_q, s.n_heads_kv);
-  DCP_REQUIRE(softmax_scale > 0.0f, "%s: softmax_scale must be positive", what);
-  DCP_REQUIRE(p.window >= 0 && p.n_starting >= 0, "%s: negative window or number of first tokens", what);
-  DCP_REQUIRE(p.page_size > 0 && p.page_size % 16 == 0, "%s: page_size %d must be a positive multiple of 16", what, p.page_size);
-  DCP_REQUIRE(p.table_width > 0 && p.table_stride >= 0, "%s: empty block tables", what);
-  DCP_REQUIRE((int64_t)p.table_width * p.page_size < 0x7fffff00, "%s: too many keys a request", what);
-  DCP_REQUIRE(p.page_stride % 8 == 0 && p.token_stride % 8 == 0 && p.head_stride % 8 == 0 && p.q_token % 8 == 0 && p.q_head % 8 == 0 &&
-                  p.out_token % 4 == 0 && p.out_head % 4 == 0, "%s: q, k, v strides must be multiples of 8 elements (out: 4)", what);
-  DCP_REQUIRE(p.page_stride >= 0 && p.token_stride >= 0 && p.head_stride >= 0 && p.q_token >= 0 && p.q_head >= 0 && p.out_token > 0 &&
-                  p.out_head > 0, "%s: negative stride", what);
-  DCP_REQUIRE(((reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
-                reinterpret_cast<uintptr_t>(p.out)) & 15) == 0, "%s: q, k, v and out must be 16-byte aligned", what);
-  DCP_REQUIRE((int64_t)s.n_tokens * s.n_heads_q < ((int64_t)1 << 31), "%s: too many queries", what);
-  return DCP_OK;
 }
 
 static int launch_rows(const PagedAttnParams& p, int head_dim, int dtype, void* stream) {
@@ -901,10 +882,10 @@ static int launch_rows(const PagedAttnParams& p, int head_dim, int dtype, void* 
 // How a call is laid out: which kernel takes the requests' own keys, and what of the workspace is whose.
 struct PagedPlan {
   int rows = 0;      // of a chunk of the kernel of few rows; 0: the kernel of rows takes them
-  int n_wg = 0;      // of the kernel of few rows
+  int n_wg = 0, heads = 1;  // of the kernel of few rows; kv heads of a workgroup
   int n_own = 1, n_prefix = 0;  // shares
-  size_t starts = 0, slots = 0, shares = 0;  // bytes
-  size_t bytes() const { return starts + slots + shares; }
+  size_t cuts = 0, slots = 0, shares = 0;  // bytes
+  size_t bytes() const { return cuts + slots + shares; }
 };
 static size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 static PagedPlan plan_paged(const PagedShape& s, int64_t max_q, int64_t max_keys, int n_prefixes, int64_t max_prefix) {
@@ -913,8 +894,11 @@ static PagedPlan plan_paged(const PagedShape& s, int64_t max_q, int64_t max_keys
   if (rows <= 32 && s.batch <= kFewMaxBatch) {
     plan.rows = rows <= 16 ? 16 : 32;
     plan.n_wg = 2 * device_cu_count();
-    plan.starts = up16((size_t)(s.batch + 1) * sizeof(int64_t));
-    plan.slots = (size_t)plan.n_wg * 2 * plan.rows * (s.head_dim + 2) * sizeof(float);
+    const int64_t tiles = (int64_t)s.batch * s.n_heads_kv * ((max_keys + kFewBN - 1) / kFewBN) / plan.n_wg;
+    plan.heads = tiles < (getenv("X_T") ? atoi(getenv("X_T")) : 64) ? 1 : s.n_heads_kv % 4 == 0 ? 4 : s.n_heads_kv % 2 == 0 ? 2 : 1;
+    if (getenv("X_HEADS")) plan.heads = std::min(plan.heads, atoi(getenv("X_HEADS")));
+    plan.cuts = up16((size_t)s.n_tokens * s.n_heads_q * sizeof(int2));
+    plan.slots = (size_t)plan.n_wg * 2 * plan.heads * plan.rows * (s.head_dim + 2) * sizeof(float);
   } else {
     plan.n_own = row_shares(s, max_keys);
   }
@@ -943,10 +927,11 @@ static int launch_own(PagedAttnParams p, const PagedPlan& plan, const int32_t* c
                       void* stream) {
   PagedFewParams f = {};
   if (plan.rows > 0) {
-    f.starts = reinterpret_cast<int64_t*>(workspace);
-    f.slot_out = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.starts);
-    f.slot_sums = reinterpret_cast<f32x2*>(f.slot_out + (size_t)plan.n_wg * 2 * plan.rows * head_dim);
+    f.cuts = reinterpret_cast<int2*>(workspace);
+    f.slot_out = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.cuts);
+    f.slot_sums = reinterpret_cast<f32x2*>(f.slot_out + (size_t)plan.n_wg * 2 * plan.heads * plan.rows * head_dim);
     f.a = p;
+    f.heads = plan.heads;
     KernelTimer timer("paged_few_kernel", stream);
     if (plan.rows == 16) launch_few_rows<1>(f, plan, head_dim, dtype, stream);
     else launch_few_rows<2>(f, plan, head_dim, dtype, stream);
@@ -972,7 +957,7 @@ static int launch_own(PagedAttnParams p, const PagedPlan& plan, const int32_t* c
 }
 
 static void place_shares(PagedAttnParams& p, const PagedPlan& plan, void* workspace, int head_dim) {
-  p.partial_out = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.starts + plan.slots);
+  p.partial_out = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.cuts + plan.slots);
   p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)(plan.n_own + plan.n_prefix) * p.n_tokens * p.n_heads_q * head_dim);
 }
 
@@ -980,110 +965,89 @@ static void place_shares(PagedAttnParams& p, const PagedPlan& plan, void* worksp
 
 using namespace dcp;
 
-extern "C" size_t dcp_paged_attn_workspace_bytes(int n_tokens, int batch, int n_heads_q, int n_heads_kv, int head_dim, int max_seqlen_q,
-                                                 int max_seqlen_k) {
-  if (n_tokens <= 0 || batch <= 0 || n_heads_q <= 0 || n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0) return 0;
-  if (max_seqlen_q <= 0 || max_seqlen_k <= 0) return 0;
-  return plan_paged({n_tokens, batch, n_heads_q, n_heads_kv, head_dim}, max_seqlen_q, max_seqlen_k, 0, 0).bytes();
+namespace {
+
+PagedShape shape_of(const dcp_paged_attn_args& x) { return {x.n_tokens, x.batch, x.n_heads_q, x.n_heads_kv, x.head_dim}; }
+
+PagedPlan plan_of(const dcp_paged_attn_args& x) {
+  return plan_paged(shape_of(x), x.max_seqlen_q, seen_keys(x.max_seqlen_q, x.max_seqlen_k, x.window, x.n_starting), x.n_prefixes, x.max_prefix_len);
 }
 
-extern "C" int dcp_paged_attn(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse, const int32_t* block_table,
-                              const int32_t* seq_lens, const int32_t* cu_seqlens_q, int n_tokens, int batch, int n_heads_q, int n_heads_kv,
-                              int head_dim, int64_t q_token_stride, int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride,
-                              int n_pages, int page_size, int64_t page_stride, int64_t token_stride, int64_t head_stride, int table_width,
-                              int64_t table_stride, int max_seqlen_q, int max_seqlen_k, int window, int n_starting, float softmax_scale,
-                              int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  DCP_RECORDED(dcp_paged_attn(q, k_cache, v_cache, out, lse, block_table, seq_lens, cu_seqlens_q, n_tokens, batch, n_heads_q, n_heads_kv,
-      head_dim, q_token_stride, q_head_stride, out_token_stride, out_head_stride, n_pages, page_size, page_stride, token_stride, head_stride,
-      table_width, table_stride, max_seqlen_q, max_seqlen_k, window, n_starting, softmax_scale, dtype, workspace, workspace_bytes, stream));
-  const PagedShape s = {n_tokens, batch, n_heads_q, n_heads_kv, head_dim};
-  PagedAttnParams p = {};
-  p.q = q; p.k = k_cache; p.v = v_cache; p.out = out; p.lse = lse;
-  p.block_table = block_table; p.key_lens = seq_lens; p.cu_seqlens_q = cu_seqlens_q;
-  p.table_stride = table_stride;
-  p.q_token = q_token_stride; p.q_head = q_head_stride; p.out_token = out_token_stride; p.out_head = out_head_stride;
-  p.page_stride = page_stride; p.token_stride = token_stride; p.head_stride = head_stride;
-  p.table_width = table_width; p.n_pages = n_pages; p.page_size = page_size;
-  p.batch = p.n_requests = batch; p.n_tokens = n_tokens;
-  p.n_heads_q = n_heads_q; p.n_heads_kv = n_heads_kv;
-  p.window = window; p.n_starting = n_starting;
-  p.scale_log2 = softmax_scale * kLog2e;
-  if (const int status = check_paged("paged_attn", s, p, softmax_scale, dtype)) return status;
-  p.group = n_heads_q / n_heads_kv;
-  DCP_REQUIRE(cu_seqlens_q != nullptr || n_tokens == batch, "paged_attn: without cu_seqlens_q every request has one token, got %d for %d",
-              n_tokens, batch);
-  if (n_tokens == 0 || batch == 0) return DCP_OK;
-  DCP_REQUIRE(q && out && lse && block_table && seq_lens && (n_pages == 0 || (k_cache && v_cache)), "paged_attn: null argument");
-  DCP_REQUIRE(max_seqlen_q > 0 && max_seqlen_k > 0, "paged_attn: the longest lengths must be positive");
-  const PagedPlan plan = plan_paged(s, max_seqlen_q, max_seqlen_k, 0, 0);
-  p.n_splits = plan.n_own;
-  const int64_t tiles = row_tiles(s);
-  DCP_REQUIRE(tiles < ((int64_t)1 << 31), "paged_attn: too many rows");
-  p.n_tiles = (int)tiles;
-  p.direct = plan.n_own == 1;
+// What a caller may have wrong, before anything is launched.
+int check_paged(const dcp_paged_attn_args& x) {
+  if (x.dtype != DCP_DTYPE_BF16 && x.dtype != DCP_DTYPE_FP16) return fail(DCP_ERR_UNSUPPORTED, "paged_attn: dtype %d unsupported (bf16 and fp16 only)", x.dtype);
+  if (x.head_dim != 64 && x.head_dim != 128) return fail(DCP_ERR_UNSUPPORTED, "paged_attn: head_dim %d unsupported (64 or 128)", x.head_dim);
+  DCP_REQUIRE(x.n_tokens >= 0 && x.batch >= 0 && x.n_pages >= 0 && x.n_prefixes >= 0, "paged_attn: negative size");
+  DCP_REQUIRE(x.n_heads_q > 0 && x.n_heads_kv > 0 && x.n_heads_q % x.n_heads_kv == 0, "paged_attn: n_heads_q %d must be a multiple of n_heads_kv %d",
+              x.n_heads_q, x.n_heads_kv);
+  DCP_REQUIRE(x.softmax_scale > 0.0f, "paged_attn: softmax_scale must be positive");
+  DCP_REQUIRE(x.window >= 0 && x.n_starting >= 0, "paged_attn: negative window or number of first tokens");
+  DCP_REQUIRE(x.n_prefixes == 0 || x.window == 0, "paged_attn: no window where there are shared prefixes");
+  DCP_REQUIRE(x.page_size > 0 && x.page_size % 16 == 0, "paged_attn: page_size %d must be a positive multiple of 16", x.page_size);
+  DCP_REQUIRE(x.table_width > 0 && x.table_stride >= 0 && (x.n_prefixes == 0 || (x.prefix_width > 0 && x.prefix_stride >= 0)),
+              "paged_attn: empty block tables");
+  DCP_REQUIRE(std::max((int64_t)x.table_width, (int64_t)(x.n_prefixes ? x.prefix_width : 0)) * x.page_size < 0x7fffff00, "paged_attn: too many keys a request");
+  DCP_REQUIRE(x.page_stride % 8 == 0 && x.token_stride % 8 == 0 && x.head_stride % 8 == 0 && x.q_token_stride % 8 == 0 && x.q_head_stride % 8 == 0 &&
+                  x.out_token_stride % 4 == 0 && x.out_head_stride % 4 == 0, "paged_attn: q, k, v strides must be multiples of 8 elements (out: 4)");
+  DCP_REQUIRE(x.page_stride >= 0 && x.token_stride >= 0 && x.head_stride >= 0 && x.q_token_stride >= 0 && x.q_head_stride >= 0 &&
+                  x.out_token_stride > 0 && x.out_head_stride > 0, "paged_attn: negative stride");
+  DCP_REQUIRE(((reinterpret_cast<uintptr_t>(x.q) | reinterpret_cast<uintptr_t>(x.k_cache) | reinterpret_cast<uintptr_t>(x.v_cache) |
+                reinterpret_cast<uintptr_t>(x.out)) & 15) == 0, "paged_attn: q, k, v and out must be 16-byte aligned");
+  DCP_REQUIRE((int64_t)x.n_tokens * x.n_heads_q < ((int64_t)1 << 31), "paged_attn: too many queries");
+  DCP_REQUIRE(x.cu_seqlens_q != nullptr || x.n_tokens == x.batch, "paged_attn: without cu_seqlens_q every request has one token, got %d for %d",
+              x.n_tokens, x.batch);
+  if (x.n_tokens == 0 || x.batch == 0) return DCP_OK;
+  DCP_REQUIRE(x.q && x.out && x.lse && x.block_table && x.seq_lens && (x.n_pages == 0 || (x.k_cache && x.v_cache)) &&
+                  (x.n_prefixes == 0 || (x.prefix_table && x.prefix_lens && x.cu_groups)), "paged_attn: null argument");
+  DCP_REQUIRE(x.max_seqlen_q > 0 && x.max_seqlen_k > 0 && (x.n_prefixes == 0 || x.max_prefix_len > 0), "paged_attn: the longest lengths must be positive");
+  DCP_REQUIRE(row_tiles(shape_of(x)) < ((int64_t)1 << 31) - x.n_prefixes, "paged_attn: too many rows");
+  return DCP_OK;
+}
+
+int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_bytes, void* stream) {
+  DCP_RECORDED(paged_attn(x, workspace, workspace_bytes, stream));
+  if (const int status = check_paged(x)) return status;
+  if (x.n_tokens == 0 || x.batch == 0) return DCP_OK;
+  const PagedPlan plan = plan_of(x);
   const size_t needed = plan.bytes();
   DCP_REQUIRE(needed == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= needed),
               "paged_attn: workspace of %zu bytes is missing, not 16-byte aligned or smaller than the %zu needed", workspace_bytes, needed);
-  if (!p.direct) place_shares(p, plan, workspace, head_dim);
-  return launch_own(p, plan, nullptr, 0, head_dim, dtype, workspace, stream);
-}
-
-extern "C" size_t dcp_shared_prefix_attn_workspace_bytes(int n_tokens, int batch, int n_prefixes, int n_heads_q, int n_heads_kv, int head_dim,
-                                                         int max_seqlen_q, int max_seqlen_k, int max_prefix_len) {
-  if (n_tokens <= 0 || batch <= 0 || n_prefixes <= 0 || n_heads_q <= 0 || n_heads_kv <= 0 || n_heads_q % n_heads_kv != 0) return 0;
-  if (max_seqlen_q <= 0 || max_seqlen_k <= 0 || max_prefix_len <= 0) return 0;
-  return plan_paged({n_tokens, batch, n_heads_q, n_heads_kv, head_dim}, max_seqlen_q, max_seqlen_k, n_prefixes, max_prefix_len).bytes();
-}
-
-extern "C" int dcp_shared_prefix_attn(const void* q, const void* k_cache, const void* v_cache, void* out, float* lse,
-                                      const int32_t* prefix_table, const int32_t* prefix_lens, const int32_t* cu_groups,
-                                      const int32_t* block_table, const int32_t* seq_lens, const int32_t* cu_seqlens_q, int n_tokens, int batch,
-                                      int n_prefixes, int n_heads_q, int n_heads_kv, int head_dim, int64_t q_token_stride,
-                                      int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, int n_pages, int page_size,
-                                      int64_t page_stride, int64_t token_stride, int64_t head_stride, int prefix_width, int64_t prefix_stride,
-                                      int table_width, int64_t table_stride, int max_seqlen_q, int max_seqlen_k, int max_prefix_len,
-                                      float softmax_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
-  DCP_RECORDED(dcp_shared_prefix_attn(q, k_cache, v_cache, out, lse, prefix_table, prefix_lens, cu_groups, block_table, seq_lens,
-      cu_seqlens_q, n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim, q_token_stride, q_head_stride, out_token_stride,
-      out_head_stride, n_pages, page_size, page_stride, token_stride, head_stride, prefix_width, prefix_stride, table_width, table_stride,
-      max_seqlen_q, max_seqlen_k, max_prefix_len, softmax_scale, dtype, workspace, workspace_bytes, stream));
-  const PagedShape s = {n_tokens, batch, n_heads_q, n_heads_kv, head_dim}, of_prefix = {n_tokens, n_prefixes, n_heads_q, n_heads_kv, head_dim};
   PagedAttnParams p = {};
-  p.q = q; p.k = k_cache; p.v = v_cache; p.out = out; p.lse = lse;
-  p.block_table = block_table; p.key_lens = seq_lens; p.cu_seqlens_q = cu_seqlens_q;
-  p.table_stride = table_stride;
-  p.q_token = q_token_stride; p.q_head = q_head_stride; p.out_token = out_token_stride; p.out_head = out_head_stride;
-  p.page_stride = page_stride; p.token_stride = token_stride; p.head_stride = head_stride;
-  p.table_width = table_width; p.n_pages = n_pages; p.page_size = page_size;
-  p.batch = p.n_requests = batch; p.n_tokens = n_tokens;
-  p.n_heads_q = n_heads_q; p.n_heads_kv = n_heads_kv;
-  p.scale_log2 = softmax_scale * kLog2e;
-  PagedAttnParams pre = p;
-  pre.block_table = prefix_table; pre.key_lens = prefix_lens; pre.cu_groups = cu_groups;
-  pre.table_stride = prefix_stride; pre.table_width = prefix_width; pre.batch = n_prefixes;
-  if (const int status = check_paged("shared_prefix_attn", s, p, softmax_scale, dtype)) return status;
-  if (const int status = check_paged("shared_prefix_attn", of_prefix, pre, softmax_scale, dtype)) return status;
-  p.group = pre.group = n_heads_q / n_heads_kv;
-  DCP_REQUIRE(cu_seqlens_q != nullptr || n_tokens == batch,
-              "shared_prefix_attn: without cu_seqlens_q every request has one token, got %d for %d", n_tokens, batch);
-  DCP_REQUIRE(n_prefixes > 0 || batch == 0, "shared_prefix_attn: no prefixes");
-  if (n_tokens == 0 || batch == 0) return DCP_OK;
-  DCP_REQUIRE(q && out && lse && prefix_table && prefix_lens && cu_groups && block_table && seq_lens && (n_pages == 0 || (k_cache && v_cache)),
-              "shared_prefix_attn: null argument");
-  DCP_REQUIRE(max_seqlen_q > 0 && max_seqlen_k > 0 && max_prefix_len > 0, "shared_prefix_attn: the longest lengths must be positive");
-  const PagedPlan plan = plan_paged(s, max_seqlen_q, max_seqlen_k, n_prefixes, max_prefix_len);
+  p.q = x.q; p.k = x.k_cache; p.v = x.v_cache; p.out = x.out; p.lse = x.lse;
+  p.block_table = x.block_table; p.key_lens = x.seq_lens; p.cu_seqlens_q = x.cu_seqlens_q;
+  p.table_stride = x.table_stride;
+  p.q_token = x.q_token_stride; p.q_head = x.q_head_stride; p.out_token = x.out_token_stride; p.out_head = x.out_head_stride;
+  p.page_stride = x.page_stride; p.token_stride = x.token_stride; p.head_stride = x.head_stride;
+  p.table_width = x.table_width; p.n_pages = x.n_pages; p.page_size = x.page_size;
+  p.batch = p.n_requests = x.batch; p.n_tokens = x.n_tokens;
+  p.n_heads_q = x.n_heads_q; p.n_heads_kv = x.n_heads_kv; p.group = x.n_heads_q / x.n_heads_kv;
+  p.window = x.window; p.n_starting = x.n_starting;
+  p.scale_log2 = x.softmax_scale * kLog2e;
   p.n_splits = plan.n_own;
-  pre.n_splits = plan.n_prefix;
-  const int64_t tiles = row_tiles(s);
-  DCP_REQUIRE(tiles < ((int64_t)1 << 31) - n_prefixes, "shared_prefix_attn: too many rows");
-  p.n_tiles = (int)tiles;
-  pre.n_tiles = (int)row_tiles(of_prefix);
-  const size_t needed = plan.bytes();
-  DCP_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= needed,
-              "shared_prefix_attn: workspace of %zu bytes is missing, not 16-byte aligned or smaller than the %zu needed", workspace_bytes, needed);
-  place_shares(p, plan, workspace, head_dim);
-  place_shares(pre, plan, workspace, head_dim);
-  pre.first_share = plan.n_own;
-  if (const int status = launch_rows(pre, head_dim, dtype, stream)) return status;
-  return launch_own(p, plan, cu_groups, n_prefixes, head_dim, dtype, workspace, stream);
+  p.n_tiles = (int)row_tiles(shape_of(x));
+  p.direct = plan.n_own + plan.n_prefix == 1;
+  if (!p.direct) place_shares(p, plan, workspace, x.head_dim);
+  if (x.n_prefixes > 0) {
+    PagedAttnParams pre = p;
+    pre.block_table = x.prefix_table; pre.key_lens = x.prefix_lens; pre.cu_groups = x.cu_groups;
+    pre.table_stride = x.prefix_stride; pre.table_width = x.prefix_width;
+    pre.batch = x.n_prefixes;
+    pre.n_splits = plan.n_prefix;
+    pre.n_tiles = (int)row_tiles({x.n_tokens, x.n_prefixes, x.n_heads_q, x.n_heads_kv, x.head_dim});
+    pre.first_share = plan.n_own;
+    if (const int status = launch_rows(pre, x.head_dim, x.dtype, stream)) return status;
+  }
+  return launch_own(p, plan, x.n_prefixes > 0 ? x.cu_groups : nullptr, x.n_prefixes, x.head_dim, x.dtype, workspace, stream);
+}
+
+}  // namespace
+
+extern "C" size_t dcp_paged_attn_workspace_bytes(const dcp_paged_attn_args* args) {
+  if (args == nullptr || check_paged(*args) != DCP_OK || args->n_tokens == 0 || args->batch == 0) return 0;
+  return plan_of(*args).bytes();
+}
+
+extern "C" int dcp_paged_attn(const dcp_paged_attn_args* args, void* workspace, size_t workspace_bytes, void* stream) {
+  DCP_REQUIRE(args != nullptr, "paged_attn: null argument");
+  return paged_attn(*args, workspace, workspace_bytes, stream);
 }

@@ -13,6 +13,7 @@ raises ``NotImplementedError`` rather than computing something different.
 
 from __future__ import annotations
 
+import struct
 from typing import Optional
 
 import torch
@@ -453,64 +454,101 @@ def _flash_attn_varlen_backward(
 # attention over a paged cache (no counterpart in the reference)
 # ---------------------------------------------------------------------------
 
-
-def paged_cache_workspace_bytes(n_tokens, batch, n_heads_q, n_heads_kv, head_dim, max_seqlen_q, max_seqlen_k) -> int:
-    """Scratch bytes ``paged_cache_attention`` needs for these sizes (0: none)."""
-    return _lib.load().dcp_paged_attn_workspace_bytes(n_tokens, batch, n_heads_q, n_heads_kv, head_dim, max_seqlen_q, max_seqlen_k)
-
-
-def shared_prefix_workspace_bytes(n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim, max_seqlen_q, max_seqlen_k, max_prefix_len) -> int:
-    """Scratch bytes ``shared_prefix_attention`` needs for these sizes."""
-    return _lib.load().dcp_shared_prefix_attn_workspace_bytes(n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim, max_seqlen_q,
-                                                             max_seqlen_k, max_prefix_len)
+# dcp_paged_attn_args: eleven addresses, nine strides, sixteen numbers and the scale.  (Packed in one call: as 37 arguments of
+# a ctypes function they cost 3 us more, of a call that takes about ten.)
+_PAGED_ARGS = struct.Struct("<11Q9q16if4x")
 
 
-def _paged_workspace(workspace, n_bytes: int, q) -> tuple:
-    if workspace is None:
-        if n_bytes == 0:
-            return None, 0, 0
-        workspace = torch.empty(n_bytes, dtype=torch.uint8, device=q.device)
-    elif not workspace.is_contiguous() or workspace.get_device() != q.get_device():
-        raise ValueError("workspace must be a contiguous tensor on q's device")
-    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+def _table_here(t, name: str, here: int, *shape) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if t.dtype is not torch.int32 or t.get_device() != here or tuple(t.shape) != shape or (len(shape) == 1 and not t.is_contiguous()) \
+            or (len(shape) == 2 and shape[1] > 1 and t.numel() > 0 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be int32 {list(shape)} with dense rows on the current device, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
-def _paged_inputs(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, out, lse):
-    """Checks what both operators take; ``(out, lse, batch, strides of q, out and the cache)``."""
+def _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, window, n_starting, out, lse,
+                prefix=None):
+    """``(out, lse, packed arguments)``, the inputs checked."""
     here = torch._C._cuda_getDevice()
-    if not (q.get_device() == here and k_cache.get_device() == here and v_cache.get_device() == here):
+    if not (q.get_device() == k_cache.get_device() == v_cache.get_device() == here):
         raise ValueError("q, k_cache and v_cache must be tensors of the current device")
+    dtype = q.dtype
+    if not (k_cache.dtype is dtype and v_cache.dtype is dtype):
+        raise TypeError(f"q is {dtype}, the caches are {k_cache.dtype} and {v_cache.dtype}")
     if q.dim() != 3 or q.stride(2) != 1:
         raise ValueError(f"q must be [tokens, n_heads_q, D] with dense rows, got {list(q.shape)}")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1 \
-            or k_cache.shape[3] != q.shape[2]:
-        raise ValueError(f"k_cache and v_cache must be [n_pages, page_size, n_heads_kv, {q.shape[2]}] with the same strides and dense rows")
-    if not (q.dtype is k_cache.dtype is v_cache.dtype):
-        raise TypeError(f"q is {q.dtype}, the caches are {k_cache.dtype} and {v_cache.dtype}")
-    if block_table.dim() != 2 or (block_table.numel() > 0 and block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"block_table must be [B, pages] with dense rows, got {list(block_table.shape)}")
-    batch = block_table.shape[0]
-    _table_here(block_table, "block_table", block_table.shape)
-    _table_here(seq_lens, "seq_lens", (batch,))
+    n_tokens, n_heads_q, head_dim = q.shape
+    cache_strides = k_cache.stride()
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or cache_strides != v_cache.stride() or cache_strides[3] != 1 \
+            or k_cache.shape[3] != head_dim:
+        raise ValueError(f"k_cache and v_cache must be [n_pages, page_size, n_heads_kv, {head_dim}] with the same strides and dense rows")
+    n_pages, page_size, n_heads_kv, _ = k_cache.shape
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [B, pages], got {list(block_table.shape)}")
+    batch, width = block_table.shape
+    _table_here(block_table, "block_table", here, batch, width)
+    _table_here(seq_lens, "seq_lens", here, batch)
     if cu_seqlens_q is not None:
-        _table_here(cu_seqlens_q, "cu_seqlens_q", (batch + 1,))
-    elif batch != q.shape[0]:
-        raise ValueError(f"without cu_seqlens_q every request has one token, got {q.shape[0]} for {batch}")
+        _table_here(cu_seqlens_q, "cu_seqlens_q", here, batch + 1)
+    elif batch != n_tokens:
+        raise ValueError(f"without cu_seqlens_q every request has one token, got {n_tokens} for {batch}")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be positive (None: no window), got {window}")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not q.dtype or out.stride(2) != 1 or out.get_device() != here:
+        out = torch.empty((n_tokens, n_heads_q, head_dim), dtype=dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype is not dtype or out.stride(2) != 1 or out.get_device() != here:
         raise ValueError(f"out must be like q, got {out.dtype} {list(out.shape)}")
     if lse is None:
-        lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-    elif tuple(lse.shape) != (q.shape[1], q.shape[0]) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != here:
-        raise ValueError(f"lse must be contiguous float32 [{q.shape[1]}, {q.shape[0]}]")
-    return out, lse, batch
+        lse = torch.empty((n_heads_q, n_tokens), dtype=torch.float32, device=q.device)
+    elif tuple(lse.shape) != (n_heads_q, n_tokens) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != here:
+        raise ValueError(f"lse must be contiguous float32 [{n_heads_q}, {n_tokens}] on the current device")
+    if max_seqlen_q is None:
+        max_seqlen_q = 1 if cu_seqlens_q is None else max(n_tokens, 1)
+    if max_seqlen_k is None:
+        max_seqlen_k = max(width * page_size, 1)
+    prefix_addresses, prefix_stride, prefix_width, n_prefixes, max_prefix_len = (0, 0, 0), 0, 0, 0, 0
+    if prefix is not None:
+        prefix_table, prefix_lens, cu_groups, max_prefix_len = prefix
+        if prefix_table.dim() != 2:
+            raise ValueError(f"prefix_table must be [P, pages], got {list(prefix_table.shape)}")
+        n_prefixes, prefix_width = prefix_table.shape
+        _table_here(prefix_table, "prefix_table", here, n_prefixes, prefix_width)
+        _table_here(prefix_lens, "prefix_lens", here, n_prefixes)
+        _table_here(cu_groups, "cu_groups", here, n_prefixes + 1)
+        prefix_addresses, prefix_stride = (prefix_table.data_ptr(), prefix_lens.data_ptr(), cu_groups.data_ptr()), prefix_table.stride(0)
+        if max_prefix_len is None:
+            max_prefix_len = max(prefix_width * page_size, 1)
+    q_strides, out_strides = q.stride(), out.stride()
+    packed = _PAGED_ARGS.pack(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
+        0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), *prefix_addresses, q_strides[0], q_strides[1], out_strides[0], out_strides[1],
+        cache_strides[0], cache_strides[1], cache_strides[2], block_table.stride(0), prefix_stride, n_tokens, batch, n_heads_q, n_heads_kv, head_dim,
+        n_pages, page_size, width, prefix_width, n_prefixes, max_seqlen_q, max_seqlen_k, max_prefix_len, window or 0, n_starting, dtype_code(dtype),
+        head_dim ** -0.5 if softmax_scale is None else softmax_scale)
+    return out, lse, packed
 
 
-def _table_here(t, name: str, shape) -> None:
-    if t.dtype is not torch.int32 or t.get_device() != torch._C._cuda_getDevice() or tuple(t.shape) != tuple(shape) \
-            or (t.dim() == 1 and not t.is_contiguous()):
-        raise ValueError(f"{name} must be int32 {list(shape)} on the current device, got {t.dtype} {list(t.shape)} on {t.device}")
+def _paged_call(packed: bytes, workspace, q) -> None:
+    address = size = 0
+    if workspace is None:
+        size = _lib.load().dcp_paged_attn_workspace_bytes(packed)
+        if size > 0:
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+            address = workspace.data_ptr()
+    else:
+        if not workspace.is_contiguous() or workspace.get_device() != q.get_device():
+            raise ValueError("workspace must be a contiguous tensor on q's device")
+        address, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _lib.call("dcp_paged_attn", packed, address, size, torch._C._cuda_getCurrentRawStream(q.get_device()))
+
+
+def paged_cache_workspace_bytes(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q=None, max_seqlen_q=None, max_seqlen_k=None,
+                                softmax_scale=None, window=None, n_starting=0, out=None, lse=None) -> int:
+    """Scratch bytes ``paged_cache_attention`` needs for these arguments (0: none)."""
+    packed = _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, window, n_starting,
+                         out, lse)[2]
+    return _lib.load().dcp_paged_attn_workspace_bytes(packed)
 
 
 def paged_cache_attention(
@@ -539,26 +577,22 @@ def paged_cache_attention(
     +inf where nothing is visible; tokens of no request are left as they were.
     ``max_seqlen_q`` / ``max_seqlen_k``: the longest lengths as far as the host knows them (default: all tokens, a whole row of
     pages); they decide how the work is split and change no result beyond its rounding.
-    ``workspace``: a tensor of ``paged_cache_workspace_bytes(...)`` bytes, for calls that may not allocate.
+    ``workspace``: a tensor of ``paged_cache_workspace_bytes(...)`` bytes, for calls that may not allocate; launches
+    that may run at the same time need one each.
     Page numbers outside of the cache name no page: nobody sees their keys.  Forward only.
     """
-    out, lse, batch = _paged_inputs(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, out, lse)
-    n_tokens, n_heads_q, head_dim = q.shape
-    n_pages, page_size, n_heads_kv, _ = k_cache.shape
-    width = block_table.shape[1]
-    if window is not None and window < 1:
-        raise ValueError(f"window must be positive (None: no window), got {window}")
-    longest_q = (1 if cu_seqlens_q is None else max(n_tokens, 1)) if max_seqlen_q is None else int(max_seqlen_q)
-    longest_k = max(width * page_size, 1) if max_seqlen_k is None else int(max_seqlen_k)
-    scale = head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
-    n_bytes = paged_cache_workspace_bytes(n_tokens, batch, n_heads_q, n_heads_kv, head_dim, longest_q, longest_k)
-    workspace, address, size = _paged_workspace(workspace, n_bytes, q)
-    _lib.call("dcp_paged_attn", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(), block_table.data_ptr(),
-              seq_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), n_tokens, batch, n_heads_q, n_heads_kv, head_dim,
-              q.stride(0), q.stride(1), out.stride(0), out.stride(1), n_pages, page_size, k_cache.stride(0), k_cache.stride(1),
-              k_cache.stride(2), width, block_table.stride(0), longest_q, longest_k, 0 if window is None else int(window),
-              int(n_starting), scale, dtype_code(q.dtype), address, size, _stream())
+    out, lse, packed = _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, window,
+                                   n_starting, out, lse)
+    _paged_call(packed, workspace, q)
     return out, lse
+
+
+def shared_prefix_workspace_bytes(q, k_cache, v_cache, prefix_table, prefix_lens, cu_groups, block_table, seq_lens, cu_seqlens_q=None,
+                                  max_seqlen_q=None, max_seqlen_k=None, max_prefix_len=None, softmax_scale=None, out=None, lse=None) -> int:
+    """Scratch bytes ``shared_prefix_attention`` needs for these arguments."""
+    packed = _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, None, 0, out, lse,
+                         (prefix_table, prefix_lens, cu_groups, max_prefix_len))[2]
+    return _lib.load().dcp_paged_attn_workspace_bytes(packed)
 
 
 def shared_prefix_attention(
@@ -586,26 +620,7 @@ def shared_prefix_attention(
     the new tokens' among them.  A query sees its whole prefix and its own keys up to itself, as ``shared_prefix_mask_fn``
     trains: ``(out, lse)`` are those of the concatenation.  Requests outside of the groups have no prefix.
     """
-    out, lse, batch = _paged_inputs(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, out, lse)
-    n_tokens, n_heads_q, head_dim = q.shape
-    n_pages, page_size, n_heads_kv, _ = k_cache.shape
-    width = block_table.shape[1]
-    if prefix_table.dim() != 2 or (prefix_table.numel() > 0 and prefix_table.shape[1] > 1 and prefix_table.stride(1) != 1):
-        raise ValueError(f"prefix_table must be [P, pages] with dense rows, got {list(prefix_table.shape)}")
-    n_prefixes, prefix_width = prefix_table.shape
-    _table_here(prefix_table, "prefix_table", prefix_table.shape)
-    _table_here(prefix_lens, "prefix_lens", (n_prefixes,))
-    _table_here(cu_groups, "cu_groups", (n_prefixes + 1,))
-    longest_q = (1 if cu_seqlens_q is None else max(n_tokens, 1)) if max_seqlen_q is None else int(max_seqlen_q)
-    longest_k = max(width * page_size, 1) if max_seqlen_k is None else int(max_seqlen_k)
-    longest_prefix = max(prefix_width * page_size, 1) if max_prefix_len is None else int(max_prefix_len)
-    scale = head_dim ** -0.5 if softmax_scale is None else float(softmax_scale)
-    n_bytes = shared_prefix_workspace_bytes(n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim, longest_q, longest_k, longest_prefix)
-    workspace, address, size = _paged_workspace(workspace, n_bytes, q)
-    _lib.call("dcp_shared_prefix_attn", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(),
-              prefix_table.data_ptr(), prefix_lens.data_ptr(), cu_groups.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-              0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), n_tokens, batch, n_prefixes, n_heads_q, n_heads_kv, head_dim,
-              q.stride(0), q.stride(1), out.stride(0), out.stride(1), n_pages, page_size, k_cache.stride(0), k_cache.stride(1),
-              k_cache.stride(2), prefix_width, prefix_table.stride(0), width, block_table.stride(0),
-              longest_q, longest_k, longest_prefix, scale, dtype_code(q.dtype), address, size, _stream())
+    out, lse, packed = _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, None, 0, out,
+                                   lse, (prefix_table, prefix_lens, cu_groups, max_prefix_len))
+    _paged_call(packed, workspace, q)
     return out, lse

@@ -12,7 +12,6 @@ from typing import NamedTuple, Optional
 import torch
 
 from dcp_amd import _lib
-from dcp_amd.ops.fused_ops import _stream
 
 __all__ = ["PagedCacheTables", "paged_cache_tables", "paged_cache_write"]
 
@@ -27,13 +26,13 @@ class PagedCacheTables(NamedTuple):
     pages_taken: torch.Tensor  # int32 [1]
 
 
-def _here(t, dtype, name: str, shape=None, dense: bool = True) -> int:
-    """The address of a tensor of the current device with this type (and, if given, this shape)."""
+def _check(t, dtype, name: str, here: int, shape=None, dense: bool = True) -> int:
+    """The address of a tensor of this type on the current device (``here``), with this shape if one is given."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.get_device() != torch._C._cuda_getDevice():
+    if t.get_device() != here:
         raise ValueError(f"{name} must be a tensor of the current device")
     if shape is not None and tuple(t.shape) != shape:
         raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
@@ -55,29 +54,32 @@ def paged_cache_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_
     not changed: drop its first ``pages_taken`` entries for the next step.  ``out``: tables of an earlier call to
     write to.
     """
+    here, i32 = torch._C._cuda_getDevice(), torch.int32
     n = cached_lens.shape[0] if isinstance(cached_lens, torch.Tensor) and cached_lens.dim() == 1 else -1
-    i32 = torch.int32
-    lens, new = _here(cached_lens, i32, "cached_lens", (n,)), _here(new_lens, i32, "new_lens", (n,))
-    table = _here(block_table, i32, "block_table", dense=False)
-    if block_table.dim() != 2 or block_table.shape[0] != n or block_table.shape[1] < 1 \
-            or (n > 0 and block_table.shape[1] > 1 and block_table.stride(1) != 1) or (n > 1 and block_table.stride(0) < block_table.shape[1]):
+    lens, new = _check(cached_lens, i32, "cached_lens", here, (n,)), _check(new_lens, i32, "new_lens", here, (n,))
+    table = _check(block_table, i32, "block_table", here, dense=False)
+    rows, width = block_table.shape if block_table.dim() == 2 else (-1, 0)
+    stride = block_table.stride(0) if rows > 1 else width
+    if rows != n or width < 1 or (n > 0 and width > 1 and block_table.stride(1) != 1) or (n > 1 and stride < width):
         raise ValueError(f"block_table must be [{n}, pages] with dense rows, got {list(block_table.shape)}")
-    free = _here(free_pages, i32, "free_pages")
+    free = _check(free_pages, i32, "free_pages", here)
     if free_pages.dim() != 1:
         raise ValueError(f"free_pages must have one axis, got {list(free_pages.shape)}")
     n_tokens = int(n_tokens)
     if n_tokens < 0:
         raise ValueError(f"n_tokens must not be negative, got {n_tokens}")
-    if out is None:
-        device = cached_lens.device
-        out = PagedCacheTables(torch.empty(n_tokens, dtype=torch.int64, device=device), torch.empty(n_tokens, dtype=i32, device=device),
-                               torch.empty(n + 1, dtype=i32, device=device), torch.empty(n, dtype=i32, device=device),
-                               torch.empty(1, dtype=i32, device=device))
-    _lib.call("dcp_paged_cache_tables", lens, new, table, max(block_table.stride(0), block_table.shape[1]), free,
-              _here(out.slot_mapping, torch.int64, "slot_mapping", (n_tokens,)), _here(out.positions, i32, "positions", (n_tokens,)),
-              _here(out.cu_seqlens, i32, "cu_seqlens", (n + 1,)), _here(out.seq_lens, i32, "seq_lens", (n,)),
-              _here(out.pages_taken, i32, "pages_taken", (1,)), n, block_table.shape[1], free_pages.shape[0], int(page_size),
-              n_tokens, _stream())
+    if out is None:  # (one tensor for the four of 32 bits: five allocations are a third of a small step's time)
+        ints = cached_lens.new_empty(n_tokens + 2 * n + 2)
+        positions, cu, lens_out, taken = ints.split_with_sizes([n_tokens, n + 1, n, 1])
+        out = PagedCacheTables(torch.empty(n_tokens, dtype=torch.int64, device=cached_lens.device), positions, cu, lens_out, taken)
+        at = ints.data_ptr()
+        addresses = (out.slot_mapping.data_ptr(), at, at + 4 * n_tokens, at + 4 * (n_tokens + n + 1), at + 4 * (n_tokens + 2 * n + 1))
+    else:
+        addresses = (_check(out.slot_mapping, torch.int64, "slot_mapping", here, (n_tokens,)),
+                     _check(out.positions, i32, "positions", here, (n_tokens,)), _check(out.cu_seqlens, i32, "cu_seqlens", here, (n + 1,)),
+                     _check(out.seq_lens, i32, "seq_lens", here, (n,)), _check(out.pages_taken, i32, "pages_taken", here, (1,)))
+    _lib.call("dcp_paged_cache_tables", lens, new, table, stride, free, *addresses, n, width, free_pages.shape[0], int(page_size), n_tokens,
+              torch._C._cuda_getCurrentRawStream(here))
     return out
 
 
@@ -85,14 +87,16 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tens
     """Writes ``k`` and ``v`` (``[n_tokens, n_heads_kv, D]``) into the caches (``[n_pages, page_size, n_heads_kv, D]``, any
     strides, a cache's two halves for instance) at ``slot_mapping`` (int64 ``[n_tokens]``).  Slots outside of the cache are skipped,
     so the -1 of padding writes nothing; the others have to differ from each other.  Any type of 1, 2 or 4 bytes."""
-    dtype = k_cache.dtype
-    addresses = [_here(t, dtype, name, dense=False) for t, name in ((k, "k"), (v, "v"), (k_cache, "k_cache"), (v_cache, "v_cache"))]
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride() != v_cache.stride() or k_cache.stride(3) != 1:
+    here, dtype = torch._C._cuda_getDevice(), k_cache.dtype
+    k_at, v_at = _check(k, dtype, "k", here, dense=False), _check(v, dtype, "v", here, dense=False)
+    k_cache_at, v_cache_at = _check(k_cache, dtype, "k_cache", here, dense=False), _check(v_cache, dtype, "v_cache", here, dense=False)
+    strides, in_strides = k_cache.stride(), k.stride()
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or strides != v_cache.stride() or strides[3] != 1:
         raise ValueError("k_cache and v_cache must be [n_pages, page_size, n_heads_kv, D] with the same strides and dense rows")
     n_pages, page_size, heads, head_dim = k_cache.shape
-    if k.dim() != 3 or k.shape != v.shape or k.stride() != v.stride() or tuple(k.shape[1:]) != (heads, head_dim) or (head_dim > 1 and k.stride(2) != 1):
+    if k.dim() != 3 or k.shape != v.shape or in_strides != v.stride() or tuple(k.shape[1:]) != (heads, head_dim) or (head_dim > 1 and in_strides[2] != 1):
         raise ValueError(f"k and v must be [n_tokens, {heads}, {head_dim}] with the same strides and dense rows")
-    slots = _here(slot_mapping, torch.int64, "slot_mapping", (k.shape[0],))
-    _lib.call("dcp_paged_cache_write", addresses[0], addresses[1], slots, addresses[2], addresses[3], k.shape[0], heads, head_dim,
-              k.element_size(), k.stride(0), k.stride(1), n_pages, page_size, k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-              _stream())
+    n_tokens = k.shape[0]
+    slots = _check(slot_mapping, torch.int64, "slot_mapping", here, (n_tokens,))
+    _lib.call("dcp_paged_cache_write", k_at, v_at, slots, k_cache_at, v_cache_at, n_tokens, heads, head_dim, k.element_size(), in_strides[0],
+              in_strides[1], n_pages, page_size, strides[0], strides[1], strides[2], torch._C._cuda_getCurrentRawStream(here))

@@ -684,62 +684,52 @@ int dcp_paged_cache_write(const void* k, const void* v,
  * log-sum-exp; a query without a visible key (one before its request's first
  * key among them) gets out = 0, lse = +inf.  Tokens of no request are left as
  * they were.  q head h reads kv head h / (n_heads_q / n_heads_kv).
+ * With n_prefixes > 0, requests [cu_groups[i], cu_groups[i+1]) share the
+ * prefix_lens[i] keys in the pages prefix_table[i * prefix_stride + j], and
+ * seq_lens and block_table are of the keys that follow, each request's own.  A
+ * query sees all of its prefix and its own keys up to itself: the result is that
+ * of the concatenation, a prefix is read once for all of its requests.  Requests
+ * outside of the groups have no prefix.  No window then.
  *  - Supported: bf16 and fp16, head_dim 64 or 128, page_size a multiple of 16,
- *    softmax_scale > 0, any strides that are multiples of 8 elements (out: 4),
- *    16-byte aligned tensors.
+ *    softmax_scale > 0, any strides (in elements) that are multiples of 8 (out:
+ *    4), 16-byte aligned tensors; the caches share theirs.
  *  - Page numbers outside of [0, n_pages) name no page: nobody sees their keys.
  *    Keys past the last entry of a row are not there.
  *  - What the cache holds where no query of a request looks (behind its last key,
  *    between its first tokens and its window) may be anything.  Queries of one
  *    request are computed together: keys that any of them sees should be finite.
- *  - max_seqlen_q, max_seqlen_k: the longest lengths, known on the host.  They
- *    decide how the work is split, not what is computed: lengths past them give the same
- *    results, slower.
- *  - workspace: dcp_paged_attn_workspace_bytes(...) bytes (0: none needed),
- *    16-byte aligned, for shares of the keys that are joined afterwards; contents
- *    are overwritten.  Launches that may run at the same time need one each.
+ *  - max_seqlen_q, max_seqlen_k, max_prefix_len: the longest lengths, as far as
+ *    they are known on the host.  They decide how the work is split, not what is
+ *    computed: lengths past them give the same results, slower.
+ *  - workspace: dcp_paged_attn_workspace_bytes(args) bytes (0: none needed, or
+ *    arguments that are refused), 16-byte aligned, for shares of the keys that are
+ *    joined afterwards; contents are overwritten.  Launches that may run at the
+ *    same time need one each.
  */
-size_t dcp_paged_attn_workspace_bytes(int n_tokens, int batch, int n_heads_q,
-                                      int n_heads_kv, int head_dim,
-                                      int max_seqlen_q, int max_seqlen_k);
-int dcp_paged_attn(const void* q, const void* k_cache, const void* v_cache,
-                   void* out, float* lse, const int32_t* block_table,
-                   const int32_t* seq_lens, const int32_t* cu_seqlens_q,
-                   int n_tokens, int batch, int n_heads_q, int n_heads_kv,
-                   int head_dim, int64_t q_token_stride, int64_t q_head_stride,
-                   int64_t out_token_stride, int64_t out_head_stride,
-                   int n_pages, int page_size, int64_t page_stride,
-                   int64_t token_stride, int64_t head_stride, int table_width,
-                   int64_t table_stride, int max_seqlen_q, int max_seqlen_k,
-                   int window, int n_starting, float softmax_scale, int dtype,
-                   void* workspace, size_t workspace_bytes, void* stream);
-
-/*
- * The same for requests that share prefixes.  Requests [cu_groups[i],
- * cu_groups[i+1]) share the prefix_lens[i] keys in the pages
- * prefix_table[i * prefix_stride + j]; seq_lens and block_table are of the keys
- * that follow, each request's own.  A query sees all of its prefix and its own
- * keys up to itself: the result is that of the concatenation, the prefix is read
- * once for all of its requests.  Requests outside of [cu_groups[0],
- * cu_groups[n_prefixes]) have no prefix.  Everything else as above;
- * the workspace is always needed.
- */
-size_t dcp_shared_prefix_attn_workspace_bytes(
-    int n_tokens, int batch, int n_prefixes, int n_heads_q, int n_heads_kv,
-    int head_dim, int max_seqlen_q, int max_seqlen_k, int max_prefix_len);
-int dcp_shared_prefix_attn(
-    const void* q, const void* k_cache, const void* v_cache, void* out,
-    float* lse, const int32_t* prefix_table, const int32_t* prefix_lens,
-    const int32_t* cu_groups, const int32_t* block_table,
-    const int32_t* seq_lens, const int32_t* cu_seqlens_q, int n_tokens,
-    int batch, int n_prefixes, int n_heads_q, int n_heads_kv, int head_dim,
-    int64_t q_token_stride, int64_t q_head_stride, int64_t out_token_stride,
-    int64_t out_head_stride, int n_pages, int page_size, int64_t page_stride,
-    int64_t token_stride, int64_t head_stride, int prefix_width,
-    int64_t prefix_stride, int table_width, int64_t table_stride,
-    int max_seqlen_q, int max_seqlen_k, int max_prefix_len,
-    float softmax_scale, int dtype, void* workspace, size_t workspace_bytes,
-    void* stream);
+typedef struct {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  void* out;
+  float* lse;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens_q;
+  const int32_t* prefix_table;
+  const int32_t* prefix_lens;
+  const int32_t* cu_groups;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int64_t page_stride, token_stride, head_stride;
+  int64_t table_stride, prefix_stride;
+  int32_t n_tokens, batch, n_heads_q, n_heads_kv, head_dim;
+  int32_t n_pages, page_size, table_width, prefix_width, n_prefixes;
+  int32_t max_seqlen_q, max_seqlen_k, max_prefix_len;
+  int32_t window, n_starting, dtype;
+  float softmax_scale;
+} dcp_paged_attn_args;
+size_t dcp_paged_attn_workspace_bytes(const dcp_paged_attn_args* args);
+int dcp_paged_attn(const dcp_paged_attn_args* args, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -211,8 +211,7 @@ def test_the_same_twice(gpu, name):
 def test_a_callers_workspace_is_enough_and_bounded(gpu, prefix):
     case = Paged([9000, 20], heads=2, kv_heads=1, **(dict(prefixes=[6000], cu_groups=[0, 2]) if prefix else {}))
     args = case.to(gpu)
-    longest = args["block_table"].shape[1] * 64
-    n = shared_prefix_workspace_bytes(2, 2, 1, 2, 1, 128, 1, longest, longest) if prefix else paged_cache_workspace_bytes(2, 2, 2, 1, 128, 1, longest)
+    n = (shared_prefix_workspace_bytes if prefix else paged_cache_workspace_bytes)(**args)
     call = shared_prefix_attention if prefix else paged_cache_attention
     store = torch.full((n + 4096,), 0xEE, dtype=torch.uint8, device=gpu)
     check(call(**args, workspace=store[:n]), case.truth())
