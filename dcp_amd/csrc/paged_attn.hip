@@ -1,21 +1,25 @@
 // Attention over a paged K/V cache for gfx950: causal or with a sliding window and first tokens that stay visible, for any
-// number of new tokens a request, and for batches that share a long prefix.
+// number of new tokens a request, and for batches that share long prefixes.
 //
 //   out = softmax(scale q K^T) V over the visible keys, lse = log sum exp
 //
 // A query's row is one (token, q head).  The rows of a kv head's group and of neighbouring tokens read the same keys, so they are
 // taken together: row r of a request stands for token r / group and head r % group of the kv head.
 //
-// The kernel of rows (paged_rows_kernel): a workgroup of 4 waves owns 128 rows of one (request, kv head), a wave 32 of them,
-// and walks its share of the key tiles (64 keys) that any of them sees.  K and V tiles go from memory straight into LDS
-// (KvTile), two stages; both products are transposed, as in the forward kernel of the plans:
+// Two kernels, by how many rows a request has for a kv head (at most, as far as the host knows): the kernel of few rows (up to 32:
+// answering token by token), which the keys' bytes bound, and the kernel of rows (prompts, and prefixes that many requests
+// share), which the matrix instructions bound.  Both form the products transposed, so that a lane holds one row:
 //
-//   S^T[key, row] = K Q^T      A = K rows from LDS, B = Q in registers
-//   O^T[d,   row] = V^T P^T    A = V columns from LDS, B = P^T straight from the S^T accumulators
+//   S^T[key, row] = K Q^T      A = rows of K, B = Q in registers
+//   O^T[d,   row] = V^T P^T    A = columns of V (transposing LDS reads), B = P^T straight from the S^T accumulators
 //
-// Keys are taken in groups of 16 that lie in one page (page sizes are multiples of 16), so a lane looks up one page a tile:
-// the lanes' 16-key group is the same for all of a wave's loads of a tile.  The window and the first tokens are two runs of such
-// groups laid end to end; nothing in between is read.
+// with 16x16x32 products: lane l = 16 g + n holds row n of 16 and keys 4 g .. 4 g + 3 of 16 (of O^T: those of d).
+//
+// Keys are taken in groups of 16 that lie in one page (page sizes are multiples of 16): a page is looked up once a group.  A window
+// and the first tokens are two runs of groups laid end to end; nothing in between is read.  What lies in a group and is
+// seen by no row (behind the last key, between the first tokens and the window, in a page that is not one) may hold anything: its
+// scores are masked by selection, and its V cleared in LDS by the lanes that brought it, since a weight of zero does not
+// make a NaN vanish.
 #include <math.h>
 
 #include <algorithm>
@@ -25,89 +29,89 @@
 
 namespace dcp {
 
-struct PagedAttnParams {
+// Keys that rows look at: the requests' own, or prefixes that requests share.
+struct PagedSource {
+  const int32_t* block_table;
+  const int32_t* key_lens;
+  const int32_t* cu_groups;  // prefixes: their requests; null for the requests' own keys
+  int64_t table_stride;
+  int table_width, batch;    // of prefixes or requests
+  int first_share, n_shares; // see PagedParams::partial_out
+  int n_tiles;               // row tiles of a kv head (kernel of rows)
+  int by_few;                // the kernel of few rows takes it
+};
+
+struct PagedParams {
   const void* q;
   const void* k;
   const void* v;
   void* out;
   float* lse;
-  const int32_t* block_table;  // of the requests, or of the shared prefixes
-  const int32_t* key_lens;
   const int32_t* cu_seqlens_q;  // null: one token a request
-  const int32_t* cu_groups;     // prefixes: the requests of a prefix; null otherwise
-  int64_t table_stride;
   int64_t q_token, q_head, out_token, out_head;  // element strides
   int64_t page_stride, token_stride, head_stride;
-  int table_width, n_pages, page_size;
-  int batch;     // requests, or prefixes
-  int n_tokens;  // of q
-  int n_requests;
+  PagedSource own, prefix;  // (prefix.batch 0: none)
+  int n_pages, page_size;
+  int n_requests, n_tokens;  // of q
   int n_heads_q, n_heads_kv, group;
-  int window, n_starting;  // window 0: none
+  int window, n_starting;  // of the own keys; window 0: none
   float scale_log2;
-  int n_tiles, n_splits;  // row tiles of a kv head; shares of a tile's keys
-  // shares, unless a tile has one and nothing is to be merged: [share][token][q head], O relative to the maximum
+  int direct;  // a row whose keys one workgroup takes is finished there
+  // Shares of a row's keys, joined afterwards: [share][token][q head], O relative to the maximum, the maximum (log2 domain) and
+  // the sum of the weights.  The own keys have shares [0, own.n_shares), the prefixes those that follow.
   float* partial_out;
-  f32x2* partial_sums;  // the maximum (log2 domain) and the sum of the weights
-  int first_share, direct;
+  f32x2* partial_sums;
+  // The kernel of few rows: pieces of the units that are cut between workgroups, and where a row's pieces are (cut_of), for the own
+  // keys and for the prefixes: [2][token][q head]
+  int2* cuts;
+  float* slot_out;   // [workgroup][2][head of the workgroup][rows][D]
+  f32x2* slot_sums;  // [workgroup][2][head of the workgroup][rows]
+  int few_rows, few_heads_log2;  // rows of a unit; kv heads a workgroup takes at once: 1, 2 or 4, with 4, 2 or 1 waves each
+  int n_few;                // workgroups
 };
-
-constexpr int kRowsThreads = 256, kRowsBM = 128, kRowsBN = 64;
-constexpr int kMinTilesPerShare = 4;
+typedef KernArgs<PagedParams> PagedArgs;
+typedef KernArgs<PagedSource> SourceArgs;
 
 // The tokens of request (or prefix) b.  Cut to the tensor, whatever the tables say.
 struct TokenRange {
   int begin, n;
 };
-__device__ __forceinline__ int first_token(const PagedAttnParams& p, int b) {
+__device__ __forceinline__ int first_token(PagedArgs& p, SourceArgs& src, int b) {
   int r = b;
-  if (p.cu_groups != nullptr) r = min(max(p.cu_groups[b], 0), p.n_requests);
+  if (src.cu_groups != nullptr) r = min(max(src.cu_groups[b], 0), p.n_requests);
   if (p.cu_seqlens_q != nullptr) r = p.cu_seqlens_q[r];
   return min(max(r, 0), p.n_tokens);
 }
-__device__ __forceinline__ TokenRange tokens_of(const PagedAttnParams& p, int b) {
-  const int begin = first_token(p, b);
-  return {begin, max(first_token(p, b + 1) - begin, 0)};
+__device__ __forceinline__ TokenRange tokens_of(PagedArgs& p, SourceArgs& src, int b) {
+  const int begin = first_token(p, src, b);
+  return {begin, max(first_token(p, src, b + 1) - begin, 0)};
 }
-
-// Row tile `tile` belongs to request b and is its tile number `index`.  Request b's tiles begin at number
-// floor(first_row / 128) + b: that leaves room for its last, partial one, and needs no sum over the requests before it.
-struct RowTile {
-  int b, index;
-};
-__device__ __forceinline__ RowTile find_row_tile(const PagedAttnParams& p, int tile) {
-  const int lane = threadIdx.x & 63;
-  auto start = [&](int b) { return (int)((int64_t)first_token(p, b) * p.group / kRowsBM) + b; };
-  int lo = 0, hi = p.batch;  // the last request that begins at or before the tile; 64 candidates a step
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 63) / 64, b = lo + lane * step;
-    const bool before = b < hi && start(b) <= tile;
-    const int n = __popcll(__ballot(before));
-    if (n > 1) lo += (n - 1) * step;
-    hi = min(lo + step, hi);
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  return {lo, tile - __builtin_amdgcn_readfirstlane(start(lo))};
+// Its keys: those that its row of pages has room for.
+__device__ __forceinline__ int keys_of(PagedArgs& p, SourceArgs& src, int b) {
+  return min(max(src.key_lens[b], 0), p.n_pages > 0 ? src.table_width * p.page_size : 0);
 }
 
 // The 16-key groups that rows at positions [first, last] see: [0, n_first) and then [begin, end).
 struct KeyGroups {
   int n_first, begin, end;
-  int window_begin, hull_end;  // keys from hull_end on, and between the first ones and the window, are seen by none
-  __device__ __forceinline__ KeyGroups(const PagedAttnParams& p, int first, int last) {
+  int window_begin, hull_end, n_starting;  // keys from hull_end on, and between the first ones and the window, are seen by none
+  __device__ __forceinline__ KeyGroups(int window, int starting, int first, int last) {
+    n_starting = starting;
     hull_end = last + 1;
     end = (hull_end + 15) / 16;
-    window_begin = p.window > 0 ? max(first - p.window + 1, 0) : 0;
+    window_begin = window > 0 ? max(first - window + 1, 0) : 0;
     begin = window_begin / 16;
-    n_first = min((int)(((int64_t)p.n_starting + 15) / 16), end);
+    n_first = min(starting / 16 + (starting % 16 != 0), end);
     if (n_first >= begin) begin = n_first = 0;  // one run
   }
   __device__ __forceinline__ int count() const { return n_first + end - begin; }
   __device__ __forceinline__ int at(int i) const { return i < n_first ? i : i - n_first + begin; }
-  __device__ __forceinline__ bool sees(const PagedAttnParams& p, int key) const {
-    return key < hull_end && (key < p.n_starting || key >= window_begin);
+  __device__ __forceinline__ bool sees(int key) const { return (key < hull_end) & ((key < n_starting) | (key >= window_begin)); }
+  __device__ __forceinline__ bool sees_all_of_16(int key) const {
+    return (key + 15 < hull_end) & ((key + 15 < n_starting) | (key >= window_begin));
   }
 };
+constexpr int kNoKey = 0x7fffff00;  // of a group that is not there: past every row's last key
 
 __device__ __forceinline__ float rows_max(float x) {  // over the lanes of one n: the four groups of 16 lanes
   const unsigned u = __float_as_uint(x);
@@ -120,185 +124,189 @@ __device__ __forceinline__ float rows_sum(float x) {
   return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// 16 bytes a lane from memory into LDS at lds_at + 16 * lane (ordered by the caller, as KvTile's loads)
+// 16 bytes a lane from memory into LDS at lds_at + 16 * lane (ordered by the caller, as KvTile's loads).  STREAM: read once, so it is
+// to take no room in the caches: four contexts of 131072 keys 369 -> 339 us.
+template <bool STREAM>
 __device__ __forceinline__ void load_async_piece(uint32_t lds_at, const uint16_t* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane(lds_at)), "v"(from)
-               : "memory");
+  if constexpr (STREAM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds_at)), "v"(from)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds_at)), "v"(from)
+                 : "memory");
 }
 
-// The same for what is read once (it takes no room in the caches).
-__device__ __forceinline__ void load_async_piece_nt(uint32_t lds_at, const uint16_t* from) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
-               :
-               : "s"(__builtin_amdgcn_readfirstlane(lds_at)), "v"(from)
-               : "memory");
+// The result of a row's 4 elements, from the sum of the weights.
+template <int DTYPE>
+__device__ __forceinline__ void store_row_piece(PagedArgs& p, int64_t token, int64_t head, int d, f32x4 o, float m, float l) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + d) =
+      u32x2{pack2<DTYPE>(o[0] * inv, o[1] * inv), pack2<DTYPE>(o[2] * inv, o[3] * inv)};
+  if (d == 0) p.lse[head * p.n_tokens + token] = l == 0.0f ? INFINITY : (m + log2f(l)) * kLn2;
 }
+
+// ---------------------------------------------------------------------------
+// The kernel of rows: a workgroup of 4 waves owns 128 rows of one (request, kv head), a wave 32 of them, and walks its share of the
+// 64-key tiles that any of them sees.  K and V tiles go from memory straight into LDS (KvTile), two stages each, K a tile
+// ahead of V: S^T of tile t + 1 is multiplied while tile t is exponentiated, MFMA by MFMA in one stream, O^T += V^T P^T
+// of tile t follows as a dense run that the SIMD's other wave fills with its own arithmetic.
+// ---------------------------------------------------------------------------
+constexpr int kRowsThreads = 256, kRowsBM = 128, kRowsBN = 64;
+constexpr int kMinTilesPerShare = 4;
+constexpr float kNoMax = -3.0e38f;  // the reference of a row that has seen nothing: below every score, and a weight of -inf against it is 0
+constexpr float kMaxTileSum = 16384.0f;  // of a lane's weights against a reference that is not their maximum: fp16 can hold them
+
+// Row tile `tile` belongs to request b and is its tile number `index` (negative: to none).  Request b's tiles begin at number
+// floor(first_row / 128) + b: that leaves room for its last, partial one, and needs no sum over the requests before it.
+struct RowTile {
+  int b, index;
+};
+__device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, int tile) {
+  const int lane = threadIdx.x & 63;
+  auto start = [&](int b) { return (int)((int64_t)first_token(p, src, b) * p.group / kRowsBM) + b; };
+  int lo = 0, hi = src.batch;  // the last request that begins at or before the tile; 64 candidates a step
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, b = lo + lane * step;
+    const bool before = b < hi && start(b) <= tile;
+    const int n = __popcll(__ballot(before));
+    if (n > 1) lo += (n - 1) * step;
+    hi = min(lo + step, hi);
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  return {lo, tile - __builtin_amdgcn_readfirstlane(start(lo))};
+}
+
+template <int D>
+constexpr int kRowsLds = 4 * KvTile<D>::SIZE * 2;
 
 template <int DTYPE, int D>
-__global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const PagedAttnParams p) {
+__device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int item, char* lds) {
   typedef KvTile<D> Tile;
-  constexpr int KS = D / 32, DT = D / 16, RT = 2, BN = kRowsBN;
-  __shared__ __attribute__((aligned(16))) uint16_t k_lds[2][Tile::SIZE];
-  __shared__ __attribute__((aligned(16))) uint16_t v_lds[2][Tile::SIZE];
+  constexpr int KS = D / 32, DT = D / 16, RT = 2, LPW = Tile::LPW;
+  constexpr int TILE_BYTES = Tile::SIZE * 2;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // ---- which rows, which share of their keys ---------------------------------
-  int item = __builtin_amdgcn_readfirstlane(blockIdx.x);
-  const int tile_number = item % p.n_tiles;
-  item /= p.n_tiles;
+  const int tile_number = __builtin_amdgcn_readfirstlane(item % src.n_tiles);
+  item = __builtin_amdgcn_readfirstlane(item / src.n_tiles);
   const int kv_head = __builtin_amdgcn_readfirstlane(item % p.n_heads_kv), share = __builtin_amdgcn_readfirstlane(item / p.n_heads_kv);
-  const RowTile tile = find_row_tile(p, tile_number);
-  const TokenRange tokens = tokens_of(p, tile.b);
+  const RowTile tile = find_row_tile(p, src, tile_number);
+  const TokenRange tokens = tokens_of(p, src, tile.b);
   const int n_rows = tokens.n * p.group;  // (at most n_tokens * group, which the host has checked)
   const int row0 = tile.index * kRowsBM;
-  if (row0 >= n_rows) return;
-  const bool prefix = p.cu_groups != nullptr;
-  const int n_keys = (int)min((int64_t)max(p.key_lens[tile.b], 0), p.n_pages > 0 ? (int64_t)p.table_width * p.page_size : 0);
+  if (tile.index < 0 || row0 >= n_rows) return;
+  const bool prefix = src.cu_groups != nullptr;
+  const int n_keys = keys_of(p, src, tile.b), window = prefix ? 0 : p.window, n_starting = p.n_starting;
   // token i of the request is at position n_keys - n + i; every token is past all of a prefix
-  const int first_tok = row0 / p.group, last_tok = min(row0 + kRowsBM, n_rows) - 1;
-  const int at0 = prefix ? n_keys - 1 : n_keys - tokens.n;
-  const int step = prefix ? 0 : 1;
-  const KeyGroups groups(p, max(at0 + first_tok * step, 0), at0 + last_tok / p.group * step);
-  const int n_groups = groups.hull_end > 0 ? groups.count() : 0;
-  const int tiles_all = (n_groups + 3) / 4;
-  const int n_shares = min(p.n_splits, max(1, tiles_all / kMinTilesPerShare));
+  const int first_tok = row0 / p.group, last_tok = (min(row0 + kRowsBM, n_rows) - 1) / p.group;
+  const int at0 = prefix ? n_keys - 1 : n_keys - tokens.n, step = prefix ? 0 : 1;
+  const KeyGroups groups(window, n_starting, max(at0 + first_tok * step, 0), at0 + last_tok * step);
+  const int n_groups = __builtin_amdgcn_readfirstlane(groups.hull_end > 0 ? groups.count() : 0);
+  const int tiles_all = (n_groups + 3) / 4, n_shares = min(src.n_shares, max(1, tiles_all / kMinTilesPerShare));
   int t_begin = 0, t_end = 0;
   if (share < n_shares) {
     t_begin = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * share / n_shares));
     t_end = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * (share + 1) / n_shares));
   }
 
-  // ---- this lane's rows: n of each of the wave's two row tiles ------------------
-  int64_t q_at[RT], out_row[RT];
-  int last_key[RT], first_key[RT];  // the last key it sees; the first of its window
-  bool live[RT];
-  int w_last = 0x7fffffff, w_first = 0;  // what every row of the wave sees: keys up to w_last, from w_first on
-  int w_hull = -1;
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int r = row0 + w * 32 + rt * 16 + n;
-    live[rt] = r < n_rows;
-    const int tok = r / p.group, head = kv_head * p.group + r % p.group;
-    q_at[rt] = (int64_t)(tokens.begin + tok) * p.q_token + head * p.q_head;
-    out_row[rt] = (int64_t)(tokens.begin + tok) * p.n_heads_q + head;
-    last_key[rt] = live[rt] ? at0 + tok * step : 0x7fffffff;  // (a row that is not there sees anything, with a zero q)
-    first_key[rt] = live[rt] && p.window > 0 ? max(last_key[rt] - p.window + 1, 0) : 0;
-    w_last = min(w_last, wave_min(last_key[rt]));
-    w_first = max(w_first, wave_max(first_key[rt]));
-    w_hull = max(w_hull, wave_max(live[rt] ? last_key[rt] : -1));
-  }
+  // ---- tiles: lane l brings pieces of rows of the tile's 16-key group l / 16, LPW of K and of V ---------
+  const int32_t* table = src.block_table + (int64_t)tile.b * src.table_stride;
+  constexpr int CH = D / 8;
+  const int lane_row = Tile::row_of(w * LPW, lane / CH) & 15;  // of load 0; the others are LOAD_ROWS further each
+  const int64_t lane_off = (int64_t)kv_head * p.head_stride + lane_row * p.token_stride + lane % CH * 8;
+  const int64_t load_step = Tile::LOAD_ROWS * p.token_stride;
+  // the first key of the lane's group of tile t
+  auto group_key = [&](int t) { return t * 4 + g < n_groups ? groups.at(t * 4 + g) * 16 : kNoKey; };
+  auto look_up = [&](int t) {
+    const int key = t < t_end ? group_key(t) : kNoKey;
+    return key != kNoKey ? table[key / p.page_size] : -1;
+  };
+  // whether the lane's group of tile t is there, and where its pieces are (of one that is not: somewhere in the cache)
+  auto is_there = [&](int t, int page) { return (group_key(t) != kNoKey) & ((unsigned)page < (unsigned)p.n_pages); };
+  auto offset_of = [&](int t, int page, bool there) -> int64_t {
+    const int64_t off = page * p.page_stride + (int64_t)(group_key(t) % p.page_size) * p.token_stride;
+    return lane_off + (there ? off : 0);
+  };
+  const uint32_t k_at = lds_address(lds), v_at = k_at + 2 * TILE_BYTES;
+  auto k_stage = [&](int t) { return reinterpret_cast<const uint16_t*>(lds + (t & 1) * TILE_BYTES); };
+  auto v_stage = [&](int t) { return reinterpret_cast<const uint16_t*>(lds + (2 + (t & 1)) * TILE_BYTES); };
+  auto load_k = [&](int t, int64_t off, int i) {
+    load_async_piece<false>(Tile::group_lds_at(k_at + (t & 1) * TILE_BYTES, w, i), reinterpret_cast<const uint16_t*>(p.k) + i * load_step + off);
+  };
+  auto load_v = [&](int t, int64_t off, int i) {
+    load_async_piece<false>(Tile::group_lds_at(v_at + (t & 1) * TILE_BYTES, w, i), reinterpret_cast<const uint16_t*>(p.v) + i * load_step + off);
+  };
+  // (the first pages are asked for before anything that does not wait for them)
+  const int page0 = look_up(t_begin), page1 = look_up(t_begin + 1);
+  int page_next = look_up(t_begin + 2);
+
+  // ---- this lane's rows: n of each of the wave's two row tiles (past the last one: the last one again, not written) ------
+  int last_key[RT];                          // the last key it sees
+  int first_last = 0x7fffffff, last_last = 0;  // of the wave's rows
   u32x4 q[RT][KS];
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt)
+  for (int rt = 0; rt < RT; ++rt) {
+    const int r = min(row0 + w * 32 + rt * 16 + n, n_rows - 1), tok = r / p.group, head = kv_head * p.group + r % p.group;
+    const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (tokens.begin + tok) * p.q_token + head * p.q_head + Tile::element16(g);
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      q[rt][ks] = u32x4{0, 0, 0, 0};
-      if (live[rt]) q[rt][ks] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(p.q) + q_at[rt] + Tile::element16(g) + Tile::step16(ks));
-    }
+    for (int ks = 0; ks < KS; ++ks) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + Tile::step16(ks));
+    last_key[rt] = at0 + tok * step;
+    first_last = min(first_last, wave_min(last_key[rt]));
+    last_last = max(last_last, wave_max(last_key[rt]));
+  }
+  const int reach = window > 0 ? window : 0x7fffffff;  // a query sees the keys less than this before its last
+  const float scale = p.scale_log2;
 
   // ---- running state ---------------------------------------------------------------
   f32x4 o[RT][DT];
-  float m_run[RT], l_run[RT];
+  float m_run[RT], l_run[RT], lsum[RT];
+  float alpha[RT];  // what O^T has to be multiplied by before the tile is added
+  bool rescale = false;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    m_run[rt] = -INFINITY;
+    m_run[rt] = kNoMax;
+    alpha[rt] = 1.0f;
     l_run[rt] = 0.0f;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-
-  // ---- tiles: lane l brings pieces of rows of the tile's 16-key group l / 16 ---------
-  const int32_t* table = p.block_table + (int64_t)tile.b * p.table_stride;
-  const uint16_t* k_base = reinterpret_cast<const uint16_t*>(p.k) + kv_head * p.head_stride;
-  const uint16_t* v_base = reinterpret_cast<const uint16_t*>(p.v) + kv_head * p.head_stride;
-  constexpr int CH = D / 8;
-  const int piece = lane % CH;
-  auto row_in_group = [&](int i) { return Tile::row_of(w * Tile::LPW + Tile::group_of_load(i), lane / CH) & 15; };
-  // the first key of the lane's group of tile t, -1 behind the last group
-  auto group_key = [&](int t) { return t * 4 + g < n_groups ? groups.at(t * 4 + g) * 16 : -1; };
-  auto look_up = [&](int t) { return t < t_end && group_key(t) >= 0 ? table[group_key(t) / p.page_size] : -1; };
-  auto request = [&](int t, int page, int stage) {
-    const int key = group_key(t);
-    const bool there = key >= 0 && (unsigned)page < (unsigned)p.n_pages;
-    const int64_t off = there ? page * p.page_stride + key % p.page_size * p.token_stride : 0;
-#pragma unroll
-    for (int i = 0; i < Tile::LPW; ++i) {
-      const int64_t at = off + row_in_group(i) * p.token_stride + piece * 8;
-      load_async_piece(Tile::group_lds_at(lds_address(k_lds[stage]), w, i), k_base + at);
-      load_async_piece(Tile::group_lds_at(lds_address(v_lds[stage]), w, i), v_base + at);
-    }
-    return there;
-  };
+  bool anchored = false;  // every row of the wave has a reference maximum
+  u32x4 pb[RT][2];        // P^T of the current tile, packed
   const int k_rd = Tile::row_base16(n, g), v_rd = Tile::col_base16(lane);
 
-  int page_next = look_up(t_begin + 1);
-  bool there = false, there_next = false;
-  if (t_begin < t_end) there_next = request(t_begin, look_up(t_begin), 0);
-  for (int t = t_begin; t < t_end; ++t) {
-    const int stage = (t - t_begin) & 1;
-    there = there_next;
-    wait_loads();
-    // What no row sees (behind the last key, between the first tokens and the window, in a page that is not one) may
-    // hold anything, and a weight of zero does not make a NaN vanish: its V is cleared by the lanes that brought it.
-    const int key0 = group_key(t);
-    const bool whole = there && key0 + 15 < groups.hull_end && (key0 + 15 < p.n_starting || key0 >= groups.window_begin);
-    if (__any(!whole)) {
+  // What the tile's keys are to the wave: is every one seen by every row; if not, the mask is put on its scores.
+  auto group_keys = [&](int t, bool there, int (&keys)[4]) {
+    const int key0 = there ? group_key(t) : kNoKey;
 #pragma unroll
-      for (int i = 0; i < Tile::LPW; ++i) {
-        if (!(there && groups.sees(p, key0 + row_in_group(i))))
-          *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(v_lds[stage]) + (Tile::group_lds_at(0, w, i) + 16 * lane)) = u32x4{0, 0, 0, 0};
-      }
-    }
-    __syncthreads();  // the tile is there, and nobody reads the other stage any more
-    if (t + 1 < t_end) there_next = request(t + 1, page_next, stage ^ 1);
-    page_next = look_up(t + 2);
-
-    // the tile's four groups: their first keys, and whether they are there
-    int group_keys[4];
-    const uint64_t there_mask = __ballot(there);
+    for (int kt = 0; kt < 4; ++kt) keys[kt] = __builtin_amdgcn_readlane(key0, 16 * kt);
+  };
+  auto is_full = [&](const int (&keys)[4]) {
+    bool full = true;
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      group_keys[kt] = __builtin_amdgcn_readlane(key0, 16 * kt);
-      if (!(there_mask >> (16 * kt) & 1)) group_keys[kt] = 0x7fffff00;  // (past every row's last key)
-    }
-    bool full = true, seen = false;
+    for (int kt = 0; kt < 4; ++kt) full = full & (keys[kt] + 15 <= first_last) & ((last_last - keys[kt] < reach) | (keys[kt] + 15 < n_starting)) & (keys[kt] != kNoKey);
+    return full;
+  };
+  auto mask = [&](const int (&keys)[4], f32x4 (&s)[RT][4]) {
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-      const int key = group_keys[kt];
-      full = full && key + 15 <= w_last && (key >= w_first || key + 15 < p.n_starting);
-      seen = seen || key <= w_hull;
-    }
-    if (!seen) continue;
-
-    f32x4 s[RT][4];
+    for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
+      for (int e = 0; e < 4; ++e) {
+        const int key = keys[kt] + 4 * g + e;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const u32x4 a = Tile::read_row16(k_lds[stage], k_rd, kt, ks);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) s[rt][kt] = mfma_16x16x32<DTYPE>(a, q[rt][ks], s[rt][kt]);
-      }
-    }
-    if (!full) {
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = group_keys[kt] + 4 * g + e;
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt) {
-            const bool visible = key <= last_key[rt] && (key < p.n_starting || key >= first_key[rt]) && group_keys[kt] < 0x7fffff00;
-            s[rt][kt][e] = visible ? s[rt][kt][e] : -INFINITY;
-          }
+        for (int rt = 0; rt < RT; ++rt) {
+          const bool visible = (key <= last_key[rt]) & ((key < n_starting) | (last_key[rt] - key < reach)) & (keys[kt] != kNoKey);
+          s[rt][kt][e] = visible ? s[rt][kt][e] : -INFINITY;
         }
-    }
-    u32x4 pb[RT][2];
+      }
+  };
+  // The maximum step: the row's reference raised to the tile's maximum, what was summed before taken relative to it.
+  auto raise = [&](const f32x4 (&s)[RT][4]) {
+    bool without = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float mx = -INFINITY;
@@ -306,86 +314,186 @@ __global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const Paged
       for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[rt][kt][e]);
-      mx = rows_max(mx * p.scale_log2);
-      const float m_new = fmaxf(m_run[rt], mx);
-      if (__any(m_new != m_run[rt])) {
-        const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_run[rt] - m_new);
-        l_run[rt] *= alpha;
+      const float m_new = fmaxf(m_run[rt], rows_max(mx * scale));
+      alpha[rt] = fast_exp2(m_run[rt] - m_new);
+      l_run[rt] *= alpha[rt];
+      m_run[rt] = m_new;
+      lsum[rt] = 0.0f;
+      without |= m_new == kNoMax;
+    }
+    anchored = !__any(without);
+    rescale = __any((alpha[0] != 1.0f) | (alpha[1] != 1.0f));
+  };
+  // Two elements of the lane's 32 weights: pair i is of row tile i / 8, key tile i / 2 % 4.  Weights are rounded to the storage type
+  // for the product (half a step each); their sum is of the unrounded ones.
+  auto weigh = [&](const f32x4 (&s)[RT][4], int i) {
+    const int rt = i / 8, kt = i / 2 % 4, e = i % 2 * 2;
+    const float x0 = fast_exp2(fmaf(s[rt][kt][e], scale, -m_run[rt])), x1 = fast_exp2(fmaf(s[rt][kt][e + 1], scale, -m_run[rt]));
+    lsum[rt] += x0 + x1;
+    pb[rt][kt / 2][2 * (kt % 2) + e / 2] = pack2<DTYPE>(x0, x1);
+  };
+
+  f32x4 s_a[RT][4], s_b[RT][4];
+  // S^T of a tile from stage k; `between(i)` goes between its 4 * KS operands
+  auto multiply_qk = [&](const uint16_t* k, f32x4 (&s)[RT][4], auto between) {
+    constexpr int N = 4 * KS, AHEAD = 2;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) s[rt][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    u32x4 a[4];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) a[i] = Tile::read_row16(k, k_rd, i & 3, i >> 2);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i + AHEAD < N) a[(i + AHEAD) & 3] = Tile::read_row16(k, k_rd, (i + AHEAD) & 3, (i + AHEAD) >> 2);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) s[rt][i & 3] = mfma_16x16x32<DTYPE>(a[i & 3], q[rt][i >> 2], s[rt][i & 3]);
+      between(i);
+      __builtin_amdgcn_sched_barrier(0);  // keeps the operand reads from being hoisted into more registers
+    }
+  };
+  auto multiply_pv = [&](const uint16_t* v) {
+    constexpr int N = 2 * DT, AHEAD = 2;
+    u32x4 a[4];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) a[i] = Tile::read_col16(v, v_rd, i / DT, i % DT);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i + AHEAD < N) a[(i + AHEAD) & 3] = Tile::read_col16(v, v_rd, (i + AHEAD) / DT, (i + AHEAD) % DT);
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) o[rt][i % DT] = mfma_16x16x32<DTYPE>(a[i & 3], pb[rt][i / DT], o[rt][i % DT]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  // ---- key loop ------------------------------------------------------------------------
+  // Tile t's V is cleared where nobody sees it; by the wave that brought it, after its loads have landed.
+  auto clear_v = [&](int t, bool there) {
+    const int key0 = group_key(t);
+    if (__any(!(there & groups.sees_all_of_16(key0)))) {
+#pragma unroll
+      for (int i = 0; i < LPW; ++i)
+        if (!(there & groups.sees(key0 + lane_row + Tile::LOAD_ROWS * i)))
+          *reinterpret_cast<u32x4*>(lds + (2 + (t & 1)) * TILE_BYTES + (Tile::group_lds_at(0, w, i) + 16 * lane)) = u32x4{0, 0, 0, 0};
+    }
+  };
+  int64_t off_next = 0;                   // of tile t + 1, whose K is there and whose V is asked for in iteration t
+  bool there = false, there_next = false;  // the lane's group of tiles t, t + 1
+  auto iteration = [&](int t, f32x4 (&s_cur)[RT][4], f32x4 (&s_nxt)[RT][4]) {
+    wait_loads();
+    clear_v(t, there);
+    __syncthreads();  // K of tile t + 1 and V of tile t are there; nobody reads K of tile t or V of tile t - 1 any more
+    int keys[4];
+    group_keys(t, there, keys);
+    const bool full = is_full(keys);
+    // the loads of K of tile t + 2 and V of tile t + 1 go out one at a time between the products
+    const bool there_k = is_there(t + 2, page_next);
+    const int64_t off_k = offset_of(t + 2, page_next, there_k);
+    // (unconditionally: past the end a page that there is comes into a stage that nobody reads any more)
+    page_next = look_up(t + 3);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) lsum[rt] = 0.0f;
+    bool taken = false;  // the tile's maximum
+    rescale = false;
+    if (__builtin_expect(!(full & anchored), 0)) {
+      if (!full) mask(keys, s_cur);
+      raise(s_cur);
+      taken = true;
+    }
+    // Where every row has a reference and sees the whole tile, its weights are taken against that without looking for its own
+    // maximum; the lanes' sums tell afterwards whether that was safe, and if not it is done again.
+    __builtin_amdgcn_s_setprio(2);
+    constexpr int N = 4 * KS, NL = 2 * LPW;
+    multiply_qk(k_stage(t + 1), s_nxt, [&](int i) {
+      constexpr int PAIRS = 16 / N;
+#pragma unroll
+      for (int x = 0; x < PAIRS; ++x) weigh(s_cur, i * PAIRS + x);
+      if ((i + 1) % (N / NL) == 0) {
+        const int load = i / (N / NL);
+        if (load < LPW) load_k(t, off_k, load);
+        else load_v(t + 1, off_next, load - LPW);
+      }
+    });
+    if (__builtin_expect(!taken & __any(!((lsum[0] < kMaxTileSum) & (lsum[1] < kMaxTileSum))), 0)) {
+      raise(s_cur);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) weigh(s_cur, i);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) l_run[rt] += lsum[rt];
+    if (__builtin_expect(rescale, 0)) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[rt][dt][e] *= alpha;
-        m_run[rt] = m_new;
-      }
-      const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-      float sum = 0.0f;
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        float x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] = fast_exp2(fmaf(s[rt][kt][e], p.scale_log2, -m_use));
-          sum += x[e];
-        }
-        // weights are rounded to the storage type for the product (half a step each); their sum is of the unrounded ones
-        pb[rt][kt / 2][2 * (kt % 2)] = pack2<DTYPE>(x[0], x[1]);
-        pb[rt][kt / 2][2 * (kt % 2) + 1] = pack2<DTYPE>(x[2], x[3]);
-      }
-      l_run[rt] += sum;
+          for (int e = 0; e < 4; ++e) o[rt][dt][e] *= alpha[rt];
     }
+    __builtin_amdgcn_s_setprio(1);
+    multiply_pv(v_stage(t));
+    __builtin_amdgcn_s_setprio(0);
+    there = there_next;
+    there_next = there_k;
+    off_next = off_k;
+  };
+  if (t_begin < t_end) {
+    there = is_there(t_begin, page0);
+    there_next = is_there(t_begin + 1, page1);
+    const int64_t off0 = offset_of(t_begin, page0, there);
+    off_next = offset_of(t_begin + 1, page1, there_next);
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2)
+    for (int i = 0; i < LPW; ++i) load_k(t_begin, off0, i);
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const u32x4 a = Tile::read_col16(v_lds[stage], v_rd, s2, dt);
+    for (int i = 0; i < LPW; ++i) load_v(t_begin, off0, i);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma_16x16x32<DTYPE>(a, pb[rt][s2], o[rt][dt]);
-      }
+    for (int i = 0; i < LPW; ++i) load_k(t_begin + 1, off_next, i);
+    wait_loads();
+    __syncthreads();
+    multiply_qk(k_stage(t_begin), s_a, [](int) {});
+    for (int t = t_begin; t < t_end; t += 2) {
+      iteration(t, s_a, s_b);
+      if (t + 1 >= t_end) break;
+      iteration(t + 1, s_b, s_a);
+    }
+    wait_loads();  // what was asked for past the end must land before the workgroup's LDS is anybody else's
   }
 
   // ---- results ---------------------------------------------------------------------
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const float l = rows_sum(l_run[rt]);
-    if (!live[rt]) continue;
+    const float l = rows_sum(l_run[rt]), m = l == 0.0f ? -INFINITY : m_run[rt];
+    const int r = row0 + w * 32 + rt * 16 + n;
+    if (r >= n_rows) continue;
+    const int64_t token = tokens.begin + r / p.group, head = kv_head * p.group + r % p.group;
     if (!p.direct) {
-      const int64_t at = (int64_t)(p.first_share + share) * p.n_tokens * p.n_heads_q + out_row[rt];
-      if (g == 0) p.partial_sums[at] = f32x2{m_run[rt], l};
+      const int64_t at = ((int64_t)(src.first_share + share) * p.n_tokens + token) * p.n_heads_q + head;
+      if (g == 0) p.partial_sums[at] = f32x2{m, l};
       if (share >= n_shares) continue;  // (nothing is read of a share without weights)
       float* to = p.partial_out + at * D + 4 * g;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(to + 16 * dt) = o[rt][dt];
       continue;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t token = out_row[rt] / p.n_heads_q, head = out_row[rt] % p.n_heads_q;
-    uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + 4 * g;
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-      *reinterpret_cast<u32x2*>(to + 16 * dt) = u32x2{pack2<DTYPE>(o[rt][dt][0] * inv, o[rt][dt][1] * inv),
-                                                      pack2<DTYPE>(o[rt][dt][2] * inv, o[rt][dt][3] * inv)};
-    if (g == 0) p.lse[head * p.n_tokens + token] = l == 0.0f ? INFINITY : (m_run[rt] + log2f(l)) * kLn2;
+    for (int dt = 0; dt < DT; ++dt) store_row_piece<DTYPE>(p, token, head, 16 * dt + 4 * g, o[rt][dt], m, l);
   }
 }
 
 // ---------------------------------------------------------------------------
-// The kernel of few rows: answering token by token.  A request has few rows a kv head (tokens * group, at most 32), so the
-// keys' bytes bound it and what counts is how many of them are under way.  The waves of a workgroup share no tile:
-// each takes tiles of 32 keys of its own, every fourth, K straight into registers in the layout of the product, V into its own
-// part of LDS, both a tile ahead, and waits for nobody until its share of the keys is done.
+// The kernel of few rows: the waves of a workgroup share no tile.  Each takes tiles of 32 keys of its own, K straight into registers
+// in the layout of the product, V into its own part of LDS, both a tile ahead, and waits for nobody until its share of the
+// keys is done: 8 waves a CU with 16 KiB under way each.
 //
-// Work is cut by length, not by request: the tiles of all (request, rows, kv head) units are laid end to end and every
-// workgroup takes the same number of them, whatever the lengths are (they are known on the device only).  A unit inside one
-// workgroup's share is finished there; of one that is cut each piece goes to the workgroup's slot (0: the share begins in the
-// unit, 1: it ends in it) and the merge kernel joins them.
+// Work is cut by length, not by request: the tiles of all (request, rows, kv heads) units, and of the prefixes' where they have few
+// rows, are laid end to end and every workgroup takes the same number of them, whatever the lengths are (they are known on
+// the device only).  A unit inside one workgroup's share is finished there; of one that is cut each piece goes to the
+// workgroup's slot (0: the share begins in the unit, 1: it ends in it) and the merge joins them.
+//
+// Several kv heads at once: in a cache by token ([page][token][head]) a head's row is 256 bytes, and four heads' waves
+// side by side read 1 KiB of a token at about the same time: four contexts of 131072 keys 382 -> 339 us, and nothing changes in a cache by head.
+// With few tiles a workgroup the waves take turns at one head's tiles instead, which makes the chain of tiles shorter.
 // ---------------------------------------------------------------------------
-struct PagedFewParams {
-  PagedAttnParams a;
-  int2* cuts;        // [token][q head]: see cut_of
-  float* slot_out;   // [workgroup][2][head of the workgroup][rows][D]
-  f32x2* slot_sums;  // [workgroup][2][head of the workgroup][rows]
-  int heads;         // kv heads a workgroup takes at once: 1, 2 or 4, as many to each of which it has 4 / heads waves
-};
 // What the merge needs to know of a row: the workgroup that begins its unit, how many the unit is cut over, the slot of the first
 // piece (the others are in slot 0) and the row in the slots.
 __device__ __forceinline__ int2 cut_of(int wg, int n_pieces, int slot, int row) { return int2{wg, n_pieces | row << 20 | slot << 28}; }
@@ -394,28 +502,37 @@ constexpr int kFewMaxBatch = 1 << 16;
 
 // What request b is to the kernel.
 struct FewRequest {
-  int first_tok, n_tok, n_keys, n_chunks, n_tiles;
-  template <typename P>
-  __device__ __forceinline__ FewRequest(const P& p, int b, int rows) {
-    const TokenRange tokens = tokens_of(p, b);
+  int first_tok, n_tok, n_keys, n_tiles;
+  __device__ __forceinline__ KeyGroups groups(PagedArgs& p, bool prefix) const {
+    return KeyGroups(prefix ? 0 : p.window, p.n_starting, prefix ? 0 : max(n_keys - n_tok, 0), n_keys - 1);
+  }
+  __device__ __forceinline__ FewRequest() {}
+  __device__ __forceinline__ FewRequest(PagedArgs& p, SourceArgs& src, int b) {
+    const TokenRange tokens = tokens_of(p, src, b);
     first_tok = tokens.begin;
     n_tok = tokens.n;
-    n_keys = (int)min((int64_t)max(p.key_lens[b], 0), p.n_pages > 0 ? (int64_t)p.table_width * p.page_size : 0);
-    n_chunks = (n_tok * p.group + rows - 1) / rows;
-    const KeyGroups groups(p, max(n_keys - n_tok, 0), n_keys - 1);
-    n_tiles = max((groups.count() + 1) / 2, 1);  // (a request without keys has its rows written all the same)
+    n_keys = keys_of(p, src, b);
+    n_tiles = max((groups(p, src.cu_groups != nullptr).count() + 1) / 2, 1);  // (a request without keys has its rows written all the same)
   }
-  __device__ __forceinline__ int64_t work(int head_groups) const { return (int64_t)n_chunks * head_groups * n_tiles; }
+  __device__ __forceinline__ int work(PagedArgs& p, int rows, int head_groups) const { return (n_tok * p.group + rows - 1) / rows * head_groups * n_tiles; }
+  __device__ __forceinline__ FewRequest of_lane(int lane) const {
+    FewRequest r;
+    r.first_tok = __builtin_amdgcn_readlane(first_tok, lane);
+    r.n_tok = __builtin_amdgcn_readlane(n_tok, lane);
+    r.n_keys = __builtin_amdgcn_readlane(n_keys, lane);
+    r.n_tiles = __builtin_amdgcn_readlane(n_tiles, lane);
+    return r;
+  }
 };
 
 // Sum over the wave's lanes up to and with this one.
-__device__ __forceinline__ int64_t wave_scan(int64_t x) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const int64_t y = __shfl_up(x, off);
-    if (lane >= off) x += y;
-  }
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
   return x;
 }
 __device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
@@ -423,101 +540,185 @@ __device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 
+// LDS of the kernel.  V of 32 keys: load r of a tile brings rows r, r + LOADS, ... side by side (1 KiB), 32 bytes of padding between
+// loads: eight consecutive rows then lie in eight different 32-byte bank windows for the transposing reads.
+template <int D, int RT>
+struct FewLds {
+  static constexpr int ROWS = 16 * RT, LOADS = kFewBN * D * 2 / 1024, LOAD_BYTES = 1024 + 32, STAGE = LOADS * LOAD_BYTES;
+  static constexpr int O_STRIDE = D + 4;  // floats: rows of a wave's result, which takes the place of its V
+  static constexpr int WAVE = 2 * STAGE > ROWS * O_STRIDE * 4 ? 2 * STAGE : ROWS * O_STRIDE * 4;
+  static constexpr int SUMS = kFewWaves * WAVE;                  // float [wave][row][2]
+  static constexpr int CHUNKS = SUMS + kFewWaves * ROWS * 2 * 4; // int [batch / 64]
+  static constexpr int BYTES = CHUNKS + 2 * kFewMaxBatch / 64 * 4;
+};
+
 template <int DTYPE, int D, int RT>
-__global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFewParams params) {
-  const PagedAttnParams& p = params.a;
-  constexpr int KS = D / 32, DT = D / 16, ROWS = 16 * RT;
-  // V of 32 keys: load r of a tile brings rows r, r + LOADS, ... side by side (1 KiB), 32 bytes of padding between loads: eight
-  // consecutive rows then lie in eight different 32-byte bank windows for the transposing reads.
-  constexpr int LOADS = kFewBN * D * 2 / 1024, LOAD_BYTES = 1024 + 32, STAGE = LOADS * LOAD_BYTES;
-  constexpr int O_STRIDE = D + 4;  // floats: rows of the joined result, a wave's
-  constexpr int WAVE_BYTES = 2 * STAGE > ROWS * O_STRIDE * 4 ? 2 * STAGE : ROWS * O_STRIDE * 4;
-  __shared__ __attribute__((aligned(16))) char lds[kFewWaves][WAVE_BYTES];
-  __shared__ float sums_lds[kFewWaves][ROWS][2];
-  __shared__ int64_t chunk_lds[kFewMaxBatch / 64];
+__device__ __forceinline__ void paged_few(int wg, char* lds) {
+  // (the arguments are read anew wherever another part of the work begins: kept in scalar registers throughout they do not fit)
+  PagedArgs& p0 = fresh_kernel_args<PagedParams>();
+  typedef FewLds<D, RT> Lds;
+  constexpr int KS = D / 32, DT = D / 16, ROWS = Lds::ROWS, LOADS = Lds::LOADS;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  float(*sums)[ROWS][2] = reinterpret_cast<float(*)[ROWS][2]>(lds + Lds::SUMS);
+  int* chunk_sums = reinterpret_cast<int*>(lds + Lds::CHUNKS);
 
-  const int heads = params.heads, head_groups = p.n_heads_kv / heads, turns = kFewWaves / heads;
-  const int my_head = w % heads, my_turn = w / heads;  // of the workgroup's heads; of the waves that share its tiles
-
-  // ---- this workgroup's share of all tiles -----------------------------------------
-  auto work_of = [&](int b) -> int64_t { return b < p.batch ? FewRequest(p, b, ROWS).work(head_groups) : 0; };
-  int64_t total, per, begin, end, before;  // before: tiles before the chunk of 64 requests in which the share begins
-  int chunk = 0;
-  const int n_chunks = (p.batch + 63) / 64;
-  int64_t scan = wave_scan(work_of(lane));
+  // ---- this workgroup's share of all tiles (the host has checked that their number fits 32 bits) ------------------------
+  // The list: the requests, padded to 64, and the prefixes behind them.
+  const int n_chunks = (p0.own.batch + 63) / 64 + (p0.prefix.by_few ? (p0.prefix.batch + 63) / 64 : 0);
+  auto own_chunks = [](PagedArgs& p) { return (p.own.batch + 63) / 64; };
+  auto source_of = [&](PagedArgs& p, int chunk) -> SourceArgs* { return chunk < own_chunks(p) ? &p.own : &p.prefix; };
+  auto requests_of = [&](int chunk, int& work) {
+    PagedArgs& p = fresh_kernel_args<PagedParams>();
+    SourceArgs& src = *source_of(p, chunk);
+    const int b = (chunk < own_chunks(p) ? chunk : chunk - own_chunks(p)) * 64 + lane;
+    FewRequest r;
+    r.first_tok = r.n_tok = r.n_keys = 0;
+    r.n_tiles = 1;
+    work = 0;
+    if (b < src.batch) {
+      r = FewRequest(p, src, b);
+      work = r.work(p, ROWS, p.n_heads_kv >> p.few_heads_log2);
+    }
+    return r;
+  };
+  int total = 0, before = 0, chunk = 0, work;
+  FewRequest requests = requests_of(0, work);
+  int scan = wave_scan(work);  // the chunk's tiles up to and with the lane's request
   if (n_chunks == 1) {
-    total = lane_value(scan, 63);
+    total = __builtin_amdgcn_readlane(scan, 63);
   } else {
     for (int i = w; i < n_chunks; i += kFewWaves) {
-      const int64_t sum = wave_scan(work_of(i * 64 + lane));
-      if (lane == 63) chunk_lds[i] = sum;
+      int more;
+      requests_of(i, more);
+      more = wave_scan(more);
+      if (lane == 63) chunk_sums[i] = more;
     }
     __syncthreads();
-    total = 0;
-    for (int i = 0; i < n_chunks; i += 64) total += lane_value(wave_scan(i + lane < n_chunks ? chunk_lds[i + lane] : 0), 63);
+    for (int i = 0; i < n_chunks; i += 64) total += __builtin_amdgcn_readlane(wave_scan(i + lane < n_chunks ? chunk_sums[i + lane] : 0), 63);
   }
-  per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)turns);
-  begin = min((int64_t)blockIdx.x * per, total);
-  end = min(begin + per, total);
+  const int per = max((total - 1) / p0.n_few + 1, kFewWaves >> p0.few_heads_log2);
+  const int begin = (int)min((int64_t)wg * per, (int64_t)total), end = (int)min((int64_t)begin + per, (int64_t)total);
   if (begin >= end) return;
-  before = 0;
   if (n_chunks > 1) {
     for (int i = 0; i < n_chunks; i += 64) {
-      const int64_t sums = before + wave_scan(i + lane < n_chunks ? chunk_lds[i + lane] : 0);
-      const int passed = __popcll(__ballot(sums <= begin));
-      if (passed > 0) before = lane_value(sums, passed - 1);
+      const int ends = before + wave_scan(i + lane < n_chunks ? chunk_sums[i + lane] : 0);
+      const int passed = __popcll(__ballot(ends <= begin));
+      if (passed > 0) before = __builtin_amdgcn_readlane(ends, passed - 1);
       chunk = i + passed;
       if (passed < 64) break;
     }
     chunk = __builtin_amdgcn_readfirstlane(min(chunk, n_chunks - 1));
-    scan = wave_scan(work_of(chunk * 64 + lane));
+    requests = requests_of(chunk, work);
+    scan = wave_scan(work);
   }
-  const int passed = min(__popcll(__ballot(before + scan <= begin)), 63);
-  int b = __builtin_amdgcn_readfirstlane(chunk * 64 + passed);
-  int64_t b_start = before + (passed > 0 ? lane_value(scan, passed - 1) : 0);
+  int index = __builtin_amdgcn_readfirstlane(min(__popcll(__ballot(before + scan <= begin)), 63));  // in the chunk
 
-  const uint32_t v_at = lds_address(lds[w]);
-  int64_t at = begin;
+  const uint32_t v_at = lds_address(lds) + w * Lds::WAVE;
+  char* v_lds = lds + w * Lds::WAVE;
+  int at = begin;
   while (at < end) {
-    const FewRequest request(p, b, ROWS);
-    const int64_t work = request.work(head_groups);
-    if (at >= b_start + work) {  // (no rows, or done)
-      b_start += work;
-      if (++b >= p.batch) break;
+    if (index == 64) {
+      before += __builtin_amdgcn_readlane(scan, 63);
+      if (++chunk >= n_chunks) break;
+      requests = requests_of(chunk, work);
+      scan = wave_scan(work);
+      index = 0;
+    }
+    const int unit_end = before + __builtin_amdgcn_readlane(scan, index);
+    if (at >= unit_end) {  // (no rows, or done)
+      ++index;
       continue;
     }
-    const int unit = __builtin_amdgcn_readfirstlane((int)((at - b_start) / request.n_tiles));
-    const int t_begin = __builtin_amdgcn_readfirstlane((int)(at - b_start - (int64_t)unit * request.n_tiles));
-    const int t_end = __builtin_amdgcn_readfirstlane((int)min((int64_t)request.n_tiles, t_begin + (end - at)));
-    const int slot = at == begin ? 0 : 1;
-    const int n_cut = t_begin == 0 ? (int)((at + request.n_tiles - 1) / per) - (int)blockIdx.x + 1 : 0;
+    PagedArgs& p = fresh_kernel_args<PagedParams>();
+    SourceArgs& src = *source_of(p, chunk);
+    const bool prefix = src.cu_groups != nullptr;
+    // the workgroup's kv heads at once, the waves that take turns at a head's tiles, and which of each the wave is
+    const int heads = 1 << p.few_heads_log2, head_groups = p.n_heads_kv >> p.few_heads_log2, turns = kFewWaves >> p.few_heads_log2;
+    const int my_head = w & (heads - 1), my_turn = w >> p.few_heads_log2;
+    const FewRequest request = requests.of_lane(index);
+    const int b = (chunk < own_chunks(p) ? chunk : chunk - own_chunks(p)) * 64 + index;
+    const int in_request = at - (unit_end - __builtin_amdgcn_readlane(work, index));
+    const int unit = __builtin_amdgcn_readfirstlane(in_request / request.n_tiles);
+    const int t_begin = in_request - unit * request.n_tiles, t_end = min(request.n_tiles, t_begin + (end - at));
     at += t_end - t_begin;
     const int kv_head0 = unit % head_groups * heads, kv_head = kv_head0 + my_head, row0 = unit / head_groups * ROWS;
-    const KeyGroups groups(p, max(request.n_keys - request.n_tok, 0), request.n_keys - 1);
-    const int n_groups = request.n_keys > 0 ? groups.count() : 0;
+    const KeyGroups groups = request.groups(p, prefix);
+    const int n_groups = request.n_keys > 0 ? groups.count() : 0, n_rows = request.n_tok * p.group;
+
+    // ---- where the wave's next 32 tiles are: lane 2 i + j holds the 16-key group j of the i-th of them ------------
+    const uint16_t* k_base = reinterpret_cast<const uint16_t*>(p.k) + kv_head * p.head_stride;
+    const uint16_t* v_base = reinterpret_cast<const uint16_t*>(p.v) + kv_head * p.head_stride;
+    int64_t lane_off = 0;
+    int lane_key = kNoKey;
+    auto look_up = [&](int step) {
+      PagedArgs& p = fresh_kernel_args<PagedParams>();
+      SourceArgs& src = *source_of(p, chunk);
+      const int group = 2 * (t_begin + my_turn + turns * (step + (lane >> 1))) + (lane & 1);
+      lane_off = 0;
+      lane_key = kNoKey;
+      if (group < n_groups && group < 2 * t_end) {
+        const int key = groups.at(group) * 16, entry = key / p.page_size;
+        const int page = src.block_table[b * src.table_stride + entry];
+        if ((unsigned)page < (unsigned)p.n_pages) {
+          lane_key = key;
+          lane_off = page * p.page_stride + (int64_t)(key - entry * p.page_size) * p.token_stride;
+        }
+      }
+    };
+    // what a lane brings of a tile: K of key n of each group, 8 elements from 32 ks + 8 g; V rows of its half's group
+    constexpr int CH = D / 8;
+    const int64_t k_lane = n * p.token_stride + 8 * g;
+    const int v_row = lane / CH % (16 / LOADS) * LOADS;  // of load 0, in the group of the lane's half
+    const int64_t v_lane = v_row * p.token_stride + lane % CH * 8, token_stride = p.token_stride;
+    const int n_steps = n_groups > 0 && t_begin + my_turn < t_end ? (t_end - t_begin - my_turn + turns - 1) / turns : 0;
+    u32x4 k[2][KS];  // K of the tile at hand, and once its products are formed of the next one
+    int64_t off[2];  // where its two groups are
+    int next_key[2], tile_key[2];
+    auto place = [&](int step) {
+      if (step % 32 == 0) look_up(step);
+      const int from = 2 * (step % 32);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        off[kt] = lane_value(lane_off, from + kt);
+        next_key[kt] = __builtin_amdgcn_readlane(lane_key, from + kt);
+      }
+    };
+    auto issue_v = [&](int stage) {
+      const uint16_t* v = v_base + (lane >= 32 ? off[1] : off[0]) + v_lane;
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
+#pragma unroll
+      for (int r = 0; r < LOADS; ++r) load_async_piece<true>(v_at + stage * Lds::STAGE + r * Lds::LOAD_BYTES, v + r * token_stride);
+    };
+    auto issue_k = [&]() {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          k[kt][ks] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_base + off[kt] + k_lane + 32 * ks));
+    };
+    if (n_steps > 0) {
+      place(0);
+      issue_v(0);
+      issue_k();
+    }
 
     // ---- this lane's rows --------------------------------------------------------------
-    int64_t out_row[RT];
     int last_key[RT], first_key[RT];
-    bool live[RT];
     int w_last = 0x7fffffff, w_first = 0;
     u32x4 q[RT][KS];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int r = row0 + rt * 16 + n;
-      live[rt] = r < request.n_tok * p.group;
-      const int tok = r / p.group, head = kv_head * p.group + r % p.group;
-      out_row[rt] = (int64_t)(request.first_tok + tok) * p.n_heads_q + head;
-      last_key[rt] = live[rt] ? request.n_keys - request.n_tok + tok : 0x7fffffff;
-      first_key[rt] = live[rt] && p.window > 0 ? max(last_key[rt] - p.window + 1, 0) : 0;
+      const int r = row0 + rt * 16 + n, tok = r / p.group, head = kv_head * p.group + r % p.group;
+      const bool live = r < n_rows;
       const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (request.first_tok + tok) * p.q_token + head * p.q_head + 8 * g;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         q[rt][ks] = u32x4{0, 0, 0, 0};
-        if (live[rt]) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + 32 * ks);
+        if (live) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + 32 * ks);
       }
+      last_key[rt] = !live ? 0x7fffffff : prefix ? request.n_keys - 1 : request.n_keys - request.n_tok + tok;
+      first_key[rt] = live && p.window > 0 && !prefix ? max(last_key[rt] - p.window + 1, 0) : 0;
       w_last = min(w_last, wave_min(last_key[rt]));
       w_first = max(w_first, wave_max(first_key[rt]));
     }
@@ -531,62 +732,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
       for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // ---- where the wave's next 32 tiles are: lane 2 i + j holds the 16-key group j of the i-th of them ------------
-    const int32_t* table = p.block_table + (int64_t)b * p.table_stride;
-    const uint16_t* k_base = reinterpret_cast<const uint16_t*>(p.k) + kv_head * p.head_stride;
-    const uint16_t* v_base = reinterpret_cast<const uint16_t*>(p.v) + kv_head * p.head_stride;
-    constexpr int kNoKey = 0x7fffff00;  // of a group that is not there: past every row's last key
-    int64_t lane_off = 0;
-    int lane_key = kNoKey;
-    auto look_up = [&](int step) {
-      const int group = 2 * (t_begin + my_turn + turns * (step + (lane >> 1))) + (lane & 1);
-      lane_off = 0;
-      lane_key = kNoKey;
-      if (group < n_groups && group < 2 * t_end) {
-        const int key = groups.at(group) * 16, index = key / p.page_size;
-        const int page = table[index];
-        if ((unsigned)page < (unsigned)p.n_pages) {
-          lane_key = key;
-          lane_off = page * p.page_stride + (int64_t)(key - index * p.page_size) * p.token_stride;
-        }
-      }
-    };
-    // what a lane brings of a tile: K of key n of each group, 8 elements from 32 ks + 8 g; V rows of its half's group
-    constexpr int CH = D / 8;
-    const int64_t k_lane = n * p.token_stride + 8 * g;
-    const int v_row = lane / CH % (16 / LOADS) * LOADS;  // of load 0, in the group of the lane's half
-    const int64_t v_lane = v_row * p.token_stride + lane % CH * 8;
-    const int n_steps = n_groups > 0 && t_begin + my_turn < t_end ? (t_end - t_begin - my_turn + turns - 1) / turns : 0;
-    u32x4 k[2][KS];  // K of the tile at hand, and once its products are formed of the next one
-    int64_t off[2];  // where its two groups are
-    int next_key[2], tile_key[2];
-    auto place = [&](int step) {
-      if (step % 32 == 0) look_up(step);
-      const int src = 2 * (step % 32);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        off[kt] = lane_value(lane_off, src + kt);
-        next_key[kt] = __builtin_amdgcn_readlane(lane_key, src + kt);
-      }
-    };
-    auto issue_v = [&](int stage) {
-      const uint16_t* v = v_base + (lane >= 32 ? off[1] : off[0]) + v_lane;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
-#pragma unroll
-      for (int r = 0; r < LOADS; ++r) load_async_piece_nt(v_at + stage * STAGE + r * LOAD_BYTES, v + r * p.token_stride);
-    };
-    auto issue_k = [&]() {
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) k[kt][ks] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_base + off[kt] + k_lane + 32 * ks));
-    };
-    const int v_rd = ((4 * g + (n >> 2)) % LOADS) * LOAD_BYTES + ((4 * g + (n >> 2)) / LOADS) * (D * 2) + 8 * (n & 3);
-    if (n_steps > 0) {
-      place(0);
-      issue_v(0);
-      issue_k();
-    }
+    const int v_rd = ((4 * g + (n >> 2)) % LOADS) * Lds::LOAD_BYTES + ((4 * g + (n >> 2)) / LOADS) * (D * 2) + 8 * (n & 3);
     for (int step = 0; step < n_steps; ++step) {
       const int stage = step & 1;
       wait_loads();
@@ -602,15 +748,15 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         const int key = tile_key[kt];
-        whole = whole && key + 15 < groups.hull_end && (key + 15 < p.n_starting || key >= groups.window_begin);
-        full = full && key + 15 <= w_last && (key >= w_first || key + 15 < p.n_starting);
+        whole = whole & groups.sees_all_of_16(key);
+        full = full & (key + 15 <= w_last) & ((key >= w_first) | (key + 15 < p.n_starting));
       }
-      if (!whole) {  // V of keys that nobody sees may be anything: cleared by the lanes that brought it
+      if (!whole) {
         const int key0 = lane >= 32 ? tile_key[1] : tile_key[0];
 #pragma unroll
         for (int r = 0; r < LOADS; ++r)
-          if (!(key0 != kNoKey && groups.sees(p, key0 + v_row + r)))
-            *reinterpret_cast<u32x4*>(lds[w] + stage * STAGE + r * LOAD_BYTES + 16 * lane) = u32x4{0, 0, 0, 0};
+          if (!((key0 != kNoKey) & groups.sees(key0 + v_row + r)))
+            *reinterpret_cast<u32x4*>(v_lds + stage * Lds::STAGE + r * Lds::LOAD_BYTES + 16 * lane) = u32x4{0, 0, 0, 0};
         asm volatile("" ::: "memory");
       }
       f32x4 s[RT][2];
@@ -634,6 +780,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
               const bool visible = (key <= last_key[rt]) & ((key < p.n_starting) | (key >= first_key[rt])) & (tile_key[kt] != kNoKey);
               s[rt][kt][e] = visible ? s[rt][kt][e] : -INFINITY;
             }
+            __builtin_amdgcn_sched_barrier(0);  // (all conditions at once need more scalar registers than there are)
           }
       }
       u32x4 pb[RT];
@@ -670,7 +817,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
       for (int dt = 0; dt < DT; ++dt) {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const uint32_t from = v_at + stage * STAGE + v_rd + 32 * dt;
+        const uint32_t from = v_at + stage * Lds::STAGE + v_rd + 32 * dt;
         const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)from));
         const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(from + 512)));  // rows 16 further
         const u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
@@ -679,107 +826,130 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedFe
       }
     }
 
-    // ---- the four waves' results joined --------------------------------------------------
+    // ---- the waves' results joined --------------------------------------------------
     asm volatile("" ::: "memory");
-    float* mine = reinterpret_cast<float*>(lds[w]);
+    float* mine = reinterpret_cast<float*>(v_lds);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float l = rows_sum(l_run[rt]);
       if (g == 0) {
-        sums_lds[w][rt * 16 + n][0] = m_run[rt];
-        sums_lds[w][rt * 16 + n][1] = l;
+        sums[w][rt * 16 + n][0] = m_run[rt];
+        sums[w][rt * 16 + n][1] = l;
       }
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mine + (rt * 16 + n) * O_STRIDE + 16 * dt + 4 * g) = o[rt][dt];
+      for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mine + (rt * 16 + n) * Lds::O_STRIDE + 16 * dt + 4 * g) = o[rt][dt];
     }
     __syncthreads();
+    PagedArgs& p_out = fresh_kernel_args<PagedParams>();
     const bool cut = t_end - t_begin < request.n_tiles;
+    const int slot = at - (t_end - t_begin) == begin ? 0 : 1;
+    const int n_cut = (at - t_end + request.n_tiles - 1) / per - wg + 1;  // (of a unit that begins here: it ends so many workgroups on)
+    const int group = p_out.group;
     constexpr int PIECES = D / 4;  // of a row
     for (int i = tid; i < heads * ROWS * PIECES; i += kFewThreads) {
       const int piece = i % PIECES, row = i / PIECES % ROWS, of = i / PIECES / ROWS, r = row0 + row;
-      if (r >= request.n_tok * p.group) continue;
+      if (r >= n_rows) continue;
       float m = -INFINITY;
-      for (int x = of; x < kFewWaves; x += heads) m = fmaxf(m, sums_lds[x][row][0]);
+      for (int x = of; x < kFewWaves; x += heads) m = fmaxf(m, sums[x][row][0]);
       const float m_use = m == -INFINITY ? 0.0f : m;
       f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
       float l = 0.0f;
       for (int x = of; x < kFewWaves; x += heads) {
-        const float weight = fast_exp2(sums_lds[x][row][0] - m_use);
-        l += weight * sums_lds[x][row][1];
-        const f32x4 o4 = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[x]) + row * O_STRIDE + 4 * piece);
+        const float weight = fast_exp2(sums[x][row][0] - m_use);
+        l += weight * sums[x][row][1];
+        const f32x4 o4 = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * Lds::WAVE) + row * Lds::O_STRIDE + 4 * piece);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
       }
-      const int64_t token = request.first_tok + r / p.group, head = (kv_head0 + of) * p.group + r % p.group;
-      if (piece == 0 && t_begin == 0) params.cuts[token * p.n_heads_q + head] = cut_of((int)blockIdx.x, n_cut, slot, of * ROWS + row);
-      if (cut || !p.direct) {
-        const int64_t to = cut ? (((int64_t)blockIdx.x * 2 + slot) * heads + of) * ROWS + row : (int64_t)p.first_share * p.n_tokens * p.n_heads_q + token * p.n_heads_q + head;
-        *reinterpret_cast<f32x4*>((cut ? params.slot_out : p.partial_out) + to * D + 4 * piece) = acc;
-        if (piece == 0) (cut ? params.slot_sums : p.partial_sums)[to] = f32x2{m, l};
+      const int64_t token = request.first_tok + r / group, head = (kv_head0 + of) * group + r % group;
+      if ((piece == 0) & (t_begin == 0))
+        p_out.cuts[((int64_t)(prefix ? p_out.n_tokens : 0) + token) * p_out.n_heads_q + head] = cut_of(wg, n_cut, slot, of * ROWS + row);
+      if (cut) {
+        const int64_t to = (((int64_t)wg * 2 + slot) * heads + of) * ROWS + row;
+        *reinterpret_cast<f32x4*>(p_out.slot_out + to * D + 4 * piece) = acc;
+        if (piece == 0) p_out.slot_sums[to] = f32x2{m, l};
+      } else if (!p_out.direct) {
+        const int64_t to = ((int64_t)source_of(p_out, chunk)->first_share * p_out.n_tokens + token) * p_out.n_heads_q + head;
+        *reinterpret_cast<f32x4*>(p_out.partial_out + to * D + 4 * piece) = acc;
+        if (piece == 0) p_out.partial_sums[to] = f32x2{m, l};
       } else {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + 4 * piece) =
-            u32x2{pack2<DTYPE>(acc[0] * inv, acc[1] * inv), pack2<DTYPE>(acc[2] * inv, acc[3] * inv)};
-        if (piece == 0) p.lse[head * p.n_tokens + token] = l == 0.0f ? INFINITY : (m + log2f(l)) * kLn2;
+        store_row_piece<DTYPE>(p_out, token, head, 4 * piece, acc, m, l);
       }
     }
     __syncthreads();  // nobody's part of LDS is filled again before all have read it
   }
 }
 
-// ---------------------------------------------------------------------------
-// The merge: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's parts, rounded once.  The parts are the pieces of a unit
-// that the kernel of few rows has cut, or the shares of the kernel of rows, or one or the other and the shares of a
-// prefix.  A workgroup takes a row: D / 4 lanes hold it in 16-byte pieces, and the 1024 / D sets of such lanes take parts in turn (a
-// wave that went through 128 parts alone took 17 us).
-// ---------------------------------------------------------------------------
-struct PagedMergeParams {
-  PagedFewParams few;       // few.cuts null: the kernel of rows has made the shares
-  const int32_t* cu_groups; // null: no prefixes
-  int n_prefixes, n_own, n_shares, rows;  // shares of the requests' own keys; with those of the prefixes, which come behind them; rows of a chunk
-};
+// ---- kernels --------------------------------------------------------------------------
+template <int DTYPE, int D>
+__global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const PagedParams) {
+  __shared__ __attribute__((aligned(16))) char lds[kRowsLds<D>];
+  PagedArgs& p = fresh_kernel_args<PagedParams>();
+  paged_rows<DTYPE, D>(p, p.own, blockIdx.x, lds);
+}
+
+template <int DTYPE, int D, int RT>
+__global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedParams) {
+  __shared__ __attribute__((aligned(16))) char lds[FewLds<D, RT>::BYTES];
+  paged_few<DTYPE, D, RT>(blockIdx.x, lds);
+}
+
+// Prefixes of many rows and the requests' own keys in one launch: the former are bound by the matrix instructions, the
+// latter by memory, so a CU takes a workgroup of each (of two consecutive ones, as long as there are both).
+template <int DTYPE, int D, int RT>
+__global__ __launch_bounds__(kFewThreads, 2) void paged_both_kernel(const PagedParams) {
+  __shared__ __attribute__((aligned(16))) char lds[std::max(FewLds<D, RT>::BYTES, kRowsLds<D>)];
+  PagedArgs& p = fresh_kernel_args<PagedParams>();
+  const int n_few = p.n_few, n_rows = gridDim.x - n_few, both = 2 * min(n_few, n_rows), wg = blockIdx.x;
+  const bool few = wg < both ? (wg & 1) != 0 : n_few > n_rows;
+  const int i = wg < both ? wg / 2 : wg - both / 2;
+  if (few) paged_few<DTYPE, D, RT>(i, lds);
+  else paged_rows<DTYPE, D>(p, p.prefix, i, lds);
+}
+
+// The merge: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's parts, rounded once.  The parts are, of the own keys and
+// of a prefix each, the pieces of a unit that the kernel of few rows has cut, or shares.  A workgroup takes a row: D / 4
+// lanes hold it in 16-byte pieces, and the 1024 / D sets of such lanes take parts in turn (a wave that went through 128
+// parts alone took 17 us).
 constexpr int kPagedMergeThreads = 256;
 template <int DTYPE, int D>
-__global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const PagedMergeParams params) {
-  const PagedAttnParams& p = params.few.a;
+__global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const PagedParams) {
+  PagedArgs& p = fresh_kernel_args<PagedParams>();
   constexpr int PIECES = D / 4, SETS = kPagedMergeThreads / PIECES;
   __shared__ f32x4 acc_lds[SETS][PIECES];
   __shared__ f32x2 sums_lds[SETS];
   const int row = blockIdx.x, tid = threadIdx.x, piece = tid % PIECES, set = tid / PIECES;
-  const int64_t n_rows = p.n_tokens * p.n_heads_q;  // (fits 32 bits)
-  // rows of no request are left as they were, and those of no prefix have no shares of one
+  const int64_t n_rows = (int64_t)p.n_tokens * p.n_heads_q;  // (fits 32 bits)
   const int token = row / p.n_heads_q, head = row % p.n_heads_q;
-  if ((token < first_token(p, 0)) | (token >= first_token(p, p.batch))) return;
-  int first = 0, end = 0x7fffffff;
-  if (params.cu_groups != nullptr) {
-    PagedAttnParams of_prefix = p;
-    of_prefix.cu_groups = params.cu_groups;
-    first = first_token(of_prefix, 0);
-    end = first_token(of_prefix, params.n_prefixes);
+  // rows of no request are left as they were, and those of no prefix have no parts of one
+  const int first = first_token(p, p.own, 0), end = first_token(p, p.own, p.own.batch);
+  int prefix_first = 0, prefix_end = 0;
+  if (p.prefix.batch > 0) {
+    prefix_first = first_token(p, p.prefix, 0);
+    prefix_end = first_token(p, p.prefix, p.prefix.batch);
   }
   // (& on purpose: of two conditions joined by && or || here, this compiler, clang 22, left the second one out)
-  const int n_shares = ((token >= first) & (token < end)) ? params.n_shares : params.n_own;
-  // the pieces of a unit that was cut come first, in the place of the own share
-  int n_cut = 0, wg = 0, slot = 0, slot_row = 0;
-  const int slot_rows = params.few.heads * params.rows;
-  if (params.few.cuts != nullptr) {
-    const int2 at = params.few.cuts[row];
-    wg = at.x;
-    n_cut = at.y & 0xfffff;
-    slot_row = at.y >> 20 & 0xff;
-    slot = at.y >> 28;
-    if (n_cut == 1) n_cut = 0;
-    if ((n_cut == 0) & (p.direct != 0)) return;  // done where it was computed
-  }
-  const int n_parts = n_cut > 0 ? n_cut + n_shares - 1 : n_shares;
+  if ((token < first) | (token >= end)) return;
+  const bool has_prefix = (token >= prefix_first) & (token < prefix_end);
+  int2 own = {0, 1}, pre = {0, 1};
+  if (p.own.by_few) own = p.cuts[row];
+  if (has_prefix & (p.prefix.by_few != 0)) pre = p.cuts[n_rows + row];
+  const int own_cut = (own.y & 0xfffff) > 1 ? own.y & 0xfffff : 0, pre_cut = (pre.y & 0xfffff) > 1 ? pre.y & 0xfffff : 0;
+  if ((p.own.by_few != 0) & (own_cut == 0) & (p.direct != 0)) return;  // done where it was computed
+  const int n_own = own_cut > 0 ? own_cut : p.own.n_shares;
+  const int n_parts = n_own + (has_prefix ? (pre_cut > 0 ? pre_cut : p.prefix.n_shares) : 0);
+  const int slot_rows = p.few_rows << p.few_heads_log2;
   // where part i is
   auto part = [&](int i, const f32x2*& sums) -> const float* {
-    if (i < n_cut) {
-      const int64_t at = ((int64_t)(wg + i) * 2 + (i == 0 ? slot : 0)) * slot_rows + slot_row;
-      sums = params.few.slot_sums + at;
-      return params.few.slot_out + at * D;
+    const bool of_prefix = i >= n_own;
+    const int j = of_prefix ? i - n_own : i;
+    const int2 cut = of_prefix ? pre : own;
+    if ((of_prefix ? pre_cut : own_cut) > 0) {
+      const int64_t at = ((int64_t)(cut.x + j) * 2 + (j == 0 ? cut.y >> 28 : 0)) * slot_rows + (cut.y >> 20 & 0xff);
+      sums = p.slot_sums + at;
+      return p.slot_out + at * D;
     }
-    const int64_t at = (i - n_cut + (n_cut > 0)) * n_rows + row;
+    const int64_t at = (int64_t)(j + (of_prefix ? p.prefix.first_share : 0)) * n_rows + row;
     sums = p.partial_sums + at;
     return p.partial_out + at * D;
   };
@@ -811,8 +981,9 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
     for (int x = 0; x < AT_ONCE; ++x) {
       const float weight = fast_exp2(ml[x][0] - m_use);
       l += weight * ml[x][1];
+      // (nothing is written of a share without weights; one that is not a number stays one)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] += weight > 0.0f ? weight * o4[x][e] : 0.0f;  // (nothing is written of a share without weights)
+      for (int e = 0; e < 4; ++e) acc[e] += weight == 0.0f ? 0.0f : weight * o4[x][e];
     }
     m = m_new;
   }
@@ -834,144 +1005,73 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
   }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + 4 * tid) =
-      u32x2{pack2<DTYPE>(acc[0] * inv, acc[1] * inv), pack2<DTYPE>(acc[2] * inv, acc[3] * inv)};
-  if (tid == 0) p.lse[(int64_t)head * p.n_tokens + token] = l == 0.0f ? INFINITY : (m + log2f(l)) * kLn2;
+  store_row_piece<DTYPE>(p, token, head, 4 * tid, acc, m, l);
 }
 
 // ---- host ---------------------------------------------------------------------------
 
-struct PagedShape {
-  int n_tokens, batch, n_heads_q, n_heads_kv, head_dim;
-};
-// Row tiles of one kv head: every request may have a partial one.
-static int64_t row_tiles(const PagedShape& s) {
-  return (int64_t)s.n_tokens * (s.n_heads_q / s.n_heads_kv) / kRowsBM + s.batch;
-}
-// Shares of a tile's keys: enough for two rounds of the device's workgroups.
-// Keys that the queries of a request see, of all of them.
-static int64_t seen_keys(int64_t max_q, int64_t max_keys, int window, int n_starting) {
-  return window > 0 ? std::min(max_keys, max_q + window + n_starting) : max_keys;
-}
-static int row_shares(const PagedShape& s, int64_t max_keys) {
-  const int64_t items = std::max<int64_t>(row_tiles(s) * s.n_heads_kv, 1);
-  const int64_t wanted = (4 * (int64_t)device_cu_count() + items - 1) / items;
-  const int64_t most = std::max<int64_t>((max_keys + kRowsBN * kMinTilesPerShare - 1) / (kRowsBN * kMinTilesPerShare), 1);
-  return (int)std::min<int64_t>({wanted, most, 256});
-}
-static size_t shares_bytes(const PagedShape& s, int n_shares) {
-  return (size_t)n_shares * s.n_tokens * s.n_heads_q * (s.head_dim + 2) * sizeof(float);
-}
-
-static int launch_rows(const PagedAttnParams& p, int head_dim, int dtype, void* stream) {
-  const int64_t n_wg = (int64_t)p.n_tiles * p.n_heads_kv * p.n_splits;
-  DCP_REQUIRE(n_wg < ((int64_t)1 << 31), "paged_attn: too many work items");
-  KernelTimer timer("paged_rows_kernel", stream);
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(kRowsThreads), 0, (hipStream_t)stream, p); };
-  if (dtype == DCP_DTYPE_BF16) {
-    if (head_dim == 128) launch(paged_rows_kernel<DCP_DTYPE_BF16, 128>);
-    else launch(paged_rows_kernel<DCP_DTYPE_BF16, 64>);
-  } else {
-    if (head_dim == 128) launch(paged_rows_kernel<DCP_DTYPE_FP16, 128>);
-    else launch(paged_rows_kernel<DCP_DTYPE_FP16, 64>);
-  }
-  return check_launch("paged_rows_kernel");
-}
-
-// How a call is laid out: which kernel takes the requests' own keys, and what of the workspace is whose.
+// How a call is laid out: which kernel takes which keys, and what of the workspace is whose.
 struct PagedPlan {
-  int rows = 0;      // of a chunk of the kernel of few rows; 0: the kernel of rows takes them
-  int n_wg = 0, heads = 1;  // of the kernel of few rows; kv heads of a workgroup
-  int n_own = 1, n_prefix = 0;  // shares
+  bool own_few = false, prefix_few = false;
+  int rows = 16, heads = 1, n_few = 0;  // of the kernel of few rows: rows of a unit, kv heads of a workgroup, workgroups
+  int n_own = 1, n_prefix = 0;          // shares
   size_t cuts = 0, slots = 0, shares = 0;  // bytes
   size_t bytes() const { return cuts + slots + shares; }
 };
-static size_t up16(size_t n) { return (n + 15) / 16 * 16; }
-static PagedPlan plan_paged(const PagedShape& s, int64_t max_q, int64_t max_keys, int n_prefixes, int64_t max_prefix) {
+
+// Row tiles of one kv head: every request may have a partial one.
+static int64_t row_tiles(const dcp_paged_attn_args& x, int batch) {
+  return (int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) / kRowsBM + batch;
+}
+// Shares of a tile's keys, so that the launch has `rounds` rounds of the device's workgroups.
+static int row_shares(const dcp_paged_attn_args& x, int batch, int64_t max_keys, int rounds) {
+  const int64_t items = std::max<int64_t>(row_tiles(x, batch) * x.n_heads_kv, 1);
+  const int64_t wanted = (rounds * 2 * (int64_t)device_cu_count() + items - 1) / items;
+  const int64_t most = std::max<int64_t>((max_keys + kRowsBN * kMinTilesPerShare - 1) / (kRowsBN * kMinTilesPerShare), 1);
+  return (int)std::min<int64_t>({wanted, most, 256});
+}
+static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
   PagedPlan plan;
-  const int64_t rows = max_q * (s.n_heads_q / s.n_heads_kv);
-  if (rows <= 32 && s.batch <= kFewMaxBatch) {
-    plan.rows = rows <= 16 ? 16 : 32;
-    plan.n_wg = 2 * device_cu_count();
-    const int64_t tiles = (int64_t)s.batch * s.n_heads_kv * ((max_keys + kFewBN - 1) / kFewBN) / plan.n_wg;
-    plan.heads = tiles < (getenv("X_T") ? atoi(getenv("X_T")) : 64) ? 1 : s.n_heads_kv % 4 == 0 ? 4 : s.n_heads_kv % 2 == 0 ? 2 : 1;
-    if (getenv("X_HEADS")) plan.heads = std::min(plan.heads, atoi(getenv("X_HEADS")));
-    plan.cuts = up16((size_t)s.n_tokens * s.n_heads_q * sizeof(int2));
-    plan.slots = (size_t)plan.n_wg * 2 * plan.heads * plan.rows * (s.head_dim + 2) * sizeof(float);
+  const auto up16 = [](size_t n) { return (n + 15) / 16 * 16; };
+  const int group = x.n_heads_q / x.n_heads_kv;
+  const int64_t keys = x.window > 0 ? std::min<int64_t>(x.max_seqlen_k, (int64_t)x.max_seqlen_q + x.window + x.n_starting) : x.max_seqlen_k;
+  // The kernel of few rows: of requests with up to 32, and of prefixes whose requests have that many together.  Its sums of
+  // tiles have to fit 32 bits whatever the lengths are.
+  const int64_t own_rows = (int64_t)x.max_seqlen_q * group, all_rows = (int64_t)x.n_tokens * group;
+  plan.own_few = own_rows <= 32;
+  plan.prefix_few = plan.own_few && x.n_prefixes > 0 && all_rows <= 32;
+  plan.rows = (plan.prefix_few ? all_rows : own_rows) <= 16 ? 16 : 32;
+  const auto most_tiles = [&](int batch, int width) {
+    return (double)(all_rows / plan.rows + batch) * x.n_heads_kv * ((double)width * x.page_size / kFewBN + 2);
+  };
+  if (most_tiles(x.batch, x.table_width) + (plan.prefix_few ? most_tiles(x.n_prefixes, x.prefix_width) : 0) > 2e9 ||
+      std::max(x.batch, x.n_prefixes) > kFewMaxBatch)
+    plan.own_few = plan.prefix_few = false;
+  if (plan.own_few) {
+    plan.n_few = 2 * device_cu_count();
+    // four heads at once from 64 tiles a workgroup on (16 for each wave): decode of 32 windows of 1016 keys, 16 tiles, 25.2 us with one
+    // head and 27.4 with four, 64 requests of up to 8192 keys, 256 tiles, 148 and 137
+    const int64_t tiles = ((int64_t)x.batch * ((keys + kFewBN - 1) / kFewBN) +
+                           (plan.prefix_few ? (int64_t)x.n_prefixes * ((x.max_prefix_len + kFewBN - 1) / kFewBN) : 0)) * x.n_heads_kv / plan.n_few;
+    plan.heads = tiles < 64 ? 1 : x.n_heads_kv % 4 == 0 ? 4 : x.n_heads_kv % 2 == 0 ? 2 : 1;
+    plan.cuts = up16((size_t)(plan.prefix_few ? 2 : 1) * x.n_tokens * x.n_heads_q * sizeof(int2));
+    plan.slots = (size_t)plan.n_few * 2 * plan.heads * plan.rows * (x.head_dim + 2) * sizeof(float);
   } else {
-    plan.n_own = row_shares(s, max_keys);
+    plan.n_own = row_shares(x, x.batch, keys, 2);
   }
-  if (n_prefixes > 0) {
-    const PagedShape of_prefix = {s.n_tokens, n_prefixes, s.n_heads_q, s.n_heads_kv, s.head_dim};
-    plan.n_prefix = row_shares(of_prefix, max_prefix);
-  }
-  if (plan.n_own + plan.n_prefix > 1) plan.shares = shares_bytes(s, plan.n_own + plan.n_prefix);
+  if (x.n_prefixes > 0) plan.n_prefix = plan.prefix_few ? 1 : row_shares(x, x.n_prefixes, x.max_prefix_len, 1);
+  if (plan.n_own + plan.n_prefix > 1) plan.shares = (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
   return plan;
 }
 
-template <int RT>
-static void launch_few_rows(const PagedFewParams& f, const PagedPlan& plan, int head_dim, int dtype, void* stream) {
-  auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3((unsigned)plan.n_wg), dim3(kFewThreads), 0, (hipStream_t)stream, f); };
-  if (dtype == DCP_DTYPE_BF16) {
-    if (head_dim == 128) launch(paged_few_kernel<DCP_DTYPE_BF16, 128, RT>);
-    else launch(paged_few_kernel<DCP_DTYPE_BF16, 64, RT>);
-  } else {
-    if (head_dim == 128) launch(paged_few_kernel<DCP_DTYPE_FP16, 128, RT>);
-    else launch(paged_few_kernel<DCP_DTYPE_FP16, 64, RT>);
-  }
-}
-
-// The requests' own keys, and the merge where there is something to join.
-static int launch_own(PagedAttnParams p, const PagedPlan& plan, const int32_t* cu_groups, int n_prefixes, int head_dim, int dtype, void* workspace,
-                      void* stream) {
-  PagedFewParams f = {};
-  if (plan.rows > 0) {
-    f.cuts = reinterpret_cast<int2*>(workspace);
-    f.slot_out = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.cuts);
-    f.slot_sums = reinterpret_cast<f32x2*>(f.slot_out + (size_t)plan.n_wg * 2 * plan.heads * plan.rows * head_dim);
-    f.a = p;
-    f.heads = plan.heads;
-    KernelTimer timer("paged_few_kernel", stream);
-    if (plan.rows == 16) launch_few_rows<1>(f, plan, head_dim, dtype, stream);
-    else launch_few_rows<2>(f, plan, head_dim, dtype, stream);
-    if (const int status = check_launch("paged_few_kernel")) return status;
-  } else {
-    if (const int status = launch_rows(p, head_dim, dtype, stream)) return status;
-    if (p.direct) return DCP_OK;
-    f.a = p;
-  }
-  const PagedMergeParams m = {f, cu_groups, n_prefixes, plan.n_own, plan.n_own + plan.n_prefix, plan.rows};
-  KernelTimer timer("paged_merge_kernel", stream);
-  auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(p.n_tokens * p.n_heads_q)), dim3(kPagedMergeThreads), 0, (hipStream_t)stream, m);
-  };
-  if (dtype == DCP_DTYPE_BF16) {
-    if (head_dim == 128) launch(paged_merge_kernel<DCP_DTYPE_BF16, 128>);
-    else launch(paged_merge_kernel<DCP_DTYPE_BF16, 64>);
-  } else {
-    if (head_dim == 128) launch(paged_merge_kernel<DCP_DTYPE_FP16, 128>);
-    else launch(paged_merge_kernel<DCP_DTYPE_FP16, 64>);
-  }
-  return check_launch("paged_merge_kernel");
-}
-
-static void place_shares(PagedAttnParams& p, const PagedPlan& plan, void* workspace, int head_dim) {
-  p.partial_out = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + plan.cuts + plan.slots);
-  p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)(plan.n_own + plan.n_prefix) * p.n_tokens * p.n_heads_q * head_dim);
-}
-
-}  // namespace dcp
-
-using namespace dcp;
+// One of the kernels of a storage type and a head size.
+#define DCP_PAGED_KERNEL(kernel, ...)                                                                   \
+  (x.dtype == DCP_DTYPE_BF16 ? (x.head_dim == 128 ? kernel<DCP_DTYPE_BF16, 128, ##__VA_ARGS__>          \
+                                                  : kernel<DCP_DTYPE_BF16, 64, ##__VA_ARGS__>)          \
+                             : (x.head_dim == 128 ? kernel<DCP_DTYPE_FP16, 128, ##__VA_ARGS__>          \
+                                                  : kernel<DCP_DTYPE_FP16, 64, ##__VA_ARGS__>))
 
 namespace {
-
-PagedShape shape_of(const dcp_paged_attn_args& x) { return {x.n_tokens, x.batch, x.n_heads_q, x.n_heads_kv, x.head_dim}; }
-
-PagedPlan plan_of(const dcp_paged_attn_args& x) {
-  return plan_paged(shape_of(x), x.max_seqlen_q, seen_keys(x.max_seqlen_q, x.max_seqlen_k, x.window, x.n_starting), x.n_prefixes, x.max_prefix_len);
-}
 
 // What a caller may have wrong, before anything is launched.
 int check_paged(const dcp_paged_attn_args& x) {
@@ -986,21 +1086,22 @@ int check_paged(const dcp_paged_attn_args& x) {
   DCP_REQUIRE(x.page_size > 0 && x.page_size % 16 == 0, "paged_attn: page_size %d must be a positive multiple of 16", x.page_size);
   DCP_REQUIRE(x.table_width > 0 && x.table_stride >= 0 && (x.n_prefixes == 0 || (x.prefix_width > 0 && x.prefix_stride >= 0)),
               "paged_attn: empty block tables");
-  DCP_REQUIRE(std::max((int64_t)x.table_width, (int64_t)(x.n_prefixes ? x.prefix_width : 0)) * x.page_size < 0x7fffff00, "paged_attn: too many keys a request");
+  DCP_REQUIRE(std::max((int64_t)x.table_width, (int64_t)(x.n_prefixes ? x.prefix_width : 0)) * x.page_size < kNoKey - 64, "paged_attn: too many keys a request");
   DCP_REQUIRE(x.page_stride % 8 == 0 && x.token_stride % 8 == 0 && x.head_stride % 8 == 0 && x.q_token_stride % 8 == 0 && x.q_head_stride % 8 == 0 &&
                   x.out_token_stride % 4 == 0 && x.out_head_stride % 4 == 0, "paged_attn: q, k, v strides must be multiples of 8 elements (out: 4)");
   DCP_REQUIRE(x.page_stride >= 0 && x.token_stride >= 0 && x.head_stride >= 0 && x.q_token_stride >= 0 && x.q_head_stride >= 0 &&
                   x.out_token_stride > 0 && x.out_head_stride > 0, "paged_attn: negative stride");
   DCP_REQUIRE(((reinterpret_cast<uintptr_t>(x.q) | reinterpret_cast<uintptr_t>(x.k_cache) | reinterpret_cast<uintptr_t>(x.v_cache) |
                 reinterpret_cast<uintptr_t>(x.out)) & 15) == 0, "paged_attn: q, k, v and out must be 16-byte aligned");
-  DCP_REQUIRE((int64_t)x.n_tokens * x.n_heads_q < ((int64_t)1 << 31), "paged_attn: too many queries");
+  DCP_REQUIRE((int64_t)x.n_tokens * x.n_heads_q < ((int64_t)1 << 31) - 256, "paged_attn: too many queries");
   DCP_REQUIRE(x.cu_seqlens_q != nullptr || x.n_tokens == x.batch, "paged_attn: without cu_seqlens_q every request has one token, got %d for %d",
               x.n_tokens, x.batch);
   if (x.n_tokens == 0 || x.batch == 0) return DCP_OK;
   DCP_REQUIRE(x.q && x.out && x.lse && x.block_table && x.seq_lens && (x.n_pages == 0 || (x.k_cache && x.v_cache)) &&
                   (x.n_prefixes == 0 || (x.prefix_table && x.prefix_lens && x.cu_groups)), "paged_attn: null argument");
   DCP_REQUIRE(x.max_seqlen_q > 0 && x.max_seqlen_k > 0 && (x.n_prefixes == 0 || x.max_prefix_len > 0), "paged_attn: the longest lengths must be positive");
-  DCP_REQUIRE(row_tiles(shape_of(x)) < ((int64_t)1 << 31) - x.n_prefixes, "paged_attn: too many rows");
+  // (every kernel's work items: at most 256 shares of a row tile)
+  DCP_REQUIRE((row_tiles(x, x.batch) + row_tiles(x, x.n_prefixes)) * x.n_heads_kv < ((int64_t)1 << 31) - (1 << 20), "paged_attn: too many rows");
   return DCP_OK;
 }
 
@@ -1008,43 +1109,72 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
   DCP_RECORDED(paged_attn(x, workspace, workspace_bytes, stream));
   if (const int status = check_paged(x)) return status;
   if (x.n_tokens == 0 || x.batch == 0) return DCP_OK;
-  const PagedPlan plan = plan_of(x);
+  const PagedPlan plan = plan_paged(x);
   const size_t needed = plan.bytes();
   DCP_REQUIRE(needed == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0 && workspace_bytes >= needed),
               "paged_attn: workspace of %zu bytes is missing, not 16-byte aligned or smaller than the %zu needed", workspace_bytes, needed);
-  PagedAttnParams p = {};
+  PagedParams p = {};
   p.q = x.q; p.k = x.k_cache; p.v = x.v_cache; p.out = x.out; p.lse = x.lse;
-  p.block_table = x.block_table; p.key_lens = x.seq_lens; p.cu_seqlens_q = x.cu_seqlens_q;
-  p.table_stride = x.table_stride;
+  p.cu_seqlens_q = x.cu_seqlens_q;
   p.q_token = x.q_token_stride; p.q_head = x.q_head_stride; p.out_token = x.out_token_stride; p.out_head = x.out_head_stride;
   p.page_stride = x.page_stride; p.token_stride = x.token_stride; p.head_stride = x.head_stride;
-  p.table_width = x.table_width; p.n_pages = x.n_pages; p.page_size = x.page_size;
-  p.batch = p.n_requests = x.batch; p.n_tokens = x.n_tokens;
+  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_own, (int)row_tiles(x, x.batch), plan.own_few};
+  if (x.n_prefixes > 0)
+    p.prefix = {x.prefix_table, x.prefix_lens, x.cu_groups, x.prefix_stride, x.prefix_width, x.n_prefixes, plan.n_own, plan.n_prefix,
+                (int)row_tiles(x, x.n_prefixes), plan.prefix_few};
+  p.n_pages = x.n_pages; p.page_size = x.page_size;
+  p.n_requests = x.batch; p.n_tokens = x.n_tokens;
   p.n_heads_q = x.n_heads_q; p.n_heads_kv = x.n_heads_kv; p.group = x.n_heads_q / x.n_heads_kv;
   p.window = x.window; p.n_starting = x.n_starting;
   p.scale_log2 = x.softmax_scale * kLog2e;
-  p.n_splits = plan.n_own;
-  p.n_tiles = (int)row_tiles(shape_of(x));
   p.direct = plan.n_own + plan.n_prefix == 1;
-  if (!p.direct) place_shares(p, plan, workspace, x.head_dim);
-  if (x.n_prefixes > 0) {
-    PagedAttnParams pre = p;
-    pre.block_table = x.prefix_table; pre.key_lens = x.prefix_lens; pre.cu_groups = x.cu_groups;
-    pre.table_stride = x.prefix_stride; pre.table_width = x.prefix_width;
-    pre.batch = x.n_prefixes;
-    pre.n_splits = plan.n_prefix;
-    pre.n_tiles = (int)row_tiles({x.n_tokens, x.n_prefixes, x.n_heads_q, x.n_heads_kv, x.head_dim});
-    pre.first_share = plan.n_own;
-    if (const int status = launch_rows(pre, x.head_dim, x.dtype, stream)) return status;
+  char* at = reinterpret_cast<char*>(workspace);
+  p.cuts = reinterpret_cast<int2*>(at);
+  p.slot_out = reinterpret_cast<float*>(at + plan.cuts);
+  p.slot_sums = reinterpret_cast<f32x2*>(p.slot_out + (size_t)plan.n_few * 2 * plan.heads * plan.rows * x.head_dim);
+  p.partial_out = reinterpret_cast<float*>(at + plan.cuts + plan.slots);
+  p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * x.head_dim);
+  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.n_few = plan.n_few;
+
+  int status = DCP_OK;
+  const auto launch = [&](auto kernel, const char* name, int64_t n_wg, int threads) {
+    if (status != DCP_OK || n_wg == 0) return;
+    if (n_wg >= (int64_t)1 << 31) {
+      status = fail(DCP_ERR_ARG, "paged_attn: too many work items");
+      return;
+    }
+    KernelTimer timer(name, stream);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(threads), 0, (hipStream_t)stream, p);
+    status = check_launch(name);
+  };
+  const auto row_items = [&](const PagedSource& src) { return (int64_t)src.n_tiles * x.n_heads_kv * src.n_shares; };
+  const bool prefix_rows = x.n_prefixes > 0 && !plan.prefix_few;
+  if (plan.own_few && prefix_rows) {
+    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_both_kernel, 1), "paged_both_kernel", row_items(p.prefix) + p.n_few, kFewThreads);
+    else launch(DCP_PAGED_KERNEL(paged_both_kernel, 2), "paged_both_kernel", row_items(p.prefix) + p.n_few, kFewThreads);
+  } else if (plan.own_few) {
+    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1), "paged_few_kernel", p.n_few, kFewThreads);
+    else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2), "paged_few_kernel", p.n_few, kFewThreads);
+  } else {
+    launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own), kRowsThreads);
+    if (prefix_rows) {
+      std::swap(p.own, p.prefix);  // (the kernel takes what it finds there)
+      launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own), kRowsThreads);
+      std::swap(p.own, p.prefix);
+    }
   }
-  return launch_own(p, plan, x.n_prefixes > 0 ? x.cu_groups : nullptr, x.n_prefixes, x.head_dim, x.dtype, workspace, stream);
+  if (plan.own_few || !p.direct) launch(DCP_PAGED_KERNEL(paged_merge_kernel), "paged_merge_kernel", (int64_t)x.n_tokens * x.n_heads_q, kPagedMergeThreads);
+  return status;
 }
 
 }  // namespace
+}  // namespace dcp
+
+using namespace dcp;
 
 extern "C" size_t dcp_paged_attn_workspace_bytes(const dcp_paged_attn_args* args) {
   if (args == nullptr || check_paged(*args) != DCP_OK || args->n_tokens == 0 || args->batch == 0) return 0;
-  return plan_of(*args).bytes();
+  return plan_paged(*args).bytes();
 }
 
 extern "C" int dcp_paged_attn(const dcp_paged_attn_args* args, void* workspace, size_t workspace_bytes, void* stream) {

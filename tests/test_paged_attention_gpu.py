@@ -78,6 +78,29 @@ def test_lengths_the_host_does_not_know(gpu, name, longest):
     check(_run(gpu, case, max_seqlen_k=longest), case.truth())
 
 
+@pytest.mark.parametrize("longest_q", [1, 5, 1000])
+@pytest.mark.parametrize("name", ["few", "five_heads", "mixed", "chunk", "window_chunk", "more_tokens_than_keys", "many", "tokens", "no_tokens",
+                                  "some_without", "empty_prefix", "no_own_keys"])
+def test_numbers_of_tokens_the_host_does_not_know(gpu, name, longest_q):
+    """max_seqlen_q chooses a kernel and no more."""
+    case = Paged(**{**SINGLE, **WINDOWS, **TOKENS, **PREFIXES}[name])
+    args = case.to(gpu)
+    if "cu_seqlens_q" not in args:
+        args["cu_seqlens_q"] = torch.tensor(case.cu, dtype=torch.int32, device=gpu)
+    got = (shared_prefix_attention if case.prefixes else paged_cache_attention)(**{**args, "max_seqlen_q": longest_q})
+    check(got, case.truth())
+
+
+def test_a_batch_of_thousands(gpu):
+    """Requests past the 64 that a wave looks at together, few and none of tokens and keys among them."""
+    n = 1500
+    case = Paged([(i * 7) % 40 for i in range(n)], new=[i % 3 for i in range(n)], heads=2, kv_heads=1, head_dim=64, page_size=16,
+                 prefixes=[i % 50 for i in range(200)], cu_groups=[7 * i + 3 for i in range(201)])
+    truth = case.truth()
+    for longest_q in (1, 2, 100):
+        check(_run(gpu, case, max_seqlen_q=longest_q), truth)
+
+
 @pytest.mark.parametrize("layout", ["apart", "by_head"])
 @pytest.mark.parametrize("new", [None, [3, 200]])
 def test_layouts_and_strides(gpu, layout, new):
@@ -126,16 +149,21 @@ def test_tokens_of_no_request_are_left(gpu, prefix, keys):
         check(_run(gpu, case, sentinel=3.0), case.truth(), untouched=3.0)
 
 
-def test_tokens_before_the_first_request_are_left(gpu):
-    case = Paged([90, 40], heads=2, kv_heads=1)
+@pytest.mark.parametrize("before", [4, 300])
+@pytest.mark.parametrize("new", [[1, 1], [40, 20]])
+@pytest.mark.parametrize("prefix", [False, True])
+def test_tokens_before_the_first_request_are_left(gpu, before, new, prefix):
+    """More of them than a tile of rows holds, too."""
+    case = Paged([90, 40], new=new, heads=2, kv_heads=1, **(dict(prefixes=[70], cu_groups=[0, 2]) if prefix else {}))
     args = case.to(gpu)
-    q = torch.cat([args["q"].new_zeros(4, 2, 128), args["q"]])
-    out, lse = torch.full_like(q, 3.0), torch.full((2, 6), 3.0, device=gpu)
-    args.update(q=q, cu_seqlens_q=torch.tensor([4, 5, 6], dtype=torch.int32, device=gpu), out=out, lse=lse)
-    for longest in (64, 100000):
-        paged_cache_attention(**args, max_seqlen_k=longest)
-        assert (out[:4] == 3).all() and (lse[:, :4] == 3).all()
-        check((out[4:], lse[:, 4:]), case.truth())
+    q = torch.cat([args["q"].new_zeros(before, 2, 128), args["q"]])
+    out, lse = torch.full_like(q, 3.0), torch.full((2, len(q)), 3.0, device=gpu)
+    args.update(q=q, cu_seqlens_q=torch.tensor(case.cu + before, dtype=torch.int32, device=gpu), out=out, lse=lse)
+    for longest_q in (1, max(new)):
+        for longest in (64, 100000):
+            (shared_prefix_attention if prefix else paged_cache_attention)(**{**args, "max_seqlen_q": longest_q, "max_seqlen_k": longest})
+            assert (out[:before] == 3).all() and (lse[:, :before] == 3).all()
+            check((out[before:], lse[:, before:]), case.truth())
 
 
 def test_no_requests_and_no_pages(gpu):

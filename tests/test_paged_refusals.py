@@ -94,7 +94,7 @@ def test_workspaces_are_none_for_nothing_and_more_for_more():
     lib = _lib.load()
     size = lambda name, **changed: lib.dcp_paged_attn_workspace_bytes(_PAGED_ARGS.pack(*{**CALLS[name], **changed}.values()))
     assert lib.dcp_paged_attn_workspace_bytes(None) == 0 and size("attention", n_tokens=0, batch=0) == 0 and size("attention", head_dim=96) == 0
-    assert 0 < size("attention") < size("attention", max_q=16) < size("prefix", max_q=16)
+    assert 0 < size("attention") < size("attention", max_q=16) and size("attention") < size("prefix") < size("prefix", max_k=1 << 20, width=1 << 16)
     # prompts of many rows need none: no share of the keys to join
     assert size("attention", n_tokens=1 << 17, cu=16, max_q=1 << 17, max_k=1 << 17, width=1 << 13) == 0
     with pytest.raises(AssertionError, match="null"):
