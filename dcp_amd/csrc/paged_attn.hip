@@ -37,7 +37,7 @@ struct PagedSource {
   int64_t table_stride;
   int table_width, batch;    // of prefixes or requests
   int first_share, n_shares; // see PagedParams::partial_out
-  int n_tiles;               // row tiles of a kv head (kernel of rows)
+  int n_tiles, xcd_group;    // row tiles of a kv head (kernel of rows); as many neighbouring work items are on one XCD
   int by_few;                // the kernel of few rows takes it
 };
 
@@ -192,7 +192,10 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // ---- which rows, which share of their keys ---------------------------------
-  const int tile_number = __builtin_amdgcn_readfirstlane(item % src.n_tiles);
+  // (row tiles of the same keys are neighbours and share an XCD's L2; those of a request's last tokens, which see the most, come first)
+  item = xcd_logical_id(item, src.xcd_group, (int64_t)src.n_tiles * p.n_heads_kv * src.n_shares);
+  if (item < 0) return;
+  const int tile_number = __builtin_amdgcn_readfirstlane(src.n_tiles - 1 - item % src.n_tiles);
   item = __builtin_amdgcn_readfirstlane(item / src.n_tiles);
   const int kv_head = __builtin_amdgcn_readfirstlane(item % p.n_heads_kv), share = __builtin_amdgcn_readfirstlane(item / p.n_heads_kv);
   const RowTile tile = find_row_tile(p, src, tile_number);
@@ -895,14 +898,15 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedPa
 }
 
 // Prefixes of many rows and the requests' own keys in one launch: the former are bound by the matrix instructions, the
-// latter by memory, so a CU takes a workgroup of each (of two consecutive ones, as long as there are both).
+// latter by memory, so a CU takes a workgroup of each, as long as there are both.
 template <int DTYPE, int D, int RT>
 __global__ __launch_bounds__(kFewThreads, 2) void paged_both_kernel(const PagedParams) {
   __shared__ __attribute__((aligned(16))) char lds[std::max(FewLds<D, RT>::BYTES, kRowsLds<D>)];
   PagedArgs& p = fresh_kernel_args<PagedParams>();
+  // (eight of the one and eight of the other in turn: consecutive workgroups go to the eight XCDs)
   const int n_few = p.n_few, n_rows = gridDim.x - n_few, both = 2 * min(n_few, n_rows), wg = blockIdx.x;
-  const bool few = wg < both ? (wg & 1) != 0 : n_few > n_rows;
-  const int i = wg < both ? wg / 2 : wg - both / 2;
+  const bool few = wg < both ? (wg & kNumXcd) != 0 : n_few > n_rows;
+  const int i = wg < both ? wg / (2 * kNumXcd) * kNumXcd + wg % kNumXcd : wg - both / 2;
   if (few) paged_few<DTYPE, D, RT>(i, lds);
   else paged_rows<DTYPE, D>(p, p.prefix, i, lds);
 }
@@ -1019,13 +1023,19 @@ struct PagedPlan {
   size_t bytes() const { return cuts + slots + shares; }
 };
 
+// Keys that a request's queries see, of the longest there are.
+static int64_t seen_keys(const dcp_paged_attn_args& x) {
+  return x.window > 0 ? std::min<int64_t>(x.max_seqlen_k, (int64_t)x.max_seqlen_q + x.window + x.n_starting) : x.max_seqlen_k;
+}
 // Row tiles of one kv head: every request may have a partial one.
 static int64_t row_tiles(const dcp_paged_attn_args& x, int batch) {
   return (int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) / kRowsBM + batch;
 }
 // Shares of a tile's keys, so that the launch has `rounds` rounds of the device's workgroups.
 static int row_shares(const dcp_paged_attn_args& x, int batch, int64_t max_keys, int rounds) {
-  const int64_t items = std::max<int64_t>(row_tiles(x, batch) * x.n_heads_kv, 1);
+  // (about as many tiles as have rows: row_tiles has room for more)
+  const int64_t rows = (int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv);
+  const int64_t items = std::max<int64_t>((rows + kRowsBM - 1) / kRowsBM, batch) * x.n_heads_kv;
   const int64_t wanted = (rounds * 2 * (int64_t)device_cu_count() + items - 1) / items;
   const int64_t most = std::max<int64_t>((max_keys + kRowsBN * kMinTilesPerShare - 1) / (kRowsBN * kMinTilesPerShare), 1);
   return (int)std::min<int64_t>({wanted, most, 256});
@@ -1034,7 +1044,7 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
   PagedPlan plan;
   const auto up16 = [](size_t n) { return (n + 15) / 16 * 16; };
   const int group = x.n_heads_q / x.n_heads_kv;
-  const int64_t keys = x.window > 0 ? std::min<int64_t>(x.max_seqlen_k, (int64_t)x.max_seqlen_q + x.window + x.n_starting) : x.max_seqlen_k;
+  const int64_t keys = seen_keys(x);
   // The kernel of few rows: of requests with up to 32, and of prefixes whose requests have that many together.  Its sums of
   // tiles have to fit 32 bits whatever the lengths are.
   const int64_t own_rows = (int64_t)x.max_seqlen_q * group, all_rows = (int64_t)x.n_tokens * group;
@@ -1118,10 +1128,10 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
   p.cu_seqlens_q = x.cu_seqlens_q;
   p.q_token = x.q_token_stride; p.q_head = x.q_head_stride; p.out_token = x.out_token_stride; p.out_head = x.out_head_stride;
   p.page_stride = x.page_stride; p.token_stride = x.token_stride; p.head_stride = x.head_stride;
-  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_own, (int)row_tiles(x, x.batch), plan.own_few};
+  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_own, (int)row_tiles(x, x.batch), 1, plan.own_few};
   if (x.n_prefixes > 0)
     p.prefix = {x.prefix_table, x.prefix_lens, x.cu_groups, x.prefix_stride, x.prefix_width, x.n_prefixes, plan.n_own, plan.n_prefix,
-                (int)row_tiles(x, x.n_prefixes), plan.prefix_few};
+                (int)row_tiles(x, x.n_prefixes), 1, plan.prefix_few};
   p.n_pages = x.n_pages; p.page_size = x.page_size;
   p.n_requests = x.batch; p.n_tokens = x.n_tokens;
   p.n_heads_q = x.n_heads_q; p.n_heads_kv = x.n_heads_kv; p.group = x.n_heads_q / x.n_heads_kv;
@@ -1147,19 +1157,29 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
     hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(threads), 0, (hipStream_t)stream, p);
     status = check_launch(name);
   };
-  const auto row_items = [&](const PagedSource& src) { return (int64_t)src.n_tiles * x.n_heads_kv * src.n_shares; };
+  // A kernel of rows' workgroups: whole groups of work items for each XCD.  A group is a request's (or a prefix's) tiles of a kv head,
+  // which read the same keys: 4 chunks of 256 tokens behind 65536 keys 1522 us one by one, 1065 in groups.  Where new tokens are more than
+  // half of what they see, tiles differ in length, and groups of them would leave XCDs idle: a prompt of 8192 tokens 592 us one
+  // by one, 654 in groups of eight.  Smaller groups where whole ones do not divide among the XCDs: 1040 items in groups of 16 359 us, of
+  // 8 278, one by one 309.
+  const auto row_items = [&](PagedSource& src, bool alike) {
+    const int64_t items = (int64_t)src.n_tiles * x.n_heads_kv * src.n_shares;
+    src.xcd_group = alike ? std::min(std::max(src.n_tiles / src.batch, 1), 128) : 1;
+    while (src.xcd_group > 1 && xcd_grid_size(items, src.xcd_group) * 20 > items * 21) --src.xcd_group;
+    return xcd_grid_size(items, src.xcd_group);
+  };
   const bool prefix_rows = x.n_prefixes > 0 && !plan.prefix_few;
   if (plan.own_few && prefix_rows) {
-    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_both_kernel, 1), "paged_both_kernel", row_items(p.prefix) + p.n_few, kFewThreads);
-    else launch(DCP_PAGED_KERNEL(paged_both_kernel, 2), "paged_both_kernel", row_items(p.prefix) + p.n_few, kFewThreads);
+    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_both_kernel, 1), "paged_both_kernel", row_items(p.prefix, true) + p.n_few, kFewThreads);
+    else launch(DCP_PAGED_KERNEL(paged_both_kernel, 2), "paged_both_kernel", row_items(p.prefix, true) + p.n_few, kFewThreads);
   } else if (plan.own_few) {
     if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1), "paged_few_kernel", p.n_few, kFewThreads);
     else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2), "paged_few_kernel", p.n_few, kFewThreads);
   } else {
-    launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own), kRowsThreads);
+    launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own, 2 * (int64_t)x.max_seqlen_q <= seen_keys(x)), kRowsThreads);
     if (prefix_rows) {
       std::swap(p.own, p.prefix);  // (the kernel takes what it finds there)
-      launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own), kRowsThreads);
+      launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own, true), kRowsThreads);
       std::swap(p.own, p.prefix);
     }
   }
