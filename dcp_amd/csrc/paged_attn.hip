@@ -180,24 +180,51 @@ __device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, 
   return {lo, tile - __builtin_amdgcn_readfirstlane(start(lo))};
 }
 
+// Which work item workgroup `wg` takes.  The items of a group, `group` neighbouring row tiles of a kv head, read the same keys and go to one
+// XCD (workgroup ids go round the eight), whose L2 then reads them once.  The groups that an XCD takes one after the other are
+// of different kv heads: in a cache by token a head's rows are 256 bytes every few KiB, so they all lie in one or two of the 16 channels of
+// an L2, and with an XCD to a head 64 requests on a prefix of 131072 keys ran at 0.63 PFLOP/s, 0.54 TB/s out of each L2.  The tiles
+// of a request's last tokens, which see the most, come first.
+struct RowItem {
+  int tile, kv_head, share;  // share: -1 for none
+};
+__device__ __forceinline__ RowItem row_item(int wg, int n_tiles, int group, int n_heads_kv, int n_shares) {
+  const int per_round = kNumXcd * group, round = wg / per_round, in_round = wg - round * per_round;
+  int i = round * kNumXcd + (in_round + round) % kNumXcd;  // the group
+  const int n_groups = (n_tiles + group - 1) / group, kv_head = i % n_heads_kv;
+  i /= n_heads_kv;
+  const int tile = n_tiles - 1 - (i % n_groups * group + in_round / kNumXcd), share = i / n_groups;
+  return {tile, kv_head, (tile >= 0) & (share < n_shares) ? share : -1};
+}
+inline int64_t row_workgroups(int64_t n_tiles, int group, int n_heads_kv, int n_shares) {
+  return xcd_grid_size((n_tiles + group - 1) / group * n_heads_kv * n_shares, 1) * group;
+}
+
+// LDS of the kernel: two stages of K and of V, and where the 16-key groups of 2 x 64 tiles are.
+constexpr int kTableTiles = 64;
 template <int D>
-constexpr int kRowsLds = 4 * KvTile<D>::SIZE * 2;
+struct RowsLds {
+  static constexpr int TILE = KvTile<D>::SIZE * 2;
+  static constexpr int OFFSETS = 4 * TILE;                     // int64 [2 * kTableTiles][4]: of a group, in the cache
+  static constexpr int ABSENT = OFFSETS + 2 * kTableTiles * 4 * 8;  // int [2 * kTableTiles][4]: it is not there (its offset is then 0)
+  static constexpr int ANY_ABSENT = ABSENT + 2 * kTableTiles * 4 * 4;  // int [2][4 waves]: one of the half's groups is not
+  static constexpr int BYTES = ANY_ABSENT + 2 * 4 * 4;
+};
 
 template <int DTYPE, int D>
 __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int item, char* lds) {
   typedef KvTile<D> Tile;
   constexpr int KS = D / 32, DT = D / 16, RT = 2, LPW = Tile::LPW;
-  constexpr int TILE_BYTES = Tile::SIZE * 2;
+  typedef RowsLds<D> Lds;
+  constexpr int TILE_BYTES = Lds::TILE;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // ---- which rows, which share of their keys ---------------------------------
-  // (row tiles of the same keys are neighbours and share an XCD's L2; those of a request's last tokens, which see the most, come first)
-  item = xcd_logical_id(item, src.xcd_group, (int64_t)src.n_tiles * p.n_heads_kv * src.n_shares);
-  if (item < 0) return;
-  const int tile_number = __builtin_amdgcn_readfirstlane(src.n_tiles - 1 - item % src.n_tiles);
-  item = __builtin_amdgcn_readfirstlane(item / src.n_tiles);
-  const int kv_head = __builtin_amdgcn_readfirstlane(item % p.n_heads_kv), share = __builtin_amdgcn_readfirstlane(item / p.n_heads_kv);
+  const RowItem at = row_item(item, src.n_tiles, src.xcd_group, p.n_heads_kv, src.n_shares);
+  if (at.share < 0) return;
+  const int tile_number = __builtin_amdgcn_readfirstlane(at.tile), kv_head = __builtin_amdgcn_readfirstlane(at.kv_head);
+  const int share = __builtin_amdgcn_readfirstlane(at.share);
   const RowTile tile = find_row_tile(p, src, tile_number);
   const TokenRange tokens = tokens_of(p, src, tile.b);
   const int n_rows = tokens.n * p.group;  // (at most n_tokens * group, which the host has checked)
@@ -218,35 +245,45 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   }
 
   // ---- tiles: lane l brings pieces of rows of the tile's 16-key group l / 16, LPW of K and of V ---------
-  const int32_t* table = src.block_table + (int64_t)tile.b * src.table_stride;
   constexpr int CH = D / 8;
   const int lane_row = Tile::row_of(w * LPW, lane / CH) & 15;  // of load 0; the others are LOAD_ROWS further each
-  const int64_t lane_off = (int64_t)kv_head * p.head_stride + lane_row * p.token_stride + lane % CH * 8;
+  const uint16_t* k_lane = reinterpret_cast<const uint16_t*>(p.k) + ((int64_t)kv_head * p.head_stride + lane_row * p.token_stride + lane % CH * 8);
   const int64_t load_step = Tile::LOAD_ROWS * p.token_stride;
-  // the first key of the lane's group of tile t
-  auto group_key = [&](int t) { return t * 4 + g < n_groups ? groups.at(t * 4 + g) * 16 : kNoKey; };
-  auto look_up = [&](int t) {
-    const int key = t < t_end ? group_key(t) : kNoKey;
-    return key != kNoKey ? table[key / p.page_size] : -1;
-  };
-  // whether the lane's group of tile t is there, and where its pieces are (of one that is not: somewhere in the cache)
-  auto is_there = [&](int t, int page) { return (group_key(t) != kNoKey) & ((unsigned)page < (unsigned)p.n_pages); };
-  auto offset_of = [&](int t, int page, bool there) -> int64_t {
-    const int64_t off = page * p.page_stride + (int64_t)(group_key(t) % p.page_size) * p.token_stride;
-    return lane_off + (there ? off : 0);
-  };
+  const int64_t v_from_k = reinterpret_cast<const uint16_t*>(p.v) - reinterpret_cast<const uint16_t*>(p.k);
   const uint32_t k_at = lds_address(lds), v_at = k_at + 2 * TILE_BYTES;
   auto k_stage = [&](int t) { return reinterpret_cast<const uint16_t*>(lds + (t & 1) * TILE_BYTES); };
   auto v_stage = [&](int t) { return reinterpret_cast<const uint16_t*>(lds + (2 + (t & 1)) * TILE_BYTES); };
   auto load_k = [&](int t, int64_t off, int i) {
-    load_async_piece<false>(Tile::group_lds_at(k_at + (t & 1) * TILE_BYTES, w, i), reinterpret_cast<const uint16_t*>(p.k) + i * load_step + off);
+    load_async_piece<false>(Tile::group_lds_at(k_at + (t & 1) * TILE_BYTES, w, i), k_lane + off + i * load_step);
   };
   auto load_v = [&](int t, int64_t off, int i) {
-    load_async_piece<false>(Tile::group_lds_at(v_at + (t & 1) * TILE_BYTES, w, i), reinterpret_cast<const uint16_t*>(p.v) + i * load_step + off);
+    load_async_piece<false>(Tile::group_lds_at(v_at + (t & 1) * TILE_BYTES, w, i), k_lane + off + (v_from_k + i * load_step));
   };
-  // (the first pages are asked for before anything that does not wait for them)
-  const int page0 = look_up(t_begin), page1 = look_up(t_begin + 1);
-  int page_next = look_up(t_begin + 2);
+  // the first key of group i of the list
+  auto group_key = [&](int i) { return i < n_groups ? groups.at(i) * 16 : kNoKey; };
+  // Where the groups are: a thread looks one up of the 64 tiles that begin with tile t_begin + rel, half a list ahead of its use.  (One
+  // tile at a time, by the lanes that load it, the divisions and 64-bit products were 40 % of the loop's instructions.)
+  int64_t* offsets = reinterpret_cast<int64_t*>(lds + Lds::OFFSETS);
+  int* absent = reinterpret_cast<int*>(lds + Lds::ABSENT);
+  int* any_absent = reinterpret_cast<int*>(lds + Lds::ANY_ABSENT);
+  auto look_up = [&](int rel) {
+    PagedArgs& p = fresh_kernel_args<PagedParams>();
+    const int i = (t_begin + rel) * 4 + tid, key = i < 4 * t_end ? group_key(i) : kNoKey;
+    int64_t off = 0;
+    bool there = false;
+    if (key != kNoKey) {
+      const int entry = key / p.page_size, page = src.block_table[tile.b * src.table_stride + entry];
+      there = (unsigned)page < (unsigned)p.n_pages;
+      if (there) off = page * p.page_stride + (int64_t)(key - entry * p.page_size) * p.token_stride;
+    }
+    const int at = (rel * 4 + tid) % (2 * kTableTiles * 4);
+    offsets[at] = off;
+    absent[at] = !there;
+    const bool any = __any(!there & (key != kNoKey));  // (what is past the end is no tile of anybody's)
+    if (lane == 0) any_absent[rel / kTableTiles % 2 * 4 + w] = any;
+  };
+  auto offset_of = [&](int t) { return offsets[((t - t_begin) * 4 + g) % (2 * kTableTiles * 4)]; };
+  if (t_begin < t_end) look_up(0);
 
   // ---- this lane's rows: n of each of the wave's two row tiles (past the last one: the last one again, not written) ------
   int last_key[RT];                          // the last key it sees
@@ -282,30 +319,32 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   u32x4 pb[RT][2];        // P^T of the current tile, packed
   const int k_rd = Tile::row_base16(n, g), v_rd = Tile::col_base16(lane);
 
-  // What the tile's keys are to the wave: is every one seen by every row; if not, the mask is put on its scores.
-  auto group_keys = [&](int t, bool there, int (&keys)[4]) {
-    const int key0 = there ? group_key(t) : kNoKey;
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt) keys[kt] = __builtin_amdgcn_readlane(key0, 16 * kt);
+  // Tiles that every row of the wave sees all of, by number: [0, full_first) in the first tokens, [full_begin, full_end) in the
+  // window.  Any other is masked.
+  const int shift = groups.n_first - groups.begin;
+  const int full_first = min(n_starting / 16, max(first_last + 1, 0) / 16) / 4;
+  const int full_begin = (max(groups.n_first, (max(last_last - reach + 1, 0) + 15) / 16 + shift) + 3) / 4;
+  const int full_count = max((max(first_last + 1, 0) / 16 + shift) / 4 - full_begin, 0);
+  auto is_full = [&](int t) {
+    const int* any = any_absent + (t - t_begin) / kTableTiles % 2 * 4;
+    const int bad = any[0] | any[1] | any[2] | any[3];
+    return (((unsigned)t < (unsigned)full_first) | ((unsigned)(t - full_begin) < (unsigned)full_count)) & (__builtin_amdgcn_readfirstlane(bad) == 0);
   };
-  auto is_full = [&](const int (&keys)[4]) {
-    bool full = true;
+  auto mask = [&](int t, f32x4 (&s)[RT][4]) {
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) full = full & (keys[kt] + 15 <= first_last) & ((last_last - keys[kt] < reach) | (keys[kt] + 15 < n_starting)) & (keys[kt] != kNoKey);
-    return full;
-  };
-  auto mask = [&](const int (&keys)[4], f32x4 (&s)[RT][4]) {
-#pragma unroll
-    for (int kt = 0; kt < 4; ++kt)
+    for (int kt = 0; kt < 4; ++kt) {
+      const bool there = absent[((t - t_begin) * 4 + kt) % (2 * kTableTiles * 4)] == 0;
+      const int key0 = group_key(t * 4 + kt);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int key = keys[kt] + 4 * g + e;
+        const int key = key0 + 4 * g + e;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          const bool visible = (key <= last_key[rt]) & ((key < n_starting) | (last_key[rt] - key < reach)) & (keys[kt] != kNoKey);
+          const bool visible = (key <= last_key[rt]) & ((key < n_starting) | (last_key[rt] - key < reach)) & there;
           s[rt][kt][e] = visible ? s[rt][kt][e] : -INFINITY;
         }
       }
+    }
   };
   // The maximum step: the row's reference raised to the tile's maximum, what was summed before taken relative to it.
   auto raise = [&](const f32x4 (&s)[RT][4]) {
@@ -372,35 +411,30 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 
   // ---- key loop ------------------------------------------------------------------------
   // Tile t's V is cleared where nobody sees it; by the wave that brought it, after its loads have landed.
-  auto clear_v = [&](int t, bool there) {
-    const int key0 = group_key(t);
-    if (__any(!(there & groups.sees_all_of_16(key0)))) {
+  auto clear_v = [&](int t) {
+    const int key0 = group_key(t * 4 + g);
+    const bool there = absent[((t - t_begin) * 4 + g) % (2 * kTableTiles * 4)] == 0;
 #pragma unroll
-      for (int i = 0; i < LPW; ++i)
-        if (!(there & groups.sees(key0 + lane_row + Tile::LOAD_ROWS * i)))
-          *reinterpret_cast<u32x4*>(lds + (2 + (t & 1)) * TILE_BYTES + (Tile::group_lds_at(0, w, i) + 16 * lane)) = u32x4{0, 0, 0, 0};
-    }
+    for (int i = 0; i < LPW; ++i)
+      if (!(there & groups.sees(key0 + lane_row + Tile::LOAD_ROWS * i)))
+        *reinterpret_cast<u32x4*>(lds + (2 + (t & 1)) * TILE_BYTES + (Tile::group_lds_at(0, w, i) + 16 * lane)) = u32x4{0, 0, 0, 0};
   };
-  int64_t off_next = 0;                   // of tile t + 1, whose K is there and whose V is asked for in iteration t
-  bool there = false, there_next = false;  // the lane's group of tiles t, t + 1
+  int64_t off_next = 0;  // of tile t + 1, whose K is there and whose V is asked for in iteration t
   auto iteration = [&](int t, f32x4 (&s_cur)[RT][4], f32x4 (&s_nxt)[RT][4]) {
     wait_loads();
-    clear_v(t, there);
+    const bool full = is_full(t);
+    if (__builtin_expect(!full, 0)) clear_v(t);
+    if (__builtin_expect((t - t_begin) % kTableTiles == kTableTiles / 2, 0)) look_up((t - t_begin) / kTableTiles * kTableTiles + kTableTiles);
     __syncthreads();  // K of tile t + 1 and V of tile t are there; nobody reads K of tile t or V of tile t - 1 any more
-    int keys[4];
-    group_keys(t, there, keys);
-    const bool full = is_full(keys);
-    // the loads of K of tile t + 2 and V of tile t + 1 go out one at a time between the products
-    const bool there_k = is_there(t + 2, page_next);
-    const int64_t off_k = offset_of(t + 2, page_next, there_k);
-    // (unconditionally: past the end a page that there is comes into a stage that nobody reads any more)
-    page_next = look_up(t + 3);
+    // The loads of K of tile t + 2 and V of tile t + 1 go out between the products, unconditionally: past the end a page that there
+    // is comes into a stage that nobody reads any more.
+    const int64_t off_k = offset_of(t + 2);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) lsum[rt] = 0.0f;
     bool taken = false;  // the tile's maximum
     rescale = false;
     if (__builtin_expect(!(full & anchored), 0)) {
-      if (!full) mask(keys, s_cur);
+      if (!full) mask(t, s_cur);
       raise(s_cur);
       taken = true;
     }
@@ -412,11 +446,8 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
       constexpr int PAIRS = 16 / N;
 #pragma unroll
       for (int x = 0; x < PAIRS; ++x) weigh(s_cur, i * PAIRS + x);
-      if ((i + 1) % (N / NL) == 0) {
-        const int load = i / (N / NL);
-        if (load < LPW) load_k(t, off_k, load);
-        else load_v(t + 1, off_next, load - LPW);
-      }
+      if (i < LPW) load_k(t, off_k, i);
+      else if (i < NL) load_v(t + 1, off_next, i - LPW);
     });
     if (__builtin_expect(!taken & __any(!((lsum[0] < kMaxTileSum) & (lsum[1] < kMaxTileSum))), 0)) {
       raise(s_cur);
@@ -436,15 +467,12 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     __builtin_amdgcn_s_setprio(1);
     multiply_pv(v_stage(t));
     __builtin_amdgcn_s_setprio(0);
-    there = there_next;
-    there_next = there_k;
     off_next = off_k;
   };
   if (t_begin < t_end) {
-    there = is_there(t_begin, page0);
-    there_next = is_there(t_begin + 1, page1);
-    const int64_t off0 = offset_of(t_begin, page0, there);
-    off_next = offset_of(t_begin + 1, page1, there_next);
+    __syncthreads();
+    const int64_t off0 = offset_of(t_begin);
+    off_next = offset_of(t_begin + 1);
 #pragma unroll
     for (int i = 0; i < LPW; ++i) load_k(t_begin, off0, i);
 #pragma unroll
@@ -886,7 +914,7 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
 // ---- kernels --------------------------------------------------------------------------
 template <int DTYPE, int D>
 __global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const PagedParams) {
-  __shared__ __attribute__((aligned(16))) char lds[kRowsLds<D>];
+  __shared__ __attribute__((aligned(16))) char lds[RowsLds<D>::BYTES];
   PagedArgs& p = fresh_kernel_args<PagedParams>();
   paged_rows<DTYPE, D>(p, p.own, blockIdx.x, lds);
 }
@@ -901,7 +929,7 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedPa
 // latter by memory, so a CU takes a workgroup of each, as long as there are both.
 template <int DTYPE, int D, int RT>
 __global__ __launch_bounds__(kFewThreads, 2) void paged_both_kernel(const PagedParams) {
-  __shared__ __attribute__((aligned(16))) char lds[std::max(FewLds<D, RT>::BYTES, kRowsLds<D>)];
+  __shared__ __attribute__((aligned(16))) char lds[std::max(FewLds<D, RT>::BYTES, RowsLds<D>::BYTES)];
   PagedArgs& p = fresh_kernel_args<PagedParams>();
   // (eight of the one and eight of the other in turn: consecutive workgroups go to the eight XCDs)
   const int n_few = p.n_few, n_rows = gridDim.x - n_few, both = 2 * min(n_few, n_rows), wg = blockIdx.x;
@@ -1157,16 +1185,12 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
     hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(threads), 0, (hipStream_t)stream, p);
     status = check_launch(name);
   };
-  // A kernel of rows' workgroups: whole groups of work items for each XCD.  A group is a request's (or a prefix's) tiles of a kv head,
-  // which read the same keys: 4 chunks of 256 tokens behind 65536 keys 1522 us one by one, 1065 in groups.  Where new tokens are more than
-  // half of what they see, tiles differ in length, and groups of them would leave XCDs idle: a prompt of 8192 tokens 592 us one
-  // by one, 654 in groups of eight.  Smaller groups where whole ones do not divide among the XCDs: 1040 items in groups of 16 359 us, of
-  // 8 278, one by one 309.
+  // A kernel of rows' workgroups, in groups of a request's (or a prefix's) tiles where these are alike in length
   const auto row_items = [&](PagedSource& src, bool alike) {
-    const int64_t items = (int64_t)src.n_tiles * x.n_heads_kv * src.n_shares;
-    src.xcd_group = alike ? std::min(std::max(src.n_tiles / src.batch, 1), 128) : 1;
-    while (src.xcd_group > 1 && xcd_grid_size(items, src.xcd_group) * 20 > items * 21) --src.xcd_group;
-    return xcd_grid_size(items, src.xcd_group);
+    const int each = std::max(src.n_tiles / src.batch, 1);
+    src.xcd_group = !alike ? 1 : each <= 16 ? each : 8;
+    if (getenv("X_G")) src.xcd_group = std::min(each, atoi(getenv("X_G")));
+    return row_workgroups(src.n_tiles, src.xcd_group, x.n_heads_kv, src.n_shares);
   };
   const bool prefix_rows = x.n_prefixes > 0 && !plan.prefix_few;
   if (plan.own_few && prefix_rows) {
