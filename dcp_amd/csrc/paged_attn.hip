@@ -1055,9 +1055,10 @@ struct PagedPlan {
 static int64_t seen_keys(const dcp_paged_attn_args& x) {
   return x.window > 0 ? std::min<int64_t>(x.max_seqlen_k, (int64_t)x.max_seqlen_q + x.window + x.n_starting) : x.max_seqlen_k;
 }
-// Row tiles of one kv head: every request may have a partial one.
+// Row tiles of one kv head: every request may have a partial one.  (Of the last one, tile floor(first_row / 128) + batch - 1 + i with
+// i < ceil(rows / 128).)
 static int64_t row_tiles(const dcp_paged_attn_args& x, int batch) {
-  return (int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) / kRowsBM + batch;
+  return ((int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) - 1) / kRowsBM + batch;
 }
 // Shares of a tile's keys, so that the launch has `rounds` rounds of the device's workgroups.
 static int row_shares(const dcp_paged_attn_args& x, int batch, int64_t max_keys, int rounds) {
