@@ -925,16 +925,16 @@ __global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedPa
   paged_few<DTYPE, D, RT>(blockIdx.x, lds);
 }
 
-// Prefixes of many rows and the requests' own keys in one launch: the former are bound by the matrix instructions, the
-// latter by memory, so a CU takes a workgroup of each, as long as there are both.
+// The requests' own keys and prefixes of many rows in one launch: a workgroup of the one starts where one of the other has ended, without
+// a kernel's end and another's start between them.  (Few rows first: 64 requests on a prefix of 32768 81 us, last 85, eight
+// workgroups of each in turn 83; on one of 131072 194, 196 and 236: dealt in turn to XCDs that are full, workgroups leave slots empty.)
 template <int DTYPE, int D, int RT>
 __global__ __launch_bounds__(kFewThreads, 2) void paged_both_kernel(const PagedParams) {
   __shared__ __attribute__((aligned(16))) char lds[std::max(FewLds<D, RT>::BYTES, RowsLds<D>::BYTES)];
   PagedArgs& p = fresh_kernel_args<PagedParams>();
-  // (eight of the one and eight of the other in turn: consecutive workgroups go to the eight XCDs)
-  const int n_few = p.n_few, n_rows = gridDim.x - n_few, both = 2 * min(n_few, n_rows), wg = blockIdx.x;
-  const bool few = wg < both ? (wg & kNumXcd) != 0 : n_few > n_rows;
-  const int i = wg < both ? wg / (2 * kNumXcd) * kNumXcd + wg % kNumXcd : wg - both / 2;
+  const int n_few = p.n_few, wg = blockIdx.x;
+  const bool few = wg < n_few;
+  const int i = few ? wg : wg - n_few;
   if (few) paged_few<DTYPE, D, RT>(i, lds);
   else paged_rows<DTYPE, D>(p, p.prefix, i, lds);
 }
