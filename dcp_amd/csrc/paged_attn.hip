@@ -38,7 +38,7 @@ struct PagedSource {
   int table_width, batch;    // of prefixes or requests
   int first_share, n_shares; // see PagedParams::partial_out
   int n_tiles, xcd_group;    // row tiles of a kv head (kernel of rows); as many neighbouring work items are on one XCD
-  int by_few;                // the kernel of few rows takes it
+  int by_few;                // the kernel of few rows takes it and may cut it (own keys)
 };
 
 struct PagedParams {
@@ -61,12 +61,13 @@ struct PagedParams {
   // the sum of the weights.  The own keys have shares [0, own.n_shares), the prefixes those that follow.
   float* partial_out;
   f32x2* partial_sums;
-  // The kernel of few rows: pieces of the units that are cut between workgroups, and where a row's pieces are (cut_of), for the own
-  // keys and for the prefixes: [2][token][q head]
+  // The kernel of few rows: pieces of the units that are cut between workgroups, and where a row's pieces are (cut_of):
+  // [token][q head]
   int2* cuts;
   float* slot_out;   // [workgroup][2][head of the workgroup][rows][D]
   f32x2* slot_sums;  // [workgroup][2][head of the workgroup][rows]
-  int few_rows, few_heads_log2;  // rows of a unit; kv heads a workgroup takes at once: 1, 2 or 4, with 4, 2 or 1 waves each
+  int few_rows, few_heads_log2;  // rows of a unit; kv heads a workgroup takes at once: 1, 2 or 4
+  int few_whole;                 // a workgroup takes a unit
   int n_few;                // workgroups
 };
 typedef KernArgs<PagedParams> PagedArgs;
@@ -512,9 +513,10 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 }
 
 // ---------------------------------------------------------------------------
-// The kernel of few rows: the waves of a workgroup share no tile.  Each takes tiles of 32 keys of its own, K straight into registers
-// in the layout of the product, V into its own part of LDS, both a tile ahead, and waits for nobody until its share of the
-// keys is done: 8 waves a CU with 16 KiB under way each.
+// The kernel of few rows: the waves of a workgroup share no tile.  Each takes tiles of 32 keys of its own, K and V into its own part of
+// LDS, and waits for nobody until its share of the keys is done.  (K straight into registers, in the layout of the product,
+// takes no LDS and no reads of it, but its 16 lanes of a row's end lie in 16 rows: a CU's loads went at a fifth of its rate, a tile took a
+// lone workgroup 3.5 us instead of 2.3, and all of them 2-10 % more.)
 //
 // Work is cut by length, not by request: the tiles of all (request, rows, kv heads) units, and of the prefixes' where they have few
 // rows, are laid end to end and every workgroup takes the same number of them, whatever the lengths are (they are known on
@@ -522,30 +524,32 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 // workgroup's slot (0: the share begins in the unit, 1: it ends in it) and the merge joins them.
 //
 // Several kv heads at once: in a cache by token ([page][token][head]) a head's row is 256 bytes, and four heads' waves
-// side by side read 1 KiB of a token at about the same time: four contexts of 131072 keys 382 -> 339 us, and nothing changes in a cache by head.
+// side by side read 1 KiB of a token at about the same time: four contexts of 131072 keys 382 -> 339 us (in a cache by head 326 and 334).
 // With few tiles a workgroup the waves take turns at one head's tiles instead, which makes the chain of tiles shorter.
 // ---------------------------------------------------------------------------
 // What the merge needs to know of a row: the workgroup that begins its unit, how many the unit is cut over, the slot of the first
 // piece (the others are in slot 0) and the row in the slots.
 __device__ __forceinline__ int2 cut_of(int wg, int n_pieces, int slot, int row) { return int2{wg, n_pieces | row << 20 | slot << 28}; }
-constexpr int kFewThreads = 256, kFewWaves = 4, kFewBN = 32;
+constexpr int kFewBN = 32;
 constexpr int kFewMaxBatch = 1 << 16;
 
 // What request b is to the kernel.
 struct FewRequest {
   int first_tok, n_tok, n_keys, n_tiles;
-  __device__ __forceinline__ KeyGroups groups(PagedArgs& p, bool prefix) const {
-    return KeyGroups(prefix ? 0 : p.window, p.n_starting, prefix ? 0 : max(n_keys - n_tok, 0), n_keys - 1);
+  __device__ __forceinline__ KeyGroups groups(PagedArgs& p) const {
+    return KeyGroups(p.window, p.n_starting, max(n_keys - n_tok, 0), n_keys - 1);
   }
   __device__ __forceinline__ FewRequest() {}
-  __device__ __forceinline__ FewRequest(PagedArgs& p, SourceArgs& src, int b) {
-    const TokenRange tokens = tokens_of(p, src, b);
+  __device__ __forceinline__ FewRequest(PagedArgs& p, int b) {
+    const TokenRange tokens = tokens_of(p, p.own, b);
     first_tok = tokens.begin;
     n_tok = tokens.n;
-    n_keys = keys_of(p, src, b);
-    n_tiles = max((groups(p, src.cu_groups != nullptr).count() + 1) / 2, 1);  // (a request without keys has its rows written all the same)
+    n_keys = keys_of(p, p.own, b);
+    n_tiles = max((groups(p).count() + 1) / 2, 1);  // (a request without keys has its rows written all the same)
   }
-  __device__ __forceinline__ int work(PagedArgs& p, int rows, int head_groups) const { return (n_tok * p.group + rows - 1) / rows * head_groups * n_tiles; }
+  __device__ __forceinline__ int units(PagedArgs& p, int rows) const {
+    return (n_tok * p.group + rows - 1) / rows * (p.n_heads_kv >> p.few_heads_log2);
+  }
   __device__ __forceinline__ FewRequest of_lane(int lane) const {
     FewRequest r;
     r.first_tok = __builtin_amdgcn_readlane(first_tok, lane);
@@ -573,53 +577,50 @@ __device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
 
 // LDS of the kernel.  V of 32 keys: load r of a tile brings rows r, r + LOADS, ... side by side (1 KiB), 32 bytes of padding between
 // loads: eight consecutive rows then lie in eight different 32-byte bank windows for the transposing reads.
-template <int D, int RT>
+template <int D, int RT, int NW>
 struct FewLds {
   static constexpr int ROWS = 16 * RT, LOADS = kFewBN * D * 2 / 1024, LOAD_BYTES = 1024 + 32, STAGE = LOADS * LOAD_BYTES;
   static constexpr int O_STRIDE = D + 4;  // floats: rows of a wave's result, which takes the place of its V
   static constexpr int WAVE = 2 * STAGE > ROWS * O_STRIDE * 4 ? 2 * STAGE : ROWS * O_STRIDE * 4;
-  static constexpr int SUMS = kFewWaves * WAVE;                  // float [wave][row][2]
-  static constexpr int CHUNKS = SUMS + kFewWaves * ROWS * 2 * 4; // int [batch / 64]
-  static constexpr int BYTES = CHUNKS + 2 * kFewMaxBatch / 64 * 4;
+  static constexpr int SUMS = NW * WAVE;                  // float [wave][row][2]
+  static constexpr int CHUNKS = SUMS + NW * ROWS * 2 * 4; // int [batch / 64]
+  static constexpr int BYTES = CHUNKS + kFewMaxBatch / 64 * 4;
 };
 
-template <int DTYPE, int D, int RT>
+template <int DTYPE, int D, int RT, int NW>
 __device__ __forceinline__ void paged_few(int wg, char* lds) {
   // (the arguments are read anew wherever another part of the work begins: kept in scalar registers throughout they do not fit)
   PagedArgs& p0 = fresh_kernel_args<PagedParams>();
-  typedef FewLds<D, RT> Lds;
+  typedef FewLds<D, RT, NW> Lds;
   constexpr int KS = D / 32, DT = D / 16, ROWS = Lds::ROWS, LOADS = Lds::LOADS;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   float(*sums)[ROWS][2] = reinterpret_cast<float(*)[ROWS][2]>(lds + Lds::SUMS);
   int* chunk_sums = reinterpret_cast<int*>(lds + Lds::CHUNKS);
 
-  // ---- this workgroup's share of all tiles (the host has checked that their number fits 32 bits) ------------------------
-  // The list: the requests, padded to 64, and the prefixes behind them.
-  const int n_chunks = (p0.own.batch + 63) / 64 + (p0.prefix.by_few ? (p0.prefix.batch + 63) / 64 : 0);
-  auto own_chunks = [](PagedArgs& p) { return (p.own.batch + 63) / 64; };
-  auto source_of = [&](PagedArgs& p, int chunk) -> SourceArgs* { return chunk < own_chunks(p) ? &p.own : &p.prefix; };
+  // ---- this workgroup's share of all tiles (the host has checked that their number fits 32 bits), or its unit -----------
+  const int n_chunks = (p0.own.batch + 63) / 64;
+  const bool whole_units = p0.few_whole != 0;
   auto requests_of = [&](int chunk, int& work) {
     PagedArgs& p = fresh_kernel_args<PagedParams>();
-    SourceArgs& src = *source_of(p, chunk);
-    const int b = (chunk < own_chunks(p) ? chunk : chunk - own_chunks(p)) * 64 + lane;
+    const int b = chunk * 64 + lane;
     FewRequest r;
     r.first_tok = r.n_tok = r.n_keys = 0;
     r.n_tiles = 1;
     work = 0;
-    if (b < src.batch) {
-      r = FewRequest(p, src, b);
-      work = r.work(p, ROWS, p.n_heads_kv >> p.few_heads_log2);
+    if (b < p.own.batch) {
+      r = FewRequest(p, b);
+      work = r.units(p, ROWS) * (whole_units ? 1 : r.n_tiles);
     }
     return r;
   };
   int total = 0, before = 0, chunk = 0, work;
   FewRequest requests = requests_of(0, work);
-  int scan = wave_scan(work);  // the chunk's tiles up to and with the lane's request
+  int scan = wave_scan(work);  // the chunk's tiles (or units) up to and with the lane's request
   if (n_chunks == 1) {
     total = __builtin_amdgcn_readlane(scan, 63);
   } else {
-    for (int i = w; i < n_chunks; i += kFewWaves) {
+    for (int i = w; i < n_chunks; i += NW) {
       int more;
       requests_of(i, more);
       more = wave_scan(more);
@@ -628,7 +629,7 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
     __syncthreads();
     for (int i = 0; i < n_chunks; i += 64) total += __builtin_amdgcn_readlane(wave_scan(i + lane < n_chunks ? chunk_sums[i + lane] : 0), 63);
   }
-  const int per = max((total - 1) / p0.n_few + 1, kFewWaves >> p0.few_heads_log2);
+  const int per = whole_units ? 1 : max((total - 1) / p0.n_few + 1, NW >> p0.few_heads_log2);
   const int begin = (int)min((int64_t)wg * per, (int64_t)total), end = (int)min((int64_t)begin + per, (int64_t)total);
   if (begin >= end) return;
   if (n_chunks > 1) {
@@ -645,8 +646,8 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
   }
   int index = __builtin_amdgcn_readfirstlane(min(__popcll(__ballot(before + scan <= begin)), 63));  // in the chunk
 
-  const uint32_t v_at = lds_address(lds) + w * Lds::WAVE;
-  char* v_lds = lds + w * Lds::WAVE;
+  char* my_lds = lds + w * Lds::WAVE;  // K of a tile and V of a tile
+  const uint32_t k_at = lds_address(lds) + w * Lds::WAVE, v_at = k_at + Lds::STAGE;
   int at = begin;
   while (at < end) {
     if (index == 64) {
@@ -662,76 +663,63 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
       continue;
     }
     PagedArgs& p = fresh_kernel_args<PagedParams>();
-    SourceArgs& src = *source_of(p, chunk);
-    const bool prefix = src.cu_groups != nullptr;
     // the workgroup's kv heads at once, the waves that take turns at a head's tiles, and which of each the wave is
-    const int heads = 1 << p.few_heads_log2, head_groups = p.n_heads_kv >> p.few_heads_log2, turns = kFewWaves >> p.few_heads_log2;
+    const int heads = 1 << p.few_heads_log2, head_groups = p.n_heads_kv >> p.few_heads_log2, turns = NW >> p.few_heads_log2;
     const int my_head = w & (heads - 1), my_turn = w >> p.few_heads_log2;
     const FewRequest request = requests.of_lane(index);
-    const int b = (chunk < own_chunks(p) ? chunk : chunk - own_chunks(p)) * 64 + index;
-    const int in_request = at - (unit_end - __builtin_amdgcn_readlane(work, index));
-    const int unit = __builtin_amdgcn_readfirstlane(in_request / request.n_tiles);
-    const int t_begin = in_request - unit * request.n_tiles, t_end = min(request.n_tiles, t_begin + (end - at));
-    at += t_end - t_begin;
+    const int b = chunk * 64 + index, in_request = at - (unit_end - __builtin_amdgcn_readlane(work, index));
+    const int unit = whole_units ? in_request : __builtin_amdgcn_readfirstlane(in_request / request.n_tiles);
+    const int t_begin = whole_units ? 0 : in_request - unit * request.n_tiles;
+    const int t_end = whole_units ? request.n_tiles : min(request.n_tiles, t_begin + (end - at));
+    const int taken = whole_units ? 1 : t_end - t_begin;
+    at += taken;
     const int kv_head0 = unit % head_groups * heads, kv_head = kv_head0 + my_head, row0 = unit / head_groups * ROWS;
-    const KeyGroups groups = request.groups(p, prefix);
+    const KeyGroups groups = request.groups(p);
     const int n_groups = request.n_keys > 0 ? groups.count() : 0, n_rows = request.n_tok * p.group;
 
     // ---- where the wave's next 32 tiles are: lane 2 i + j holds the 16-key group j of the i-th of them ------------
-    const uint16_t* k_base = reinterpret_cast<const uint16_t*>(p.k) + kv_head * p.head_stride;
-    const uint16_t* v_base = reinterpret_cast<const uint16_t*>(p.v) + kv_head * p.head_stride;
     int64_t lane_off = 0;
     int lane_key = kNoKey;
     auto look_up = [&](int step) {
       PagedArgs& p = fresh_kernel_args<PagedParams>();
-      SourceArgs& src = *source_of(p, chunk);
       const int group = 2 * (t_begin + my_turn + turns * (step + (lane >> 1))) + (lane & 1);
       lane_off = 0;
       lane_key = kNoKey;
       if (group < n_groups && group < 2 * t_end) {
         const int key = groups.at(group) * 16, entry = key / p.page_size;
-        const int page = src.block_table[b * src.table_stride + entry];
+        const int page = p.own.block_table[b * p.own.table_stride + entry];
         if ((unsigned)page < (unsigned)p.n_pages) {
           lane_key = key;
           lane_off = page * p.page_stride + (int64_t)(key - entry * p.page_size) * p.token_stride;
         }
       }
     };
-    // what a lane brings of a tile: K of key n of each group, 8 elements from 32 ks + 8 g; V rows of its half's group
+    // what a lane brings of a tile's K and V: a piece of LOADS rows of its half's group
     constexpr int CH = D / 8;
-    const int64_t k_lane = n * p.token_stride + 8 * g;
-    const int v_row = lane / CH % (16 / LOADS) * LOADS;  // of load 0, in the group of the lane's half
-    const int64_t v_lane = v_row * p.token_stride + lane % CH * 8, token_stride = p.token_stride;
+    const int lane_row = lane / CH % (16 / LOADS) * LOADS;  // of load 0
+    const int64_t token_stride = p.token_stride;
+    const uint16_t* k_lane = reinterpret_cast<const uint16_t*>(p.k) + (kv_head * p.head_stride + lane_row * token_stride + lane % CH * 8);
+    const int64_t v_from_k = reinterpret_cast<const uint16_t*>(p.v) - reinterpret_cast<const uint16_t*>(p.k);
     const int n_steps = n_groups > 0 && t_begin + my_turn < t_end ? (t_end - t_begin - my_turn + turns - 1) / turns : 0;
-    u32x4 k[2][KS];  // K of the tile at hand, and once its products are formed of the next one
-    int64_t off[2];  // where its two groups are
+    int64_t off = 0;  // where the lane's group of the next tile is
     int next_key[2], tile_key[2];
     auto place = [&](int step) {
       if (step % 32 == 0) look_up(step);
       const int from = 2 * (step % 32);
+      const int64_t off0 = lane_value(lane_off, from), off1 = lane_value(lane_off, from + 1);
+      off = lane >= 32 ? off1 : off0;
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        off[kt] = lane_value(lane_off, from + kt);
-        next_key[kt] = __builtin_amdgcn_readlane(lane_key, from + kt);
-      }
+      for (int kt = 0; kt < 2; ++kt) next_key[kt] = __builtin_amdgcn_readlane(lane_key, from + kt);
     };
-    auto issue_v = [&](int stage) {
-      const uint16_t* v = v_base + (lane >= 32 ? off[1] : off[0]) + v_lane;
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's last reads are done
+    auto issue = [&](uint32_t at, int64_t from_k) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of what is there are done
 #pragma unroll
-      for (int r = 0; r < LOADS; ++r) load_async_piece<true>(v_at + stage * Lds::STAGE + r * Lds::LOAD_BYTES, v + r * token_stride);
-    };
-    auto issue_k = [&]() {
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          k[kt][ks] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k_base + off[kt] + k_lane + 32 * ks));
+      for (int r = 0; r < LOADS; ++r) load_async_piece<true>(at + r * Lds::LOAD_BYTES, k_lane + off + (from_k + r * token_stride));
     };
     if (n_steps > 0) {
       place(0);
-      issue_v(0);
-      issue_k();
+      issue(k_at, 0);
+      issue(v_at, v_from_k);
     }
 
     // ---- this lane's rows --------------------------------------------------------------
@@ -748,8 +736,8 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
         q[rt][ks] = u32x4{0, 0, 0, 0};
         if (live) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + 32 * ks);
       }
-      last_key[rt] = !live ? 0x7fffffff : prefix ? request.n_keys - 1 : request.n_keys - request.n_tok + tok;
-      first_key[rt] = live && p.window > 0 && !prefix ? max(last_key[rt] - p.window + 1, 0) : 0;
+      last_key[rt] = live ? request.n_keys - request.n_tok + tok : 0x7fffffff;
+      first_key[rt] = live && p.window > 0 ? max(last_key[rt] - p.window + 1, 0) : 0;
       w_last = min(w_last, wave_min(last_key[rt]));
       w_first = max(w_first, wave_max(first_key[rt]));
     }
@@ -763,43 +751,37 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
       for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int v_rd = ((4 * g + (n >> 2)) % LOADS) * Lds::LOAD_BYTES + ((4 * g + (n >> 2)) / LOADS) * (D * 2) + 8 * (n & 3);
+    auto row_at = [](int row) { return row % LOADS * Lds::LOAD_BYTES + row / LOADS * (D * 2); };  // 16 rows further: 512 bytes
+    const int k_rd = row_at(n) + 16 * g, v_rd = row_at(4 * g + (n >> 2)) + 8 * (n & 3);
     for (int step = 0; step < n_steps; ++step) {
-      const int stage = step & 1;
-      wait_loads();
+      // K and V of the next tile are asked for as soon as those of this one have been read, and waited for on their own: under
+      // way are K of a tile while V is at work and V while K is.
+      __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS);  // all loads but the last LOADS, which are V's
       asm volatile("" ::: "memory");
-      tile_key[0] = next_key[0];
-      tile_key[1] = next_key[1];
       const bool more = step + 1 < n_steps;
-      if (more) {
-        place(step + 1);
-        issue_v(stage ^ 1);
-      }
       bool whole = true, full = true;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        const int key = tile_key[kt];
+        const int key = tile_key[kt] = next_key[kt];
         whole = whole & groups.sees_all_of_16(key);
         full = full & (key + 15 <= w_last) & ((key >= w_first) | (key + 15 < p.n_starting));
       }
-      if (!whole) {
-        const int key0 = lane >= 32 ? tile_key[1] : tile_key[0];
-#pragma unroll
-        for (int r = 0; r < LOADS; ++r)
-          if (!((key0 != kNoKey) & groups.sees(key0 + v_row + r)))
-            *reinterpret_cast<u32x4*>(v_lds + stage * Lds::STAGE + r * Lds::LOAD_BYTES + 16 * lane) = u32x4{0, 0, 0, 0};
-        asm volatile("" ::: "memory");
-      }
       f32x4 s[RT][2];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int kt = 0; kt < 2; ++kt) {
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          s[rt][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int ks = 0; ks < KS; ++ks) s[rt][kt] = mfma_16x16x32<DTYPE>(k[kt][ks], q[rt][ks], s[rt][kt]);
+        for (int ks = 0; ks < KS; ++ks) {
+          const u32x4 a = *reinterpret_cast<const u32x4*>(my_lds + k_rd + 512 * kt + 64 * ks);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][kt] = mfma_16x16x32<DTYPE>(a, q[rt][ks], s[rt][kt]);
         }
-      if (more) issue_k();
+      }
+      if (more) {
+        place(step + 1);
+        issue(k_at, 0);
+      }
       if (!(whole & full)) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -844,22 +826,34 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
           pb[rt][2 * kt + 1] = pack2<DTYPE>(x[2], x[3]);
         }
       }
+      if (more) __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS);  // (the last LOADS are the next K)
+      else wait_loads();
+      asm volatile("" ::: "memory");
+      if (!whole) {
+        const int key0 = lane >= 32 ? tile_key[1] : tile_key[0];
+#pragma unroll
+        for (int r = 0; r < LOADS; ++r)
+          if (!((key0 != kNoKey) & groups.sees(key0 + lane_row + r)))
+            *reinterpret_cast<u32x4*>(my_lds + Lds::STAGE + r * Lds::LOAD_BYTES + 16 * lane) = u32x4{0, 0, 0, 0};
+        asm volatile("" ::: "memory");
+      }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) {
         typedef short s16x4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const uint32_t from = v_at + stage * Lds::STAGE + v_rd + 32 * dt;
+        const uint32_t from = v_at + v_rd + 32 * dt;
         const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)from));
-        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(from + 512)));  // rows 16 further
+        const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(uintptr_t)(from + 512)));
         const u32x4 a = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) o[rt][dt] = mfma_16x16x32<DTYPE>(a, pb[rt], o[rt][dt]);
       }
+      if (more) issue(v_at, v_from_k);
     }
 
     // ---- the waves' results joined --------------------------------------------------
     asm volatile("" ::: "memory");
-    float* mine = reinterpret_cast<float*>(v_lds);
+    float* mine = reinterpret_cast<float*>(my_lds);
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float l = rows_sum(l_run[rt]);
@@ -873,19 +867,19 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
     __syncthreads();
     PagedArgs& p_out = fresh_kernel_args<PagedParams>();
     const bool cut = t_end - t_begin < request.n_tiles;
-    const int slot = at - (t_end - t_begin) == begin ? 0 : 1;
-    const int n_cut = (at - t_end + request.n_tiles - 1) / per - wg + 1;  // (of a unit that begins here: it ends so many workgroups on)
+    const int slot = at - taken == begin ? 0 : 1;
+    const int n_cut = (at - taken + request.n_tiles - 1) / per - wg + 1;  // (of a unit that begins here: it ends so many workgroups on)
     const int group = p_out.group;
     constexpr int PIECES = D / 4;  // of a row
-    for (int i = tid; i < heads * ROWS * PIECES; i += kFewThreads) {
+    for (int i = tid; i < heads * ROWS * PIECES; i += NW * 64) {
       const int piece = i % PIECES, row = i / PIECES % ROWS, of = i / PIECES / ROWS, r = row0 + row;
       if (r >= n_rows) continue;
       float m = -INFINITY;
-      for (int x = of; x < kFewWaves; x += heads) m = fmaxf(m, sums[x][row][0]);
+      for (int x = of; x < NW; x += heads) m = fmaxf(m, sums[x][row][0]);
       const float m_use = m == -INFINITY ? 0.0f : m;
       f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
       float l = 0.0f;
-      for (int x = of; x < kFewWaves; x += heads) {
+      for (int x = of; x < NW; x += heads) {
         const float weight = fast_exp2(sums[x][row][0] - m_use);
         l += weight * sums[x][row][1];
         const f32x4 o4 = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * Lds::WAVE) + row * Lds::O_STRIDE + 4 * piece);
@@ -893,14 +887,13 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
         for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
       }
       const int64_t token = request.first_tok + r / group, head = (kv_head0 + of) * group + r % group;
-      if ((piece == 0) & (t_begin == 0))
-        p_out.cuts[((int64_t)(prefix ? p_out.n_tokens : 0) + token) * p_out.n_heads_q + head] = cut_of(wg, n_cut, slot, of * ROWS + row);
+      if ((piece == 0) & (t_begin == 0) & !whole_units) p_out.cuts[token * p_out.n_heads_q + head] = cut_of(wg, n_cut, slot, of * ROWS + row);
       if (cut) {
         const int64_t to = (((int64_t)wg * 2 + slot) * heads + of) * ROWS + row;
         *reinterpret_cast<f32x4*>(p_out.slot_out + to * D + 4 * piece) = acc;
         if (piece == 0) p_out.slot_sums[to] = f32x2{m, l};
       } else if (!p_out.direct) {
-        const int64_t to = ((int64_t)source_of(p_out, chunk)->first_share * p_out.n_tokens + token) * p_out.n_heads_q + head;
+        const int64_t to = ((int64_t)p_out.own.first_share * p_out.n_tokens + token) * p_out.n_heads_q + head;
         *reinterpret_cast<f32x4*>(p_out.partial_out + to * D + 4 * piece) = acc;
         if (piece == 0) p_out.partial_sums[to] = f32x2{m, l};
       } else {
@@ -919,28 +912,28 @@ __global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const Paged
   paged_rows<DTYPE, D>(p, p.own, blockIdx.x, lds);
 }
 
-template <int DTYPE, int D, int RT>
-__global__ __launch_bounds__(kFewThreads, 2) void paged_few_kernel(const PagedParams) {
-  __shared__ __attribute__((aligned(16))) char lds[FewLds<D, RT>::BYTES];
-  paged_few<DTYPE, D, RT>(blockIdx.x, lds);
+template <int DTYPE, int D, int RT, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void paged_few_kernel(const PagedParams) {
+  __shared__ __attribute__((aligned(16))) char lds[FewLds<D, RT, NW>::BYTES];
+  paged_few<DTYPE, D, RT, NW>(blockIdx.x, lds);
 }
 
 // The requests' own keys and prefixes of many rows in one launch: a workgroup of the one starts where one of the other has ended, without
 // a kernel's end and another's start between them.  (Few rows first: 64 requests on a prefix of 32768 81 us, last 85, eight
 // workgroups of each in turn 83; on one of 131072 194, 196 and 236: dealt in turn to XCDs that are full, workgroups leave slots empty.)
 template <int DTYPE, int D, int RT>
-__global__ __launch_bounds__(kFewThreads, 2) void paged_both_kernel(const PagedParams) {
-  __shared__ __attribute__((aligned(16))) char lds[std::max(FewLds<D, RT>::BYTES, RowsLds<D>::BYTES)];
+__global__ __launch_bounds__(256, 2) void paged_both_kernel(const PagedParams) {
+  __shared__ __attribute__((aligned(16))) char lds[std::max(FewLds<D, RT, 4>::BYTES, RowsLds<D>::BYTES)];
   PagedArgs& p = fresh_kernel_args<PagedParams>();
   const int n_few = p.n_few, wg = blockIdx.x;
   const bool few = wg < n_few;
   const int i = few ? wg : wg - n_few;
-  if (few) paged_few<DTYPE, D, RT>(i, lds);
+  if (few) paged_few<DTYPE, D, RT, 4>(i, lds);
   else paged_rows<DTYPE, D>(p, p.prefix, i, lds);
 }
 
-// The merge: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's parts, rounded once.  The parts are, of the own keys and
-// of a prefix each, the pieces of a unit that the kernel of few rows has cut, or shares.  A workgroup takes a row: D / 4
+// The merge: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's parts, rounded once.  The parts are the pieces
+// of a unit that the kernel of few rows has cut, or shares of the own keys, and the shares of a prefix.  A workgroup takes a row: D / 4
 // lanes hold it in 16-byte pieces, and the 1024 / D sets of such lanes take parts in turn (a wave that went through 128
 // parts alone took 17 us).
 constexpr int kPagedMergeThreads = 256;
@@ -963,25 +956,20 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   // (& on purpose: of two conditions joined by && or || here, this compiler, clang 22, left the second one out)
   if ((token < first) | (token >= end)) return;
   const bool has_prefix = (token >= prefix_first) & (token < prefix_end);
-  int2 own = {0, 1}, pre = {0, 1};
-  if (p.own.by_few) own = p.cuts[row];
-  if (has_prefix & (p.prefix.by_few != 0)) pre = p.cuts[n_rows + row];
-  const int own_cut = (own.y & 0xfffff) > 1 ? own.y & 0xfffff : 0, pre_cut = (pre.y & 0xfffff) > 1 ? pre.y & 0xfffff : 0;
-  if ((p.own.by_few != 0) & (own_cut == 0) & (p.direct != 0)) return;  // done where it was computed
-  const int n_own = own_cut > 0 ? own_cut : p.own.n_shares;
-  const int n_parts = n_own + (has_prefix ? (pre_cut > 0 ? pre_cut : p.prefix.n_shares) : 0);
+  int2 cut = {0, 1};
+  if (p.own.by_few) cut = p.cuts[row];
+  const int n_cut = (cut.y & 0xfffff) > 1 ? cut.y & 0xfffff : 0;
+  if ((p.own.by_few != 0) & (n_cut == 0) & (p.direct != 0)) return;  // done where it was computed
+  const int n_own = n_cut > 0 ? n_cut : p.own.n_shares, n_parts = n_own + (has_prefix ? p.prefix.n_shares : 0);
   const int slot_rows = p.few_rows << p.few_heads_log2;
   // where part i is
   auto part = [&](int i, const f32x2*& sums) -> const float* {
-    const bool of_prefix = i >= n_own;
-    const int j = of_prefix ? i - n_own : i;
-    const int2 cut = of_prefix ? pre : own;
-    if ((of_prefix ? pre_cut : own_cut) > 0) {
-      const int64_t at = ((int64_t)(cut.x + j) * 2 + (j == 0 ? cut.y >> 28 : 0)) * slot_rows + (cut.y >> 20 & 0xff);
+    if (i < n_cut) {
+      const int64_t at = ((int64_t)(cut.x + i) * 2 + (i == 0 ? cut.y >> 28 : 0)) * slot_rows + (cut.y >> 20 & 0xff);
       sums = p.slot_sums + at;
       return p.slot_out + at * D;
     }
-    const int64_t at = (int64_t)(j + (of_prefix ? p.prefix.first_share : 0)) * n_rows + row;
+    const int64_t at = (int64_t)(i < n_own ? i : i - n_own + p.prefix.first_share) * n_rows + row;
     sums = p.partial_sums + at;
     return p.partial_out + at * D;
   };
@@ -1044,8 +1032,9 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
 
 // How a call is laid out: which kernel takes which keys, and what of the workspace is whose.
 struct PagedPlan {
-  bool own_few = false, prefix_few = false;
-  int rows = 16, heads = 1, n_few = 0;  // of the kernel of few rows: rows of a unit, kv heads of a workgroup, workgroups
+  bool few = false;    // the kernel of few rows takes the requests' own keys
+  bool whole = false;  // a workgroup (of 8 waves) takes a unit of it; otherwise one of 4 an equal share of all tiles
+  int rows = 16, heads = 1, n_few = 0;  // rows of a unit, kv heads of a workgroup, workgroups
   int n_own = 1, n_prefix = 0;          // shares
   size_t cuts = 0, slots = 0, shares = 0;  // bytes
   size_t bytes() const { return cuts + slots + shares; }
@@ -1074,31 +1063,33 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
   const auto up16 = [](size_t n) { return (n + 15) / 16 * 16; };
   const int group = x.n_heads_q / x.n_heads_kv;
   const int64_t keys = seen_keys(x);
-  // The kernel of few rows: of requests with up to 32, and of prefixes whose requests have that many together.  Its sums of
-  // tiles have to fit 32 bits whatever the lengths are.
+  // The kernel of few rows: of requests with up to 32.  Its sums of tiles have to fit 32 bits whatever the lengths are.
   const int64_t own_rows = (int64_t)x.max_seqlen_q * group, all_rows = (int64_t)x.n_tokens * group;
-  plan.own_few = own_rows <= 32;
-  plan.prefix_few = plan.own_few && x.n_prefixes > 0 && all_rows <= 32;
-  plan.rows = (plan.prefix_few ? all_rows : own_rows) <= 16 ? 16 : 32;
-  const auto most_tiles = [&](int batch, int width) {
-    return (double)(all_rows / plan.rows + batch) * x.n_heads_kv * ((double)width * x.page_size / kFewBN + 2);
-  };
-  if (most_tiles(x.batch, x.table_width) + (plan.prefix_few ? most_tiles(x.n_prefixes, x.prefix_width) : 0) > 2e9 ||
-      std::max(x.batch, x.n_prefixes) > kFewMaxBatch)
-    plan.own_few = plan.prefix_few = false;
-  if (plan.own_few) {
-    plan.n_few = 2 * device_cu_count();
-    // four heads at once from 64 tiles a workgroup on (16 for each wave): decode of 32 windows of 1016 keys, 16 tiles, 25.2 us with one
-    // head and 27.4 with four, 64 requests of up to 8192 keys, 256 tiles, 148 and 137
-    const int64_t tiles = ((int64_t)x.batch * ((keys + kFewBN - 1) / kFewBN) +
-                           (plan.prefix_few ? (int64_t)x.n_prefixes * ((x.max_prefix_len + kFewBN - 1) / kFewBN) : 0)) * x.n_heads_kv / plan.n_few;
-    plan.heads = tiles < 64 ? 1 : x.n_heads_kv % 4 == 0 ? 4 : x.n_heads_kv % 2 == 0 ? 2 : 1;
-    plan.cuts = up16((size_t)(plan.prefix_few ? 2 : 1) * x.n_tokens * x.n_heads_q * sizeof(int2));
-    plan.slots = (size_t)plan.n_few * 2 * plan.heads * plan.rows * (x.head_dim + 2) * sizeof(float);
+  plan.rows = own_rows <= 16 ? 16 : 32;
+  // (as many units as there can be, and about as many as there are)
+  const int64_t most_units = (all_rows + (int64_t)x.batch * (plan.rows - 1)) / plan.rows * x.n_heads_kv;
+  const int64_t units = std::max<int64_t>(x.batch, all_rows / plan.rows) * x.n_heads_kv;
+  plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2) < 2e9;
+  if (plan.few) {
+    // Whole units where every CU has at most one, and the chain of an eighth of its tiles (2.3 us each) is shorter than what cutting costs
+    // (a second kernel and more) and the equal shares take (of lengths that are half the longest on average, at 5.4 TB/s).  us, whole
+    // and cut: one request of 256 keys 7.3 and 9.8, of 1000 14.4 and 10.3; 32 of 1000 27.4 and 31.7, of up to 1024 20.2 and 24.4;
+    // 32 windows of 1016 keys, head size 64, 18.1 and 23.2; 16 of up to 2048 29.3 and 24.0; 64 of 256 20.8 and 19.4.
+    // Beside a prefix's shares, which are joined anyway, always as long as units are short: 64 requests on a prefix of 32768 80 and 87.
+    const double unit_us = keys * (2.3 / 256), all_us = 0.5 * units * keys * x.head_dim * 4 / 5.4e6;
+    plan.whole = keys <= 2048 && (x.n_prefixes > 0 || (units <= device_cu_count() && unit_us < 5 + all_us));
+    plan.n_few = plan.whole ? (int)most_units : 2 * device_cu_count();
+    // Four heads at once from 64 tiles a workgroup on (16 for each wave).
+    const int64_t tiles = (int64_t)x.batch * ((keys + kFewBN - 1) / kFewBN) * x.n_heads_kv / plan.n_few;
+    plan.heads = plan.whole || tiles < 64 ? 1 : x.n_heads_kv % 4 == 0 ? 4 : x.n_heads_kv % 2 == 0 ? 2 : 1;
+    if (!plan.whole) {
+      plan.cuts = up16((size_t)x.n_tokens * x.n_heads_q * sizeof(int2));
+      plan.slots = (size_t)plan.n_few * 2 * plan.heads * plan.rows * (x.head_dim + 2) * sizeof(float);
+    }
   } else {
     plan.n_own = row_shares(x, x.batch, keys, 2);
   }
-  if (x.n_prefixes > 0) plan.n_prefix = plan.prefix_few ? 1 : row_shares(x, x.n_prefixes, x.max_prefix_len, 1);
+  if (x.n_prefixes > 0) plan.n_prefix = row_shares(x, x.n_prefixes, x.max_prefix_len, 1);
   if (plan.n_own + plan.n_prefix > 1) plan.shares = (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
   return plan;
 }
@@ -1157,10 +1148,10 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
   p.cu_seqlens_q = x.cu_seqlens_q;
   p.q_token = x.q_token_stride; p.q_head = x.q_head_stride; p.out_token = x.out_token_stride; p.out_head = x.out_head_stride;
   p.page_stride = x.page_stride; p.token_stride = x.token_stride; p.head_stride = x.head_stride;
-  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_own, (int)row_tiles(x, x.batch), 1, plan.own_few};
+  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_own, (int)row_tiles(x, x.batch), 1, plan.few && !plan.whole};
   if (x.n_prefixes > 0)
     p.prefix = {x.prefix_table, x.prefix_lens, x.cu_groups, x.prefix_stride, x.prefix_width, x.n_prefixes, plan.n_own, plan.n_prefix,
-                (int)row_tiles(x, x.n_prefixes), 1, plan.prefix_few};
+                (int)row_tiles(x, x.n_prefixes), 1, 0};
   p.n_pages = x.n_pages; p.page_size = x.page_size;
   p.n_requests = x.batch; p.n_tokens = x.n_tokens;
   p.n_heads_q = x.n_heads_q; p.n_heads_kv = x.n_heads_kv; p.group = x.n_heads_q / x.n_heads_kv;
@@ -1173,7 +1164,7 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
   p.slot_sums = reinterpret_cast<f32x2*>(p.slot_out + (size_t)plan.n_few * 2 * plan.heads * plan.rows * x.head_dim);
   p.partial_out = reinterpret_cast<float*>(at + plan.cuts + plan.slots);
   p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * x.head_dim);
-  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.n_few = plan.n_few;
+  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.few_whole = plan.whole; p.n_few = plan.n_few;
 
   int status = DCP_OK;
   const auto launch = [&](auto kernel, const char* name, int64_t n_wg, int threads) {
@@ -1190,25 +1181,28 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
   const auto row_items = [&](PagedSource& src, bool alike) {
     const int each = std::max(src.n_tiles / src.batch, 1);
     src.xcd_group = !alike ? 1 : each <= 16 ? each : 8;
-    if (getenv("X_G")) src.xcd_group = std::min(each, atoi(getenv("X_G")));
     return row_workgroups(src.n_tiles, src.xcd_group, x.n_heads_kv, src.n_shares);
   };
-  const bool prefix_rows = x.n_prefixes > 0 && !plan.prefix_few;
-  if (plan.own_few && prefix_rows) {
-    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_both_kernel, 1), "paged_both_kernel", row_items(p.prefix, true) + p.n_few, kFewThreads);
-    else launch(DCP_PAGED_KERNEL(paged_both_kernel, 2), "paged_both_kernel", row_items(p.prefix, true) + p.n_few, kFewThreads);
-  } else if (plan.own_few) {
-    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1), "paged_few_kernel", p.n_few, kFewThreads);
-    else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2), "paged_few_kernel", p.n_few, kFewThreads);
+  const bool alike = 2 * (int64_t)x.max_seqlen_q <= seen_keys(x);
+  if (plan.few && x.n_prefixes > 0) {
+    const int64_t n_wg = row_items(p.prefix, true) + p.n_few;
+    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_both_kernel, 1), "paged_both_kernel", n_wg, 256);
+    else launch(DCP_PAGED_KERNEL(paged_both_kernel, 2), "paged_both_kernel", n_wg, 256);
+  } else if (plan.few && plan.whole) {
+    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1, 8), "paged_few_kernel", p.n_few, 512);
+    else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2, 8), "paged_few_kernel", p.n_few, 512);
+  } else if (plan.few) {
+    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1, 4), "paged_few_kernel", p.n_few, 256);
+    else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2, 4), "paged_few_kernel", p.n_few, 256);
   } else {
-    launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own, 2 * (int64_t)x.max_seqlen_q <= seen_keys(x)), kRowsThreads);
-    if (prefix_rows) {
+    launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own, alike), kRowsThreads);
+    if (x.n_prefixes > 0) {
       std::swap(p.own, p.prefix);  // (the kernel takes what it finds there)
       launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own, true), kRowsThreads);
       std::swap(p.own, p.prefix);
     }
   }
-  if (plan.own_few || !p.direct) launch(DCP_PAGED_KERNEL(paged_merge_kernel), "paged_merge_kernel", (int64_t)x.n_tokens * x.n_heads_q, kPagedMergeThreads);
+  if (p.own.by_few || !p.direct) launch(DCP_PAGED_KERNEL(paged_merge_kernel), "paged_merge_kernel", (int64_t)x.n_tokens * x.n_heads_q, kPagedMergeThreads);
   return status;
 }
 

@@ -91,6 +91,15 @@ def test_numbers_of_tokens_the_host_does_not_know(gpu, name, longest_q):
     check(got, case.truth())
 
 
+@pytest.mark.parametrize("longest", [64, 700, 5000])
+@pytest.mark.parametrize("name", ["short", "empty_rows", "group_24", "fp16_d64", "window_and_first", "first_touch_window", "few", "groups",
+                                  "some_without"])
+def test_units_whole_and_cut(gpu, name, longest):
+    """What max_seqlen_k says of short requests decides whether a workgroup takes all keys of its rows."""
+    case = Paged(**{**SINGLE, **WINDOWS, **TOKENS, **PREFIXES}[name])
+    check(_run(gpu, case, max_seqlen_k=longest), case.truth())
+
+
 def test_a_batch_of_thousands(gpu):
     """Requests past the 64 that a wave looks at together, few and none of tokens and keys among them."""
     n = 1500
@@ -98,7 +107,8 @@ def test_a_batch_of_thousands(gpu):
                  prefixes=[i % 50 for i in range(200)], cu_groups=[7 * i + 3 for i in range(201)])
     truth = case.truth()
     for longest_q in (1, 2, 100):
-        check(_run(gpu, case, max_seqlen_q=longest_q), truth)
+        for longest_k in (48, 5000):
+            check(_run(gpu, case, max_seqlen_q=longest_q, max_seqlen_k=longest_k), truth)
 
 
 @pytest.mark.parametrize("layout", ["apart", "by_head"])

@@ -13,8 +13,8 @@ TABLES = dict(cached=16, new=16, table=16, stride=4, free=16, slots=16, position
 WRITE = dict(k=16, v=16, slots=16, k_cache=16, v_cache=16, n_tokens=3, heads=2, head_dim=64, elem=2, token=128, head=64, n_pages=4,
              page_size=16, page=2048, cache_token=128, cache_head=64, stream=0)
 ATTN = dict(q=16, k=16, v=16, out=16, lse=16, table=16, lens=16, cu=0, prefix_table=0, prefix_lens=0, groups=0, q_token=512, q_head=128, out_token=512,
-            out_head=128, page=4096, token=256, head=128, stride=4, prefix_stride=0, n_tokens=2, batch=2, heads=4, kv_heads=2, head_dim=128, n_pages=4,
-            page_size=16, width=4, prefix_width=0, n_prefixes=0, max_q=1, max_k=64, max_prefix=0, window=0, n_starting=0, dtype=0, scale=1.0)
+            out_head=128, page=4096, token=256, head=128, stride=256, prefix_stride=0, n_tokens=2, batch=2, heads=4, kv_heads=2, head_dim=128, n_pages=4,
+            page_size=16, width=256, prefix_width=0, n_prefixes=0, max_q=1, max_k=4096, max_prefix=0, window=0, n_starting=0, dtype=0, scale=1.0)
 PREFIX = dict(ATTN, prefix_table=16, prefix_lens=16, groups=16, prefix_stride=4, prefix_width=4, n_prefixes=1, max_prefix=64)
 CALLS = {"dcp_paged_cache_tables": TABLES, "dcp_paged_cache_write": WRITE, "attention": ATTN, "prefix": PREFIX}
 
