@@ -177,13 +177,17 @@ def last_error() -> str:
 
 
 def call(name: str, *args) -> None:
-    """Call an entry point; a nonzero status becomes an exception carrying the
+    """Call an entry point; a nonzero status becomes an exception (``fail``)."""
+    status = getattr(load(), name)(*args)
+    if status != 0:
+        fail(name, status)
+
+
+def fail(name: str, status: int) -> None:
+    """Raise for a nonzero status of an entry point, with the
     library's message: ``ValueError`` for unsupported types (status 2),
     ``AssertionError`` for argument preconditions (status 1), as the reference
     operators raise for the same conditions."""
-    status = getattr(load(), name)(*args)
-    if status == 0:
-        return
     message = f"{name}: {last_error()}"
     if status == 2:
         raise ValueError(message)

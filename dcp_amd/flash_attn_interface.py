@@ -459,80 +459,80 @@ def _flash_attn_varlen_backward(
 _PAGED_ARGS = struct.Struct("<11Q9q16if4x")
 
 
-def _table_here(t, name: str, here: int, *shape) -> None:
+def _table_here(t, name: str, here: int, shape) -> int:
+    """The address of an int32 table of this shape on the current device (``here``)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
-    if t.dtype is not torch.int32 or t.get_device() != here or tuple(t.shape) != shape or (len(shape) == 1 and not t.is_contiguous()) \
-            or (len(shape) == 2 and shape[1] > 1 and t.numel() > 0 and t.stride(1) != 1):
+    if t.dtype is not torch.int32 or t.get_device() != here or t.shape != shape or not (t.is_contiguous() or (len(shape) == 2 and t.stride(1) == 1)):
         raise ValueError(f"{name} must be int32 {list(shape)} with dense rows on the current device, got {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
+# A short decoding step is as long as its call: what is checked here is checked once and with few questions (a call takes 11 us of
+# the host, 5 of them its launches; with an attribute asked for wherever it is used 16).
 def _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, window, n_starting, out, lse,
                 prefix=None):
     """``(out, lse, packed arguments)``, the inputs checked."""
-    here = torch._C._cuda_getDevice()
+    here, dtype, cache_shape, cache_strides, q_strides = torch._C._cuda_getDevice(), q.dtype, k_cache.shape, k_cache.stride(), q.stride()
     if not (q.get_device() == k_cache.get_device() == v_cache.get_device() == here):
         raise ValueError("q, k_cache and v_cache must be tensors of the current device")
-    dtype = q.dtype
     if not (k_cache.dtype is dtype and v_cache.dtype is dtype):
         raise TypeError(f"q is {dtype}, the caches are {k_cache.dtype} and {v_cache.dtype}")
-    if q.dim() != 3 or q.stride(2) != 1:
+    if len(q_strides) != 3 or q_strides[2] != 1:
         raise ValueError(f"q must be [tokens, n_heads_q, D] with dense rows, got {list(q.shape)}")
     n_tokens, n_heads_q, head_dim = q.shape
-    cache_strides = k_cache.stride()
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or cache_strides != v_cache.stride() or cache_strides[3] != 1 \
-            or k_cache.shape[3] != head_dim:
+    if len(cache_shape) != 4 or cache_shape != v_cache.shape or cache_strides != v_cache.stride() or cache_strides[3] != 1 or cache_shape[3] != head_dim:
         raise ValueError(f"k_cache and v_cache must be [n_pages, page_size, n_heads_kv, {head_dim}] with the same strides and dense rows")
-    n_pages, page_size, n_heads_kv, _ = k_cache.shape
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be [B, pages], got {list(block_table.shape)}")
     batch, width = block_table.shape
-    _table_here(block_table, "block_table", here, batch, width)
-    _table_here(seq_lens, "seq_lens", here, batch)
+    table_at = _table_here(block_table, "block_table", here, (batch, width))
+    lens_at = _table_here(seq_lens, "seq_lens", here, (batch,))
+    cu_at = 0
     if cu_seqlens_q is not None:
-        _table_here(cu_seqlens_q, "cu_seqlens_q", here, batch + 1)
+        cu_at = _table_here(cu_seqlens_q, "cu_seqlens_q", here, (batch + 1,))
     elif batch != n_tokens:
         raise ValueError(f"without cu_seqlens_q every request has one token, got {n_tokens} for {batch}")
     if window is not None and window < 1:
         raise ValueError(f"window must be positive (None: no window), got {window}")
     if out is None:
-        out = torch.empty((n_tokens, n_heads_q, head_dim), dtype=dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype is not dtype or out.stride(2) != 1 or out.get_device() != here:
-        raise ValueError(f"out must be like q, got {out.dtype} {list(out.shape)}")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out_token, out_head = n_heads_q * head_dim, head_dim
+    else:
+        if out.shape != q.shape or out.dtype is not dtype or out.stride(2) != 1 or out.get_device() != here:
+            raise ValueError(f"out must be like q, got {out.dtype} {list(out.shape)}")
+        out_token, out_head, _ = out.stride()
     if lse is None:
-        lse = torch.empty((n_heads_q, n_tokens), dtype=torch.float32, device=q.device)
-    elif tuple(lse.shape) != (n_heads_q, n_tokens) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != here:
+        lse = seq_lens.new_empty((n_heads_q, n_tokens), dtype=torch.float32)
+    elif lse.shape != (n_heads_q, n_tokens) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != here:
         raise ValueError(f"lse must be contiguous float32 [{n_heads_q}, {n_tokens}] on the current device")
     if max_seqlen_q is None:
-        max_seqlen_q = 1 if cu_seqlens_q is None else max(n_tokens, 1)
+        max_seqlen_q = 1 if cu_at == 0 else max(n_tokens, 1)
     if max_seqlen_k is None:
-        max_seqlen_k = max(width * page_size, 1)
-    prefix_addresses, prefix_stride, prefix_width, n_prefixes, max_prefix_len = (0, 0, 0), 0, 0, 0, 0
+        max_seqlen_k = max(width * cache_shape[1], 1)
+    prefix_at = lens_of_prefixes_at = groups_at = prefix_stride = prefix_width = n_prefixes = max_prefix_len = 0
     if prefix is not None:
         prefix_table, prefix_lens, cu_groups, max_prefix_len = prefix
         if prefix_table.dim() != 2:
             raise ValueError(f"prefix_table must be [P, pages], got {list(prefix_table.shape)}")
         n_prefixes, prefix_width = prefix_table.shape
-        _table_here(prefix_table, "prefix_table", here, n_prefixes, prefix_width)
-        _table_here(prefix_lens, "prefix_lens", here, n_prefixes)
-        _table_here(cu_groups, "cu_groups", here, n_prefixes + 1)
-        prefix_addresses, prefix_stride = (prefix_table.data_ptr(), prefix_lens.data_ptr(), cu_groups.data_ptr()), prefix_table.stride(0)
+        prefix_at, prefix_stride = _table_here(prefix_table, "prefix_table", here, (n_prefixes, prefix_width)), prefix_table.stride(0)
+        lens_of_prefixes_at = _table_here(prefix_lens, "prefix_lens", here, (n_prefixes,))
+        groups_at = _table_here(cu_groups, "cu_groups", here, (n_prefixes + 1,))
         if max_prefix_len is None:
-            max_prefix_len = max(prefix_width * page_size, 1)
-    q_strides, out_strides = q.stride(), out.stride()
-    packed = _PAGED_ARGS.pack(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(),
-        0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), *prefix_addresses, q_strides[0], q_strides[1], out_strides[0], out_strides[1],
-        cache_strides[0], cache_strides[1], cache_strides[2], block_table.stride(0), prefix_stride, n_tokens, batch, n_heads_q, n_heads_kv, head_dim,
-        n_pages, page_size, width, prefix_width, n_prefixes, max_seqlen_q, max_seqlen_k, max_prefix_len, window or 0, n_starting, dtype_code(dtype),
+            max_prefix_len = max(prefix_width * cache_shape[1], 1)
+    return out, lse, _PAGED_ARGS.pack(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(), table_at, lens_at, cu_at, prefix_at,
+        lens_of_prefixes_at, groups_at, q_strides[0], q_strides[1], out_token, out_head, cache_strides[0], cache_strides[1], cache_strides[2],
+        block_table.stride(0), prefix_stride, n_tokens, batch, n_heads_q, cache_shape[2], head_dim, cache_shape[0], cache_shape[1], width,
+        prefix_width, n_prefixes, max_seqlen_q, max_seqlen_k, max_prefix_len, window or 0, n_starting, dtype_code(dtype),
         head_dim ** -0.5 if softmax_scale is None else softmax_scale)
-    return out, lse, packed
 
 
 def _paged_call(packed: bytes, workspace, q) -> None:
-    address = size = 0
+    lib, address, size = _lib.load(), 0, 0
     if workspace is None:
-        size = _lib.load().dcp_paged_attn_workspace_bytes(packed)
+        size = lib.dcp_paged_attn_workspace_bytes(packed)
         if size > 0:
             workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
             address = workspace.data_ptr()
@@ -540,7 +540,9 @@ def _paged_call(packed: bytes, workspace, q) -> None:
         if not workspace.is_contiguous() or workspace.get_device() != q.get_device():
             raise ValueError("workspace must be a contiguous tensor on q's device")
         address, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _lib.call("dcp_paged_attn", packed, address, size, torch._C._cuda_getCurrentRawStream(q.get_device()))
+    status = lib.dcp_paged_attn(packed, address, size, torch._C._cuda_getCurrentRawStream(q.get_device()))
+    if status != 0:
+        _lib.fail("dcp_paged_attn", status)
 
 
 def paged_cache_workspace_bytes(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q=None, max_seqlen_q=None, max_seqlen_k=None,
