@@ -69,6 +69,7 @@ struct PagedParams {
   int few_rows, few_heads_log2;  // rows of a unit; kv heads a workgroup takes at once: 1, 2 or 4
   int few_whole;                 // a workgroup takes a unit
   int n_few;                // workgroups
+  int merge_sets;           // of lanes that share a row in the merge, a power of two
 };
 typedef KernArgs<PagedParams> PagedArgs;
 typedef KernArgs<PagedSource> SourceArgs;
@@ -182,10 +183,9 @@ __device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, 
 }
 
 // Which work item workgroup `wg` takes.  The items of a group, `group` neighbouring row tiles of a kv head, read the same keys and go to one
-// XCD (workgroup ids go round the eight), whose L2 then reads them once.  The groups that an XCD takes one after the other are
-// of different kv heads: in a cache by token a head's rows are 256 bytes every few KiB, so they all lie in one or two of the 16 channels of
-// an L2, and with an XCD to a head 64 requests on a prefix of 131072 keys ran at 0.63 PFLOP/s, 0.54 TB/s out of each L2.  The tiles
-// of a request's last tokens, which see the most, come first.
+// XCD (workgroup ids go round the eight), whose L2 then reads them once.  From one round of eight groups to the next the XCDs
+// move on by one, so that the groups of one kv head do not all go to the same XCD where there are eight.  The tiles of a request's last
+// tokens, which see the most, come first.
 struct RowItem {
   int tile, kv_head, share;  // share: -1 for none
 };
@@ -933,9 +933,9 @@ __global__ __launch_bounds__(256, 2) void paged_both_kernel(const PagedParams) {
 }
 
 // The merge: out = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over a row's parts, rounded once.  The parts are the pieces
-// of a unit that the kernel of few rows has cut, or shares of the own keys, and the shares of a prefix.  A workgroup takes a row: D / 4
-// lanes hold it in 16-byte pieces, and the 1024 / D sets of such lanes take parts in turn (a wave that went through 128
-// parts alone took 17 us).
+// of a unit that the kernel of few rows has cut, or shares of the own keys, and the shares of a prefix.  D / 4 lanes hold a
+// row in 16-byte pieces; as many sets of such lanes as p.merge_sets take parts of one row in turn (a wave that went through 128
+// parts alone took 17 us), the other sets of the workgroup take other rows (a workgroup for each of 32768 rows of two parts 27 us).
 constexpr int kPagedMergeThreads = 256;
 template <int DTYPE, int D>
 __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const PagedParams) {
@@ -943,9 +943,10 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   constexpr int PIECES = D / 4, SETS = kPagedMergeThreads / PIECES;
   __shared__ f32x4 acc_lds[SETS][PIECES];
   __shared__ f32x2 sums_lds[SETS];
-  const int row = blockIdx.x, tid = threadIdx.x, piece = tid % PIECES, set = tid / PIECES;
+  const int tid = threadIdx.x, piece = tid % PIECES, set = tid / PIECES, row_sets = p.merge_sets, turn = set % row_sets;
   const int64_t n_rows = (int64_t)p.n_tokens * p.n_heads_q;  // (fits 32 bits)
-  const int token = row / p.n_heads_q, head = row % p.n_heads_q;
+  const int64_t row64 = (int64_t)blockIdx.x * (SETS / row_sets) + set / row_sets;
+  const int row = (int)min(row64, n_rows - 1), token = row / p.n_heads_q, head = row % p.n_heads_q;
   // rows of no request are left as they were, and those of no prefix have no parts of one
   const int first = first_token(p, p.own, 0), end = first_token(p, p.own, p.own.batch);
   int prefix_first = 0, prefix_end = 0;
@@ -954,13 +955,13 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
     prefix_end = first_token(p, p.prefix, p.prefix.batch);
   }
   // (& on purpose: of two conditions joined by && or || here, this compiler, clang 22, left the second one out)
-  if ((token < first) | (token >= end)) return;
   const bool has_prefix = (token >= prefix_first) & (token < prefix_end);
   int2 cut = {0, 1};
   if (p.own.by_few) cut = p.cuts[row];
   const int n_cut = (cut.y & 0xfffff) > 1 ? cut.y & 0xfffff : 0;
-  if ((p.own.by_few != 0) & (n_cut == 0) & (p.direct != 0)) return;  // done where it was computed
-  const int n_own = n_cut > 0 ? n_cut : p.own.n_shares, n_parts = n_own + (has_prefix ? p.prefix.n_shares : 0);
+  // (a row of few that was not cut is done where it was computed, if there is nothing else of it)
+  const bool mine = (row64 < n_rows) & (token >= first) & (token < end) & ((p.own.by_few == 0) | (n_cut > 0) | (p.direct == 0));
+  const int n_own = n_cut > 0 ? n_cut : p.own.n_shares, n_parts = mine ? n_own + (has_prefix ? p.prefix.n_shares : 0) : 0;
   const int slot_rows = p.few_rows << p.few_heads_log2;
   // where part i is
   auto part = [&](int i, const f32x2*& sums) -> const float* {
@@ -975,24 +976,24 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   };
   float m = -INFINITY, l = 0.0f;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  constexpr int AT_ONCE = 4;
-  for (int i0 = set; i0 < n_parts; i0 += SETS * AT_ONCE) {
+  constexpr int AT_ONCE = 8;
+  for (int i0 = turn; i0 < n_parts; i0 += row_sets * AT_ONCE) {
     f32x2 ml[AT_ONCE];
     f32x4 o4[AT_ONCE];
 #pragma unroll
     for (int x = 0; x < AT_ONCE; ++x) {
-      const int i = min(i0 + x * SETS, n_parts - 1);
-      const f32x2* sums;
-      const float* from = part(i, sums);
-      ml[x] = *sums;
-      o4[x] = *reinterpret_cast<const f32x4*>(from + 4 * piece);
+      ml[x] = f32x2{-INFINITY, 0.0f};
+      o4[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (i0 + x * row_sets < n_parts) {
+        const f32x2* sums;
+        const float* from = part(i0 + x * row_sets, sums);
+        ml[x] = *sums;
+        o4[x] = *reinterpret_cast<const f32x4*>(from + 4 * piece);
+      }
     }
     float m_new = m;
 #pragma unroll
-    for (int x = 0; x < AT_ONCE; ++x) {
-      if (i0 + x * SETS >= n_parts) ml[x] = f32x2{-INFINITY, 0.0f};
-      m_new = fmaxf(m_new, ml[x][0]);
-    }
+    for (int x = 0; x < AT_ONCE; ++x) m_new = fmaxf(m_new, ml[x][0]);
     const float m_use = m_new == -INFINITY ? 0.0f : m_new, old = fast_exp2(m - m_use);
     l *= old;
 #pragma unroll
@@ -1007,25 +1008,25 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
     }
     m = m_new;
   }
-  acc_lds[set][piece] = acc;
-  if (piece == 0) sums_lds[set] = f32x2{m, l};
-  __syncthreads();
-  if (tid >= PIECES) return;
-  m = -INFINITY;
+  if (row_sets > 1) {
+    acc_lds[set][piece] = acc;
+    if (piece == 0) sums_lds[set] = f32x2{m, l};
+    __syncthreads();
+    if (turn > 0) return;
+    m = -INFINITY;
+    for (int x = set; x < set + row_sets; ++x) m = fmaxf(m, sums_lds[x][0]);
+    const float m_use = m == -INFINITY ? 0.0f : m;
+    l = 0.0f;
+    acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int x = set; x < set + row_sets; ++x) {
+      const float weight = fast_exp2(sums_lds[x][0] - m_use);
+      l += weight * sums_lds[x][1];
+      const f32x4 o4 = acc_lds[x][piece];
 #pragma unroll
-  for (int x = 0; x < SETS; ++x) m = fmaxf(m, sums_lds[x][0]);
-  const float m_use = m == -INFINITY ? 0.0f : m;
-  l = 0.0f;
-  acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int x = 0; x < SETS; ++x) {
-    const float weight = fast_exp2(sums_lds[x][0] - m_use);
-    l += weight * sums_lds[x][1];
-    const f32x4 o4 = acc_lds[x][tid];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
+      for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
+    }
   }
-  store_row_piece<DTYPE>(p, token, head, 4 * tid, acc, m, l);
+  if (mine) store_row_piece<DTYPE>(p, token, head, 4 * piece, acc, m, l);
 }
 
 // ---- host ---------------------------------------------------------------------------
@@ -1049,14 +1050,30 @@ static int64_t seen_keys(const dcp_paged_attn_args& x) {
 static int64_t row_tiles(const dcp_paged_attn_args& x, int batch) {
   return ((int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) - 1) / kRowsBM + batch;
 }
-// Shares of a tile's keys, so that the launch has `rounds` rounds of the device's workgroups.
-static int row_shares(const dcp_paged_attn_args& x, int batch, int64_t max_keys, int rounds) {
+// Shares of a tile's keys: the number that by these figures takes least (us, head size 128, at the longest lengths).  A workgroup begins
+// and ends in 8 and takes 1.25 a tile where it has a CU to itself, 2.0 where two share one; the shares are written and
+// read at 3 TB/s, in a kernel that takes 6 more.  Measured, us by shares: a prompt of 1024 (256 workgroups at one share) 30 at 1, 39 at 2, 50 at
+// 4; 300 tokens behind 8192 keys 153 at 1, 90 at 2, 70 at 4, 89 at 16; 64 requests on a prefix of 32768 120 at 8, 87 at 16, 81 at 24, 87 at 32,
+// 101 at 64; 64 tokens behind 131072 keys 2490 at 1, 339 at 8, 202 at 16, 173 at 32.
+static int row_shares(const dcp_paged_attn_args& x, int batch, int64_t max_keys, bool joined_anyway) {
   // (about as many tiles as have rows: row_tiles has room for more)
   const int64_t rows = (int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv);
   const int64_t items = std::max<int64_t>((rows + kRowsBM - 1) / kRowsBM, batch) * x.n_heads_kv;
-  const int64_t wanted = (rounds * 2 * (int64_t)device_cu_count() + items - 1) / items;
-  const int64_t most = std::max<int64_t>((max_keys + kRowsBN * kMinTilesPerShare - 1) / (kRowsBN * kMinTilesPerShare), 1);
-  return (int)std::min<int64_t>({wanted, most, 256});
+  const int64_t tiles = (max_keys + kRowsBN - 1) / kRowsBN;
+  const int most = (int)std::min<int64_t>(std::max<int64_t>(tiles / kMinTilesPerShare, 1), 64), n_cu = device_cu_count();
+  const double share_us = (double)x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float) * 2 / 3e6;
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= most; ++s) {
+    const int64_t n_wg = items * s, rounds = (n_wg + 2 * n_cu - 1) / (2 * n_cu);
+    const double us = rounds * (8 + (double)tiles / s * (n_wg <= n_cu ? 1.25 : 2.0) * x.head_dim / 128) + (s > 1 || joined_anyway ? s * share_us : 0) +
+                      (s > 1 && !joined_anyway ? 6 : 0);
+    if (us < least) {
+      least = us;
+      best = s;
+    }
+  }
+  return best;
 }
 static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
   PagedPlan plan;
@@ -1087,9 +1104,9 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
       plan.slots = (size_t)plan.n_few * 2 * plan.heads * plan.rows * (x.head_dim + 2) * sizeof(float);
     }
   } else {
-    plan.n_own = row_shares(x, x.batch, keys, 2);
+    plan.n_own = row_shares(x, x.batch, keys, x.n_prefixes > 0);
   }
-  if (x.n_prefixes > 0) plan.n_prefix = row_shares(x, x.n_prefixes, x.max_prefix_len, 1);
+  if (x.n_prefixes > 0) plan.n_prefix = row_shares(x, x.n_prefixes, x.max_prefix_len, true);
   if (plan.n_own + plan.n_prefix > 1) plan.shares = (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
   return plan;
 }
@@ -1130,7 +1147,7 @@ int check_paged(const dcp_paged_attn_args& x) {
   DCP_REQUIRE(x.q && x.out && x.lse && x.block_table && x.seq_lens && (x.n_pages == 0 || (x.k_cache && x.v_cache)) &&
                   (x.n_prefixes == 0 || (x.prefix_table && x.prefix_lens && x.cu_groups)), "paged_attn: null argument");
   DCP_REQUIRE(x.max_seqlen_q > 0 && x.max_seqlen_k > 0 && (x.n_prefixes == 0 || x.max_prefix_len > 0), "paged_attn: the longest lengths must be positive");
-  // (every kernel's work items: at most 256 shares of a row tile)
+  // (every kernel's work items: at most 64 shares of a row tile)
   DCP_REQUIRE((row_tiles(x, x.batch) + row_tiles(x, x.n_prefixes)) * x.n_heads_kv < ((int64_t)1 << 31) - (1 << 20), "paged_attn: too many rows");
   return DCP_OK;
 }
@@ -1164,7 +1181,7 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
   p.slot_sums = reinterpret_cast<f32x2*>(p.slot_out + (size_t)plan.n_few * 2 * plan.heads * plan.rows * x.head_dim);
   p.partial_out = reinterpret_cast<float*>(at + plan.cuts + plan.slots);
   p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * x.head_dim);
-  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.few_whole = plan.whole; p.n_few = plan.n_few;
+  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.few_whole = plan.whole; p.merge_sets = 1; p.n_few = plan.n_few;
 
   int status = DCP_OK;
   const auto launch = [&](auto kernel, const char* name, int64_t n_wg, int threads) {
@@ -1177,15 +1194,15 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
     hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(threads), 0, (hipStream_t)stream, p);
     status = check_launch(name);
   };
-  // A kernel of rows' workgroups, in groups of a request's (or a prefix's) tiles where these are alike in length
-  const auto row_items = [&](PagedSource& src, bool alike) {
-    const int each = std::max(src.n_tiles / src.batch, 1);
-    src.xcd_group = !alike ? 1 : each <= 16 ? each : 8;
+  // A kernel of rows' workgroups, in groups of a request's (or a prefix's) tiles, 16 at most and about equal.  us, single tiles and groups:
+  // two prompts of 2048 behind 14336 keys 330 and 265, 16 of 100 behind 900 54 and 43, one of 8192 from its start 520 and 502.
+  const auto row_items = [&](PagedSource& src) {
+    const int each = std::max(src.n_tiles / src.batch, 1), n = (each + 15) / 16;
+    src.xcd_group = (each + n - 1) / n;
     return row_workgroups(src.n_tiles, src.xcd_group, x.n_heads_kv, src.n_shares);
   };
-  const bool alike = 2 * (int64_t)x.max_seqlen_q <= seen_keys(x);
   if (plan.few && x.n_prefixes > 0) {
-    const int64_t n_wg = row_items(p.prefix, true) + p.n_few;
+    const int64_t n_wg = row_items(p.prefix) + p.n_few;
     if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_both_kernel, 1), "paged_both_kernel", n_wg, 256);
     else launch(DCP_PAGED_KERNEL(paged_both_kernel, 2), "paged_both_kernel", n_wg, 256);
   } else if (plan.few && plan.whole) {
@@ -1195,14 +1212,21 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
     if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1, 4), "paged_few_kernel", p.n_few, 256);
     else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2, 4), "paged_few_kernel", p.n_few, 256);
   } else {
-    launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own, alike), kRowsThreads);
+    launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own), kRowsThreads);
     if (x.n_prefixes > 0) {
       std::swap(p.own, p.prefix);  // (the kernel takes what it finds there)
-      launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own, true), kRowsThreads);
+      launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own), kRowsThreads);
       std::swap(p.own, p.prefix);
     }
   }
-  if (p.own.by_few || !p.direct) launch(DCP_PAGED_KERNEL(paged_merge_kernel), "paged_merge_kernel", (int64_t)x.n_tokens * x.n_heads_q, kPagedMergeThreads);
+  if (p.own.by_few || !p.direct) {
+    // eight parts a set of lanes, as far as the longest lengths tell how many there are
+    const int64_t units = std::max<int64_t>((int64_t)x.batch * x.n_heads_kv / plan.heads, 1);
+    const int64_t parts = (plan.few && !plan.whole ? plan.n_few / units + 2 : plan.n_own) + plan.n_prefix;
+    const int sets = kPagedMergeThreads / (x.head_dim / 4);
+    while (p.merge_sets < sets && parts > 8 * p.merge_sets) p.merge_sets *= 2;
+    launch(DCP_PAGED_KERNEL(paged_merge_kernel), "paged_merge_kernel", ((int64_t)x.n_tokens * x.n_heads_q * p.merge_sets + sets - 1) / sets, kPagedMergeThreads);
+  }
   return status;
 }
 
