@@ -9,6 +9,7 @@
 // paged_cache_write_kernel moves the new tokens' rows of K and V into the cache.  HBM-bound: 16 bytes a lane, four
 // of them in flight.
 #include <algorithm>
+#include <utility>
 
 #include "common.h"
 #include "record.h"
@@ -191,6 +192,18 @@ extern "C" int dcp_paged_cache_tables(const int32_t* cached_lens, const int32_t*
   DCP_REQUIRE(cu_seqlens && pages_taken && (batch == 0 || (cached_lens && new_lens && block_table && seq_lens)) &&
                   (n_free == 0 || free_pages) && (n_tokens == 0 || (slot_mapping && positions)),
               "paged_cache_tables: null argument");
+  // (workgroups read the lengths and the free list while others write: the last step's seq_lens, say, are not both)
+  const auto overlap = [](const void* a, int64_t n, const void* b, int64_t m) {
+    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+    return x < y + (uintptr_t)m && y < x + (uintptr_t)n;
+  };
+  const int64_t n = 4 * (int64_t)batch, tokens = n_tokens;
+  const std::pair<const void*, int64_t> read[] = {{cached_lens, n}, {new_lens, n}, {free_pages, 4 * (int64_t)n_free}};
+  const std::pair<const void*, int64_t> written[] = {{seq_lens, n}, {cu_seqlens, n + 4}, {pages_taken, 4}, {positions, 4 * tokens}, {slot_mapping, 8 * tokens},
+                                                     {block_table, 4 * (std::max<int64_t>(batch - 1, 0) * table_stride + table_width)}};
+  for (const auto& w : written)
+    for (const auto& r : read)
+      DCP_REQUIRE(batch == 0 || r.second == 0 || w.second == 0 || !overlap(w.first, w.second, r.first, r.second), "paged_cache_tables: an input is also written to");
   CacheTablesParams p = {cached_lens, new_lens, block_table, table_stride, free_pages, slot_mapping, positions, cu_seqlens,
                          seq_lens, pages_taken, batch, table_width, n_free, page_size, n_tokens};
   const int64_t most = std::max(n_tokens, 1);

@@ -52,7 +52,7 @@ def paged_cache_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_
     fit are not entered).  ``pages_taken`` says how many pages the step takes: where that is more than there are,
     the missing ones are entered as -1 and their tokens get slot -1, as do tokens past ``W`` pages.  ``free_pages`` itself is
     not changed: drop its first ``pages_taken`` entries for the next step.  ``out``: tables of an earlier call to
-    write to.
+    write to, none of which may be an input (the last step's ``seq_lens`` as ``cached_lens``: copy them first).
     """
     here, i32 = torch._C._cuda_getDevice(), torch.int32
     n = cached_lens.shape[0] if isinstance(cached_lens, torch.Tensor) and cached_lens.dim() == 1 else -1

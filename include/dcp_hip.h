@@ -647,6 +647,7 @@ int dcp_greedy_stage_selection(
  *  - n_tokens: length of slot_mapping and positions.  Tokens past the last
  *    request's have slot -1, position 0; those that do not fit are not entered.
  *  - Negative lengths count as 0.
+ *  - No output may lie in cached_lens, new_lens or free_pages (status 1).
  */
 int dcp_paged_cache_tables(const int32_t* cached_lens, const int32_t* new_lens,
                            int32_t* block_table, int64_t table_stride,

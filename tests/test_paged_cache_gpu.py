@@ -81,7 +81,7 @@ def test_tables_take_strided_rows_and_out(gpu):
     assert again.slot_mapping.data_ptr() == first.slot_mapping.data_ptr() and again.pages_taken.tolist() == [6]
     for wrong in (dict(block_table=wide[:, :3].t()), dict(block_table=wide[:1, :3].expand(3, 3)), dict(block_table=wide[:, :3].long()),
                   dict(new_lens=new[:2]), dict(cached_lens=cached.cpu()), dict(page_size=0), dict(n_tokens=-1), dict(n_tokens=60, out=first),
-                  dict(free_pages=free.view(2, 3))):
+                  dict(cached_lens=first.seq_lens, out=first), dict(free_pages=free.view(2, 3))):
         with pytest.raises((ValueError, TypeError, AssertionError)):
             paged_cache_tables(**{**dict(cached_lens=cached, new_lens=new, block_table=wide[:, 2:5], free_pages=free, page_size=16, n_tokens=61), **wrong})
 

@@ -8,7 +8,7 @@ import pytest
 from dcp_amd import _lib
 from dcp_amd.flash_attn_interface import _PAGED_ARGS
 
-TABLES = dict(cached=16, new=16, table=16, stride=4, free=16, slots=16, positions=16, cu=16, lens=16, taken=16, batch=2, width=4, n_free=3,
+TABLES = dict(cached=16, new=16, table=256, stride=4, free=32, slots=512, positions=512, cu=512, lens=512, taken=512, batch=2, width=4, n_free=3,
               page_size=16, n_tokens=5, stream=0)
 WRITE = dict(k=16, v=16, slots=16, k_cache=16, v_cache=16, n_tokens=3, heads=2, head_dim=64, elem=2, token=128, head=64, n_pages=4,
              page_size=16, page=2048, cache_token=128, cache_head=64, stream=0)
@@ -44,6 +44,8 @@ def built():
     ("dcp_paged_cache_tables", dict(width=0), "do not make a table"),
     ("dcp_paged_cache_tables", dict(stride=3), "do not make a table"),
     *[("dcp_paged_cache_tables", {x: 0}, "null") for x in ("cached", "new", "table", "free", "slots", "positions", "cu", "lens", "taken")],
+    *[("dcp_paged_cache_tables", {a: 4096, b: 4100}, "also written") for a in ("cached", "new", "free") for b in ("lens", "cu", "slots", "positions", "table")],
+    ("dcp_paged_cache_tables", dict(free=4096, taken=4104), "also written"),
     ("dcp_paged_cache_write", dict(elem=8), "element size"),
     ("dcp_paged_cache_write", dict(n_tokens=-1), "sizes"),
     ("dcp_paged_cache_write", dict(heads=0), "sizes"),
