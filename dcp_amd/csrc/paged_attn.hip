@@ -668,6 +668,7 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
     const int my_head = w & (heads - 1), my_turn = w >> p.few_heads_log2;
     const FewRequest request = requests.of_lane(index);
     const int b = chunk * 64 + index, in_request = at - (unit_end - __builtin_amdgcn_readlane(work, index));
+    if (in_request < 0) break;  // (tables whose tokens are many times those there are: their sums wrap)
     const int unit = whole_units ? in_request : __builtin_amdgcn_readfirstlane(in_request / request.n_tiles);
     const int t_begin = whole_units ? 0 : in_request - unit * request.n_tiles;
     const int t_end = whole_units ? request.n_tiles : min(request.n_tiles, t_begin + (end - at));
@@ -958,7 +959,9 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   const bool has_prefix = (token >= prefix_first) & (token < prefix_end);
   int2 cut = {0, 1};
   if (p.own.by_few) cut = p.cuts[row];
-  const int n_cut = (cut.y & 0xfffff) > 1 ? cut.y & 0xfffff : 0;
+  // (kept to the slots there are, also where cu_seqlens is of more tokens than there are and a row has no entry)
+  cut.x = min(max(cut.x, 0), p.n_few);
+  const int n_pieces = min(cut.y & 0xfffff, p.n_few - cut.x), n_cut = n_pieces > 1 ? n_pieces : 0;
   // (a row of few that was not cut is done where it was computed, if there is nothing else of it)
   const bool mine = (row64 < n_rows) & (token >= first) & (token < end) & ((p.own.by_few == 0) | (n_cut > 0) | (p.direct == 0));
   const int n_own = n_cut > 0 ? n_cut : p.own.n_shares, n_parts = mine ? n_own + (has_prefix ? p.prefix.n_shares : 0) : 0;
@@ -966,7 +969,7 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   // where part i is
   auto part = [&](int i, const f32x2*& sums) -> const float* {
     if (i < n_cut) {
-      const int64_t at = ((int64_t)(cut.x + i) * 2 + (i == 0 ? cut.y >> 28 : 0)) * slot_rows + (cut.y >> 20 & 0xff);
+      const int64_t at = ((int64_t)(cut.x + i) * 2 + (i == 0 ? cut.y >> 28 & 1 : 0)) * slot_rows + min(cut.y >> 20 & 0xff, slot_rows - 1);
       sums = p.slot_sums + at;
       return p.slot_out + at * D;
     }

@@ -521,12 +521,16 @@ def _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_se
         groups_at = _table_here(cu_groups, "cu_groups", here, (n_prefixes + 1,))
         if max_prefix_len is None:
             max_prefix_len = max(prefix_width * cache_shape[1], 1)
-    return out, lse, _PAGED_ARGS.pack(
+    args = (
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), lse.data_ptr(), table_at, lens_at, cu_at, prefix_at,
         lens_of_prefixes_at, groups_at, q_strides[0], q_strides[1], out_token, out_head, cache_strides[0], cache_strides[1], cache_strides[2],
         block_table.stride(0), prefix_stride, n_tokens, batch, n_heads_q, cache_shape[2], head_dim, cache_shape[0], cache_shape[1], width,
         prefix_width, n_prefixes, max_seqlen_q, max_seqlen_k, max_prefix_len, window or 0, n_starting, dtype_code(dtype),
         head_dim ** -0.5 if softmax_scale is None else softmax_scale)
+    try:
+        return out, lse, _PAGED_ARGS.pack(*args)
+    except struct.error as e:
+        raise ValueError(f"sizes, lengths, window and n_starting must be whole numbers of 32 bits, softmax_scale a number: {e}") from None
 
 
 def _paged_call(packed: bytes, workspace, q) -> None:
@@ -581,7 +585,8 @@ def paged_cache_attention(
     pages); they decide how the work is split and change no result beyond its rounding.
     ``workspace``: a tensor of ``paged_cache_workspace_bytes(...)`` bytes, for calls that may not allocate; launches
     that may run at the same time need one each.
-    Page numbers outside of the cache name no page: nobody sees their keys.  Forward only.
+    Page numbers outside of the cache name no page: nobody sees their keys.  What no query of a request sees may hold anything; a key
+    or value that is not finite and that one of its queries sees may reach the request's other queries.  Forward only.
     """
     out, lse, packed = _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, window,
                                    n_starting, out, lse)

@@ -1,6 +1,8 @@
 """Attention over a paged cache and over shared prefixes on the GPU, against their definitions in 64 bits.  Every place of the
 cache that no query of its request sees holds NaN."""
 
+import math
+
 import pytest
 import torch
 
@@ -109,6 +111,28 @@ def test_a_batch_of_thousands(gpu):
     for longest_q in (1, 2, 100):
         for longest_k in (48, 5000):
             check(_run(gpu, case, max_seqlen_q=longest_q, max_seqlen_k=longest_k), truth)
+
+
+def test_more_requests_than_the_kernel_of_few_rows_takes(gpu):
+    """Past 65536 requests every one has a row tile of the kernel of rows."""
+    n, n_pages = 65600, 4
+    k, v = (torch.randn(n_pages, 16, 1, 64, device=gpu).to(torch.bfloat16) for _ in range(2))
+    q = torch.randn(n, 1, 64, device=gpu).to(torch.bfloat16)
+    table = torch.arange(n, dtype=torch.int32, device=gpu)[:, None] % n_pages
+    lens = torch.arange(n, dtype=torch.int32, device=gpu) % 17
+    got = paged_cache_attention(q, k, v, table, lens)
+    k64, v64 = (x[table[:, 0].long(), :, 0].double() for x in (k, v))
+    s = (q.double() * k64).sum(-1) * 64**-0.5
+    s.masked_fill_(torch.arange(16, device=gpu) >= lens[:, None], -math.inf)
+    weights = torch.exp(s - s.amax(1, keepdim=True).clamp_min(-1e30))
+    total = weights.sum(1)
+    truth = ((weights[..., None] * v64).sum(1) / total.clamp_min(1e-300)[:, None])[:, None]
+    # weights and results are rounded to bf16, half a step each, of values up to the largest |v| (and fp32 sums of 80 terms)
+    assert (got[0].double() - truth).abs().max() <= (2 * 2.0**-8 + 2.0**-15) * v64.abs().max()
+    some = lens > 0
+    lse = s.amax(1) + total.log()
+    assert (got[1][0][some].double() - lse[some]).abs().max() <= 2.0**-16 * (1 + lse[some].abs().max())
+    assert torch.isinf(got[1][0][~some]).all() and (got[0][~some] == 0).all()
 
 
 @pytest.mark.parametrize("layout", ["apart", "by_head"])
@@ -293,7 +317,7 @@ def test_captured_and_replayed_with_other_lengths(gpu, prefix):
 
 
 @pytest.mark.parametrize("wrong", ["q_type", "cache_type", "q_axes", "cache_strides", "tables", "lens", "cu", "no_cu", "out", "lse", "dim", "fp32",
-                                   "window", "scale", "page_size", "aligned", "cpu", "heads"])
+                                   "window", "wide_window", "half_a_token", "scale", "page_size", "aligned", "cpu", "heads"])
 def test_refusals(gpu, wrong):
     case = Paged([70, 30], head_dim=128)
     args = case.to(gpu)
@@ -303,7 +327,8 @@ def test_refusals(gpu, wrong):
         tables=dict(block_table=table.long()), lens=dict(seq_lens=args["seq_lens"][:1]), cu=dict(cu_seqlens_q=args["seq_lens"]),
         no_cu=dict(q=torch.cat([q, q])), out=dict(out=q[:1].clone()), lse=dict(lse=torch.empty(2, 8, device=gpu)),
         dim=dict(q=q[..., :96].contiguous(), k_cache=k[..., :96], v_cache=v[..., :96]),
-        fp32=dict(q=q.float(), k_cache=k.float(), v_cache=v.float()), window=dict(window=0), scale=dict(softmax_scale=0.0),
+        fp32=dict(q=q.float(), k_cache=k.float(), v_cache=v.float()), window=dict(window=0), wide_window=dict(window=1 << 40),
+        half_a_token=dict(window=9, n_starting=1.5), scale=dict(softmax_scale=0.0),
         page_size=dict(k_cache=k[:, :40], v_cache=v[:, :40]),
         aligned=dict(q=torch.empty(2 * 8 * 128 + 8, dtype=q.dtype, device=gpu)[4 : 4 + 2 * 8 * 128].view(2, 8, 128)),
         cpu=dict(k_cache=k.cpu(), v_cache=v.cpu()), heads=dict(q=q[:, :5].contiguous()))[wrong]
