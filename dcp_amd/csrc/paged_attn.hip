@@ -948,34 +948,45 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   const int64_t n_rows = (int64_t)p.n_tokens * p.n_heads_q;  // (fits 32 bits)
   const int64_t row64 = (int64_t)blockIdx.x * (SETS / row_sets) + set / row_sets;
   const int row = (int)min(row64, n_rows - 1), token = row / p.n_heads_q, head = row % p.n_heads_q;
-  // rows of no request are left as they were, and those of no prefix have no parts of one
-  const int first = first_token(p, p.own, 0), end = first_token(p, p.own, p.own.batch);
-  int prefix_first = 0, prefix_end = 0;
-  if (p.prefix.batch > 0) {
-    prefix_first = first_token(p, p.prefix, 0);
-    prefix_end = first_token(p, p.prefix, p.prefix.batch);
-  }
-  // (& on purpose: of two conditions joined by && or || here, this compiler, clang 22, left the second one out)
-  const bool has_prefix = (token >= prefix_first) & (token < prefix_end);
+  // Every trip to memory here is as long as the sums themselves, so there are three: where the row's parts are and which groups share
+  // prefixes; the parts and which tokens the groups and requests have; the stores.  The parts are read before it is known whether the row
+  // has any: whatever the entry of a row of no request holds, it is kept to the slots there are, and shares there are of every row.
   int2 cut = {0, 1};
   if (p.own.by_few) cut = p.cuts[row];
-  // (kept to the slots there are, also where cu_seqlens is of more tokens than there are and a row has no entry)
+  const bool prefixes = p.prefix.batch > 0;
+  int first = 0, end = p.n_requests, prefix_first = 0, prefix_end = 0;  // requests, then tokens
+  if (prefixes) {
+    prefix_first = min(max(p.prefix.cu_groups[0], 0), end);
+    prefix_end = min(max(p.prefix.cu_groups[p.prefix.batch], 0), end);
+  }
+  if (p.cu_seqlens_q != nullptr) {
+    const int32_t* cu = p.cu_seqlens_q;
+    const int a = cu[first], b = cu[end], c = cu[prefix_first], d = cu[prefix_end];
+    first = a; end = b; prefix_first = c; prefix_end = d;
+  }
   cut.x = min(max(cut.x, 0), p.n_few);
   const int n_pieces = min(cut.y & 0xfffff, p.n_few - cut.x), n_cut = n_pieces > 1 ? n_pieces : 0;
-  // (a row of few that was not cut is done where it was computed, if there is nothing else of it)
-  const bool mine = (row64 < n_rows) & (token >= first) & (token < end) & ((p.own.by_few == 0) | (n_cut > 0) | (p.direct == 0));
-  const int n_own = n_cut > 0 ? n_cut : p.own.n_shares, n_parts = mine ? n_own + (has_prefix ? p.prefix.n_shares : 0) : 0;
-  const int slot_rows = p.few_rows << p.few_heads_log2;
+  const int n_own = n_cut > 0 ? n_cut : p.direct ? 0 : p.own.n_shares;  // (no memory for shares where rows are done at once)
+  const int n_parts = n_own + (prefixes ? p.prefix.n_shares : 0);
+  const int slot_rows = p.few_rows << p.few_heads_log2, slot_row = min(cut.y >> 20 & 0xff, slot_rows - 1), slot = cut.y >> 28 & 1;
+  // (& on purpose: of two conditions joined by && or || here, this compiler, clang 22, left the second one out)
+  const bool has_prefix = prefixes & (token >= prefix_first) & (token < prefix_end);
+  // rows of no request are left as they were; one that has no parts is done where it was computed
+  const bool mine = (row64 < n_rows) & (token >= first) & (token < end) & (n_parts > 0);
+  // (kept in registers: a choice between two of the arguments was made by loading the chosen one, for every part anew)
+  typedef __attribute__((address_space(1))) const f32x4 GlobalOut;
+  typedef __attribute__((address_space(1))) const f32x2 GlobalSums;
+  GlobalOut *slot_out = (GlobalOut*)p.slot_out, *partial_out = (GlobalOut*)p.partial_out;
+  GlobalSums *slot_sums = (GlobalSums*)p.slot_sums, *partial_sums = (GlobalSums*)p.partial_sums;
+  asm("" : "+s"(slot_out), "+s"(partial_out), "+s"(slot_sums), "+s"(partial_sums));
   // where part i is
-  auto part = [&](int i, const f32x2*& sums) -> const float* {
-    if (i < n_cut) {
-      const int64_t at = ((int64_t)(cut.x + i) * 2 + (i == 0 ? cut.y >> 28 & 1 : 0)) * slot_rows + min(cut.y >> 20 & 0xff, slot_rows - 1);
-      sums = p.slot_sums + at;
-      return p.slot_out + at * D;
-    }
-    const int64_t at = (int64_t)(i < n_own ? i : i - n_own + p.prefix.first_share) * n_rows + row;
-    sums = p.partial_sums + at;
-    return p.partial_out + at * D;
+  const int prefix_shift = p.prefix.first_share - n_own;
+  auto part = [&](int i, GlobalSums*& sums) -> GlobalOut* {
+    const bool in_slot = i < n_cut;
+    const int64_t at = in_slot ? ((int64_t)(cut.x + i) * 2 + (i == 0 ? slot : 0)) * slot_rows + slot_row
+                               : (int64_t)(i < n_own ? i : i + prefix_shift) * n_rows + row;
+    sums = (in_slot ? slot_sums : partial_sums) + at;
+    return (in_slot ? slot_out : partial_out) + at * PIECES + piece;
   };
   float m = -INFINITY, l = 0.0f;
   f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -988,15 +999,17 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
       ml[x] = f32x2{-INFINITY, 0.0f};
       o4[x] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (i0 + x * row_sets < n_parts) {
-        const f32x2* sums;
-        const float* from = part(i0 + x * row_sets, sums);
+        GlobalSums* sums;
+        o4[x] = *part(i0 + x * row_sets, sums);
         ml[x] = *sums;
-        o4[x] = *reinterpret_cast<const f32x4*>(from + 4 * piece);
       }
     }
     float m_new = m;
 #pragma unroll
-    for (int x = 0; x < AT_ONCE; ++x) m_new = fmaxf(m_new, ml[x][0]);
+    for (int x = 0; x < AT_ONCE; ++x) {
+      if (!((i0 + x * row_sets < n_own) | has_prefix)) ml[x] = f32x2{-INFINITY, 0.0f};
+      m_new = fmaxf(m_new, ml[x][0]);
+    }
     const float m_use = m_new == -INFINITY ? 0.0f : m_new, old = fast_exp2(m - m_use);
     l *= old;
 #pragma unroll

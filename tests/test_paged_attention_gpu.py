@@ -113,6 +113,13 @@ def test_a_batch_of_thousands(gpu):
             check(_run(gpu, case, max_seqlen_q=longest_q, max_seqlen_k=longest_k), truth)
 
 
+@pytest.mark.parametrize("keys", [64, 65])
+def test_shares_that_end_with_a_request(gpu, keys):
+    """As many requests as workgroups twice over, of the same length: none is cut, or nearly all are."""
+    case = Paged([keys] * 1024, heads=2, kv_heads=1, head_dim=64, page_size=16)
+    check(_run(gpu, case, max_seqlen_k=5000), case.truth())
+
+
 def test_more_requests_than_the_kernel_of_few_rows_takes(gpu):
     """Past 65536 requests every one has a row tile of the kernel of rows."""
     n, n_pages = 65600, 4
