@@ -166,20 +166,27 @@ constexpr float kMaxTileSum = 16384.0f;  // of a lane's weights against a refere
 // floor(first_row / 128) + b: that leaves room for its last, partial one, and needs no sum over the requests before it.
 struct RowTile {
   int b, index;
+  TokenRange tokens;
+  int n_keys;
 };
 __device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, int tile) {
   const int lane = threadIdx.x & 63;
-  auto start = [&](int b) { return (int)((int64_t)first_token(p, src, b) * p.group / kRowsBM) + b; };
+  auto start = [&](int first, int b) { return (int)((int64_t)first * p.group / kRowsBM) + b; };
   int lo = 0, hi = src.batch;  // the last request that begins at or before the tile; 64 candidates a step
-  while (hi - lo > 1) {
+  while (hi - lo > 64) {
     const int step = (hi - lo + 63) / 64, b = lo + lane * step;
-    const bool before = b < hi && start(b) <= tile;
+    const bool before = b < hi && start(first_token(p, src, b), b) <= tile;
     const int n = __popcll(__ballot(before));
     if (n > 1) lo += (n - 1) * step;
     hi = min(lo + step, hi);
   }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  return {lo, tile - __builtin_amdgcn_readfirstlane(start(lo))};
+  // A lane looks at one request, and at all there is to know of it: another trip to memory for the one that is found is a microsecond.
+  const int b = min(lo + lane, hi - 1);
+  const TokenRange tokens = tokens_of(p, src, b);
+  const int n_keys = keys_of(p, src, b), first_tile = start(tokens.begin, b);
+  const int at = __builtin_amdgcn_readfirstlane(max(__popcll(__ballot((lo + lane < hi) & (first_tile <= tile))) - 1, 0));
+  auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+  return {of(b), tile - of(first_tile), {of(tokens.begin), of(tokens.n)}, of(n_keys)};
 }
 
 // Which work item workgroup `wg` takes.  The items of a group, `group` neighbouring row tiles of a kv head, read the same keys and go to one
@@ -227,12 +234,12 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   const int tile_number = __builtin_amdgcn_readfirstlane(at.tile), kv_head = __builtin_amdgcn_readfirstlane(at.kv_head);
   const int share = __builtin_amdgcn_readfirstlane(at.share);
   const RowTile tile = find_row_tile(p, src, tile_number);
-  const TokenRange tokens = tokens_of(p, src, tile.b);
+  const TokenRange tokens = tile.tokens;
   const int n_rows = tokens.n * p.group;  // (at most n_tokens * group, which the host has checked)
   const int row0 = tile.index * kRowsBM;
   if (tile.index < 0 || row0 >= n_rows) return;
   const bool prefix = src.cu_groups != nullptr;
-  const int n_keys = keys_of(p, src, tile.b), window = prefix ? 0 : p.window, n_starting = p.n_starting;
+  const int n_keys = tile.n_keys, window = prefix ? 0 : p.window, n_starting = p.n_starting;
   // token i of the request is at position n_keys - n + i; every token is past all of a prefix
   const int first_tok = row0 / p.group, last_tok = (min(row0 + kRowsBM, n_rows) - 1) / p.group;
   const int at0 = prefix ? n_keys - 1 : n_keys - tokens.n, step = prefix ? 0 : 1;
@@ -284,7 +291,6 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     if (lane == 0) any_absent[rel / kTableTiles % 2 * 4 + w] = any;
   };
   auto offset_of = [&](int t) { return offsets[((t - t_begin) * 4 + g) % (2 * kTableTiles * 4)]; };
-  if (t_begin < t_end) look_up(0);
 
   // ---- this lane's rows: n of each of the wave's two row tiles (past the last one: the last one again, not written) ------
   int last_key[RT];                          // the last key it sees
@@ -300,6 +306,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     first_last = min(first_last, wave_min(last_key[rt]));
     last_last = max(last_last, wave_max(last_key[rt]));
   }
+  if (t_begin < t_end) look_up(0);  // (after the rows were asked for)
   const int reach = window > 0 ? window : 0x7fffffff;  // a query sees the keys less than this before its last
   const float scale = p.scale_log2;
 
