@@ -68,7 +68,7 @@ struct PagedParams {
   f32x2* slot_sums;  // [workgroup][2][head of the workgroup][rows]
   int few_rows, few_heads_log2;  // rows of a unit; kv heads a workgroup takes at once: 1, 2 or 4
   int few_whole;                 // a workgroup takes a unit
-  int n_few;                // workgroups
+  int n_few, few_first;     // workgroups; of paged_both_kernel those before the ones of rows
   int merge_sets;           // of lanes that share a row in the merge, a power of two
 };
 typedef KernArgs<PagedParams> PagedArgs;
@@ -927,15 +927,16 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_few_kernel(const PagedParams
 }
 
 // The requests' own keys and prefixes of many rows in one launch: a workgroup of the one starts where one of the other has ended, without
-// a kernel's end and another's start between them.  (Few rows first: 64 requests on a prefix of 32768 81 us, last 85, eight
-// workgroups of each in turn 83; on one of 131072 194, 196 and 236: dealt in turn to XCDs that are full, workgroups leave slots empty.)
+// a kernel's end and another's start between them.  p.few_first workgroups of few rows come first, then those of rows, then the other
+// few: all of the few, or one a CU, so that a CU has one of each kind, of which one waits for memory and the other for products.  (In
+// turns it is the CUs that take turns: of an XCD's every second has two of rows.)
 template <int DTYPE, int D, int RT>
 __global__ __launch_bounds__(256, 2) void paged_both_kernel(const PagedParams) {
   __shared__ __attribute__((aligned(16))) char lds[std::max(FewLds<D, RT, 4>::BYTES, RowsLds<D>::BYTES)];
   PagedArgs& p = fresh_kernel_args<PagedParams>();
-  const int n_few = p.n_few, wg = blockIdx.x;
-  const bool few = wg < n_few;
-  const int i = few ? wg : wg - n_few;
+  const int wg = blockIdx.x, before = p.few_first, n_rows = gridDim.x - p.n_few;
+  const bool few = (wg < before) | (wg >= before + n_rows);
+  const int i = wg < before ? wg : few ? wg - n_rows : wg - before;
   if (few) paged_few<DTYPE, D, RT, 4>(i, lds);
   else paged_rows<DTYPE, D>(p, p.prefix, i, lds);
 }
@@ -1059,6 +1060,7 @@ struct PagedPlan {
   bool few = false;    // the kernel of few rows takes the requests' own keys
   bool whole = false;  // a workgroup (of 8 waves) takes a unit of it; otherwise one of 4 an equal share of all tiles
   int rows = 16, heads = 1, n_few = 0;  // rows of a unit, kv heads of a workgroup, workgroups
+  int few_first = 0;                    // those before a prefix's
   int n_own = 1, n_prefix = 0;          // shares
   size_t cuts = 0, slots = 0, shares = 0;  // bytes
   size_t bytes() const { return cuts + slots + shares; }
@@ -1078,23 +1080,23 @@ static int64_t row_tiles(const dcp_paged_attn_args& x, int batch) {
 // read at 3 TB/s, in a kernel that takes 6 more.  Measured, us by shares: a prompt of 1024 (256 workgroups at one share) 30 at 1, 39 at 2, 50 at
 // 4; 300 tokens behind 8192 keys 153 at 1, 90 at 2, 70 at 4, 89 at 16; 64 requests on a prefix of 32768 120 at 8, 87 at 16, 81 at 24, 87 at 32,
 // 101 at 64; 64 tokens behind 131072 keys 2490 at 1, 339 at 8, 202 at 16, 173 at 32.
-static int row_shares(const dcp_paged_attn_args& x, int batch, int64_t max_keys, bool joined_anyway) {
+struct RowShares {
+  int n;
+  double us;
+};
+static RowShares row_shares(const dcp_paged_attn_args& x, int batch, int64_t max_keys, bool joined_anyway) {
   // (about as many tiles as have rows: row_tiles has room for more)
   const int64_t rows = (int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv);
   const int64_t items = std::max<int64_t>((rows + kRowsBM - 1) / kRowsBM, batch) * x.n_heads_kv;
   const int64_t tiles = (max_keys + kRowsBN - 1) / kRowsBN;
   const int most = (int)std::min<int64_t>(std::max<int64_t>(tiles / kMinTilesPerShare, 1), 64), n_cu = device_cu_count();
   const double share_us = (double)x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float) * 2 / 3e6;
-  int best = 1;
-  double least = 1e30;
+  RowShares best = {1, 1e30};
   for (int s = 1; s <= most; ++s) {
     const int64_t n_wg = items * s, rounds = (n_wg + 2 * n_cu - 1) / (2 * n_cu);
     const double us = rounds * (8 + (double)tiles / s * (n_wg <= n_cu ? 1.25 : 2.0) * x.head_dim / 128) + (s > 1 || joined_anyway ? s * share_us : 0) +
                       (s > 1 && !joined_anyway ? 6 : 0);
-    if (us < least) {
-      least = us;
-      best = s;
-    }
+    if (us < best.us) best = {s, us};
   }
   return best;
 }
@@ -1110,14 +1112,16 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
   const int64_t most_units = (all_rows + (int64_t)x.batch * (plan.rows - 1)) / plan.rows * x.n_heads_kv;
   const int64_t units = std::max<int64_t>(x.batch, all_rows / plan.rows) * x.n_heads_kv;
   plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2) < 2e9;
+  double few_us = 0;
   if (plan.few) {
     // Whole units where every CU has at most one, and the chain of an eighth of its tiles (2.3 us each) is shorter than what cutting costs
     // (a second kernel and more) and the equal shares take (of lengths that are half the longest on average, at 5.4 TB/s).  us, whole
     // and cut: one request of 256 keys 7.3 and 9.8, of 1000 14.4 and 10.3; 32 of 1000 27.4 and 31.7, of up to 1024 20.2 and 24.4;
     // 32 windows of 1016 keys, head size 64, 18.1 and 23.2; 16 of up to 2048 29.3 and 24.0; 64 of 256 20.8 and 19.4.
     // Beside a prefix's shares, which are joined anyway, always as long as units are short: 64 requests on a prefix of 32768 80 and 87.
-    const double unit_us = keys * (2.3 / 256), all_us = 0.5 * units * keys * x.head_dim * 4 / 5.4e6;
-    plan.whole = keys <= 2048 && (x.n_prefixes > 0 || (units <= device_cu_count() && unit_us < 5 + all_us));
+    const double unit_us = keys * (2.3 / 256);
+    few_us = 0.5 * units * keys * x.head_dim * 4 / 5.4e6;
+    plan.whole = keys <= 2048 && (x.n_prefixes > 0 || (units <= device_cu_count() && unit_us < 5 + few_us));
     plan.n_few = plan.whole ? (int)most_units : 2 * device_cu_count();
     // Four heads at once from 64 tiles a workgroup on (16 for each wave).
     const int64_t tiles = (int64_t)x.batch * ((keys + kFewBN - 1) / kFewBN) * x.n_heads_kv / plan.n_few;
@@ -1127,9 +1131,16 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
       plan.slots = (size_t)plan.n_few * 2 * plan.heads * plan.rows * (x.head_dim + 2) * sizeof(float);
     }
   } else {
-    plan.n_own = row_shares(x, x.batch, keys, x.n_prefixes > 0);
+    plan.n_own = row_shares(x, x.batch, keys, x.n_prefixes > 0).n;
   }
-  if (x.n_prefixes > 0) plan.n_prefix = row_shares(x, x.n_prefixes, x.max_prefix_len, true);
+  if (x.n_prefixes > 0) {
+    const RowShares shares = row_shares(x, x.n_prefixes, x.max_prefix_len, true);
+    plan.n_prefix = shares.n;
+    // All of the few first where theirs is most of the time: the prefix's then fill what they leave at their end.  us, all first and one
+    // a CU first: 64 requests of up to 1024 own keys on a prefix of 32768 84 and 75, of 64 own keys 77 and 66; 256 of up to 600 on 8192
+    // 114 and 97; 128 of up to 2000 on 8192 110 and 115; 64 of up to 6000 on 16384 122 and 125.
+    plan.few_first = few_us < 1.5 * shares.us ? std::min(plan.n_few, device_cu_count()) : plan.n_few;
+  }
   if (plan.n_own + plan.n_prefix > 1) plan.shares = (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
   return plan;
 }
@@ -1204,7 +1215,7 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
   p.slot_sums = reinterpret_cast<f32x2*>(p.slot_out + (size_t)plan.n_few * 2 * plan.heads * plan.rows * x.head_dim);
   p.partial_out = reinterpret_cast<float*>(at + plan.cuts + plan.slots);
   p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * x.head_dim);
-  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.few_whole = plan.whole; p.merge_sets = 1; p.n_few = plan.n_few;
+  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.few_whole = plan.whole; p.merge_sets = 1; p.n_few = plan.n_few; p.few_first = plan.few_first;
 
   int status = DCP_OK;
   const auto launch = [&](auto kernel, const char* name, int64_t n_wg, int threads) {
