@@ -158,7 +158,7 @@ __device__ __forceinline__ void store_row_piece(PagedArgs& p, int64_t token, int
 // of tile t follows as a dense run that the SIMD's other wave fills with its own arithmetic.
 // ---------------------------------------------------------------------------
 constexpr int kRowsThreads = 256, kRowsBM = 128, kRowsBN = 64;
-constexpr int kMinTilesPerShare = 4;
+constexpr int kMinTilesPerShare = 2;
 constexpr float kNoMax = -3.0e38f;  // the reference of a row that has seen nothing: below every score, and a weight of -inf against it is 0
 constexpr float kMaxTileSum = 16384.0f;  // of a lane's weights against a reference that is not their maximum: fp16 can hold them
 
@@ -1058,7 +1058,8 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
 // How a call is laid out: which kernel takes which keys, and what of the workspace is whose.
 struct PagedPlan {
   bool few = false;    // the kernel of few rows takes the requests' own keys
-  bool whole = false;  // a workgroup (of 8 waves) takes a unit of it; otherwise one of 4 an equal share of all tiles
+  bool whole = false;  // a workgroup takes a unit of it; otherwise an equal share of all tiles
+  int waves = 4;       // of a workgroup of it
   int rows = 16, heads = 1, n_few = 0;  // rows of a unit, kv heads of a workgroup, workgroups
   int few_first = 0;                    // those before a prefix's
   int n_own = 1, n_prefix = 0;          // shares
@@ -1075,11 +1076,18 @@ static int64_t seen_keys(const dcp_paged_attn_args& x) {
 static int64_t row_tiles(const dcp_paged_attn_args& x, int batch) {
   return ((int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) - 1) / kRowsBM + batch;
 }
+// Row tiles that go to one XCD together: of one request (or prefix), 16 at most and about equal.  us, single tiles and groups:
+// two prompts of 2048 behind 14336 keys 330 and 265, 16 of 100 behind 900 54 and 43, one of 8192 from its start 520 and 502.
+static int row_group(const dcp_paged_attn_args& x, int batch) {
+  const int each = std::max((int)(row_tiles(x, batch) / batch), 1), n = (each + 15) / 16;
+  return (each + n - 1) / n;
+}
 // Shares of a tile's keys: the number that by these figures takes least (us, head size 128, at the longest lengths).  A workgroup begins
-// and ends in 8 and takes 1.25 a tile where it has a CU to itself, 2.0 where two share one; the shares are written and
-// read at 3 TB/s, in a kernel that takes 6 more.  Measured, us by shares: a prompt of 1024 (256 workgroups at one share) 30 at 1, 39 at 2, 50 at
-// 4; 300 tokens behind 8192 keys 153 at 1, 90 at 2, 70 at 4, 89 at 16; 64 requests on a prefix of 32768 120 at 8, 87 at 16, 81 at 24, 87 at 32,
-// 101 at 64; 64 tokens behind 131072 keys 2490 at 1, 339 at 8, 202 at 16, 173 at 32.
+// and ends in 7 and takes 1.1 a tile where it has a CU to itself, 2.0 where two share one; the shares are written and
+// read at 3 TB/s, in a kernel that takes 3.5 more.  Measured, us by shares: a prompt of 1024 (256 workgroups at one share) 29 at 1, 41 at 2,
+// 49 at 4; 3 of 13 tokens of 542 keys 18 at 1 and 16 at 4; 300 tokens behind 8192 keys 152 at 1, 90 at 2, 68 at 4, 60 at 6, 82 at 16;
+// 64 requests on a prefix of 32768 106 at 8, 75 at 16, 81 at 32; 83 on one of 13447 47 at 8, 35 at 16 and 43 at 21, where an XCD has 33
+// workgroups for its 32 CUs; 64 tokens behind 131072 keys 2490 at 1, 337 at 8, 198 at 16, 162 at 32.
 struct RowShares {
   int n;
   double us;
@@ -1087,15 +1095,16 @@ struct RowShares {
 static RowShares row_shares(const dcp_paged_attn_args& x, int batch, int64_t max_keys, bool joined_anyway) {
   // (about as many tiles as have rows: row_tiles has room for more)
   const int64_t rows = (int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv);
-  const int64_t items = std::max<int64_t>((rows + kRowsBM - 1) / kRowsBM, batch) * x.n_heads_kv;
+  const int64_t row_tiles_there = std::max<int64_t>((rows + kRowsBM - 1) / kRowsBM, batch), group = row_group(x, batch);
+  const int64_t groups = (row_tiles_there + group - 1) / group * x.n_heads_kv;
   const int64_t tiles = (max_keys + kRowsBN - 1) / kRowsBN;
   const int most = (int)std::min<int64_t>(std::max<int64_t>(tiles / kMinTilesPerShare, 1), 64), n_cu = device_cu_count();
   const double share_us = (double)x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float) * 2 / 3e6;
   RowShares best = {1, 1e30};
   for (int s = 1; s <= most; ++s) {
-    const int64_t n_wg = items * s, rounds = (n_wg + 2 * n_cu - 1) / (2 * n_cu);
-    const double us = rounds * (8 + (double)tiles / s * (n_wg <= n_cu ? 1.25 : 2.0) * x.head_dim / 128) + (s > 1 || joined_anyway ? s * share_us : 0) +
-                      (s > 1 && !joined_anyway ? 6 : 0);
+    const int64_t n_wg = xcd_grid_size(groups * s, 1) * group, rounds = (n_wg + 2 * n_cu - 1) / (2 * n_cu);
+    const double us = rounds * (7 + (double)tiles / s * (n_wg <= n_cu ? 1.1 : 2.0) * x.head_dim / 128) + (s > 1 || joined_anyway ? s * share_us : 0) +
+                      (s > 1 && !joined_anyway ? 3.5 : 0);
     if (us < best.us) best = {s, us};
   }
   return best;
@@ -1114,15 +1123,19 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
   plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2) < 2e9;
   double few_us = 0;
   if (plan.few) {
-    // Whole units where every CU has at most one, and the chain of an eighth of its tiles (2.3 us each) is shorter than what cutting costs
-    // (a second kernel and more) and the equal shares take (of lengths that are half the longest on average, at 5.4 TB/s).  us, whole
-    // and cut: one request of 256 keys 7.3 and 9.8, of 1000 14.4 and 10.3; 32 of 1000 27.4 and 31.7, of up to 1024 20.2 and 24.4;
-    // 32 windows of 1016 keys, head size 64, 18.1 and 23.2; 16 of up to 2048 29.3 and 24.0; 64 of 256 20.8 and 19.4.
-    // Beside a prefix's shares, which are joined anyway, always as long as units are short: 64 requests on a prefix of 32768 80 and 87.
-    const double unit_us = keys * (2.3 / 256);
+    // Whole units where they are short: the chain of one's tiles (of a fourth of them) against what cutting costs, a second kernel and
+    // more, and, as far as that goes, against the equal shares' time (of lengths that are half the longest on average, at 5.4 TB/s).
+    // us, whole and cut, 8 kv heads of 128: 4 requests of 32 keys 6.0 and 18, of 512 11.2 and 11.0, of 1024 17 and 12; 32 of 512 16 and 21,
+    // of 1024 26 and 31, of up to 1024 20 and 23, of up to 2048 32 and 32; 64 of up to 64 9 and 22, of up to 2048 50 and 45;
+    // 192 of up to 256 32 and 54, of 1024 132 and 141.  Beside a prefix's shares, which are joined anyway, always as
+    // long as units are short: 64 requests on a prefix of 32768 80 and 87.
+    const double unit_us = keys * (0.004 + 0.007 * x.head_dim / 128);
     few_us = 0.5 * units * keys * x.head_dim * 4 / 5.4e6;
-    plan.whole = keys <= 2048 && (x.n_prefixes > 0 || (units <= device_cu_count() && unit_us < 5 + few_us));
+    plan.whole = x.n_prefixes > 0 ? keys <= 2048 : unit_us < 8 + std::min(few_us, 9.0);
     plan.n_few = plan.whole ? (int)most_units : 2 * device_cu_count();
+    // Of eight waves where a CU has at most one and could hold two (head size 64): 32 windows of 1016 keys 14.1, of four 14.6; 16 of
+    // 2048 20.6 and 22.2, of 256 7.4 and 7.0.
+    plan.waves = plan.whole && x.head_dim == 64 && x.n_prefixes == 0 && units <= device_cu_count() && keys > 512 ? 8 : 4;
     // Four heads at once from 64 tiles a workgroup on (16 for each wave).
     const int64_t tiles = (int64_t)x.batch * ((keys + kFewBN - 1) / kFewBN) * x.n_heads_kv / plan.n_few;
     plan.heads = plan.whole || tiles < 64 ? 1 : x.n_heads_kv % 4 == 0 ? 4 : x.n_heads_kv % 2 == 0 ? 2 : 1;
@@ -1228,20 +1241,19 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
     hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(threads), 0, (hipStream_t)stream, p);
     status = check_launch(name);
   };
-  // A kernel of rows' workgroups, in groups of a request's (or a prefix's) tiles, 16 at most and about equal.  us, single tiles and groups:
-  // two prompts of 2048 behind 14336 keys 330 and 265, 16 of 100 behind 900 54 and 43, one of 8192 from its start 520 and 502.
+  // A kernel of rows' workgroups
   const auto row_items = [&](PagedSource& src) {
-    const int each = std::max(src.n_tiles / src.batch, 1), n = (each + 15) / 16;
-    src.xcd_group = (each + n - 1) / n;
+    src.xcd_group = row_group(x, src.batch);
     return row_workgroups(src.n_tiles, src.xcd_group, x.n_heads_kv, src.n_shares);
   };
   if (plan.few && x.n_prefixes > 0) {
     const int64_t n_wg = row_items(p.prefix) + p.n_few;
     if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_both_kernel, 1), "paged_both_kernel", n_wg, 256);
     else launch(DCP_PAGED_KERNEL(paged_both_kernel, 2), "paged_both_kernel", n_wg, 256);
-  } else if (plan.few && plan.whole) {
-    if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1, 8), "paged_few_kernel", p.n_few, 512);
-    else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2, 8), "paged_few_kernel", p.n_few, 512);
+  } else if (plan.few && plan.waves == 8) {
+    launch(x.dtype == DCP_DTYPE_BF16 ? (plan.rows == 16 ? paged_few_kernel<DCP_DTYPE_BF16, 64, 1, 8> : paged_few_kernel<DCP_DTYPE_BF16, 64, 2, 8>)
+                                     : (plan.rows == 16 ? paged_few_kernel<DCP_DTYPE_FP16, 64, 1, 8> : paged_few_kernel<DCP_DTYPE_FP16, 64, 2, 8>),
+           "paged_few_kernel", p.n_few, 512);
   } else if (plan.few) {
     if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1, 4), "paged_few_kernel", p.n_few, 256);
     else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2, 4), "paged_few_kernel", p.n_few, 256);

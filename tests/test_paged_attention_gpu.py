@@ -102,6 +102,14 @@ def test_units_whole_and_cut(gpu, name, longest):
     check(_run(gpu, case, max_seqlen_k=longest), case.truth())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, F16])
+@pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2]])
+def test_whole_units_of_head_size_64(gpu, new, dtype):
+    """Long enough for workgroups of eight waves; 8 and 24 rows."""
+    case = Paged([900, 5, 640], new=new, heads=16, kv_heads=2, head_dim=64, page_size=16, dtype=dtype, window=700, n_starting=20)
+    check(_run(gpu, case, max_seqlen_q=max(new), max_seqlen_k=900), case.truth())
+
+
 def test_a_batch_of_thousands(gpu):
     """Requests past the 64 that a wave looks at together, few and none of tokens and keys among them."""
     n = 1500
