@@ -1103,7 +1103,7 @@ static RowShares row_shares(const dcp_paged_attn_args& x, int batch, int64_t max
   RowShares best = {1, 1e30};
   for (int s = 1; s <= most; ++s) {
     const int64_t n_wg = xcd_grid_size(groups * s, 1) * group, rounds = (n_wg + 2 * n_cu - 1) / (2 * n_cu);
-    const double us = rounds * (7 + (double)tiles / s * (n_wg <= n_cu ? 1.1 : 2.0) * x.head_dim / 128) + (s > 1 || joined_anyway ? s * share_us : 0) +
+    const double us = rounds * (7 + (double)tiles / s * (n_wg <= n_cu ? 1.0 + 0.1 * x.head_dim / 128 : 0.5 + 1.5 * x.head_dim / 128)) + (s > 1 || joined_anyway ? s * share_us : 0) +
                       (s > 1 && !joined_anyway ? 3.5 : 0);
     if (us < best.us) best = {s, us};
   }
@@ -1132,13 +1132,18 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
     const double unit_us = keys * (0.004 + 0.007 * x.head_dim / 128);
     few_us = 0.5 * units * keys * x.head_dim * 4 / 5.4e6;
     plan.whole = x.n_prefixes > 0 ? keys <= 2048 : unit_us < 8 + std::min(few_us, 9.0);
-    plan.n_few = plan.whole ? (int)most_units : 2 * device_cu_count();
+    const int slots = 2 * device_cu_count();
     // Of eight waves where a CU has at most one and could hold two (head size 64): 32 windows of 1016 keys 14.1, of four 14.6; 16 of
     // 2048 20.6 and 22.2, of 256 7.4 and 7.0.
     plan.waves = plan.whole && x.head_dim == 64 && x.n_prefixes == 0 && units <= device_cu_count() && keys > 512 ? 8 : 4;
-    // Four heads at once from 64 tiles a workgroup on (16 for each wave).
-    const int64_t tiles = (int64_t)x.batch * ((keys + kFewBN - 1) / kFewBN) * x.n_heads_kv / plan.n_few;
-    plan.heads = plan.whole || tiles < 64 ? 1 : x.n_heads_kv % 4 == 0 ? 4 : x.n_heads_kv % 2 == 0 ? 2 : 1;
+    // Heads at once, a wave or two for each: of whole units while there are more than the CUs hold and a wave's chain stays short,
+    // which its start and end outlast (us, one, two and four heads: 128 requests of 16 keys 15, 9.6 and 9.9, of 256 31.5, 27.9 and 28.0; 512 of
+    // 64 64, 44 and 35, of up to 512 105, 82 and 87; 64 of 64 8.2, 8.7 and 10.8); of equal shares four from 64 tiles a workgroup on.
+    const int64_t tiles = (int64_t)x.batch * ((keys + kFewBN - 1) / kFewBN) * x.n_heads_kv / slots;
+    while (plan.heads < 4 && x.n_heads_kv % (2 * plan.heads) == 0 &&
+           (plan.whole ? units / plan.heads > slots && 2 * plan.heads * keys <= 1280 : tiles >= 64))
+      plan.heads *= 2;
+    plan.n_few = plan.whole ? (int)(most_units / plan.heads) : slots;
     if (!plan.whole) {
       plan.cuts = up16((size_t)x.n_tokens * x.n_heads_q * sizeof(int2));
       plan.slots = (size_t)plan.n_few * 2 * plan.heads * plan.rows * (x.head_dim + 2) * sizeof(float);

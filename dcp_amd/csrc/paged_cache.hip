@@ -15,7 +15,6 @@
 
 namespace dcp {
 
-constexpr int kTablesThreads = 256;
 
 struct CacheTablesParams {
   const int32_t* cached_lens;
@@ -50,10 +49,11 @@ struct StepSums {
   int64_t tokens, pages;
 };
 
-__global__ __launch_bounds__(kTablesThreads) void paged_cache_tables_kernel(const CacheTablesParams p) {
-  __shared__ StepSums ends[kTablesThreads];  // sums up to and with each thread's requests
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_cache_tables_kernel(const CacheTablesParams p) {
+  __shared__ StepSums ends[THREADS];  // sums up to and with each thread's requests
   const int tid = threadIdx.x;
-  const int per_thread = (p.batch + kTablesThreads - 1) / kTablesThreads;
+  const int per_thread = (p.batch + THREADS - 1) / THREADS;
   const int b0 = min(tid * per_thread, p.batch), b1 = min(b0 + per_thread, p.batch);
   StepSums sum = {0, 0};
   for (int b = b0; b < b1; ++b) {
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kTablesThreads) void paged_cache_tables_kernel(cons
   }
   ends[tid] = sum;
   __syncthreads();
-  for (int step = 1; step < kTablesThreads; step *= 2) {
+  for (int step = 1; step < THREADS; step *= 2) {
     StepSums before = {0, 0};
     if (tid >= step) before = ends[tid - step];
     __syncthreads();
@@ -71,12 +71,12 @@ __global__ __launch_bounds__(kTablesThreads) void paged_cache_tables_kernel(cons
     ends[tid].pages += before.pages;
     __syncthreads();
   }
-  const StepSums all = ends[kTablesThreads - 1];
-  const int first = blockIdx.x * kTablesThreads + tid, stride = gridDim.x * kTablesThreads;
+  const StepSums all = ends[THREADS - 1];
+  const int first = blockIdx.x * THREADS + tid, stride = gridDim.x * THREADS;
 
   // the request that holds the `index`-th of the tokens or pages, and the sums before it
   auto find = [&](int64_t index, auto of, StepSums& before) -> int {
-    int lo = 0, hi = kTablesThreads - 1;  // the first thread whose sum passes it
+    int lo = 0, hi = THREADS - 1;  // the first thread whose sum passes it
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
       if (of(ends[mid]) > index) hi = mid;
@@ -211,9 +211,15 @@ extern "C" int dcp_paged_cache_tables(const int32_t* cached_lens, const int32_t*
   CacheTablesParams p = {cached_lens, new_lens, block_table, table_stride, free_pages, slot_mapping, positions, cu_seqlens,
                          seq_lens, pages_taken, batch, table_width, n_free, page_size, n_tokens};
   const int64_t most = std::max(n_tokens, 1);
-  const int n_wg = (int)std::min<int64_t>((most + kTablesThreads - 1) / kTablesThreads, 2 * device_cu_count());
   KernelTimer timer("paged_cache_tables_kernel", stream);
-  hipLaunchKernelGGL(paged_cache_tables_kernel, dim3(n_wg), dim3(kTablesThreads), 0, (hipStream_t)stream, p);
+  const auto launch = [&](auto kernel, int threads) {
+    const int n_wg = (int)std::min<int64_t>((most + threads - 1) / threads, 2 * device_cu_count());
+    hipLaunchKernelGGL(kernel, dim3(n_wg), dim3(threads), 0, (hipStream_t)stream, p);
+  };
+  // A thread takes the lengths of batch / threads requests one after the other, and as many again for a token or page.
+  // us, of 256 and of 1024 threads: 4090 requests 18.5 and 12.2, 1024 7.9 and 8.0.
+  if (batch <= 1024) launch(paged_cache_tables_kernel<256>, 256);
+  else launch(paged_cache_tables_kernel<1024>, 1024);
   return check_launch("paged_cache_tables_kernel");
 }
 

@@ -61,6 +61,12 @@ def test_tables_of_random_lengths(gpu):
         _tables(gpu, cached, new, int(rng.choice([1, 16, 48, 64])), int(rng.integers(1, 40)), int(rng.integers(0, 3000)), int(rng.integers(0, 9)), seed)
 
 
+def test_tables_of_thousands_of_requests(gpu):
+    rng = np.random.default_rng(3)
+    for n in (1024, 1025, 3001):
+        _tables(gpu, rng.integers(0, 100, n).tolist(), rng.integers(0, 3, n).tolist(), 16, 9, 2000, 5, n)
+
+
 def test_tables_with_lengths_near_the_types_end(gpu):
     """Sums that pass 32 bits: no token is entered twice, nothing outside of the tables is touched."""
     most = 2**31 - 1
