@@ -162,17 +162,32 @@ constexpr int kMinTilesPerShare = 2;
 constexpr float kNoMax = -3.0e38f;  // the reference of a row that has seen nothing: below every score, and a weight of -inf against it is 0
 constexpr float kMaxTileSum = 16384.0f;  // of a lane's weights against a reference that is not their maximum: fp16 can hold them
 
-// Row tile `tile` belongs to request b and is its tile number `index` (negative: to none).  Request b's tiles begin at number
-// floor(first_row / 128) + b: that leaves room for its last, partial one, and needs no sum over the requests before it.
+// Sum over the wave's lanes up to and with this one.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
+// The row tile of place `place`, the last one first: tile number `index` of request b's (negative: there is none).
 struct RowTile {
   int b, index;
   TokenRange tokens;
   int n_keys;
 };
-__device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, int tile) {
+__device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, int place) {
   const int lane = threadIdx.x & 63;
+  // Up to 64 requests are counted.  Of more, request b's tiles begin at number floor(first_row / 128) + b: that leaves room for its last,
+  // partial one, and needs no sum over the requests before it, but its places without a tile lie among the others, and CUs with two tiles
+  // beside CUs with none (24 requests of 128 rows on 1024 keys, nearly half of the places empty: 40 us, counted 35; 64 of 64 rows on 4096 267
+  // and 213).
   auto start = [&](int first, int b) { return (int)((int64_t)first * p.group / kRowsBM) + b; };
-  int lo = 0, hi = src.batch;  // the last request that begins at or before the tile; 64 candidates a step
+  const bool counted = src.batch <= 64;
+  int tile = src.n_tiles - 1 - place, lo = 0, hi = src.batch;  // the last request that begins at or before the tile; 64 candidates a step
   while (hi - lo > 64) {
     const int step = (hi - lo + 63) / 64, b = lo + lane * step;
     const bool before = b < hi && start(first_token(p, src, b), b) <= tile;
@@ -183,26 +198,36 @@ __device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, 
   // A lane looks at one request, and at all there is to know of it: another trip to memory for the one that is found is a microsecond.
   const int b = min(lo + lane, hi - 1);
   const TokenRange tokens = tokens_of(p, src, b);
-  const int n_keys = keys_of(p, src, b), first_tile = start(tokens.begin, b);
-  const int at = __builtin_amdgcn_readfirstlane(max(__popcll(__ballot((lo + lane < hi) & (first_tile <= tile))) - 1, 0));
+  const int n_keys = keys_of(p, src, b), n_tiles = (tokens.n * p.group + kRowsBM - 1) / kRowsBM;
+  int first_tile = start(tokens.begin, b), passed;
+  if (counted) {
+    const int ends = wave_scan(lane < hi ? n_tiles : 0);
+    tile = __builtin_amdgcn_readlane(ends, 63) - 1 - place;
+    first_tile = ends - n_tiles;
+    passed = __popcll(__ballot((lane < hi) & (ends <= tile)));
+  } else {
+    passed = max(__popcll(__ballot((lo + lane < hi) & (first_tile <= tile))) - 1, 0);
+  }
+  const int at = __builtin_amdgcn_readfirstlane(min(passed, hi - lo - 1));
   auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-  return {of(b), tile - of(first_tile), {of(tokens.begin), of(tokens.n)}, of(n_keys)};
+  const int index = of(tile - first_tile);
+  return {of(b), (tile >= 0) & (index < of(n_tiles)) ? index : -1, {of(tokens.begin), of(tokens.n)}, of(n_keys)};
 }
 
 // Which work item workgroup `wg` takes.  The items of a group, `group` neighbouring row tiles of a kv head, read the same keys and go to one
 // XCD (workgroup ids go round the eight), whose L2 then reads them once.  From one round of eight groups to the next the XCDs
 // move on by one, so that the groups of one kv head do not all go to the same XCD where there are eight.  The tiles of a request's last
-// tokens, which see the most, come first.
+// tokens, which see the most, come first, places without a tile last.
 struct RowItem {
-  int tile, kv_head, share;  // share: -1 for none
+  int place, kv_head, share;  // share: -1 for none
 };
 __device__ __forceinline__ RowItem row_item(int wg, int n_tiles, int group, int n_heads_kv, int n_shares) {
   const int per_round = kNumXcd * group, round = wg / per_round, in_round = wg - round * per_round;
   int i = round * kNumXcd + (in_round + round) % kNumXcd;  // the group
-  const int n_groups = (n_tiles + group - 1) / group, kv_head = i % n_heads_kv;
+  const int kv_head = i % n_heads_kv;
   i /= n_heads_kv;
-  const int tile = n_tiles - 1 - (i % n_groups * group + in_round / kNumXcd), share = i / n_groups;
-  return {tile, kv_head, (tile >= 0) & (share < n_shares) ? share : -1};
+  const int place = i / n_shares * group + in_round / kNumXcd, share = i % n_shares;
+  return {place, kv_head, place < n_tiles ? share : -1};
 }
 inline int64_t row_workgroups(int64_t n_tiles, int group, int n_heads_kv, int n_shares) {
   return xcd_grid_size((n_tiles + group - 1) / group * n_heads_kv * n_shares, 1) * group;
@@ -231,13 +256,13 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   // ---- which rows, which share of their keys ---------------------------------
   const RowItem at = row_item(item, src.n_tiles, src.xcd_group, p.n_heads_kv, src.n_shares);
   if (at.share < 0) return;
-  const int tile_number = __builtin_amdgcn_readfirstlane(at.tile), kv_head = __builtin_amdgcn_readfirstlane(at.kv_head);
+  const int place = __builtin_amdgcn_readfirstlane(at.place), kv_head = __builtin_amdgcn_readfirstlane(at.kv_head);
   const int share = __builtin_amdgcn_readfirstlane(at.share);
-  const RowTile tile = find_row_tile(p, src, tile_number);
+  const RowTile tile = find_row_tile(p, src, place);
   const TokenRange tokens = tile.tokens;
   const int n_rows = tokens.n * p.group;  // (at most n_tokens * group, which the host has checked)
   const int row0 = tile.index * kRowsBM;
-  if (tile.index < 0 || row0 >= n_rows) return;
+  if (tile.index < 0) return;
   const bool prefix = src.cu_groups != nullptr;
   const int n_keys = tile.n_keys, window = prefix ? 0 : p.window, n_starting = p.n_starting;
   // token i of the request is at position n_keys - n + i; every token is past all of a prefix
@@ -567,16 +592,6 @@ struct FewRequest {
   }
 };
 
-// Sum over the wave's lanes up to and with this one.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
-  return x;
-}
 __device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
   const uint32_t lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
   return (int64_t)(((uint64_t)hi << 32) | lo);

@@ -102,6 +102,14 @@ def test_units_whole_and_cut(gpu, name, longest):
     check(_run(gpu, case, max_seqlen_k=longest), case.truth())
 
 
+@pytest.mark.parametrize("requests", [63, 64, 65, 130])
+def test_row_tiles_of_many_requests(gpu, requests):
+    """Tiles counted and not, of requests without tokens, with a part of a tile and with several."""
+    new = [(0, 3, 17, 64, 65)[(i * 7 + i // 5) % 5] for i in range(requests)]
+    case = Paged([n + (i * 13) % 60 for i, n in enumerate(new)], new=new, heads=4, kv_heads=2, head_dim=64, page_size=16)
+    check(_run(gpu, case), case.truth())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, F16])
 @pytest.mark.parametrize("new", [[1, 1, 1], [3, 1, 2]])
 def test_whole_units_of_head_size_64(gpu, new, dtype):
