@@ -299,27 +299,32 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   int64_t* offsets = reinterpret_cast<int64_t*>(lds + Lds::OFFSETS);
   int* absent = reinterpret_cast<int*>(lds + Lds::ABSENT);
   int* any_absent = reinterpret_cast<int*>(lds + Lds::ANY_ABSENT);
-  auto look_up = [&](int rel) {
+  struct Entry {
+    int key, in_page, page;
+  };
+  auto read_entry = [&](int rel) -> Entry {
     PagedArgs& p = fresh_kernel_args<PagedParams>();
     const int i = (t_begin + rel) * 4 + tid, key = i < 4 * t_end ? group_key(i) : kNoKey;
-    int64_t off = 0;
-    bool there = false;
-    if (key != kNoKey) {
-      const int entry = key / p.page_size, page = src.block_table[tile.b * src.table_stride + entry];
-      there = (unsigned)page < (unsigned)p.n_pages;
-      if (there) off = page * p.page_stride + (int64_t)(key - entry * p.page_size) * p.token_stride;
-    }
+    if (key == kNoKey) return {key, 0, -1};
+    const int entry = key / p.page_size;
+    return {key, key - entry * p.page_size, src.block_table[tile.b * src.table_stride + entry]};
+  };
+  auto look_up = [&](int rel, Entry entry) {
+    PagedArgs& p = fresh_kernel_args<PagedParams>();
+    const bool there = (unsigned)entry.page < (unsigned)p.n_pages;
     const int at = (rel * 4 + tid) % (2 * kTableTiles * 4);
-    offsets[at] = off;
+    offsets[at] = there ? entry.page * p.page_stride + entry.in_page * p.token_stride : 0;
     absent[at] = !there;
-    const bool any = __any(!there & (key != kNoKey));  // (what is past the end is no tile of anybody's)
+    const bool any = __any(!there & (entry.key != kNoKey));  // (what is past the end is no tile of anybody's)
     if (lane == 0) any_absent[rel / kTableTiles % 2 * 4 + w] = any;
   };
   auto offset_of = [&](int t) { return offsets[((t - t_begin) * 4 + g) % (2 * kTableTiles * 4)]; };
 
+  Entry first_entry = {kNoKey, 0, -1};
+  if (t_begin < t_end) first_entry = read_entry(0);
+
   // ---- this lane's rows: n of each of the wave's two row tiles (past the last one: the last one again, not written) ------
   int last_key[RT];                          // the last key it sees
-  int first_last = 0x7fffffff, last_last = 0;  // of the wave's rows
   u32x4 q[RT][KS];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -328,10 +333,10 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + Tile::step16(ks));
     last_key[rt] = at0 + tok * step;
-    first_last = min(first_last, wave_min(last_key[rt]));
-    last_last = max(last_last, wave_max(last_key[rt]));
   }
-  if (t_begin < t_end) look_up(0);  // (after the rows were asked for)
+  // of the wave's rows (they do not decrease from lane to lane and tile to tile)
+  const int first_last = __builtin_amdgcn_readlane(last_key[0], 0), last_last = __builtin_amdgcn_readlane(last_key[RT - 1], 15);
+  if (t_begin < t_end) look_up(0, first_entry);  // (asked for before the rows, there before them)
   const int reach = window > 0 ? window : 0x7fffffff;  // a query sees the keys less than this before its last
   const float scale = p.scale_log2;
 
@@ -457,7 +462,10 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     wait_loads();
     const bool full = is_full(t);
     if (__builtin_expect(!full, 0)) clear_v(t);
-    if (__builtin_expect((t - t_begin) % kTableTiles == kTableTiles / 2, 0)) look_up((t - t_begin) / kTableTiles * kTableTiles + kTableTiles);
+    if (__builtin_expect((t - t_begin) % kTableTiles == kTableTiles / 2, 0)) {
+      const int rel = (t - t_begin) / kTableTiles * kTableTiles + kTableTiles;
+      look_up(rel, read_entry(rel));
+    }
     __syncthreads();  // K of tile t + 1 and V of tile t are there; nobody reads K of tile t or V of tile t - 1 any more
     // The loads of K of tile t + 2 and V of tile t + 1 go out between the products, unconditionally: past the end a page that there
     // is comes into a stage that nobody reads any more.
