@@ -317,6 +317,41 @@ def test_on_another_stream(gpu, prefix):
     check(got, truth)
 
 
+def test_calls_at_the_same_time(gpu):
+    """Two streams, and two graphs with a workspace each, replayed side by side."""
+    cases = [Paged([3000, 9, 700], heads=4, kv_heads=2), Paged([2500, 30], heads=4, kv_heads=2, prefixes=[3000], cu_groups=[0, 2], seed=1)]
+    calls = [(paged_cache_attention, paged_cache_workspace_bytes), (shared_prefix_attention, shared_prefix_workspace_bytes)]
+    args, truths, streams = [c.to(gpu) for c in cases], [c.truth() for c in cases], [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(calls[i][0](**args[i]))
+    torch.cuda.synchronize()
+    for results, truth in zip(got, truths):
+        for result in results:
+            check(result, truth)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in cases], []
+    for i, graph in enumerate(graphs):
+        more = dict(out=torch.empty_like(args[i]["q"]), lse=torch.empty(args[i]["q"].shape[1::-1], device=gpu),
+                    workspace=torch.empty(calls[i][1](**args[i]), dtype=torch.uint8, device=gpu))
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=streams[i]):
+            calls[i][0](**args[i], **more)
+        outs.append(more)
+    for _ in range(3):
+        for more in outs:
+            more["out"].fill_(9)
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for more, truth in zip(outs, truths):
+            check((more["out"], more["lse"]), truth)
+
+
 @pytest.mark.parametrize("prefix", [False, True])
 def test_captured_and_replayed_with_other_lengths(gpu, prefix):
     """One graph for all steps: lengths are read on the device."""
