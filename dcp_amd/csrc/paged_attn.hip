@@ -664,6 +664,9 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
   // ---- this workgroup's share of all tiles (the host has checked that their number fits 32 bits), or its unit -----------
   const int n_chunks = (p0.own.batch + 63) / 64;
   const bool whole_units = p0.few_whole != 0;
+  // Shares are counted in turns of the waves at a head's tiles: a cut inside one would cost both of its sides a whole one.  (One context
+  // of 1500 keys, 8 heads, which 47 tiles a head then fit no better: counted in tiles 14.4 us, in turns 11.4.)
+  const int turns_log2 = (NW == 8 ? 3 : 2) - p0.few_heads_log2, turns = 1 << turns_log2;
   auto requests_of = [&](int chunk, int& work) {
     PagedArgs& p = fresh_kernel_args<PagedParams>();
     const int b = chunk * 64 + lane;
@@ -673,7 +676,7 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
     work = 0;
     if (b < p.own.batch) {
       r = FewRequest(p, b);
-      work = r.units(p, ROWS) * (whole_units ? 1 : r.n_tiles);
+      work = r.units(p, ROWS) * (whole_units ? 1 : (r.n_tiles + turns - 1) >> turns_log2);
     }
     return r;
   };
@@ -692,7 +695,7 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
     __syncthreads();
     for (int i = 0; i < n_chunks; i += 64) total += __builtin_amdgcn_readlane(wave_scan(i + lane < n_chunks ? chunk_sums[i + lane] : 0), 63);
   }
-  const int per = whole_units ? 1 : max((total - 1) / p0.n_few + 1, NW >> p0.few_heads_log2);
+  const int per = whole_units ? 1 : (total - 1) / p0.n_few + 1;
   const int begin = (int)min((int64_t)wg * per, (int64_t)total), end = (int)min((int64_t)begin + per, (int64_t)total);
   if (begin >= end) return;
   if (n_chunks > 1) {
@@ -727,15 +730,15 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
     }
     PagedArgs& p = fresh_kernel_args<PagedParams>();
     // the workgroup's kv heads at once, the waves that take turns at a head's tiles, and which of each the wave is
-    const int heads = 1 << p.few_heads_log2, head_groups = p.n_heads_kv >> p.few_heads_log2, turns = NW >> p.few_heads_log2;
+    const int heads = 1 << p.few_heads_log2, head_groups = p.n_heads_kv >> p.few_heads_log2;
     const int my_head = w & (heads - 1), my_turn = w >> p.few_heads_log2;
     const FewRequest request = requests.of_lane(index);
     const int b = chunk * 64 + index, in_request = at - (unit_end - __builtin_amdgcn_readlane(work, index));
     if (in_request < 0) break;  // (tables whose tokens are many times those there are: their sums wrap)
-    const int unit = whole_units ? in_request : __builtin_amdgcn_readfirstlane(in_request / request.n_tiles);
-    const int t_begin = whole_units ? 0 : in_request - unit * request.n_tiles;
-    const int t_end = whole_units ? request.n_tiles : min(request.n_tiles, t_begin + (end - at));
-    const int taken = whole_units ? 1 : t_end - t_begin;
+    const int unit_turns = whole_units ? 1 : (request.n_tiles + turns - 1) >> turns_log2;
+    const int unit = __builtin_amdgcn_readfirstlane(in_request / unit_turns);
+    const int first_turn = in_request - unit * unit_turns, taken = min(unit_turns - first_turn, end - at);
+    const int t_begin = whole_units ? 0 : first_turn * turns, t_end = whole_units ? request.n_tiles : min(request.n_tiles, t_begin + taken * turns);
     at += taken;
     const int kv_head0 = unit % head_groups * heads, kv_head = kv_head0 + my_head, row0 = unit / head_groups * ROWS;
     const KeyGroups groups = request.groups(p);
@@ -930,9 +933,9 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
     }
     __syncthreads();
     PagedArgs& p_out = fresh_kernel_args<PagedParams>();
-    const bool cut = t_end - t_begin < request.n_tiles;
+    const bool cut = taken < unit_turns;
     const int slot = at - taken == begin ? 0 : 1;
-    const int n_cut = (at - taken + request.n_tiles - 1) / per - wg + 1;  // (of a unit that begins here: it ends so many workgroups on)
+    const int n_cut = (at - taken + unit_turns - 1) / per - wg + 1;  // (of a unit that begins here: it ends so many workgroups on)
     const int group = p_out.group;
     constexpr int PIECES = D / 4;  // of a row
     for (int i = tid; i < heads * ROWS * PIECES; i += NW * 64) {
@@ -1181,13 +1184,13 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
   if (plan.few) {
     // Whole units where they are short: the chain of one's tiles (of a fourth of them) against what cutting costs, a second kernel and
     // more, and, as far as that goes, against the equal shares' time (of lengths that are half the longest on average, at 5.4 TB/s).
-    // us, whole and cut, 8 kv heads of 128: 4 requests of 32 keys 6.0 and 18, of 512 11.2 and 11.0, of 1024 17 and 12; 32 of 512 16 and 21,
-    // of 1024 26 and 31, of up to 1024 20 and 23, of up to 2048 32 and 32; 64 of up to 64 9 and 22, of up to 2048 50 and 45;
-    // 192 of up to 256 32 and 54, of 1024 132 and 141.  Beside a prefix's shares, which are joined anyway, always as
+    // us, whole and cut, 8 kv heads of 128: 1 request of 100 keys 6.8 and 9.5, of 512 9.5 and 10.9, of 1024 15 and 11; 16 of 300 11 and 13, of
+    // 1024 20 and 21, of up to 1024 18 and 15; 32 of 512 16 and 21, of 1400 34 and 42, of up to 1400 25 and 27, of 2048 48 and 52, of up
+    // to 2048 33 and 30; 64 of up to 200 11 and 16, of up to 1400 37 and 40.  Beside a prefix's shares, which are joined anyway, always as
     // long as units are short: 64 requests on a prefix of 32768 80 and 87.
     const double unit_us = keys * (0.004 + 0.007 * x.head_dim / 128);
     few_us = 0.5 * units * keys * x.head_dim * 4 / 5.4e6;
-    plan.whole = x.n_prefixes > 0 ? keys <= 2048 : unit_us < 8 + std::min(few_us, 9.0);
+    plan.whole = x.n_prefixes > 0 ? keys <= 2048 : unit_us < 5.5 + std::min(0.6 * few_us, 10.5);
     const int slots = 2 * device_cu_count();
     // Of eight waves where a CU has at most one and could hold two (head size 64): 32 windows of 1016 keys 14.1, of four 14.6; 16 of
     // 2048 20.6 and 22.2, of 256 7.4 and 7.0.
