@@ -1180,17 +1180,18 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
   const int64_t most_units = (all_rows + (int64_t)x.batch * (plan.rows - 1)) / plan.rows * x.n_heads_kv;
   const int64_t units = std::max<int64_t>(x.batch, all_rows / plan.rows) * x.n_heads_kv;
   plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2) < 2e9;
+  const RowShares prefix_shares = x.n_prefixes > 0 ? row_shares(x, x.n_prefixes, x.max_prefix_len, true) : RowShares{0, 0};
   double few_us = 0;
   if (plan.few) {
     // Whole units where they are short: the chain of one's tiles (of a fourth of them) against what cutting costs, a second kernel and
     // more, and, as far as that goes, against the equal shares' time (of lengths that are half the longest on average, at 5.4 TB/s).
     // us, whole and cut, 8 kv heads of 128: 1 request of 100 keys 6.8 and 9.5, of 512 9.5 and 10.9, of 1024 15 and 11; 16 of 300 11 and 13, of
     // 1024 20 and 21, of up to 1024 18 and 15; 32 of 512 16 and 21, of 1400 34 and 42, of up to 1400 25 and 27, of 2048 48 and 52, of up
-    // to 2048 33 and 30; 64 of up to 200 11 and 16, of up to 1400 37 and 40.  Beside a prefix's shares, which are joined anyway, always as
-    // long as units are short: 64 requests on a prefix of 32768 80 and 87.
+    // to 2048 33 and 30; 64 of up to 200 11 and 16, of up to 1400 37 and 40.  Beside a prefix's shares, which are joined anyway, also
+    // where these take as long: 64 requests of up to 1024 own keys on a prefix of 32768 80 and 87, but 4 of up to 2000 on one of 2000 33 and 18.
     const double unit_us = keys * (0.004 + 0.007 * x.head_dim / 128);
     few_us = 0.5 * units * keys * x.head_dim * 4 / 5.4e6;
-    plan.whole = x.n_prefixes > 0 ? keys <= 2048 : unit_us < 5.5 + std::min(0.6 * few_us, 10.5);
+    plan.whole = unit_us < std::max(5.5 + std::min(0.6 * few_us, 10.5), keys <= 2048 ? prefix_shares.us - 6 : 0.0);
     const int slots = 2 * device_cu_count();
     // Of eight waves where a CU has at most one and could hold two (head size 64): 32 windows of 1016 keys 14.1, of four 14.6; 16 of
     // 2048 20.6 and 22.2, of 256 7.4 and 7.0.
@@ -1211,12 +1212,11 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
     plan.n_own = row_shares(x, x.batch, keys, x.n_prefixes > 0).n;
   }
   if (x.n_prefixes > 0) {
-    const RowShares shares = row_shares(x, x.n_prefixes, x.max_prefix_len, true);
-    plan.n_prefix = shares.n;
+    plan.n_prefix = prefix_shares.n;
     // All of the few first where theirs is most of the time: the prefix's then fill what they leave at their end.  us, all first and one
     // a CU first: 64 requests of up to 1024 own keys on a prefix of 32768 84 and 75, of 64 own keys 77 and 66; 256 of up to 600 on 8192
     // 114 and 97; 128 of up to 2000 on 8192 110 and 115; 64 of up to 6000 on 16384 122 and 125.
-    plan.few_first = few_us < 1.5 * shares.us ? std::min(plan.n_few, device_cu_count()) : plan.n_few;
+    plan.few_first = few_us < 1.5 * prefix_shares.us ? std::min(plan.n_few, device_cu_count()) : plan.n_few;
   }
   if (plan.n_own + plan.n_prefix > 1) plan.shares = (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
   return plan;
