@@ -5,10 +5,13 @@ reference executor imports from its flash-attention fork
 ``dcp/runtime/flash_attention/executor.py:161-184`` and ``:303-334``), with the
 same argument order, backed by the gfx950 kernels of ``libdcp_hip.so``.
 
-Only the configuration the executor uses is implemented: no dropout, no causal
+Only the configuration the executor uses is implemented of them: no dropout, no causal
 flag, no sliding window, no softcap, no alibi; masking comes from
 ``attn_range`` and all tensors are paged through block tables.  Anything else
 raises ``NotImplementedError`` rather than computing something different.
+
+Beside them, with no counterpart in the reference, what answering takes: attention over a paged K/V cache
+(``paged_cache_attention``) and of requests that share prefixes in it (``shared_prefix_attention``), forward only.
 """
 
 from __future__ import annotations

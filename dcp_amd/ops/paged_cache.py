@@ -86,7 +86,8 @@ def paged_cache_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_
 def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor) -> None:
     """Writes ``k`` and ``v`` (``[n_tokens, n_heads_kv, D]``) into the caches (``[n_pages, page_size, n_heads_kv, D]``, any
     strides, a cache's two halves for instance) at ``slot_mapping`` (int64 ``[n_tokens]``).  Slots outside of the cache are skipped,
-    so the -1 of padding writes nothing; the others have to differ from each other.  Any type of 1, 2 or 4 bytes."""
+    so the -1 of padding writes nothing; the others have to differ from each other, and ``k`` and ``v`` may not lie in the caches.
+    Any type of 1, 2 or 4 bytes."""
     here, dtype = torch._C._cuda_getDevice(), k_cache.dtype
     k_at, v_at = _check(k, dtype, "k", here, dense=False), _check(v, dtype, "v", here, dense=False)
     k_cache_at, v_cache_at = _check(k_cache, dtype, "k_cache", here, dense=False), _check(v_cache, dtype, "v_cache", here, dense=False)
