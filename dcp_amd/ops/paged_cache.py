@@ -41,6 +41,13 @@ def _check(t, dtype, name: str, here: int, shape=None, dense: bool = True) -> in
     return t.data_ptr()
 
 
+def _number(x, name: str) -> int:
+    """A whole number of 32 bits, which is what the library takes: the call would cut any other without a word."""
+    if not -(2**31) <= x < 2**31 or int(x) != x:
+        raise ValueError(f"{name} must be a whole number of 32 bits, got {x}")
+    return int(x)
+
+
 def paged_cache_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                        page_size: int, n_tokens: int, out: Optional[PagedCacheTables] = None) -> PagedCacheTables:
     """The tables of a step in which request ``b``, with ``cached_lens[b]`` tokens in the cache, adds ``new_lens[b]``.
@@ -65,7 +72,8 @@ def paged_cache_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_
     free = _check(free_pages, i32, "free_pages", here)
     if free_pages.dim() != 1:
         raise ValueError(f"free_pages must have one axis, got {list(free_pages.shape)}")
-    n_tokens = int(n_tokens)
+    n_tokens, page_size, n_free = _number(n_tokens, "n_tokens"), _number(page_size, "page_size"), free_pages.shape[0]
+    _number(max(n, width, n_free), "the longest of the tables")
     if n_tokens < 0:
         raise ValueError(f"n_tokens must not be negative, got {n_tokens}")
     if out is None:  # (one tensor for the four of 32 bits: five allocations are a third of a small step's time)
@@ -78,7 +86,7 @@ def paged_cache_tables(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_
         addresses = (_check(out.slot_mapping, torch.int64, "slot_mapping", here, (n_tokens,)),
                      _check(out.positions, i32, "positions", here, (n_tokens,)), _check(out.cu_seqlens, i32, "cu_seqlens", here, (n + 1,)),
                      _check(out.seq_lens, i32, "seq_lens", here, (n,)), _check(out.pages_taken, i32, "pages_taken", here, (1,)))
-    _lib.call("dcp_paged_cache_tables", lens, new, table, stride, free, *addresses, n, width, free_pages.shape[0], int(page_size), n_tokens,
+    _lib.call("dcp_paged_cache_tables", lens, new, table, stride, free, *addresses, n, width, n_free, page_size, n_tokens,
               torch._C._cuda_getCurrentRawStream(here))
     return out
 
@@ -98,6 +106,7 @@ def paged_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tens
     if k.dim() != 3 or k.shape != v.shape or in_strides != v.stride() or tuple(k.shape[1:]) != (heads, head_dim) or (head_dim > 1 and in_strides[2] != 1):
         raise ValueError(f"k and v must be [n_tokens, {heads}, {head_dim}] with the same strides and dense rows")
     n_tokens = k.shape[0]
+    _number(max(n_tokens, page_size, heads, head_dim), "the largest size")
     slots = _check(slot_mapping, torch.int64, "slot_mapping", here, (n_tokens,))
     _lib.call("dcp_paged_cache_write", k_at, v_at, slots, k_cache_at, v_cache_at, n_tokens, heads, head_dim, k.element_size(), in_strides[0],
               in_strides[1], n_pages, page_size, strides[0], strides[1], strides[2], torch._C._cuda_getCurrentRawStream(here))
