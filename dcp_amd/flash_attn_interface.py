@@ -532,7 +532,7 @@ def _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_se
         head_dim ** -0.5 if softmax_scale is None else softmax_scale)
     try:
         return out, lse, _PAGED_ARGS.pack(*args)
-    except struct.error as e:
+    except (struct.error, OverflowError) as e:  # (the second: a scale past the type's end)
         raise ValueError(f"sizes, lengths, window and n_starting must be whole numbers of 32 bits, softmax_scale a number: {e}") from None
 
 

@@ -52,3 +52,13 @@ def test_sizes_of_writes_that_do_not(here, wrong):
     with pytest.raises(ValueError, match="32 bits"):
         _write(**wrong)
     assert not here
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, "half"])
+def test_a_scale_that_32_bits_do_not_hold(here, scale):
+    from dcp_amd.flash_attn_interface import _paged_args
+
+    bf16 = torch.bfloat16
+    q, cache = _empty(2, 4, 64, dtype=bf16), _empty(3, 16, 2, 64, dtype=bf16)
+    with pytest.raises(ValueError, match="softmax_scale"):
+        _paged_args(q, cache, cache, _empty(2, 3), _empty(2), None, None, None, scale, None, 0, None, None)
