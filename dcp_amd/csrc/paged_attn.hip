@@ -257,9 +257,11 @@ struct RowsLds {
 };
 
 // CORRECTED: O is divided by the sum of the rounded weights instead of theirs (l / rounded times as much), so that rounding a weight that
-// outweighs the others cancels: rms error against 64 bits of prefixes 0.0023 -> 0.0019 in bf16 (0.0017 is the result's own rounding), lse
-// as it was.  Beside a prefix's chain of tiles the second sum costs nothing (64 requests on one of 32768 74.3 and 74.6 us), a prompt of 8192
-// 481 and 521, with an error of 0.0023 and 0.0022: not there.
+// outweighs the others cancels, lse as it was.  Prefixes have it in every launch: what the host says of the longest lengths chooses the
+// launch, and is not to choose the rounding.  rms error against 64 bits in bf16 (0.0017 is the result's own rounding): one token a
+// request 0.0023 -> 0.0019, 64 tokens each 0.0023 -> 0.0020.  Beside a prefix's chain of tiles the second sum costs nothing (64 requests of
+// one token on a prefix of 32768 74.3 and 74.6 us), where products bound it 3-4 % (32 requests of 256 tokens on one of 4096 663 and 690, 4
+// of 2048 on 16384 2105 and 2178).  Own keys have it not: a prompt of 8192 481 and 521 us, for an error of 0.0023 and 0.0022.
 template <int DTYPE, int D, bool CORRECTED>
 __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int item, char* lds) {
   typedef KvTile<D> Tile;
@@ -972,11 +974,11 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
 }
 
 // ---- kernels --------------------------------------------------------------------------
-template <int DTYPE, int D>
+template <int DTYPE, int D, bool CORRECTED>
 __global__ __launch_bounds__(kRowsThreads, 2) void paged_rows_kernel(const PagedParams) {
   __shared__ __attribute__((aligned(16))) char lds[RowsLds<D>::BYTES];
   PagedArgs& p = fresh_kernel_args<PagedParams>();
-  paged_rows<DTYPE, D, false>(p, p.own, blockIdx.x, lds);
+  paged_rows<DTYPE, D, CORRECTED>(p, p.own, blockIdx.x, lds);
 }
 
 template <int DTYPE, int D, int RT, int NW>
@@ -1322,10 +1324,10 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
     if (plan.rows == 16) launch(DCP_PAGED_KERNEL(paged_few_kernel, 1, 4), "paged_few_kernel", p.n_few, 256);
     else launch(DCP_PAGED_KERNEL(paged_few_kernel, 2, 4), "paged_few_kernel", p.n_few, 256);
   } else {
-    launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own), kRowsThreads);
+    launch(DCP_PAGED_KERNEL(paged_rows_kernel, false), "paged_rows_kernel", row_items(p.own), kRowsThreads);
     if (x.n_prefixes > 0) {
       std::swap(p.own, p.prefix);  // (the kernel takes what it finds there)
-      launch(DCP_PAGED_KERNEL(paged_rows_kernel), "paged_rows_kernel", row_items(p.own), kRowsThreads);
+      launch(DCP_PAGED_KERNEL(paged_rows_kernel, true), "paged_rows_kernel", row_items(p.own), kRowsThreads);
       std::swap(p.own, p.prefix);
     }
   }
