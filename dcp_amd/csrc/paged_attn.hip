@@ -1038,10 +1038,9 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
   const int n_own = n_cut > 0 ? n_cut : p.direct ? 0 : p.own.n_shares;  // (no memory for shares where rows are done at once)
   const int n_parts = n_own + (prefixes ? p.prefix.n_shares : 0);
   const int slot_rows = p.few_rows << p.few_heads_log2, slot_row = min(cut.y >> 20 & 0xff, slot_rows - 1), slot = cut.y >> 28 & 1;
-  // (& on purpose: of two conditions joined by && or || here, this compiler, clang 22, left the second one out)
-  const bool has_prefix = prefixes & (token >= prefix_first) & (token < prefix_end);
+  const bool has_prefix = prefixes && token >= prefix_first && token < prefix_end;
   // rows of no request are left as they were; one that has no parts is done where it was computed
-  const bool mine = (row64 < n_rows) & (token >= first) & (token < end) & (n_parts > 0);
+  const bool mine = row64 < n_rows && token >= first && token < end && n_parts > 0;
   // (kept in registers: a choice between two of the arguments was made by loading the chosen one, for every part anew)
   typedef __attribute__((address_space(1))) const f32x4 GlobalOut;
   typedef __attribute__((address_space(1))) const f32x2 GlobalSums;
@@ -1076,7 +1075,7 @@ __global__ __launch_bounds__(kPagedMergeThreads) void paged_merge_kernel(const P
     float m_new = m;
 #pragma unroll
     for (int x = 0; x < AT_ONCE; ++x) {
-      if (!((i0 + x * row_sets < n_own) | has_prefix)) ml[x] = f32x2{-INFINITY, 0.0f};
+      if (i0 + x * row_sets >= n_own && !has_prefix) ml[x] = f32x2{-INFINITY, 0.0f};
       m_new = fmaxf(m_new, ml[x][0]);
     }
     const float m_use = m_new == -INFINITY ? 0.0f : m_new, old = fast_exp2(m - m_use);
