@@ -139,7 +139,7 @@ __device__ __forceinline__ float add_pair(uint32_t pair, float sum) {
 }
 
 // 16 bytes a lane from memory into LDS at lds_at + 16 * lane (ordered by the caller, as KvTile's loads).  STREAM: read once, so it is
-// to take no room in the caches: four contexts of 131072 keys 369 -> 339 us.
+// to take no room in the caches: four contexts of 131072 keys 363 us without and 321 with it.
 template <bool STREAM>
 __device__ __forceinline__ void load_async_piece(uint32_t lds_at, const uint16_t* from) {
   if constexpr (STREAM)
@@ -593,14 +593,15 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 // takes no LDS and no reads of it, but its 16 lanes of a row's end lie in 16 rows: a CU's loads went at a fifth of its rate, a tile took a
 // lone workgroup 3.5 us instead of 2.3, and all of them 2-10 % more.)
 //
-// Work is cut by length, not by request: the tiles of all (request, rows, kv heads) units, and of the prefixes' where they have few
-// rows, are laid end to end and every workgroup takes the same number of them, whatever the lengths are (they are known on
-// the device only).  A unit inside one workgroup's share is finished there; of one that is cut each piece goes to the
-// workgroup's slot (0: the share begins in the unit, 1: it ends in it) and the merge joins them.
+// Work is cut by length, not by request: the tiles of all (request, rows, kv heads) units are laid end to end and every workgroup
+// takes the same number of them, whatever the lengths are (they are known on the device only).  A unit inside one workgroup's
+// share is finished there; of one that is cut each piece goes to the workgroup's slot (0: the share begins in the unit, 1: it
+// ends in it) and the merge joins them.
 //
 // Several kv heads at once: in a cache by token ([page][token][head]) a head's row is 256 bytes, and four heads' waves
-// side by side read 1 KiB of a token at about the same time: four contexts of 131072 keys 382 -> 339 us (in a cache by head 326 and 334).
-// With few tiles a workgroup the waves take turns at one head's tiles instead, which makes the chain of tiles shorter.
+// side by side read 1 KiB of a token at about the same time: four contexts of 131072 keys 344 us by one head and 321 by four (in a
+// cache by head 319 and 335).  With few tiles a workgroup the waves take turns at one head's tiles instead, which makes the chain of
+// tiles shorter.
 // ---------------------------------------------------------------------------
 // What the merge needs to know of a row: the workgroup that begins its unit, how many the unit is cut over, the slot of the first
 // piece (the others are in slot 0) and the row in the slots.
@@ -645,7 +646,7 @@ __device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
 template <int D, int RT, int NW>
 struct FewLds {
   static constexpr int ROWS = 16 * RT, LOADS = kFewBN * D * 2 / 1024, LOAD_BYTES = 1024 + 32, STAGE = LOADS * LOAD_BYTES;
-  static constexpr int O_STRIDE = D + 4;  // floats: rows of a wave's result, which takes the place of its V
+  static constexpr int O_STRIDE = D + 4;  // floats: rows of a wave's result, which takes the place of its K and as much of its V as it needs
   static constexpr int WAVE = 2 * STAGE > ROWS * O_STRIDE * 4 ? 2 * STAGE : ROWS * O_STRIDE * 4;
   static constexpr int SUMS = NW * WAVE;                  // float [wave][row][2]
   static constexpr int CHUNKS = SUMS + NW * ROWS * 2 * 4; // int [batch / 64]
@@ -891,7 +892,9 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
             x[e] = fast_exp2(fmaf(s[rt][kt][e], p.scale_log2, -m_use));
             l_run[rt] += x[e];
           }
-          pb[rt][2 * kt] = pack2<DTYPE>(x[0], x[1]);  // (rounded for the product, summed unrounded, as above)
+          // Rounded for the product, summed unrounded, and not CORRECTED: the reference is the row's maximum, whose weight of 1 is
+          // exact, and the second sum changed neither the time nor the error (0.0018 in bf16).
+          pb[rt][2 * kt] = pack2<DTYPE>(x[0], x[1]);
           pb[rt][2 * kt + 1] = pack2<DTYPE>(x[2], x[3]);
         }
       }

@@ -706,6 +706,7 @@ int dcp_paged_cache_write(const void* k, const void* v,
  *    arguments that are refused), 16-byte aligned, for shares of the keys that are
  *    joined afterwards; contents are overwritten.  Launches that may run at the
  *    same time need one each.
+ *  - *args is read in the call, and a recorded call keeps a copy of it.
  */
 typedef struct {
   const void* q;
