@@ -20,111 +20,12 @@
 // seen by no row (behind the last key, between the first tokens and the window, in a page that is not one) may hold anything: its
 // scores are masked by selection, and its V cleared in LDS by the lanes that brought it, since a weight of zero does not
 // make a NaN vanish.
-#include <math.h>
-
 #include <algorithm>
 
-#include "attn_common.h"
+#include "paged_common.h"
 #include "record.h"
 
 namespace dcp {
-
-// Keys that rows look at: the requests' own, or prefixes that requests share.
-struct PagedSource {
-  const int32_t* block_table;
-  const int32_t* key_lens;
-  const int32_t* cu_groups;  // prefixes: their requests; null for the requests' own keys
-  int64_t table_stride;
-  int table_width, batch;    // of prefixes or requests
-  int first_share, n_shares; // see PagedParams::partial_out
-  int n_tiles, xcd_group;    // row tiles of a kv head (kernel of rows); as many neighbouring work items are on one XCD
-  int by_few;                // the kernel of few rows takes it and may cut it (own keys)
-};
-
-struct PagedParams {
-  const void* q;
-  const void* k;
-  const void* v;
-  void* out;
-  float* lse;
-  const int32_t* cu_seqlens_q;  // null: one token a request
-  int64_t q_token, q_head, out_token, out_head;  // element strides
-  int64_t page_stride, token_stride, head_stride;
-  PagedSource own, prefix;  // (prefix.batch 0: none)
-  int n_pages, page_size;
-  int n_requests, n_tokens;  // of q
-  int n_heads_q, n_heads_kv, group;
-  int window, n_starting;  // of the own keys; window 0: none
-  float scale_log2;
-  int direct;  // a row whose keys one workgroup takes is finished there
-  // Shares of a row's keys, joined afterwards: [share][token][q head], O relative to the maximum, the maximum (log2 domain) and
-  // the sum of the weights.  The own keys have shares [0, own.n_shares), the prefixes those that follow.
-  float* partial_out;
-  f32x2* partial_sums;
-  // The kernel of few rows: pieces of the units that are cut between workgroups, and where a row's pieces are (cut_of):
-  // [token][q head]
-  int2* cuts;
-  float* slot_out;   // [workgroup][2][head of the workgroup][rows][D]
-  f32x2* slot_sums;  // [workgroup][2][head of the workgroup][rows]
-  int few_rows, few_heads_log2;  // rows of a unit; kv heads a workgroup takes at once: 1, 2 or 4
-  int few_whole;                 // a workgroup takes a unit
-  int n_few, few_first;     // workgroups; of paged_both_kernel those before the ones of rows
-  int merge_sets;           // of lanes that share a row in the merge, a power of two
-};
-typedef KernArgs<PagedParams> PagedArgs;
-typedef KernArgs<PagedSource> SourceArgs;
-
-// The tokens of request (or prefix) b.  Cut to the tensor, whatever the tables say.
-struct TokenRange {
-  int begin, n;
-};
-__device__ __forceinline__ int first_token(PagedArgs& p, SourceArgs& src, int b) {
-  int r = b;
-  if (src.cu_groups != nullptr) r = min(max(src.cu_groups[b], 0), p.n_requests);
-  if (p.cu_seqlens_q != nullptr) r = p.cu_seqlens_q[r];
-  return min(max(r, 0), p.n_tokens);
-}
-__device__ __forceinline__ TokenRange tokens_of(PagedArgs& p, SourceArgs& src, int b) {
-  const int begin = first_token(p, src, b);
-  return {begin, max(first_token(p, src, b + 1) - begin, 0)};
-}
-// Its keys: those that its row of pages has room for.
-__device__ __forceinline__ int keys_of(PagedArgs& p, SourceArgs& src, int b) {
-  return min(max(src.key_lens[b], 0), p.n_pages > 0 ? src.table_width * p.page_size : 0);
-}
-
-// The 16-key groups that rows at positions [first, last] see: [0, n_first) and then [begin, end).
-struct KeyGroups {
-  int n_first, begin, end;
-  int window_begin, hull_end, n_starting;  // keys from hull_end on, and between the first ones and the window, are seen by none
-  __device__ __forceinline__ KeyGroups(int window, int starting, int first, int last) {
-    n_starting = starting;
-    hull_end = last + 1;
-    end = (hull_end + 15) / 16;
-    window_begin = window > 0 ? max(first - window + 1, 0) : 0;
-    begin = window_begin / 16;
-    n_first = min(starting / 16 + (starting % 16 != 0), end);
-    if (n_first >= begin) begin = n_first = 0;  // one run
-  }
-  __device__ __forceinline__ int count() const { return n_first + end - begin; }
-  __device__ __forceinline__ int at(int i) const { return i < n_first ? i : i - n_first + begin; }
-  __device__ __forceinline__ bool sees(int key) const { return (key < hull_end) & ((key < n_starting) | (key >= window_begin)); }
-  __device__ __forceinline__ bool sees_all_of_16(int key) const {
-    return (key + 15 < hull_end) & ((key + 15 < n_starting) | (key >= window_begin));
-  }
-};
-constexpr int kNoKey = 0x7fffff00;  // of a group that is not there: past every row's last key
-
-__device__ __forceinline__ float rows_max(float x) {  // over the lanes of one n: the four groups of 16 lanes
-  const unsigned u = __float_as_uint(x);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float rows_sum(float x) {
-  const unsigned u = __float_as_uint(x);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
 
 // sum + the two weights of a pair.
 template <int DTYPE>
@@ -154,96 +55,14 @@ __device__ __forceinline__ void load_async_piece(uint32_t lds_at, const uint16_t
                  : "memory");
 }
 
-// The result of a row's 4 elements, from the sum of the weights.
-template <int DTYPE>
-__device__ __forceinline__ void store_row_piece(PagedArgs& p, int64_t token, int64_t head, int d, f32x4 o, float m, float l) {
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(p.out) + token * p.out_token + head * p.out_head + d) =
-      u32x2{pack2<DTYPE>(o[0] * inv, o[1] * inv), pack2<DTYPE>(o[2] * inv, o[3] * inv)};
-  if (d == 0) p.lse[head * p.n_tokens + token] = l == 0.0f ? INFINITY : (m + log2f(l)) * kLn2;
-}
-
 // ---------------------------------------------------------------------------
 // The kernel of rows: a workgroup of 4 waves owns 128 rows of one (request, kv head), a wave 32 of them, and walks its share of the
 // 64-key tiles that any of them sees.  K and V tiles go from memory straight into LDS (KvTile), two stages each, K a tile
 // ahead of V: S^T of tile t + 1 is multiplied while tile t is exponentiated, MFMA by MFMA in one stream, O^T += V^T P^T
 // of tile t follows as a dense run that the SIMD's other wave fills with its own arithmetic.
 // ---------------------------------------------------------------------------
-constexpr int kRowsThreads = 256, kRowsBM = 128, kRowsBN = 64;
-constexpr int kMinTilesPerShare = 2;
 constexpr float kNoMax = -3.0e38f;  // the reference of a row that has seen nothing: below every score, and a weight of -inf against it is 0
 constexpr float kMaxTileSum = 16384.0f;  // of a lane's weights against a reference that is not their maximum: fp16 can hold them
-
-// Sum over the wave's lanes up to and with this one.
-__device__ __forceinline__ int wave_scan(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr:1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);   // row_shr:2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);   // row_shr:4
-  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);   // row_shr:8
-  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
-  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
-  return x;
-}
-
-// The row tile of place `place`, the last one first: tile number `index` of request b's (negative: there is none).
-struct RowTile {
-  int b, index;
-  TokenRange tokens;
-  int n_keys;
-};
-__device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, int place) {
-  const int lane = threadIdx.x & 63;
-  // Up to 64 requests are counted.  Of more, request b's tiles begin at number floor(first_row / 128) + b: that leaves room for its last,
-  // partial one, and needs no sum over the requests before it, but its places without a tile lie among the others, and CUs with two tiles
-  // beside CUs with none (24 requests of 128 rows on 1024 keys, nearly half of the places empty: 40 us, counted 35; 64 of 64 rows on 4096 267
-  // and 213).
-  auto start = [&](int first, int b) { return (int)((int64_t)first * p.group / kRowsBM) + b; };
-  const bool counted = src.batch <= 64;
-  int tile = src.n_tiles - 1 - place, lo = 0, hi = src.batch;  // the last request that begins at or before the tile; 64 candidates a step
-  while (hi - lo > 64) {
-    const int step = (hi - lo + 63) / 64, b = lo + lane * step;
-    const bool before = b < hi && start(first_token(p, src, b), b) <= tile;
-    const int n = __popcll(__ballot(before));
-    if (n > 1) lo += (n - 1) * step;
-    hi = min(lo + step, hi);
-  }
-  // A lane looks at one request, and at all there is to know of it: another trip to memory for the one that is found is a microsecond.
-  const int b = min(lo + lane, hi - 1);
-  const TokenRange tokens = tokens_of(p, src, b);
-  const int n_keys = keys_of(p, src, b), n_tiles = (tokens.n * p.group + kRowsBM - 1) / kRowsBM;
-  int first_tile = start(tokens.begin, b), passed;
-  if (counted) {
-    const int ends = wave_scan(lane < hi ? n_tiles : 0);
-    tile = __builtin_amdgcn_readlane(ends, 63) - 1 - place;
-    first_tile = ends - n_tiles;
-    passed = __popcll(__ballot((lane < hi) & (ends <= tile)));
-  } else {
-    passed = max(__popcll(__ballot((lo + lane < hi) & (first_tile <= tile))) - 1, 0);
-  }
-  const int at = __builtin_amdgcn_readfirstlane(min(passed, hi - lo - 1));
-  auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-  const int index = of(tile - first_tile);
-  return {of(b), (tile >= 0) & (index < of(n_tiles)) ? index : -1, {of(tokens.begin), of(tokens.n)}, of(n_keys)};
-}
-
-// Which work item workgroup `wg` takes.  The items of a group, `group` neighbouring row tiles of a kv head, read the same keys and go to one
-// XCD (workgroup ids go round the eight), whose L2 then reads them once.  From one round of eight groups to the next the XCDs
-// move on by one, so that the groups of one kv head do not all go to the same XCD where there are eight.  The tiles of a request's last
-// tokens, which see the most, come first, places without a tile last.
-struct RowItem {
-  int place, kv_head, share;  // share: -1 for none
-};
-__device__ __forceinline__ RowItem row_item(int wg, int n_tiles, int group, int n_heads_kv, int n_shares) {
-  const int per_round = kNumXcd * group, round = wg / per_round, in_round = wg - round * per_round;
-  int i = round * kNumXcd + (in_round + round) % kNumXcd;  // the group
-  const int kv_head = i % n_heads_kv;
-  i /= n_heads_kv;
-  const int place = i / n_shares * group + in_round / kNumXcd, share = i % n_shares;
-  return {place, kv_head, place < n_tiles ? share : -1};
-}
-inline int64_t row_workgroups(int64_t n_tiles, int group, int n_heads_kv, int n_shares) {
-  return xcd_grid_size((n_tiles + group - 1) / group * n_heads_kv * n_shares, 1) * group;
-}
 
 // LDS of the kernel: two stages of K and of V, and where the 16-key groups of 2 x 64 tiles are.
 constexpr int kTableTiles = 64;
@@ -603,44 +422,6 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 // cache by head 319 and 335).  With few tiles a workgroup the waves take turns at one head's tiles instead, which makes the chain of
 // tiles shorter.
 // ---------------------------------------------------------------------------
-// What the merge needs to know of a row: the workgroup that begins its unit, how many the unit is cut over, the slot of the first
-// piece (the others are in slot 0) and the row in the slots.
-__device__ __forceinline__ int2 cut_of(int wg, int n_pieces, int slot, int row) { return int2{wg, n_pieces | row << 20 | slot << 28}; }
-constexpr int kFewBN = 32;
-constexpr int kFewMaxBatch = 1 << 16;
-
-// What request b is to the kernel.
-struct FewRequest {
-  int first_tok, n_tok, n_keys, n_tiles;
-  __device__ __forceinline__ KeyGroups groups(PagedArgs& p) const {
-    return KeyGroups(p.window, p.n_starting, max(n_keys - n_tok, 0), n_keys - 1);
-  }
-  __device__ __forceinline__ FewRequest() {}
-  __device__ __forceinline__ FewRequest(PagedArgs& p, int b) {
-    const TokenRange tokens = tokens_of(p, p.own, b);
-    first_tok = tokens.begin;
-    n_tok = tokens.n;
-    n_keys = keys_of(p, p.own, b);
-    n_tiles = max((groups(p).count() + 1) / 2, 1);  // (a request without keys has its rows written all the same)
-  }
-  __device__ __forceinline__ int units(PagedArgs& p, int rows) const {
-    return (n_tok * p.group + rows - 1) / rows * (p.n_heads_kv >> p.few_heads_log2);
-  }
-  __device__ __forceinline__ FewRequest of_lane(int lane) const {
-    FewRequest r;
-    r.first_tok = __builtin_amdgcn_readlane(first_tok, lane);
-    r.n_tok = __builtin_amdgcn_readlane(n_tok, lane);
-    r.n_keys = __builtin_amdgcn_readlane(n_keys, lane);
-    r.n_tiles = __builtin_amdgcn_readlane(n_tiles, lane);
-    return r;
-  }
-};
-
-__device__ __forceinline__ int64_t lane_value(int64_t x, int lane) {
-  const uint32_t lo = __builtin_amdgcn_readlane((int)x, lane), hi = __builtin_amdgcn_readlane((int)(x >> 32), lane);
-  return (int64_t)(((uint64_t)hi << 32) | lo);
-}
-
 // LDS of the kernel.  V of 32 keys: load r of a tile brings rows r, r + LOADS, ... side by side (1 KiB), 32 bytes of padding between
 // loads: eight consecutive rows then lie in eight different 32-byte bank windows for the transposing reads.
 template <int D, int RT, int NW>
@@ -656,7 +437,6 @@ struct FewLds {
 template <int DTYPE, int D, int RT, int NW>
 __device__ __forceinline__ void paged_few(int wg, char* lds) {
   // (the arguments are read anew wherever another part of the work begins: kept in scalar registers throughout they do not fit)
-  PagedArgs& p0 = fresh_kernel_args<PagedParams>();
   typedef FewLds<D, RT, NW> Lds;
   constexpr int KS = D / 32, DT = D / 16, ROWS = Lds::ROWS, LOADS = Lds::LOADS;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
@@ -664,85 +444,17 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
   float(*sums)[ROWS][2] = reinterpret_cast<float(*)[ROWS][2]>(lds + Lds::SUMS);
   int* chunk_sums = reinterpret_cast<int*>(lds + Lds::CHUNKS);
 
-  // ---- this workgroup's share of all tiles (the host has checked that their number fits 32 bits), or its unit -----------
-  const int n_chunks = (p0.own.batch + 63) / 64;
-  const bool whole_units = p0.few_whole != 0;
-  // Shares are counted in turns of the waves at a head's tiles: a cut inside one would cost both of its sides a whole one.  (One context
-  // of 1500 keys, 8 heads, which 47 tiles a head then fit no better: counted in tiles 14.4 us, in turns 11.4.)
-  const int turns_log2 = (NW == 8 ? 3 : 2) - p0.few_heads_log2, turns = 1 << turns_log2;
-  auto requests_of = [&](int chunk, int& work) {
-    PagedArgs& p = fresh_kernel_args<PagedParams>();
-    const int b = chunk * 64 + lane;
-    FewRequest r;
-    r.first_tok = r.n_tok = r.n_keys = 0;
-    r.n_tiles = 1;
-    work = 0;
-    if (b < p.own.batch) {
-      r = FewRequest(p, b);
-      work = r.units(p, ROWS) * (whole_units ? 1 : (r.n_tiles + turns - 1) >> turns_log2);
-    }
-    return r;
-  };
-  int total = 0, before = 0, chunk = 0, work;
-  FewRequest requests = requests_of(0, work);
-  int scan = wave_scan(work);  // the chunk's tiles (or units) up to and with the lane's request
-  if (n_chunks == 1) {
-    total = __builtin_amdgcn_readlane(scan, 63);
-  } else {
-    for (int i = w; i < n_chunks; i += NW) {
-      int more;
-      requests_of(i, more);
-      more = wave_scan(more);
-      if (lane == 63) chunk_sums[i] = more;
-    }
-    __syncthreads();
-    for (int i = 0; i < n_chunks; i += 64) total += __builtin_amdgcn_readlane(wave_scan(i + lane < n_chunks ? chunk_sums[i + lane] : 0), 63);
-  }
-  const int per = whole_units ? 1 : (total - 1) / p0.n_few + 1;
-  const int begin = (int)min((int64_t)wg * per, (int64_t)total), end = (int)min((int64_t)begin + per, (int64_t)total);
-  if (begin >= end) return;
-  if (n_chunks > 1) {
-    for (int i = 0; i < n_chunks; i += 64) {
-      const int ends = before + wave_scan(i + lane < n_chunks ? chunk_sums[i + lane] : 0);
-      const int passed = __popcll(__ballot(ends <= begin));
-      if (passed > 0) before = __builtin_amdgcn_readlane(ends, passed - 1);
-      chunk = i + passed;
-      if (passed < 64) break;
-    }
-    chunk = __builtin_amdgcn_readfirstlane(min(chunk, n_chunks - 1));
-    requests = requests_of(chunk, work);
-    scan = wave_scan(work);
-  }
-  int index = __builtin_amdgcn_readfirstlane(min(__popcll(__ballot(before + scan <= begin)), 63));  // in the chunk
-
+  FewWalk<ROWS, NW> walk(wg, chunk_sums);
+  FewUnit u;
   char* my_lds = lds + w * Lds::WAVE;  // K of a tile and V of a tile
   const uint32_t k_at = lds_address(lds) + w * Lds::WAVE, v_at = k_at + Lds::STAGE;
-  int at = begin;
-  while (at < end) {
-    if (index == 64) {
-      before += __builtin_amdgcn_readlane(scan, 63);
-      if (++chunk >= n_chunks) break;
-      requests = requests_of(chunk, work);
-      scan = wave_scan(work);
-      index = 0;
-    }
-    const int unit_end = before + __builtin_amdgcn_readlane(scan, index);
-    if (at >= unit_end) {  // (no rows, or done)
-      ++index;
-      continue;
-    }
+  while (walk.next(u)) {
     PagedArgs& p = fresh_kernel_args<PagedParams>();
     // the workgroup's kv heads at once, the waves that take turns at a head's tiles, and which of each the wave is
-    const int heads = 1 << p.few_heads_log2, head_groups = p.n_heads_kv >> p.few_heads_log2;
+    const int heads = 1 << p.few_heads_log2, head_groups = p.n_heads_kv >> p.few_heads_log2, turns = NW >> p.few_heads_log2;
     const int my_head = w & (heads - 1), my_turn = w >> p.few_heads_log2;
-    const FewRequest request = requests.of_lane(index);
-    const int b = chunk * 64 + index, in_request = at - (unit_end - __builtin_amdgcn_readlane(work, index));
-    if (in_request < 0) break;  // (tables whose tokens are many times those there are: their sums wrap)
-    const int unit_turns = whole_units ? 1 : (request.n_tiles + turns - 1) >> turns_log2;
-    const int unit = __builtin_amdgcn_readfirstlane(in_request / unit_turns);
-    const int first_turn = in_request - unit * unit_turns, taken = min(unit_turns - first_turn, end - at);
-    const int t_begin = whole_units ? 0 : first_turn * turns, t_end = whole_units ? request.n_tiles : min(request.n_tiles, t_begin + taken * turns);
-    at += taken;
+    const FewRequest& request = u.request;
+    const int b = u.b, unit = u.unit, t_begin = u.t_begin, t_end = u.t_end;
     const int kv_head0 = unit % head_groups * heads, kv_head = kv_head0 + my_head, row0 = unit / head_groups * ROWS;
     const KeyGroups groups = request.groups(p);
     const int n_groups = request.n_keys > 0 ? groups.count() : 0, n_rows = request.n_tok * p.group;
@@ -937,41 +649,7 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mine + (rt * 16 + n) * Lds::O_STRIDE + 16 * dt + 4 * g) = o[rt][dt];
     }
     __syncthreads();
-    PagedArgs& p_out = fresh_kernel_args<PagedParams>();
-    const bool cut = taken < unit_turns;
-    const int slot = at - taken == begin ? 0 : 1;
-    const int n_cut = (at - taken + unit_turns - 1) / per - wg + 1;  // (of a unit that begins here: it ends so many workgroups on)
-    const int group = p_out.group;
-    constexpr int PIECES = D / 4;  // of a row
-    for (int i = tid; i < heads * ROWS * PIECES; i += NW * 64) {
-      const int piece = i % PIECES, row = i / PIECES % ROWS, of = i / PIECES / ROWS, r = row0 + row;
-      if (r >= n_rows) continue;
-      float m = -INFINITY;
-      for (int x = of; x < NW; x += heads) m = fmaxf(m, sums[x][row][0]);
-      const float m_use = m == -INFINITY ? 0.0f : m;
-      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-      float l = 0.0f;
-      for (int x = of; x < NW; x += heads) {
-        const float weight = fast_exp2(sums[x][row][0] - m_use);
-        l += weight * sums[x][row][1];
-        const f32x4 o4 = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds + x * Lds::WAVE) + row * Lds::O_STRIDE + 4 * piece);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
-      }
-      const int64_t token = request.first_tok + r / group, head = (kv_head0 + of) * group + r % group;
-      if ((piece == 0) & (t_begin == 0) & !whole_units) p_out.cuts[token * p_out.n_heads_q + head] = cut_of(wg, n_cut, slot, of * ROWS + row);
-      if (cut) {
-        const int64_t to = (((int64_t)wg * 2 + slot) * heads + of) * ROWS + row;
-        *reinterpret_cast<f32x4*>(p_out.slot_out + to * D + 4 * piece) = acc;
-        if (piece == 0) p_out.slot_sums[to] = f32x2{m, l};
-      } else if (!p_out.direct) {
-        const int64_t to = ((int64_t)p_out.own.first_share * p_out.n_tokens + token) * p_out.n_heads_q + head;
-        *reinterpret_cast<f32x4*>(p_out.partial_out + to * D + 4 * piece) = acc;
-        if (piece == 0) p_out.partial_sums[to] = f32x2{m, l};
-      } else {
-        store_row_piece<DTYPE>(p_out, token, head, 4 * piece, acc, m, l);
-      }
-    }
+    join_few<DTYPE, D, ROWS, NW, Lds::WAVE>(walk, u, lds, sums, kv_head0, row0);
     __syncthreads();  // nobody's part of LDS is filled again before all have read it
   }
 }
@@ -1233,6 +911,19 @@ static PagedPlan plan_paged(const dcp_paged_attn_args& x) {
                              : (x.head_dim == 128 ? kernel<DCP_DTYPE_FP16, 128, ##__VA_ARGS__>          \
                                                   : kernel<DCP_DTYPE_FP16, 64, ##__VA_ARGS__>))
 
+int launch_paged_merge(PagedParams& p, int dtype, int head_dim, int64_t parts, void* stream) {
+  const struct { int dtype, head_dim; } x = {dtype, head_dim};
+  // eight parts a set of lanes, as far as the longest lengths tell how many there are
+  const int sets = kPagedMergeThreads / (head_dim / 4);
+  p.merge_sets = 1;
+  while (p.merge_sets < sets && parts > 8 * p.merge_sets) p.merge_sets *= 2;
+  const int64_t n_wg = ((int64_t)p.n_tokens * p.n_heads_q * p.merge_sets + sets - 1) / sets;
+  if (n_wg >= (int64_t)1 << 31) return fail(DCP_ERR_ARG, "paged_attn: too many work items");
+  KernelTimer timer("paged_merge_kernel", stream);
+  hipLaunchKernelGGL((DCP_PAGED_KERNEL(paged_merge_kernel)), dim3((unsigned)n_wg), dim3(kPagedMergeThreads), 0, (hipStream_t)stream, p);
+  return check_launch("paged_merge_kernel");
+}
+
 namespace {
 
 // What a caller may have wrong, before anything is launched.
@@ -1296,7 +987,7 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
   p.slot_sums = reinterpret_cast<f32x2*>(p.slot_out + (size_t)plan.n_few * 2 * plan.heads * plan.rows * x.head_dim);
   p.partial_out = reinterpret_cast<float*>(at + plan.cuts + plan.slots);
   p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)(plan.n_own + plan.n_prefix) * x.n_tokens * x.n_heads_q * x.head_dim);
-  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.few_whole = plan.whole; p.merge_sets = 1; p.n_few = plan.n_few; p.few_first = plan.few_first;
+  p.few_rows = plan.rows; p.few_heads_log2 = plan.heads / 2; p.few_whole = plan.whole; p.n_few = plan.n_few; p.few_first = plan.few_first;
 
   int status = DCP_OK;
   const auto launch = [&](auto kernel, const char* name, int64_t n_wg, int threads) {
@@ -1334,12 +1025,9 @@ int paged_attn(const dcp_paged_attn_args& x, void* workspace, size_t workspace_b
     }
   }
   if (p.own.by_few || !p.direct) {
-    // eight parts a set of lanes, as far as the longest lengths tell how many there are
     const int64_t units = std::max<int64_t>((int64_t)x.batch * x.n_heads_kv / plan.heads, 1);
-    const int64_t parts = (plan.few && !plan.whole ? plan.n_few / units + 2 : plan.n_own) + plan.n_prefix;
-    const int sets = kPagedMergeThreads / (x.head_dim / 4);
-    while (p.merge_sets < sets && parts > 8 * p.merge_sets) p.merge_sets *= 2;
-    launch(DCP_PAGED_KERNEL(paged_merge_kernel), "paged_merge_kernel", ((int64_t)x.n_tokens * x.n_heads_q * p.merge_sets + sets - 1) / sets, kPagedMergeThreads);
+    if (status == DCP_OK)
+      status = launch_paged_merge(p, x.dtype, x.head_dim, (plan.few && !plan.whole ? plan.n_few / units + 2 : plan.n_own) + plan.n_prefix, stream);
   }
   return status;
 }
