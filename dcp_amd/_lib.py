@@ -58,6 +58,10 @@ SIGNATURES = {
     "dcp_paged_cache_write": [_P] * 5 + [_I] * 4 + [_L] * 3 + [_I] + [_L] * 3 + [_P],
     "dcp_paged_attn_workspace_bytes": [_P],
     "dcp_paged_attn": [_P, _P, c_size_t, _P],
+    "dcp_quantized_cache_write": [_P] * 4 + [_I] * 4 + [_L] * 3 + [_I, _L, _L, _P],
+    "dcp_quantized_cache_read": [_P] * 4 + [_I] * 4 + [_L] * 3 + [_I, _L, _L, _P],
+    "dcp_quantized_attn_workspace_bytes": [_P],
+    "dcp_quantized_attn": [_P, _P, c_size_t, _P],
     "dcp_greedy_stage_selection": [_I, _P, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _L, _P, _P, _P],
 }
 
@@ -94,7 +98,8 @@ def load():
             fn.restype = {"dcp_last_error": c_char_p, "dcp_record_begin": c_void_p, "dcp_record_free": None, "dcp_attn_bwd_workspace_bytes": c_size_t,
                           "dcp_attn_fwd_workspace_bytes": c_size_t,
                           "dcp_attn_bwd_static_scratch_bytes": c_size_t,
-                          "dcp_attn_bwd_workspace_bytes_kv": c_size_t, "dcp_paged_attn_workspace_bytes": c_size_t}.get(name, c_int)
+                          "dcp_attn_bwd_workspace_bytes_kv": c_size_t, "dcp_paged_attn_workspace_bytes": c_size_t,
+                          "dcp_quantized_attn_workspace_bytes": c_size_t}.get(name, c_int)
         _lib = lib
     return _lib
 

@@ -11,7 +11,8 @@ flag, no sliding window, no softcap, no alibi; masking comes from
 raises ``NotImplementedError`` rather than computing something different.
 
 Beside them, with no counterpart in the reference, what answering takes: attention over a paged K/V cache
-(``paged_cache_attention``) and of requests that share prefixes in it (``shared_prefix_attention``), forward only.
+(``paged_cache_attention``), over one held in 4 bits (``quantized_cache_attention``), and of requests that share prefixes
+(``shared_prefix_attention``), forward only.
 """
 
 from __future__ import annotations
@@ -23,6 +24,7 @@ import torch
 
 from dcp_amd import _lib
 from dcp_amd.ops.fused_ops import dtype_code
+from dcp_amd.ops.quantized_cache import _cache_args
 
 __all__ = [
     "_flash_attn_varlen_forward",
@@ -31,6 +33,8 @@ __all__ = [
     "backward_workspace_bytes",
     "paged_cache_attention",
     "paged_cache_workspace_bytes",
+    "quantized_cache_attention",
+    "quantized_cache_workspace_bytes",
     "shared_prefix_attention",
     "shared_prefix_workspace_bytes",
 ]
@@ -633,4 +637,106 @@ def shared_prefix_attention(
     out, lse, packed = _paged_args(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, None, 0, out,
                                    lse, (prefix_table, prefix_lens, cu_groups, max_prefix_len))
     _paged_call(packed, workspace, q)
+    return out, lse
+
+
+# ---------------------------------------------------------------------------
+# attention over a paged cache held in 4 bits (no counterpart in the reference)
+# ---------------------------------------------------------------------------
+
+# dcp_quantized_attn_args: seven addresses, seven strides, thirteen numbers and the scale
+_QUANTIZED_ARGS = struct.Struct("<7Q7q13if")
+
+
+def _quantized_args(q, cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, window, n_starting, out, lse):
+    """``(out, lse, packed arguments)``, the inputs checked."""
+    here, dtype, q_strides = torch._C._cuda_getDevice(), q.dtype, q.stride()
+    cache_at, n_heads_kv, head_dim, n_pages, page_size, page_stride, head_stride = _cache_args(cache, here)
+    if q.get_device() != here:
+        raise ValueError("q must be a tensor of the current device")
+    if len(q_strides) != 3 or q_strides[2] != 1 or q.shape[2] != head_dim:
+        raise ValueError(f"q must be [tokens, n_heads_q, {head_dim}] with dense rows, got {list(q.shape)}")
+    n_tokens, n_heads_q, _ = q.shape
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [B, pages], got {list(block_table.shape)}")
+    batch, width = block_table.shape
+    table_at = _table_here(block_table, "block_table", here, (batch, width))
+    lens_at = _table_here(seq_lens, "seq_lens", here, (batch,))
+    cu_at = 0
+    if cu_seqlens_q is not None:
+        cu_at = _table_here(cu_seqlens_q, "cu_seqlens_q", here, (batch + 1,))
+    elif batch != n_tokens:
+        raise ValueError(f"without cu_seqlens_q every request has one token, got {n_tokens} for {batch}")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be positive (None: no window), got {window}")
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out_token, out_head = n_heads_q * head_dim, head_dim
+    else:
+        if out.shape != q.shape or out.dtype is not dtype or out.stride(2) != 1 or out.get_device() != here:
+            raise ValueError(f"out must be like q, got {out.dtype} {list(out.shape)}")
+        out_token, out_head, _ = out.stride()
+    if lse is None:
+        lse = seq_lens.new_empty((n_heads_q, n_tokens), dtype=torch.float32)
+    elif lse.shape != (n_heads_q, n_tokens) or lse.dtype is not torch.float32 or not lse.is_contiguous() or lse.get_device() != here:
+        raise ValueError(f"lse must be contiguous float32 [{n_heads_q}, {n_tokens}] on the current device")
+    if max_seqlen_q is None:
+        max_seqlen_q = 1 if cu_at == 0 else max(n_tokens, 1)
+    if max_seqlen_k is None:
+        max_seqlen_k = max(width * page_size, 1)
+    args = (
+        q.data_ptr(), cache_at, out.data_ptr(), lse.data_ptr(), table_at, lens_at, cu_at, q_strides[0], q_strides[1], out_token, out_head,
+        page_stride, head_stride, block_table.stride(0), n_tokens, batch, n_heads_q, n_heads_kv, head_dim, n_pages, page_size, width,
+        max_seqlen_q, max_seqlen_k, window or 0, n_starting, dtype_code(dtype), head_dim ** -0.5 if softmax_scale is None else softmax_scale)
+    try:
+        return out, lse, _QUANTIZED_ARGS.pack(*args)
+    except (struct.error, OverflowError) as e:  # (the second: a scale past the type's end)
+        raise ValueError(f"sizes, lengths, window and n_starting must be whole numbers of 32 bits, softmax_scale a number: {e}") from None
+
+
+def quantized_cache_workspace_bytes(q, cache, block_table, seq_lens, cu_seqlens_q=None, max_seqlen_q=None, max_seqlen_k=None, softmax_scale=None,
+                                    window=None, n_starting=0, out=None, lse=None) -> int:
+    """Scratch bytes ``quantized_cache_attention`` needs for these arguments (0: none)."""
+    packed = _quantized_args(q, cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, window, n_starting, out, lse)[2]
+    return _lib.load().dcp_quantized_attn_workspace_bytes(packed)
+
+
+def quantized_cache_attention(
+    q,
+    cache,
+    block_table,
+    seq_lens,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    max_seqlen_q: Optional[int] = None,
+    max_seqlen_k: Optional[int] = None,
+    softmax_scale: Optional[float] = None,
+    window: Optional[int] = None,
+    n_starting: int = 0,
+    out: Optional[torch.Tensor] = None,
+    lse: Optional[torch.Tensor] = None,
+    workspace: Optional[torch.Tensor] = None,
+):
+    """``paged_cache_attention`` over a cache held in 4 bits (``dcp_amd.ops.quantized_cache_pages``, uint8
+    ``[n_pages, n_heads_kv, page_size // 16, 17 * D]``; pages and heads at any strides that are multiples of 16); returns ``(out, lse)``.
+
+    Every other argument is as there, ``workspace`` of ``quantized_cache_workspace_bytes(...)`` bytes.  q is bf16 or fp16, and of a
+    type that holds what the cache stands for, as the type does that it was written from.  Keys and values are exactly what
+    ``quantized_cache_read`` gives in that type.  What no query of a request sees may hold anything; a block that is no number and that one of its
+    queries sees may reach the request's other queries.  Forward only.
+    """
+    out, lse, packed = _quantized_args(q, cache, block_table, seq_lens, cu_seqlens_q, max_seqlen_q, max_seqlen_k, softmax_scale, window, n_starting,
+                                       out, lse)
+    lib, address, size = _lib.load(), 0, 0
+    if workspace is None:
+        size = lib.dcp_quantized_attn_workspace_bytes(packed)
+        if size > 0:
+            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
+            address = workspace.data_ptr()
+    else:
+        if not workspace.is_contiguous() or workspace.get_device() != q.get_device():
+            raise ValueError("workspace must be a contiguous tensor on q's device")
+        address, size = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    status = lib.dcp_quantized_attn(packed, address, size, torch._C._cuda_getCurrentRawStream(q.get_device()))
+    if status != 0:
+        _lib.fail("dcp_quantized_attn", status)
     return out, lse

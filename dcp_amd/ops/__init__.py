@@ -16,3 +16,4 @@ from dcp_amd.ops.fused_ops import (  # noqa: F401
     warmup_triton_ops,
 )
 from dcp_amd.ops.paged_cache import PagedCacheTables, paged_cache_tables, paged_cache_write  # noqa: F401
+from dcp_amd.ops.quantized_cache import quantized_cache_pages, quantized_cache_read, quantized_cache_write  # noqa: F401

@@ -733,6 +733,79 @@ size_t dcp_paged_attn_workspace_bytes(const dcp_paged_attn_args* args);
 int dcp_paged_attn(const dcp_paged_attn_args* args, void* workspace,
                    size_t workspace_bytes, void* stream);
 
+/*
+ * A paged K/V cache held in 4 bits (no counterpart in the reference).
+ *
+ * Every 32 neighbouring elements of a token's key or value are a block of
+ * numbers c 2^e: c one of +-{0, 0.5, 1, 1.5, 2, 3, 4, 6} in 4 bits (sign, two
+ * bits of exponent, one of mantissa; in this order 0 to 7, the sign in the
+ * highest bit), e in [-127, 127] in a byte that holds e + 127 (255: the block is
+ * no number).  Elements 2 i and 2 i + 1 are the low and the high half of a byte.
+ * The cache is [n_pages][n_heads_kv][page_size / 16][17 * head_dim] bytes, pages
+ * and heads at any strides that are multiples of 16.  Of the bytes of 16 tokens
+ * of a head, D = head_dim:
+ *   [0, 8 D)           K's codes, [16 tokens][D / 2]
+ *   [8 D, 16 D)        V's codes, [4][16 pieces][4 tokens][D / 32]: piece i is
+ *                      elements i D / 16 .., tokens 4 j to 4 j + 3 the j-th four
+ *   [16 D, + D / 2)    K's exponents, [16 tokens][D / 32]
+ *   [.., + D / 2)      V's exponents, [4][D / 32][4 tokens]
+ *
+ * dcp_quantized_cache_write: tokens' rows of K and V ([n_tokens][n_heads_kv][D],
+ * strides in elements) at their slots (page * page_size + offset).  e is the
+ * smallest with no element's size past 7 * 2^e; an element goes to the nearest of
+ * the numbers that its type can hold, ties to the even code, so it is off by at
+ * most 2^e where the block's largest is in (3.5, 7] * 2^e (a quarter of it where
+ * that largest is among the type's last; by 2^-129 where all are below 2^-127).
+ * A block with an infinity or a NaN is no number as a whole.  Slots outside of the
+ * cache are skipped; the others have to differ from each other, and the inputs
+ * may not lie in the cache.
+ *
+ * dcp_quantized_cache_read: the rows at these slots in 16 bits, into k and v.
+ * What was written from the same type is exact, what the type does not hold is
+ * rounded.  Rows of slots outside of the cache are zeros.
+ *  - Supported: bf16 and fp16, head_dim 64 or 128, page_size a multiple of 16;
+ *    16-byte aligned rows (strides multiples of 8 elements).
+ */
+int dcp_quantized_cache_write(const void* k, const void* v,
+                              const int64_t* slot_mapping, void* cache,
+                              int n_tokens, int n_heads_kv, int head_dim,
+                              int dtype, int64_t token_stride,
+                              int64_t head_stride, int64_t n_pages,
+                              int page_size, int64_t cache_page_stride,
+                              int64_t cache_head_stride, void* stream);
+int dcp_quantized_cache_read(const void* cache, const int64_t* slot_mapping,
+                             void* k, void* v, int n_tokens, int n_heads_kv,
+                             int head_dim, int dtype, int64_t token_stride,
+                             int64_t head_stride, int64_t n_pages,
+                             int page_size, int64_t cache_page_stride,
+                             int64_t cache_head_stride, void* stream);
+
+/*
+ * Attention over a cache held in 4 bits: dcp_paged_attn's own keys, with its
+ * masks, lengths and results (without shared prefixes), q and out in a type that
+ * holds what the cache stands for.  page_stride and head_stride are in bytes,
+ * the other strides in elements.
+ */
+typedef struct {
+  const void* q;
+  const void* cache;
+  void* out;
+  float* lse;
+  const int32_t* block_table;
+  const int32_t* seq_lens;
+  const int32_t* cu_seqlens_q;
+  int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+  int64_t page_stride, head_stride, table_stride;
+  int32_t n_tokens, batch, n_heads_q, n_heads_kv, head_dim;
+  int32_t n_pages, page_size, table_width;
+  int32_t max_seqlen_q, max_seqlen_k;
+  int32_t window, n_starting, dtype;
+  float softmax_scale;
+} dcp_quantized_attn_args;
+size_t dcp_quantized_attn_workspace_bytes(const dcp_quantized_attn_args* args);
+int dcp_quantized_attn(const dcp_quantized_attn_args* args, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
