@@ -14,8 +14,7 @@
 // more than 14 bits of the largest: scores were off by 5e-6 of the sum of their products' sizes, here by 1e-7.)
 #include <algorithm>
 
-#include "paged_common.h"
-#include "quantized_cache.h"
+#include "paged_rows.h"
 #include "record.h"
 
 namespace dcp {
@@ -26,13 +25,6 @@ struct QuantFewLds {
   static constexpr int SUMS = NW * WAVE;                           // float [wave][row][2]
   static constexpr int CHUNKS = SUMS + NW * ROWS * 2 * 4;          // int [batch / 64]
   static constexpr int BYTES = CHUNKS + kFewMaxBatch / 64 * 4;
-};
-
-// What a lane reads of 16 keys.
-template <int D>
-struct QuantGroup {
-  typename QuantTile<D>::Codes k, v;
-  uint32_t k_exp, v_exp;
 };
 
 // The operands of V for two groups of 16 keys: those of elements n D / 16 + 2 U and the one after it.
@@ -118,10 +110,10 @@ __global__ __launch_bounds__(NW * 64, RT == 1 ? 3 : 2) void quantized_few_kernel
         const char* at = head + lane_value(lane_off, from);
         next_key[kt] = __builtin_amdgcn_readlane(lane_key, from);
         typedef typename Tile::Codes Codes;
-        next[kt].k = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(at + (n * 4 + g) * Tile::LANE_BYTES));
-        next[kt].k_exp = *reinterpret_cast<const uint8_t*>(at + Tile::k_exp_of(n, g));
-        next[kt].v = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(at + Tile::V + lane * Tile::LANE_BYTES));
-        next[kt].v_exp = *reinterpret_cast<const uint32_t*>(at + Tile::v_exp_of(n, g));
+        next[kt].k = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(at + Tile::k_of(lane)));
+        next[kt].k_exp = *reinterpret_cast<const uint8_t*>(at + Tile::k_exp_of(lane));
+        next[kt].v = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(at + Tile::v_of(lane)));
+        next[kt].v_exp = *reinterpret_cast<const uint32_t*>(at + Tile::v_exp_of(lane));
       }
     };
     if (n_steps > 0) load(0);
@@ -184,8 +176,7 @@ __global__ __launch_bounds__(NW * 64, RT == 1 ? 3 : 2) void quantized_few_kernel
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = tile_key[kt] + 4 * g + e;
-            // what no row sees may hold anything: with this exponent it is finite, and its weight is 0
-            if (!((tile_key[kt] != kNoKey) & groups.sees(key))) x[kt].v_exp &= ~(0xffu << (8 * e));
+            if (!((tile_key[kt] != kNoKey) & groups.sees(key))) x[kt].clear_v(e);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
               const bool visible = (key <= last_key[rt]) & ((key < p.n_starting) | (key >= first_key[rt])) & (tile_key[kt] != kNoKey);
@@ -255,24 +246,46 @@ __global__ __launch_bounds__(NW * 64, RT == 1 ? 3 : 2) void quantized_few_kernel
   }
 }
 
+template <int DTYPE, int D>
+__global__ __launch_bounds__(kRowsThreads, 2) void quantized_rows_kernel(const PagedParams) {
+  __shared__ __attribute__((aligned(16))) char lds[RowsLds<D>::BYTES];
+  PagedArgs& p = fresh_kernel_args<PagedParams>();
+  paged_rows<DTYPE, D, false, true>(p, p.own, blockIdx.x, lds);
+}
+
 // ---- host ---------------------------------------------------------------------------
 
 // How a call is laid out, and what of the workspace is whose.
 struct QuantPlan {
-  bool whole = false;  // a workgroup takes a unit; otherwise an equal share of all tiles
+  bool few = false;    // the kernel of few rows
+  bool whole = false;  // a workgroup takes a unit of it; otherwise an equal share of all tiles
   int rows = 16, n_few = 0;
-  size_t cuts = 0, slots = 0;  // bytes
-  size_t bytes() const { return cuts + slots; }
+  int n_shares = 1;    // of a row's keys, by the kernel of rows
+  size_t cuts = 0, slots = 0, shares = 0;  // bytes
+  size_t bytes() const { return cuts + slots + shares; }
 };
+
+// Keys that a request's queries see, of the longest there are.
+static int64_t seen_keys(const dcp_quantized_attn_args& x) {
+  return x.window > 0 ? std::min<int64_t>(x.max_seqlen_k, (int64_t)x.max_seqlen_q + x.window + x.n_starting) : x.max_seqlen_k;
+}
 
 static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
   QuantPlan plan;
   const int group = x.n_heads_q / x.n_heads_kv;
-  const int64_t own_rows = (int64_t)x.max_seqlen_q * group;
+  // The kernel of few rows: of requests with up to 32.  Its sums of tiles have to fit 32 bits whatever the lengths are.
+  const int64_t own_rows = (int64_t)x.max_seqlen_q * group, all_rows = (int64_t)x.n_tokens * group;
   plan.rows = own_rows <= 16 ? 16 : 32;
-  plan.n_few = (plan.rows == 16 ? 3 : 2) * device_cu_count();
-  plan.cuts = ((size_t)x.n_tokens * x.n_heads_q * sizeof(int2) + 15) / 16 * 16;
-  plan.slots = (size_t)plan.n_few * 2 * plan.rows * (x.head_dim + 2) * sizeof(float);
+  const int64_t most_units = (all_rows + (int64_t)x.batch * (plan.rows - 1)) / plan.rows * x.n_heads_kv;
+  plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2) < 2e9;
+  if (plan.few) {
+    plan.n_few = (plan.rows == 16 ? 3 : 2) * device_cu_count();
+    plan.cuts = ((size_t)x.n_tokens * x.n_heads_q * sizeof(int2) + 15) / 16 * 16;
+    plan.slots = (size_t)plan.n_few * 2 * plan.rows * (x.head_dim + 2) * sizeof(float);
+  } else {
+    plan.n_shares = row_shares(x, x.batch, seen_keys(x), false).n;
+    if (plan.n_shares > 1) plan.shares = (size_t)plan.n_shares * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
+  }
   return plan;
 }
 
@@ -308,8 +321,8 @@ int check_quantized(const dcp_quantized_attn_args& x) {
   if (x.n_tokens == 0 || x.batch == 0) return DCP_OK;
   DCP_REQUIRE(x.q && x.out && x.lse && x.block_table && x.seq_lens && (x.n_pages == 0 || x.cache), "quantized_attn: null argument");
   DCP_REQUIRE(x.max_seqlen_q > 0 && x.max_seqlen_k > 0, "quantized_attn: the longest lengths must be positive");
-  const double most_units = ((double)x.n_tokens * (x.n_heads_q / x.n_heads_kv) / 16 + x.batch) * x.n_heads_kv;
-  DCP_REQUIRE(x.batch <= kFewMaxBatch && most_units * ((double)x.table_width * x.page_size / kFewBN + 2) < 2e9, "quantized_attn: too many rows");
+  // (every kernel's work items: at most 64 shares of a row tile)
+  DCP_REQUIRE(row_tiles(x, x.batch) * x.n_heads_kv < ((int64_t)1 << 31) - (1 << 20), "quantized_attn: too many rows");
   return DCP_OK;
 }
 
@@ -326,28 +339,34 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
   p.cu_seqlens_q = x.cu_seqlens_q;
   p.q_token = x.q_token_stride; p.q_head = x.q_head_stride; p.out_token = x.out_token_stride; p.out_head = x.out_head_stride;
   p.page_stride = x.page_stride; p.head_stride = x.head_stride;
-  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, 1, 0, 1, !plan.whole};
+  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_shares, (int)row_tiles(x, x.batch), row_group(x, x.batch), plan.few && !plan.whole};
   p.n_pages = x.n_pages; p.page_size = x.page_size;
   p.n_requests = x.batch; p.n_tokens = x.n_tokens;
   p.n_heads_q = x.n_heads_q; p.n_heads_kv = x.n_heads_kv; p.group = x.n_heads_q / x.n_heads_kv;
   p.window = x.window; p.n_starting = x.n_starting;
   p.scale_log2 = x.softmax_scale * kLog2e;
-  p.direct = 1;
+  p.direct = plan.n_shares == 1;
   char* at = reinterpret_cast<char*>(workspace);
   p.cuts = reinterpret_cast<int2*>(at);
   p.slot_out = reinterpret_cast<float*>(at + plan.cuts);
   p.slot_sums = reinterpret_cast<f32x2*>(p.slot_out + (size_t)plan.n_few * 2 * plan.rows * x.head_dim);
+  p.partial_out = reinterpret_cast<float*>(at + plan.cuts + plan.slots);
+  p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)plan.n_shares * x.n_tokens * x.n_heads_q * x.head_dim);
   p.few_rows = plan.rows; p.few_whole = plan.whole; p.n_few = plan.n_few;
-  const auto launch = [&](auto kernel, const char* name, int64_t n_wg, int threads) {
+  const auto launch = [&](auto kernel, const char* name, int64_t n_wg) {
+    if (n_wg >= (int64_t)1 << 31) return fail(DCP_ERR_ARG, "quantized_attn: too many work items");
     KernelTimer timer(name, stream);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(threads), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(256), 0, (hipStream_t)stream, p);
     return check_launch(name);
   };
-  int status = plan.rows == 16 ? launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 4), "quantized_few_kernel", p.n_few, 256)
-                               : launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 4), "quantized_few_kernel", p.n_few, 256);
-  if (status == DCP_OK) {
+  int status;
+  if (!plan.few)
+    status = launch(DCP_QUANT_KERNEL(quantized_rows_kernel), "quantized_rows_kernel", row_workgroups(p.own.n_tiles, p.own.xcd_group, x.n_heads_kv, plan.n_shares));
+  else if (plan.rows == 16) status = launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 4), "quantized_few_kernel", p.n_few);
+  else status = launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 4), "quantized_few_kernel", p.n_few);
+  if (status == DCP_OK && (p.own.by_few || !p.direct)) {
     const int64_t units = std::max<int64_t>((int64_t)x.batch * x.n_heads_kv, 1);
-    status = launch_paged_merge(p, x.dtype, x.head_dim, plan.n_few / units + 2, stream);
+    status = launch_paged_merge(p, x.dtype, x.head_dim, plan.few ? plan.n_few / units + 2 : plan.n_shares, stream);
   }
   return status;
 }

@@ -32,8 +32,11 @@ struct QuantTile {
   // what lane (n, g) reads, and bytes that it takes of K or V
   static constexpr int LANE_BYTES = D / 8;
   typedef uint32_t Codes __attribute__((ext_vector_type(D / 32)));
-  static __device__ __forceinline__ int k_exp_of(int n, int g) { return K_EXP + n * BLOCKS + g * BLOCKS / 4; }
-  static __device__ __forceinline__ int v_exp_of(int n, int g) { return V_EXP + (g * BLOCKS + n * BLOCKS / 16) * 4; }
+  // where lane 16 g + n finds them
+  static __device__ __forceinline__ int k_of(int lane) { return ((lane & 15) * 4 + (lane >> 4)) * LANE_BYTES; }
+  static __device__ __forceinline__ int k_exp_of(int lane) { return K_EXP + ((lane & 15) * 4 + (lane >> 4)) * BLOCKS / 4; }
+  static __device__ __forceinline__ int v_of(int lane) { return V + lane * LANE_BYTES; }
+  static __device__ __forceinline__ int v_exp_of(int lane) { return V_EXP + lane * BLOCKS / 16 * 4; }  // (g BLOCKS + n BLOCKS / 16) 4
 };
 
 // Two elements of byte SEL of `codes`, times the power of two in scale's exponent bits (its other bits are ignored).
@@ -52,5 +55,22 @@ __device__ __forceinline__ u32x4 eight_of_codes(uint32_t codes, float scale) {
 __device__ __forceinline__ float exponent_scale(uint32_t exponents, int i) {
   return __uint_as_float(i == 3 ? exponents >> 1 : exponents << (23 - 8 * i));
 }
+
+// What a lane reads of 16 tokens.
+template <int D>
+struct QuantGroup {
+  typename QuantTile<D>::Codes k, v;
+  uint32_t k_exp, v_exp;
+  __device__ __forceinline__ void load_k(const char* at, int lane) {
+    k = *reinterpret_cast<const typename QuantTile<D>::Codes*>(at + QuantTile<D>::k_of(lane));
+    k_exp = *reinterpret_cast<const uint8_t*>(at + QuantTile<D>::k_exp_of(lane));
+  }
+  __device__ __forceinline__ void load_v(const char* at, int lane) {
+    v = *reinterpret_cast<const typename QuantTile<D>::Codes*>(at + QuantTile<D>::v_of(lane));
+    v_exp = *reinterpret_cast<const uint32_t*>(at + QuantTile<D>::v_exp_of(lane));
+  }
+  // what nobody sees of the lane's token j may hold anything: with this exponent it is finite
+  __device__ __forceinline__ void clear_v(int j) { v_exp &= ~(0xffu << (8 * j)); }
+};
 
 }  // namespace dcp

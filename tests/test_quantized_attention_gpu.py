@@ -76,7 +76,7 @@ def test_shares_that_end_with_a_request(gpu, keys):
     check(_run(gpu, case, max_seqlen_k=5000), case.truth())
 
 
-@pytest.mark.parametrize("requests", [65536])
+@pytest.mark.parametrize("requests", [65536, 65600])
 def test_tens_of_thousands_of_requests(gpu, requests):
     n, n_pages = requests, 4
     x = torch.randn(2, n_pages * 16, 1, 64, device=gpu).to(torch.bfloat16)
