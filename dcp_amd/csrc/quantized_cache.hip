@@ -1,8 +1,9 @@
 // Writes into a paged K/V cache held in 4 bits, and its rows taken back to 16 bits (quantized_cache.h has the layout).
 //
-// Both are bound by HBM where there is enough to do, by a launch and one or two trips to memory where there is not.  A lane has 8
-// elements of a token's row, the 16 bytes that it moves of the 16-bit side at once; four lanes are a block, whose largest element
-// they find together.
+// Both are bound by HBM where there is enough to do, by a launch and two trips to memory where there is not.  A lane takes 8 elements
+// of a token's row, 16 bytes of the 16-bit side and 4 of the other, for several heads one after the other; the lanes of a wave
+// are 4 tokens (8 at head size 64) with all of their pieces, so that of neighbouring slots both K and V are 256 bytes in a row: lanes of one
+// token and four heads would touch four times that of V.
 #include <algorithm>
 
 #include "quantized_cache.h"
@@ -19,32 +20,35 @@ struct QuantRowsParams {
   int64_t page_stride, head_stride;  // of the cache in bytes
   int64_t n_slots;
   int n_tokens, page_size, n_heads;
-  int token_pieces;  // 8-element pieces of a token's K and V
+  int head_groups;  // of kQuantHeads heads
 };
 
-// Where a token's 17 D bytes begin, and its number among the 16.
+// Which rows a thread has: token `token`, piece `piece` of heads [head, head_end).
+constexpr int kQuantThreads = 256, kQuantHeads = 4;
 template <int D>
-__device__ __forceinline__ char* tile_of_slot(const QuantRowsParams& p, int64_t slot, int head, int& j) {
+struct QuantRows {
+  static constexpr int PIECES = D / 8, TOKENS = kQuantThreads / PIECES;  // of a row, of a workgroup
+  int token, piece, head, head_end;
+  __device__ __forceinline__ QuantRows(const QuantRowsParams& p) {
+    const int wg = blockIdx.x / p.head_groups;
+    token = (int)min((int64_t)wg * TOKENS + threadIdx.x / PIECES, (int64_t)0x7fffffff);
+    piece = threadIdx.x % PIECES;
+    head = (blockIdx.x - wg * p.head_groups) * kQuantHeads;
+    head_end = min(head + kQuantHeads, p.n_heads);
+  }
+};
+// Where the 17 D bytes of head 0 begin that hold a slot's token, and its number j among the 16.
+template <int D>
+__device__ __forceinline__ char* tile_of_slot(const QuantRowsParams& p, int64_t slot, int& j) {
   const int64_t page = p.n_slots < 0x7fffffff ? (uint32_t)slot / (uint32_t)p.page_size : slot / p.page_size;
   const int offset = (int)(slot - page * p.page_size);
   j = offset % kQuantTokens;
-  return p.cache + page * p.page_stride + head * p.head_stride + (int64_t)(offset / kQuantTokens) * QuantTile<D>::BYTES;
+  return p.cache + page * p.page_stride + (int64_t)(offset / kQuantTokens) * QuantTile<D>::BYTES;
 }
 
-constexpr int kQuantThreads = 256;
-
-template <int DTYPE, int D>
-__global__ __launch_bounds__(kQuantThreads) void quantized_write_kernel(const QuantRowsParams p) {
-  typedef QuantTile<D> Tile;
-  constexpr int ROW = D / 8;  // pieces of a row
-  const int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x;
-  const int64_t token = i / p.token_pieces;
-  if (token >= p.n_tokens) return;  // (a block's four lanes are of one token)
-  const int in_token = (int)(i - token * p.token_pieces), half = p.token_pieces / 2;
-  const bool is_v = in_token >= half;
-  const int at = is_v ? in_token - half : in_token, head = at / ROW, piece = at % ROW;
-  const u32x4 x = *reinterpret_cast<const u32x4*>((is_v ? p.v : p.k) + token * p.token + head * p.head + piece * 16);
-  const int64_t slot = p.slots[token];
+// Eight elements, of which four lanes have a block, in 4 bits; `byte`: the block's exponent.
+template <int DTYPE>
+__device__ __forceinline__ uint32_t to_codes(u32x4 x, uint32_t& byte) {
   float f[8];
   uint32_t top = 0;  // bits of the largest size: as whole numbers sizes are in their own order, and what is no number is above them
 #pragma unroll
@@ -54,15 +58,14 @@ __global__ __launch_bounds__(kQuantThreads) void quantized_write_kernel(const Qu
   }
   top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, true));  // quad_perm 1 0 3 2
   top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, true));  // quad_perm 2 3 0 1
-  if ((slot < 0) | (slot >= p.n_slots)) return;
   // e + 127, the smallest with top <= 7 2^e: two less than top's own exponent, one more where its mantissa is past 1.75.  (Below the
   // type's normal numbers 0, which holds all of them.)
-  const uint32_t byte = top >= 0x7f800000u ? 255u : (uint32_t)max((int)(top + 0x1fffffu >> 23) - 2, 0);
+  byte = top >= 0x7f800000u ? 255u : (uint32_t)max((int)((top + 0x1fffffu) >> 23) - 2, 0);
   const float scale = __uint_as_float(byte << 23);
-  // The conversion takes the nearest, ties to the even code, and 6 for what is past 5.  Where a block has the type's largest number 4 2^e is
+  // The conversion takes the nearest, ties to the even code, and 6 for what is past 5.  Where a block has the type's largest numbers 4 2^e is
   // past the type's end: sizes past 3 2^e are 3 2^e there.
   constexpr uint32_t LAST = DTYPE == DCP_DTYPE_BF16 ? 126 + 127 : 14 + 127;
-  if (byte == LAST) {
+  if (__builtin_expect(byte == LAST, 0)) {
     const float most = 3.0f * scale;
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = fminf(fmaxf(f[e], -most), most);
@@ -72,54 +75,85 @@ __global__ __launch_bounds__(kQuantThreads) void quantized_write_kernel(const Qu
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[2], f[3], scale, 1);
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[4], f[5], scale, 2);
   codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, f[6], f[7], scale, 3);
+  return codes;
+}
+
+template <int DTYPE, int D>
+__global__ __launch_bounds__(kQuantThreads) void quantized_write_kernel(const QuantRowsParams p) {
+  typedef QuantTile<D> Tile;
+  const QuantRows<D> rows(p);
+  if (rows.token >= p.n_tokens) return;  // (a block's four lanes are of one token)
+  const int64_t slot = p.slots[rows.token], from = rows.token * p.token + rows.piece * 16;
+  u32x4 x[kQuantHeads][2];
+#pragma unroll
+  for (int h = 0; h < kQuantHeads; ++h) {
+    if (rows.head + h >= rows.head_end) break;
+    x[h][0] = *reinterpret_cast<const u32x4*>(p.k + from + (rows.head + h) * p.head);
+    x[h][1] = *reinterpret_cast<const u32x4*>(p.v + from + (rows.head + h) * p.head);
+  }
+  if ((slot < 0) | (slot >= p.n_slots)) return;
   int j;
-  char* tile = tile_of_slot<D>(p, slot, head, j);
-  if (!is_v) {
-    *reinterpret_cast<uint32_t*>(tile + j * (D / 2) + piece * 4) = codes;
-    if (piece % 4 == 0) tile[Tile::K_EXP + j * Tile::BLOCKS + piece / 4] = (char)byte;
-    return;
+  char* tile = tile_of_slot<D>(p, slot, j) + rows.head * p.head_stride;
+#pragma unroll
+  for (int h = 0; h < kQuantHeads; ++h, tile += p.head_stride) {
+    if (rows.head + h >= rows.head_end) break;
+    uint32_t k_exp, v_exp;
+    const uint32_t k = to_codes<DTYPE>(x[h][0], k_exp), v = to_codes<DTYPE>(x[h][1], v_exp);
+    *reinterpret_cast<uint32_t*>(tile + j * (D / 2) + rows.piece * 4) = k;
+    char* to = tile + Tile::V + j / 4 * (2 * D) + j % 4 * Tile::V_PIECE + rows.piece * 16;  // a sixteenth of a row: 4 V_PIECE bytes further each
+    if constexpr (D == 128) {
+      *reinterpret_cast<uint32_t*>(to) = v;
+    } else {
+      *reinterpret_cast<uint16_t*>(to) = (uint16_t)v;
+      *reinterpret_cast<uint16_t*>(to + 8) = (uint16_t)(v >> 16);
+    }
+    if (rows.piece % 4 == 0) {
+      tile[Tile::K_EXP + j * Tile::BLOCKS + rows.piece / 4] = (char)k_exp;
+      tile[Tile::V_EXP + (j / 4 * Tile::BLOCKS + rows.piece / 4) * 4 + j % 4] = (char)v_exp;
+    }
   }
-  char* to = tile + Tile::V + j / 4 * (2 * D) + j % 4 * Tile::V_PIECE;  // sixteenth n: 4 V_PIECE bytes further each
-  if constexpr (D == 128) {
-    *reinterpret_cast<uint32_t*>(to + piece * 16) = codes;
-  } else {
-    *reinterpret_cast<uint16_t*>(to + piece * 16) = (uint16_t)codes;
-    *reinterpret_cast<uint16_t*>(to + piece * 16 + 8) = (uint16_t)(codes >> 16);
-  }
-  if (piece % 4 == 0) tile[Tile::V_EXP + (j / 4 * Tile::BLOCKS + piece / 4) * 4 + j % 4] = (char)byte;
 }
 
 template <int DTYPE, int D>
 __global__ __launch_bounds__(kQuantThreads) void quantized_read_kernel(const QuantRowsParams p) {
   typedef QuantTile<D> Tile;
-  constexpr int ROW = D / 8;
-  const int64_t i = (int64_t)blockIdx.x * kQuantThreads + threadIdx.x;
-  const int64_t token = i / p.token_pieces;
-  if (token >= p.n_tokens) return;
-  const int in_token = (int)(i - token * p.token_pieces), half = p.token_pieces / 2;
-  const bool is_v = in_token >= half;
-  const int at = is_v ? in_token - half : in_token, head = at / ROW, piece = at % ROW;
-  const int64_t slot = p.slots[token];
-  u32x4 x = {0, 0, 0, 0};
-  if ((slot >= 0) & (slot < p.n_slots)) {
+  const QuantRows<D> rows(p);
+  if (rows.token >= p.n_tokens) return;
+  const int64_t slot = p.slots[rows.token], to = rows.token * p.token + rows.piece * 16;
+  const bool there = (slot >= 0) & (slot < p.n_slots);
+  uint32_t codes[kQuantHeads][2], exps[kQuantHeads][2];
+  if (there) {
     int j;
-    const char* tile = tile_of_slot<D>(p, slot, head, j);
-    uint32_t codes, byte;
-    if (!is_v) {
-      codes = *reinterpret_cast<const uint32_t*>(tile + j * (D / 2) + piece * 4);
-      byte = (uint8_t)tile[Tile::K_EXP + j * Tile::BLOCKS + piece / 4];
-    } else {
-      const char* from = tile + Tile::V + j / 4 * (2 * D) + j % 4 * Tile::V_PIECE + piece * 16;
-      if constexpr (D == 128) codes = *reinterpret_cast<const uint32_t*>(from);
-      else codes = *reinterpret_cast<const uint16_t*>(from) | (uint32_t)*reinterpret_cast<const uint16_t*>(from + 8) << 16;
-      byte = (uint8_t)tile[Tile::V_EXP + (j / 4 * Tile::BLOCKS + piece / 4) * 4 + j % 4];
+    const char* tile = tile_of_slot<D>(p, slot, j) + rows.head * p.head_stride;
+#pragma unroll
+    for (int h = 0; h < kQuantHeads; ++h, tile += p.head_stride) {
+      if (rows.head + h >= rows.head_end) break;
+      codes[h][0] = *reinterpret_cast<const uint32_t*>(tile + j * (D / 2) + rows.piece * 4);
+      const char* from = tile + Tile::V + j / 4 * (2 * D) + j % 4 * Tile::V_PIECE + rows.piece * 16;
+      if constexpr (D == 128) codes[h][1] = *reinterpret_cast<const uint32_t*>(from);
+      else codes[h][1] = *reinterpret_cast<const uint16_t*>(from) | (uint32_t)*reinterpret_cast<const uint16_t*>(from + 8) << 16;
+      exps[h][0] = (uint8_t)tile[Tile::K_EXP + j * Tile::BLOCKS + rows.piece / 4];
+      exps[h][1] = (uint8_t)tile[Tile::V_EXP + (j / 4 * Tile::BLOCKS + rows.piece / 4) * 4 + j % 4];
     }
-    x = eight_of_codes<DTYPE>(codes, exponent_scale(byte, 0));
   }
-  *reinterpret_cast<u32x4*>((is_v ? p.v : p.k) + token * p.token + head * p.head + piece * 16) = x;
+#pragma unroll
+  for (int h = 0; h < kQuantHeads; ++h) {
+    if (rows.head + h >= rows.head_end) break;
+#pragma unroll
+    for (int of = 0; of < 2; ++of) {
+      u32x4 x = {0, 0, 0, 0};
+      if (there) x = eight_of_codes<DTYPE>(codes[h][of], exponent_scale(exps[h][of], 0));
+      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>((of ? p.v : p.k) + to + (rows.head + h) * p.head));
+    }
+  }
 }
 
 namespace {
+
+int64_t row_workgroups(const QuantRowsParams& p, int head_dim) {
+  const int64_t tokens = kQuantThreads / (head_dim / 8);  // of a workgroup
+  return (p.n_tokens + tokens - 1) / tokens * p.head_groups;
+}
 
 // What the two calls have in common: their arguments, checked, as the kernels take them.
 int quantized_rows(const char* what, QuantRowsParams& p, const void* k, const void* v, const int64_t* slot_mapping, const void* cache, int n_tokens,
@@ -139,17 +173,15 @@ int quantized_rows(const char* what, QuantRowsParams& p, const void* k, const vo
   DCP_REQUIRE(k && v && slot_mapping && (n_pages == 0 || cache), "%s: null argument", what);
   DCP_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)cache) & 15) == 0, "%s: k, v and the cache must be 16-byte aligned", what);
   p = {(char*)k, (char*)v, slot_mapping, (char*)cache, token_stride * 2, head_stride * 2, cache_page_stride, cache_head_stride, n_pages * page_size,
-       n_tokens, page_size, n_heads_kv, 2 * n_heads_kv * (head_dim / 8)};
-  const int64_t n_wg = ((int64_t)n_tokens * p.token_pieces + kQuantThreads - 1) / kQuantThreads;
-  DCP_REQUIRE(n_wg < (int64_t)1 << 31, "%s: too many rows", what);
+       n_tokens, page_size, n_heads_kv, (n_heads_kv + kQuantHeads - 1) / kQuantHeads};
+  DCP_REQUIRE(row_workgroups(p, head_dim) < (int64_t)1 << 31, "%s: too many rows", what);
   return DCP_OK;
 }
 
 template <typename Kernel>
-int launch_rows(Kernel kernel, const char* name, const QuantRowsParams& p, void* stream) {
-  const int64_t n_wg = ((int64_t)p.n_tokens * p.token_pieces + kQuantThreads - 1) / kQuantThreads;
+int launch_rows(Kernel kernel, const char* name, const QuantRowsParams& p, int head_dim, void* stream) {
   KernelTimer timer(name, stream);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(kQuantThreads), 0, (hipStream_t)stream, p);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)row_workgroups(p, head_dim)), dim3(kQuantThreads), 0, (hipStream_t)stream, p);
   return check_launch(name);
 }
 
@@ -172,7 +204,7 @@ extern "C" int dcp_quantized_cache_write(const void* k, const void* v, const int
                                         head_stride, n_pages, page_size, cache_page_stride, cache_head_stride))
     return status;
   if (n_tokens == 0 || n_pages == 0) return DCP_OK;
-  return launch_rows(DCP_QUANT_KERNEL(quantized_write_kernel), "quantized_write_kernel", p, stream);
+  return launch_rows(DCP_QUANT_KERNEL(quantized_write_kernel), "quantized_write_kernel", p, head_dim, stream);
 }
 
 extern "C" int dcp_quantized_cache_read(const void* cache, const int64_t* slot_mapping, void* k, void* v, int n_tokens, int n_heads_kv, int head_dim,
@@ -185,5 +217,5 @@ extern "C" int dcp_quantized_cache_read(const void* cache, const int64_t* slot_m
                                         head_stride, n_pages, page_size, cache_page_stride, cache_head_stride))
     return status;
   if (n_tokens == 0) return DCP_OK;
-  return launch_rows(DCP_QUANT_KERNEL(quantized_read_kernel), "quantized_read_kernel", p, stream);
+  return launch_rows(DCP_QUANT_KERNEL(quantized_read_kernel), "quantized_read_kernel", p, head_dim, stream);
 }

@@ -31,24 +31,40 @@ def quantized_cache_pages(n_pages: int, page_size: int, n_heads_kv: int, head_di
     return torch.zeros(n_pages, n_heads_kv, page_size // 16, 17 * head_dim, dtype=torch.uint8, device=device)
 
 
+# A short call is as long as its checks and its launch (3 of 6 us), so what is as it should be passes in one expression; what is not is told
+# apart afterwards.
 def _cache_args(cache: torch.Tensor, here: int) -> tuple:
     """``(address, heads, head size, pages, page size, page stride, head stride)`` of a cache on the current device."""
-    at = _check(cache, torch.uint8, "cache", here, dense=False)
-    shape, strides = cache.shape, cache.stride()
-    if len(shape) != 4 or shape[3] not in (17 * 64, 17 * 128) or strides[3] != 1 or (strides[2] != shape[3] and shape[2] > 1) or shape[2] < 1:
+    try:
+        shape, strides = cache.shape, cache.stride()
+        good = (len(shape) == 4 and (shape[3] == 2176 or shape[3] == 1088) and strides[3] == 1 and shape[2] > 0 and
+                (strides[2] == shape[3] or shape[2] == 1) and cache.dtype is torch.uint8 and cache.get_device() == here)
+    except AttributeError:
+        good = False
+    if not good:
+        _check(cache, torch.uint8, "cache", here, dense=False)
         raise ValueError("cache must be [n_pages, n_heads_kv, page_size // 16, 17 * head_dim] of head size 64 or 128, dense in the "
                          f"last two, got {list(shape)} with strides {list(strides)}")
-    return at, shape[1], shape[3] // 17, shape[0], 16 * shape[2], strides[0], strides[1]
+    return cache.data_ptr(), shape[1], shape[3] // 17, shape[0], 16 * shape[2], strides[0], strides[1]
 
 
 def _rows(k, v, slot_mapping, heads: int, head_dim: int, here: int) -> tuple:
     """``(k, v, slots, n_tokens, dtype, token stride, head stride)`` of rows that belong into a cache of these sizes."""
-    dtype = k.dtype if isinstance(k, torch.Tensor) else None
-    k_at, v_at = _check(k, dtype, "k", here, dense=False), _check(v, dtype, "v", here, dense=False)
-    strides = k.stride()
-    if k.dim() != 3 or k.shape != v.shape or strides != v.stride() or tuple(k.shape[1:]) != (heads, head_dim) or strides[2] != 1:
-        raise ValueError(f"k and v must be [n_tokens, {heads}, {head_dim}] with the same strides and dense rows")
-    return k_at, v_at, _check(slot_mapping, torch.int64, "slot_mapping", here, (k.shape[0],)), k.shape[0], dtype_code(dtype), strides[0], strides[1]
+    try:
+        dtype, shape, strides = k.dtype, k.shape, k.stride()
+        good = (len(shape) == 3 and shape[1] == heads and shape[2] == head_dim and strides[2] == 1 and shape == v.shape and strides == v.stride() and
+                v.dtype is dtype and k.get_device() == here and v.get_device() == here)
+        slots_good = (slot_mapping.dtype is torch.int64 and slot_mapping.dim() == 1 and slot_mapping.get_device() == here and
+                      slot_mapping.is_contiguous())
+    except AttributeError:
+        good, dtype = False, getattr(k, "dtype", torch.bfloat16)
+    if not good:
+        _check(k, dtype, "k", here, dense=False), _check(v, dtype, "v", here, dense=False)
+        if isinstance(slot_mapping, torch.Tensor):
+            raise ValueError(f"k and v must be [n_tokens, {heads}, {head_dim}] with the same strides and dense rows")
+    if not good or not slots_good or slot_mapping.shape[0] != shape[0]:
+        _check(slot_mapping, torch.int64, "slot_mapping", here, (shape[0],))
+    return k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), shape[0], dtype_code(dtype), strides[0], strides[1]
 
 
 def quantized_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, cache: torch.Tensor) -> None:
@@ -78,11 +94,16 @@ def quantized_cache_read(cache: torch.Tensor, slot_mapping: torch.Tensor, dtype:
     here = torch._C._cuda_getDevice()
     cache_at, heads, head_dim, n_pages, page_size, page, head = _cache_args(cache, here)
     if out is None:
-        n_tokens = slot_mapping.shape[0] if isinstance(slot_mapping, torch.Tensor) and slot_mapping.dim() == 1 else 0
-        kv = torch.empty((2, n_tokens, heads, head_dim), dtype=dtype, device=cache.device)
-        out = (kv[0], kv[1])
-    k, v = out
-    k_at, v_at, slots, n_tokens, code, token_stride, head_stride = _rows(k, v, slot_mapping, heads, head_dim, here)
+        _check(slot_mapping, torch.int64, "slot_mapping", here)
+        if slot_mapping.dim() != 1:
+            raise ValueError(f"slot_mapping must have one axis, got {list(slot_mapping.shape)}")
+        n_tokens, code = slot_mapping.shape[0], dtype_code(dtype)
+        k = cache.new_empty((n_tokens, heads, head_dim), dtype=dtype)
+        v = torch.empty_like(k)
+        k_at, v_at, slots, token_stride, head_stride = k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), heads * head_dim, head_dim
+    else:
+        k, v = out
+        k_at, v_at, slots, n_tokens, code, token_stride, head_stride = _rows(k, v, slot_mapping, heads, head_dim, here)
     if (n_tokens | page_size | heads) >> 31:
         _in_32_bits(n_tokens=n_tokens, page_size=page_size, n_heads_kv=heads)
     _lib.call("dcp_quantized_cache_read", cache_at, slots, k_at, v_at, n_tokens, heads, head_dim, code, token_stride, head_stride, n_pages,
