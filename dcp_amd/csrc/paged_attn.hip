@@ -270,7 +270,8 @@ __device__ __forceinline__ void paged_few(int wg, char* lds) {
       for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(mine + (rt * 16 + n) * Lds::O_STRIDE + 16 * dt + 4 * g) = o[rt][dt];
     }
     __syncthreads();
-    join_few<DTYPE, D, ROWS, NW, Lds::WAVE>(walk, u, lds, sums, kv_head0, row0);
+    join_few<DTYPE, D, ROWS, NW, Lds::WAVE>(walk, u, walk.slot(u), walk.n_cut(u), lds, sums, kv_head0, row0,
+                                            [](PagedArgs& p, int r) { return r / p.group; });
     __syncthreads();  // nobody's part of LDS is filled again before all have read it
   }
 }

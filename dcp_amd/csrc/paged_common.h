@@ -8,6 +8,18 @@
 
 namespace dcp {
 
+// Whole numbers from 0 up to 2^31 divided by one that the host knows: 2 n mul / 2^(32 + shift) with mul = floor(2^(31 + shift) / d) + 1 and d
+// at most 2^shift is n / d and less than 1 / d more.  (Three instructions; a division by any number is some twenty-five.)
+struct Divider {
+  uint32_t mul, shift;
+  static Divider of(int d) {
+    uint32_t shift = 0;
+    while (((int64_t)1 << shift) < d) ++shift;
+    return {(uint32_t)(((uint64_t)1 << (31 + shift)) / (uint64_t)d) + 1, shift};
+  }
+};
+__device__ __forceinline__ int divide(int n, KernArgs<Divider>& by) { return (int)(__umulhi(2u * (uint32_t)n, by.mul) >> by.shift); }
+
 // Keys that rows look at: the requests' own, or prefixes that requests share.
 struct PagedSource {
   const int32_t* block_table;
@@ -49,6 +61,7 @@ struct PagedParams {
   int few_whole;                 // a workgroup takes a unit
   int n_few, few_first;     // workgroups; of paged_both_kernel those before the ones of rows
   int merge_sets;           // of lanes that share a row in the merge, a power of two
+  Divider by_page, by_group, by_heads;  // page_size / 16, group, n_heads_kv (quantized_few_kernel)
 };
 typedef KernArgs<PagedParams> PagedArgs;
 typedef KernArgs<PagedSource> SourceArgs;
@@ -237,7 +250,8 @@ struct FewUnit {
 // together, unit by unit.  Shares are counted in turns of the waves at a head's tiles: a cut inside one would cost both of its sides a whole
 // one.  (One context of 1500 keys, 8 heads, which 47 tiles a head then fit no better: counted in tiles 14.4 us, in turns 11.4.)
 // `chunk_sums`: LDS, an int for every 64 requests.
-template <int ROWS, int NW>
+// WHOLE: it is known to be a unit.  START: turns that the start of a unit is counted as, so that a workgroup of many short units has fewer.
+template <int ROWS, int NW, bool WHOLE = false, int START = 0>
 struct FewWalk {
   int lane, wg, n_chunks, turns_log2, per, begin, end, at;
   int before = 0, chunk = 0, work, scan, index;
@@ -253,7 +267,7 @@ struct FewWalk {
     work = 0;
     if (b < p.own.batch) {
       r = FewRequest(p, b);
-      work = r.units(p, ROWS) * (whole_units ? 1 : (r.n_tiles + turns - 1) >> turns_log2);
+      work = r.units(p, ROWS) * (WHOLE || whole_units ? 1 : START + ((r.n_tiles + turns - 1) >> turns_log2));
     }
     return r;
   }
@@ -263,7 +277,7 @@ struct FewWalk {
     lane = threadIdx.x & 63;
     wg = wg_;
     n_chunks = (p0.own.batch + 63) / 64;
-    whole_units = p0.few_whole != 0;
+    whole_units = WHOLE || p0.few_whole != 0;
     turns_log2 = (NW == 8 ? 3 : 2) - p0.few_heads_log2;
     int total = 0;
     requests = requests_of(0, work);
@@ -319,8 +333,13 @@ struct FewWalk {
       const int in_request = at - (unit_end - __builtin_amdgcn_readlane(work, index)), turns = 1 << turns_log2;
       if (in_request < 0) return false;  // (tables whose tokens are many times those there are: their sums wrap)
       u.turns = whole_units ? 1 : (u.request.n_tiles + turns - 1) >> turns_log2;
-      u.unit = __builtin_amdgcn_readfirstlane(in_request / u.turns);
-      const int first_turn = in_request - u.unit * u.turns;
+      u.unit = __builtin_amdgcn_readfirstlane(in_request / (u.turns + START));
+      int first_turn = in_request - u.unit * (u.turns + START) - START;
+      if (START > 0 && first_turn < 0) {
+        at -= first_turn;
+        first_turn = 0;
+        if (at >= end) return false;
+      }
       u.taken = min(u.turns - first_turn, end - at);
       u.t_begin = whole_units ? 0 : first_turn * turns;
       u.t_end = whole_units ? u.request.n_tiles : min(u.request.n_tiles, u.t_begin + u.taken * turns);
@@ -335,14 +354,15 @@ struct FewWalk {
   __device__ __forceinline__ int n_cut(const FewUnit& u) const { return (at - u.taken + u.turns - 1) / per - wg + 1; }
 };
 
-// The waves' results of a unit's piece joined and stored.  Wave x has row r's O, relative to its maximum, at lds + x * WAVE as
+// The waves' results of a unit's piece joined and stored; `slot` and `n_cut` as FewWalk has them of it.  Wave x has row r's O, relative to its maximum, at lds + x * WAVE as
 // float [row][D + 4], the maximum and the sum of the weights in sums[x][row]; it is of the workgroup's kv head x % heads.
-template <int DTYPE, int D, int ROWS, int NW, int WAVE>
-__device__ __forceinline__ void join_few(const FewWalk<ROWS, NW>& walk, const FewUnit& u, const char* lds, const float (*sums)[ROWS][2], int kv_head0, int row0) {
+// `token_of(p, r)`: r / group.  ONE_HEAD: the workgroup has one kv head.
+template <int DTYPE, int D, int ROWS, int NW, int WAVE, bool ONE_HEAD = false, typename Walk, typename TokenOf>
+__device__ __forceinline__ void join_few(const Walk& walk, const FewUnit& u, int slot, int n_cut, const char* lds, const float (*sums)[ROWS][2],
+                                         int kv_head0, int row0, TokenOf token_of) {
   PagedArgs& p = fresh_kernel_args<PagedParams>();
-  const int heads = 1 << p.few_heads_log2, n_rows = u.request.n_tok * p.group, group = p.group;
+  const int heads = ONE_HEAD ? 1 : 1 << p.few_heads_log2, n_rows = u.request.n_tok * p.group, group = p.group;
   const bool cut = u.taken < u.turns;
-  const int slot = walk.slot(u), n_cut = walk.n_cut(u);
   constexpr int PIECES = D / 4;  // of a row
   for (int i = threadIdx.x; i < heads * ROWS * PIECES; i += NW * 64) {
     const int piece = i % PIECES, row = i / PIECES % ROWS, of = i / PIECES / ROWS, r = row0 + row;
@@ -359,7 +379,8 @@ __device__ __forceinline__ void join_few(const FewWalk<ROWS, NW>& walk, const Fe
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[e] += weight * o4[e];
     }
-    const int64_t token = u.request.first_tok + r / group, head = (kv_head0 + of) * group + r % group;
+    const int tok = token_of(p, r);
+    const int64_t token = u.request.first_tok + tok, head = (kv_head0 + of) * group + (r - tok * group);
     if ((piece == 0) & (u.t_begin == 0) & !walk.whole_units) p.cuts[token * p.n_heads_q + head] = cut_of(walk.wg, n_cut, slot, of * ROWS + row);
     if (cut) {
       const int64_t to = (((int64_t)walk.wg * 2 + slot) * heads + of) * ROWS + row;

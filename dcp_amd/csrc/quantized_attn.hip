@@ -19,12 +19,19 @@
 
 namespace dcp {
 
+// LDS of the kernel of few rows.  A wave has STAGES tiles of 32 keys under way: of both groups of 16 their codes as they lie in the cache (K's pieces
+// in the order of the lanes that take them), then their exponents.  Its result takes the place of its tiles, of EARLY_ROWS and
+// fewer that of the second alone.
 template <int D, int RT, int NW>
 struct QuantFewLds {
-  static constexpr int ROWS = 16 * RT, WAVE = ROWS * (D + 4) * 4;  // a wave's result: float [row][D + 4]
-  static constexpr int SUMS = NW * WAVE;                           // float [wave][row][2]
-  static constexpr int CHUNKS = SUMS + NW * ROWS * 2 * 4;          // int [batch / 64]
-  static constexpr int BYTES = CHUNKS + kFewMaxBatch / 64 * 4;
+  static constexpr int ROWS = 16 * RT, STAGES = 2, GROUP = 16 * D, EXPS = 2 * GROUP, GROUP_EXPS = 256, STAGE = EXPS + 2 * GROUP_EXPS;
+  static constexpr int RESULT = ROWS * (D + 4) * 4;  // float [row][D + 4]
+  static constexpr int EARLY_ROWS = 8;
+  static_assert(EARLY_ROWS * (D + 4) * 4 <= STAGE, "");
+  static constexpr int WAVE = STAGES * STAGE > RESULT ? STAGES * STAGE : RESULT;
+  static constexpr int SUMS = NW * WAVE;                   // float [wave][row][2]
+  static constexpr int BYTES = SUMS + NW * ROWS * 2 * 4;
+  static_assert(kFewMaxBatch / 64 * 4 <= SUMS, "");        // (FewWalk's sums, before there are tiles)
 };
 
 // The operands of V for two groups of 16 keys: those of elements n D / 16 + 2 U and the one after it.
@@ -56,14 +63,21 @@ __device__ __forceinline__ void multiply_v(const QuantGroup<D> (&x)[2], const fl
       o[rt][2 * U] = mfma_16x16x32<DTYPE>(even, pb[rt], o[rt][2 * U]);
       o[rt][2 * U + 1] = mfma_16x16x32<DTYPE>(odd, pb[rt], o[rt][2 * U + 1]);
     }
-    multiply_v<DTYPE, D, RT, U + 1>(x, scale, pb, o);
+      multiply_v<DTYPE, D, RT, U + 1>(x, scale, pb, o);
   }
 }
 
 // The kernel of few rows: the waves of a workgroup share no tile.  Each takes tiles of 32 keys of its own and waits for nobody until its
-// share of the keys is done; work is cut as over a cache of 16 bits (FewWalk).
-template <int DTYPE, int D, int RT, int NW>
-__global__ __launch_bounds__(NW * 64, RT == 1 ? 3 : 2) void quantized_few_kernel(const PagedParams) {
+// share of the keys is done; work is cut as over a cache of 16 bits (FewWalk), or whole units where they are short (WHOLE).
+//
+// What bounds it is the number of instructions: with 4 bits a key the memory would let a SIMD issue 280 of them a tile.  64 conversions
+// and 32 of their results put in order are what the tile cannot do without; whether it has to be masked is asked once for 32 of them, and
+// weights are taken against a reference maximum that the tile's own is only looked for where the weights' sum says so.  What is done once a
+// piece is bound by the fetch of its instructions (some 15 ns each the first time they are met), so each step stands once in the
+// code, whichever piece it is of, tiles are not unrolled over their places in LDS, and there is no division by a number known on the host.
+constexpr int kStartTurns = 2;
+template <int DTYPE, int D, int RT, int NW, bool WHOLE>
+__global__ __launch_bounds__(NW * 64, NW == 4 && (RT == 1 || D == 64) ? (RT == 1 && D == 64 ? 4 : 3) : 2) void quantized_few_kernel(const PagedParams) {
   typedef QuantFewLds<D, RT, NW> Lds;
   typedef QuantTile<D> Tile;
   __shared__ __attribute__((aligned(16))) char lds[Lds::BYTES];
@@ -72,90 +86,171 @@ __global__ __launch_bounds__(NW * 64, RT == 1 ? 3 : 2) void quantized_few_kernel
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   float(*sums)[ROWS][2] = reinterpret_cast<float(*)[ROWS][2]>(lds + Lds::SUMS);
 
-  FewWalk<ROWS, NW> walk(blockIdx.x, reinterpret_cast<int*>(lds + Lds::CHUNKS));
+  FewWalk<ROWS, NW, WHOLE, WHOLE ? 0 : kStartTurns> walk(blockIdx.x, reinterpret_cast<int*>(lds));
+  if (walk.n_chunks > 1) __syncthreads();
+  // ---- the piece at work -------------------------------------------------------------------
   FewUnit u;
-  while (walk.next(u)) {
+  int kv_head = 0, row0 = 0, n_groups = 0, n_steps = 0;
+  const char* head = nullptr;
+  int all_last = 0, all_first = 0;  // every row sees the keys up to the one and, of those behind the first tokens, from the other on
+  int last_key[RT];                 // of the lane's rows (past the last one: the last one again, not written)
+  u32x4 q[RT][KS];                  // slots of product ks: D / 4 elements from g D / 4 on, eight at a time
+  // Of 32 of the wave's tiles of it lane 2 i + j holds the 16-key group j of the i-th: where it is, and its first key.  Tiles are asked for two
+  // steps ahead, so the keys of the next 32 are known before the last two of these are done.
+  int lane_page, lane_tile, lane_key, lane_key_ahead;
+  int64_t lane_off;
+  uint64_t full = 0, full_ahead;  // bit 2 i + j: every row sees all of that group
+  auto ask = [&](int step) {
     PagedArgs& p = fresh_kernel_args<PagedParams>();
-    const FewRequest& request = u.request;
-    const int kv_head = u.unit % p.n_heads_kv, row0 = u.unit / p.n_heads_kv * ROWS, n_rows = request.n_tok * p.group;
-    const KeyGroups groups = request.groups(p);
-    const int n_groups = request.n_keys > 0 ? groups.count() : 0;
+    const int group = 2 * (u.t_begin + w + NW * (step + (lane >> 1))) + (lane & 1);
+    lane_key_ahead = kNoKey;
+    lane_page = -1;
+    lane_tile = 0;
+    if (group < n_groups && group < 2 * u.t_end) {
+      const int at = u.request.groups(p).at(group), entry = divide(at, p.by_page);
+      lane_key_ahead = at * 16;
+      lane_tile = at - entry * (p.page_size / 16);
+      lane_page = p.own.block_table[u.b * p.own.table_stride + entry];
+    }
+  };
+  auto told = [&]() {
+    PagedArgs& p = fresh_kernel_args<PagedParams>();
+    const bool there = (unsigned)lane_page < (unsigned)p.n_pages;
+    lane_off = there ? lane_page * p.page_stride + lane_tile * Tile::BYTES : 0;
+    const int key = lane_key_ahead = there ? lane_key_ahead : kNoKey;
+    full_ahead = __ballot((key + 15 <= all_last) & ((key >= all_first) | (key + 15 < p.n_starting)));
+  };
 
-    // ---- where the wave's next 32 tiles are: lane 2 i + j holds the 16-key group j of the i-th of them ------------
-    int64_t lane_off = 0;
-    int lane_key = kNoKey;
-    auto look_up = [&](int step) {
+  // ---- a tile goes from memory straight into LDS, into the place of the one two before it, which the wave has read by then ---------
+  char* my_lds = lds + w * Lds::WAVE;
+  const uint32_t my_at = lds_address(lds) + w * Lds::WAVE;
+  const uint32_t k_from = D == 128 ? Tile::k_of(lane) : 16 * lane, v_from = Tile::v_of(lane), exps_from = Tile::K_EXP + lane % (D / 4) * 4;
+  constexpr int LOADS = D == 128 ? 6 : 4;
+  auto issue = [&](int step) {
+    const uint32_t to = my_at + (step & 1) * Lds::STAGE;
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the last reads of what is there are done
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const uint64_t at = (uint64_t)(head + lane_value(lane_off, 2 * (step % 32) + kt));
+      KvTile<D>::load_group_at_streaming(to + kt * Lds::GROUP, at, k_from);  // (at head size 64 with V)
+      if constexpr (D == 128) KvTile<D>::load_group_at_streaming(to + kt * Lds::GROUP + Tile::V, at, v_from);
+      load_async_dword(to + Lds::EXPS + kt * Lds::GROUP_EXPS, exps_from, reinterpret_cast<const void*>(at));
+    }
+  };
+  const char* k_read = my_lds + (D == 128 ? 16 * lane : Tile::k_of(lane));
+  const char* v_read = my_lds + Tile::v_of(lane);
+  const char* k_exp_read = my_lds + Lds::EXPS - Tile::K_EXP + Tile::k_exp_of(lane);
+  const char* v_exp_read = my_lds + Lds::EXPS - Tile::K_EXP + Tile::v_exp_of(lane);
+
+  f32x4 o[RT][DT];
+  float m_run[RT], l_run[RT];
+  int have = 0;  // results to be joined
+  asm("" : "+s"(have));  // (not known to be none: the compiler would write the first turn out on its own)
+  FewUnit done = {};
+  int slot = 0, n_cut = 0, done_head = 0, done_row0 = 0;
+  while (true) {
+    // ---- the next piece's pages and rows are asked for, the waves' results of the last one are joined ----------------------
+    const bool more = walk.next(u) & (!WHOLE | !have);
+    if (!more && !have) return;
+    if (more) {
       PagedArgs& p = fresh_kernel_args<PagedParams>();
-      const int group = 2 * (u.t_begin + w + NW * (step + (lane >> 1))) + (lane & 1);
-      lane_off = 0;
-      lane_key = kNoKey;
-      if (group < n_groups && group < 2 * u.t_end) {
-        const int key = groups.at(group) * 16, entry = key / p.page_size;
-        const int page = p.own.block_table[u.b * p.own.table_stride + entry];
-        if ((unsigned)page < (unsigned)p.n_pages) {
-          lane_key = key;
-          lane_off = page * p.page_stride + (int64_t)((key - entry * p.page_size) / 16) * Tile::BYTES;
+      const int chunk = divide(u.unit, p.by_heads);
+      kv_head = u.unit - chunk * p.n_heads_kv;
+      row0 = chunk * ROWS;
+      n_groups = u.request.n_keys > 0 ? u.request.groups(p).count() : 0;
+      n_steps = max((min(u.t_end, n_groups) - u.t_begin - w + NW - 1) / NW, 0);  // (a tile or more has a group)
+      head = reinterpret_cast<const char*>(p.k) + kv_head * p.head_stride;
+      ask(0);
+    }
+    // Results of few rows lie in the second tile's place, so that the first tile of the next piece need not wait for them to be read.
+    const bool early = done.request.n_tok * fresh_kernel_args<PagedParams>().group - done_row0 <= Lds::EARLY_ROWS;
+    if (have) {  // element (4 g + e) D / 16 + dt is o[dt][e]
+      float* result = reinterpret_cast<float*>(my_lds + (early ? Lds::STAGE : 0));
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float l = rows_sum(l_run[rt]);
+        if (g == 0) {
+          sums[w][rt * 16 + n][0] = l == 0.0f ? -INFINITY : m_run[rt];
+          sums[w][rt * 16 + n][1] = l;
+        }
+        if (!early | (rt * 16 + n < Lds::EARLY_ROWS)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int dt = 0; dt < DT; dt += 4)
+              *reinterpret_cast<f32x4*>(result + (rt * 16 + n) * (D + 4) + (4 * g + e) * DT + dt) =
+                  f32x4{o[rt][dt][e], o[rt][dt + 1][e], o[rt][dt + 2][e], o[rt][dt + 3][e]};
         }
       }
-    };
-    const char* head = reinterpret_cast<const char*>(p.k) + kv_head * p.head_stride;
-    const int n_steps = n_groups > 0 && u.t_begin + w < u.t_end ? (u.t_end - u.t_begin - w + NW - 1) / NW : 0;
-    QuantGroup<D> next[2];
-    int next_key[2];
-    auto load = [&](int step) {
-      if (step % 32 == 0) look_up(step);
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        const int from = 2 * (step % 32) + kt;
-        const char* at = head + lane_value(lane_off, from);
-        next_key[kt] = __builtin_amdgcn_readlane(lane_key, from);
-        typedef typename Tile::Codes Codes;
-        next[kt].k = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(at + Tile::k_of(lane)));
-        next[kt].k_exp = *reinterpret_cast<const uint8_t*>(at + Tile::k_exp_of(lane));
-        next[kt].v = __builtin_nontemporal_load(reinterpret_cast<const Codes*>(at + Tile::v_of(lane)));
-        next[kt].v_exp = *reinterpret_cast<const uint32_t*>(at + Tile::v_exp_of(lane));
-      }
-    };
-    if (n_steps > 0) load(0);
-
-    // ---- this lane's rows --------------------------------------------------------------
-    int last_key[RT], first_key[RT];
-    int w_last = 0x7fffffff, w_first = 0;
-    u32x4 q[RT][KS];  // slots of product ks: D / 4 elements from g D / 4 on, eight at a time
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const int r = row0 + rt * 16 + n, tok = r / p.group, q_head = kv_head * p.group + r % p.group;
-      const bool live = r < n_rows;
-      const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (request.first_tok + tok) * p.q_token + q_head * p.q_head + g * (D / 4);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        q[rt][ks] = u32x4{0, 0, 0, 0};
-        if (live) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + 8 * ks);
-      }
-      last_key[rt] = live ? request.n_keys - request.n_tok + tok : 0x7fffffff;
-      first_key[rt] = live && p.window > 0 ? max(last_key[rt] - p.window + 1, 0) : 0;
-      w_last = min(w_last, wave_min(last_key[rt]));
-      w_first = max(w_first, wave_max(first_key[rt]));
     }
-    f32x4 o[RT][DT];
-    float m_run[RT], l_run[RT];
+    if (more) {
+      PagedArgs& p = fresh_kernel_args<PagedParams>();
+      const int at0 = u.request.n_keys - u.request.n_tok, last_row = u.request.n_tok * p.group - 1;
+      all_last = at0 + divide(row0, p.by_group);
+      all_first = p.window > 0 ? max(at0 + divide(min(row0 + ROWS - 1, last_row), p.by_group) - p.window + 1, 0) : 0;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = min(row0 + rt * 16 + n, last_row), tok = divide(r, p.by_group), q_head = kv_head * p.group + r - tok * p.group;
+        const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (u.request.first_tok + tok) * p.q_token + q_head * p.q_head + g * (D / 4);
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + 8 * ks);
+        last_key[rt] = at0 + tok;
+      }
+    }
+    if (have) phase_barrier();
+    wait_loads();  // of pages and rows: no product is to wait for rows that may be under way, and with them for tiles that are
+    told();
+    const bool issued = more & early & (n_steps > 0) & (have != 0);
+    if (issued) issue(0);
+    if (have) {
+      join_few<DTYPE, D, ROWS, NW, Lds::WAVE, true>(walk, done, slot, n_cut, lds + (early ? Lds::STAGE : 0), sums, done_head, done_row0,
+                                              [](PagedArgs& p, int r) { return divide(r, p.by_group); });
+      if (!more) return;
+      phase_barrier();  // nobody's part of LDS is filled again before all have read it
+    }
+    for (int i = issued ? 1 : 0; i < min(n_steps, 2); ++i) issue(i);
+
+    const float scale_log2 = fresh_kernel_args<PagedParams>().scale_log2;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      m_run[rt] = -INFINITY;
+      m_run[rt] = kNoMax;
       l_run[rt] = 0.0f;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-
+    bool anchored = false;  // every row has a reference maximum
     for (int step = 0; step < n_steps; ++step) {
-      QuantGroup<D> x[2] = {next[0], next[1]};
-      const int tile_key[2] = {next_key[0], next_key[1]};
-      if (step + 1 < n_steps) load(step + 1);
-      bool whole = true, full = true;
+      if (step % 32 == 0) {
+        lane_key = lane_key_ahead;
+        full = full_ahead;
+      }
+      const int left = n_steps - step;
+      if (left > 1) __builtin_amdgcn_s_waitcnt(0x0F70 | LOADS);  // all loads but those of the tile behind it
+      else wait_loads();
+      asm volatile("" ::: "memory");
+      typedef typename Tile::Codes Codes;
+      QuantGroup<D> x[2];
+      const int stage = (step & 1) * Lds::STAGE;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        whole = whole & groups.sees_all_of_16(tile_key[kt]);
-        full = full & (tile_key[kt] + 15 <= w_last) & ((tile_key[kt] >= w_first) | (tile_key[kt] + 15 < p.n_starting));
+        x[kt].k = *reinterpret_cast<const Codes*>(k_read + (stage + kt * Lds::GROUP));
+        x[kt].v = *reinterpret_cast<const Codes*>(v_read + (stage + kt * Lds::GROUP));
+        x[kt].k_exp = *reinterpret_cast<const uint8_t*>(k_exp_read + (stage + kt * Lds::GROUP_EXPS));
+        x[kt].v_exp = *reinterpret_cast<const uint32_t*>(v_exp_read + (stage + kt * Lds::GROUP_EXPS));
+      }
+      const int from = 2 * (step % 32);
+      const bool is_full = (full >> from & 3) == 3;
+      int tile_key[2] = {0, 0};
+      if (!is_full) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) tile_key[kt] = __builtin_amdgcn_readlane(lane_key, from + kt);
+      }
+      if (left > 2) {
+        if ((step + 2) % 32 == 0) {
+          ask(step + 2);
+          told();
+        }
+        issue(step + 2);
       }
       f32x4 s[RT][2];
 #pragma unroll
@@ -170,7 +265,10 @@ __global__ __launch_bounds__(NW * 64, RT == 1 ? 3 : 2) void quantized_few_kernel
           for (int rt = 0; rt < RT; ++rt) s[rt][kt] = mfma_16x16x32<DTYPE>(a, q[rt][ks], s[rt][kt]);
         }
       }
-      if (!(whole & full)) {
+      if (__builtin_expect(!is_full, 0)) {
+        PagedArgs& p = fresh_kernel_args<PagedParams>();
+        const KeyGroups groups = u.request.groups(p);
+        const int reach = p.window > 0 ? p.window : 0x7fffffff;  // a query sees the keys less than this before its last
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -179,43 +277,57 @@ __global__ __launch_bounds__(NW * 64, RT == 1 ? 3 : 2) void quantized_few_kernel
             if (!((tile_key[kt] != kNoKey) & groups.sees(key))) x[kt].clear_v(e);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-              const bool visible = (key <= last_key[rt]) & ((key < p.n_starting) | (key >= first_key[rt])) & (tile_key[kt] != kNoKey);
+              const bool visible = (key <= last_key[rt]) & ((key < p.n_starting) | (last_key[rt] - key < reach)) & (tile_key[kt] != kNoKey);
               s[rt][kt][e] = visible ? s[rt][kt][e] : -INFINITY;
             }
             __builtin_amdgcn_sched_barrier(0);  // (all conditions at once need more scalar registers than there are)
           }
       }
       u32x4 pb[RT];
+      float sum[RT];
+      for (bool raise = !anchored;; raise = true) {
+        if (__builtin_expect(raise, 0)) {  // the reference to the tile's maximum, what was summed before taken relative to it
+          bool without = false, summed = false;
+          float alpha[RT];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float mx = fmaxf(s[rt][0][0], s[rt][1][0]);
+          for (int rt = 0; rt < RT; ++rt) {
+            float mx = s[rt][0][0];
 #pragma unroll
-        for (int e = 1; e < 4; ++e) mx = fmaxf(mx, fmaxf(s[rt][0][e], s[rt][1][e]));
-        mx = rows_max(mx * p.scale_log2);
-        const float m_new = fmaxf(m_run[rt], mx);
-        if (__any(m_new != m_run[rt])) {
-          const float alpha = m_new == -INFINITY ? 1.0f : fast_exp2(m_run[rt] - m_new);
-          l_run[rt] *= alpha;
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[rt][dt][e] *= alpha;
-          m_run[rt] = m_new;
-        }
-        const float m_use = m_new == -INFINITY ? 0.0f : m_new;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-          float y[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y[e] = fast_exp2(fmaf(s[rt][kt][e], p.scale_log2, -m_use));
-            l_run[rt] += y[e];
+            for (int e = 1; e < 8; ++e) mx = fmaxf(mx, s[rt][e / 4][e % 4]);
+            const float m_new = fmaxf(m_run[rt], rows_max(mx * scale_log2));
+            alpha[rt] = fast_exp2(m_run[rt] - m_new);
+            m_run[rt] = m_new;
+            without |= m_new == kNoMax;
+            summed |= l_run[rt] != 0.0f;
           }
-          // Rounded for the product, to half a step of q's type, summed unrounded: the largest weight is 1, which is exact.
-          pb[rt][2 * kt] = pack2<DTYPE>(y[0], y[1]);
-          pb[rt][2 * kt + 1] = pack2<DTYPE>(y[2], y[3]);
+          anchored = !__any(without);
+          if (__any(summed)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              l_run[rt] *= alpha[rt];
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[rt][dt][e] *= alpha[rt];
+            }
+          }
         }
+        bool again = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = fast_exp2(fmaf(s[rt][e / 4][e % 4], scale_log2, -m_run[rt]));
+          sum[rt] = ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+          again |= !(sum[rt] < kMaxTileSum);
+          // Rounded for the product, to half a step of q's type, summed unrounded.
+#pragma unroll
+          for (int i = 0; i < 4; ++i) pb[rt][i] = pack2<DTYPE>(y[2 * i], y[2 * i + 1]);
+        }
+        if (__builtin_expect(raise || !__any(again), 1)) break;
       }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) l_run[rt] += sum[rt];
       float scale[2][4];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
@@ -223,26 +335,14 @@ __global__ __launch_bounds__(NW * 64, RT == 1 ? 3 : 2) void quantized_few_kernel
         for (int j = 0; j < 4; ++j) scale[kt][j] = exponent_scale(x[kt].v_exp, j);
       multiply_v<DTYPE, D, RT>(x, scale, pb, o);
     }
-
-    // ---- the waves' results joined: element (4 g + e) D / 16 + dt is o[dt][e] --------------------------------
-    float* mine = reinterpret_cast<float*>(lds + w * Lds::WAVE);
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float l = rows_sum(l_run[rt]);
-      if (g == 0) {
-        sums[w][rt * 16 + n][0] = m_run[rt];
-        sums[w][rt * 16 + n][1] = l;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int dt = 0; dt < DT; dt += 4)
-          *reinterpret_cast<f32x4*>(mine + (rt * 16 + n) * (D + 4) + (4 * g + e) * DT + dt) =
-              f32x4{o[rt][dt][e], o[rt][dt + 1][e], o[rt][dt + 2][e], o[rt][dt + 3][e]};
+    have = 1;
+    done = u;
+    done_head = kv_head;
+    done_row0 = row0;
+    if constexpr (!WHOLE) {
+      slot = walk.slot(u);
+      n_cut = walk.n_cut(u);
     }
-    __syncthreads();
-    join_few<DTYPE, D, ROWS, NW, Lds::WAVE>(walk, u, lds, sums, kv_head, row0);
-    __syncthreads();  // nobody's part of LDS is filled again before all have read it
   }
 }
 
@@ -259,6 +359,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void quantized_rows_kernel(const P
 struct QuantPlan {
   bool few = false;    // the kernel of few rows
   bool whole = false;  // a workgroup takes a unit of it; otherwise an equal share of all tiles
+  int waves = 4;       // of a workgroup of it
   int rows = 16, n_few = 0;
   int n_shares = 1;    // of a row's keys, by the kernel of rows
   size_t cuts = 0, slots = 0, shares = 0;  // bytes
@@ -279,9 +380,25 @@ static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
   const int64_t most_units = (all_rows + (int64_t)x.batch * (plan.rows - 1)) / plan.rows * x.n_heads_kv;
   plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2) < 2e9;
   if (plan.few) {
-    plan.n_few = (plan.rows == 16 ? 3 : 2) * device_cu_count();
-    plan.cuts = ((size_t)x.n_tokens * x.n_heads_q * sizeof(int2) + 15) / 16 * 16;
-    plan.slots = (size_t)plan.n_few * 2 * plan.rows * (x.head_dim + 2) * sizeof(float);
+    // Whole units where they are short: a unit's chain of tiles, by eight waves where every unit has a CU to itself, against what cutting costs,
+    // a second kernel and more starts, which grows with the bytes there are (at 7 TB/s, if all were as long as the longest).  us, whole and cut,
+    // 8 kv heads of 128: 1 request of 100 keys 6.0 and 9.0, of 1000 9.1 and 10.4, of 1500 11.1 and 10.4; 16 of 2000 12.7 and 15.6; 32 of 2000
+    // 15.5 and 20, of 4000 25 and 30, of up to 4000 19.6 and 19.5; 64 of 500 9.8 and 12.4, of up to 2000 16.5 and 19.3, of up to 4000 28 and 27,
+    // of up to 8192 51 and 40; 128 of up to 300 10.5 and 19.4.  Head size 64: 1 of 1000 7.8 and 10.5, of 2000 10.5 and 10.6; windows of 1016 keys
+    // of 32 8.4 and 13.7.  32 rows: 4 of 1000 12.4 and 14.7, of 4000 26 and 18; 24 of up to 1000 12.4 and 14.9, of up to 4000 26 and 22.
+    const int64_t keys = seen_keys(x), units = std::max<int64_t>(x.batch, all_rows / plan.rows) * x.n_heads_kv;
+    plan.waves = units <= device_cu_count() ? 8 : 4;
+    const double chain_us = keys * (plan.waves == 8 ? 0.0032 : 0.0045) * (x.head_dim == 128 ? 1.0 : 0.6) * (plan.rows == 16 ? 1.0 : 1.6);
+    const double bytes_us = (double)units * keys * x.head_dim * 17 / 16 / 7e6;
+    plan.whole = chain_us < (plan.rows == 16 ? 4.5 : 6.5) + std::min(0.45 * bytes_us, 12.0);
+    if (!plan.whole) plan.waves = 4;
+    // Two workgroups a CU are enough for the memory, of head size 64 (half of the bytes under way) four.  us, one, two, three and four: four
+    // contexts of 131072 keys 93-96, 96, 96-99, 98; 64 of up to 8192 48, 40, 42, 42; at head size 64 40, 29.5, 29, 28.
+    plan.n_few = plan.whole ? (int)most_units : (x.head_dim == 128 ? 2 : 4) * device_cu_count();
+    if (!plan.whole) {
+      plan.cuts = ((size_t)x.n_tokens * x.n_heads_q * sizeof(int2) + 15) / 16 * 16;
+      plan.slots = (size_t)plan.n_few * 2 * plan.rows * (x.head_dim + 2) * sizeof(float);
+    }
   } else {
     plan.n_shares = row_shares(x, x.batch, seen_keys(x), false).n;
     if (plan.n_shares > 1) plan.shares = (size_t)plan.n_shares * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
@@ -352,18 +469,27 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
   p.slot_sums = reinterpret_cast<f32x2*>(p.slot_out + (size_t)plan.n_few * 2 * plan.rows * x.head_dim);
   p.partial_out = reinterpret_cast<float*>(at + plan.cuts + plan.slots);
   p.partial_sums = reinterpret_cast<f32x2*>(p.partial_out + (size_t)plan.n_shares * x.n_tokens * x.n_heads_q * x.head_dim);
+  p.by_page = Divider::of(x.page_size / kQuantTokens); p.by_group = Divider::of(p.group); p.by_heads = Divider::of(x.n_heads_kv);
   p.few_rows = plan.rows; p.few_whole = plan.whole; p.n_few = plan.n_few;
-  const auto launch = [&](auto kernel, const char* name, int64_t n_wg) {
+  const auto launch = [&](auto kernel, const char* name, int64_t n_wg, int threads) {
     if (n_wg >= (int64_t)1 << 31) return fail(DCP_ERR_ARG, "quantized_attn: too many work items");
     KernelTimer timer(name, stream);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(256), 0, (hipStream_t)stream, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(threads), 0, (hipStream_t)stream, p);
     return check_launch(name);
   };
   int status;
   if (!plan.few)
-    status = launch(DCP_QUANT_KERNEL(quantized_rows_kernel), "quantized_rows_kernel", row_workgroups(p.own.n_tiles, p.own.xcd_group, x.n_heads_kv, plan.n_shares));
-  else if (plan.rows == 16) status = launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 4), "quantized_few_kernel", p.n_few);
-  else status = launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 4), "quantized_few_kernel", p.n_few);
+    status = launch(DCP_QUANT_KERNEL(quantized_rows_kernel), "quantized_rows_kernel", row_workgroups(p.own.n_tiles, p.own.xcd_group, x.n_heads_kv, plan.n_shares),
+                    kRowsThreads);
+  else if (plan.whole && plan.waves == 8)
+    status = plan.rows == 16 ? launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 8, true), "quantized_few_kernel", p.n_few, 512)
+                             : launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 8, true), "quantized_few_kernel", p.n_few, 512);
+  else if (plan.whole)
+    status = plan.rows == 16 ? launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 4, true), "quantized_few_kernel", p.n_few, 256)
+                             : launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 4, true), "quantized_few_kernel", p.n_few, 256);
+  else
+    status = plan.rows == 16 ? launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 4, false), "quantized_few_kernel", p.n_few, 256)
+                             : launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 4, false), "quantized_few_kernel", p.n_few, 256);
   if (status == DCP_OK && (p.own.by_few || !p.direct)) {
     const int64_t units = std::max<int64_t>((int64_t)x.batch * x.n_heads_kv, 1);
     status = launch_paged_merge(p, x.dtype, x.head_dim, plan.few ? plan.n_few / units + 2 : plan.n_shares, stream);

@@ -128,6 +128,15 @@ def test_entries_that_name_no_page(gpu, kind):
     check(_run(gpu, case), case.truth())
 
 
+@pytest.mark.parametrize("longest", [1, 1 << 20])
+@pytest.mark.parametrize("window", [0, 9000])
+def test_missing_pages_far_into_a_unit(gpu, longest, window):
+    """A wave finds its tiles 32 at a time; what is missing of the last of them and of the first of the next."""
+    missing = [(0, i, lambda n: -1) for tile in (31 * 4, 31 * 8, 32 * 4 + 3, 63 * 4 + 1, 64 * 8 + 7) for i in (2 * tile,)]
+    case = Quantized([17500], bad=missing, page_size=16, heads=2, kv_heads=1, window=window, n_starting=100 if window else 0)
+    check(_run(gpu, case, max_seqlen_k=longest), case.truth())
+
+
 @pytest.mark.parametrize("keys", [[100, 9], [9000, 9]])
 @pytest.mark.parametrize("new", [None, [2, 0], [90, 0]])
 def test_tokens_of_no_request_are_left(gpu, keys, new):
@@ -292,6 +301,6 @@ def test_refusals(gpu, wrong):
         scale=dict(softmax_scale=0.0), huge_scale=dict(softmax_scale=1e39),
         aligned=dict(q=torch.empty(2 * 8 * 128 + 8, dtype=q.dtype, device=gpu)[4 : 4 + 2 * 8 * 128].view(2, 8, 128)), cache_aligned=dict(cache=shifted),
         cpu=dict(cache=cache.cpu()), q_cpu=dict(q=q.cpu()), heads=dict(q=q[:, :5].contiguous()),
-        workspace=dict(workspace=torch.empty(16, dtype=torch.uint8, device=gpu)))[wrong]
+        workspace=dict(workspace=torch.empty(16, dtype=torch.uint8, device=gpu), max_seqlen_k=100000))[wrong]
     with pytest.raises((ValueError, TypeError, AssertionError)):
         quantized_cache_attention(**{**args, **change})
