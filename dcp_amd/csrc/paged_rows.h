@@ -36,6 +36,34 @@ __device__ __forceinline__ void load_async_piece(uint32_t lds_at, const uint16_t
                  : "memory");
 }
 
+// The row tile of rank `rank` (negative index: there is none), the ones that see the most keys first, by steps of 64: the last ones to start are
+// the shortest, so that no CU is left with a long one.  A request's tiles that see more than 64 t keys are its last ones, and their number is
+// known from its lengths; t is found by halving.  For up to 64 requests, one a lane.
+__device__ __forceinline__ RowTile find_ranked_tile(PagedArgs& p, SourceArgs& src, int rank) {
+  const int lane = threadIdx.x & 63, b = min(lane, src.batch - 1);
+  const TokenRange tokens = tokens_of(p, src, b);
+  const int n_keys = keys_of(p, src, b), n_rows = lane < src.batch ? tokens.n * p.group : 0, at0 = n_keys - tokens.n;
+  const int n_tiles = (n_rows + kRowsBM - 1) / kRowsBM;
+  const int room = src.table_width * p.page_size / kRowsBN;
+  const int most = p.window > 0 ? min((int)(((uint32_t)p.window + (uint32_t)p.n_starting) / kRowsBN), room) + 1 : room + 1;  // what a row can see
+  auto seeing_more = [&](int t) {  // tiles of the lane's request, all of them for t = 0
+    const uint32_t first = kRowsBN * t > at0 ? (uint32_t)(kRowsBN * t) - (uint32_t)at0 : 0;  // the first token that sees more
+    const int n = first < (uint32_t)tokens.n ? max(n_tiles - (int)first * p.group / kRowsBM, 0) : 0;
+    return t == 0 ? n_tiles : t < most ? n : 0;
+  };
+  auto total = [&](int n) { return __builtin_amdgcn_readlane(wave_scan(n), 63); };
+  if (rank >= total(n_tiles)) return {0, -1, {0, 0}, 0};
+  int t = 0;
+  for (int step = 1 << (31 - __builtin_clz(most)); step > 0; step >>= 1)
+    if (t + step < most && total(seeing_more(t + step)) > rank) t += step;
+  const int longer = seeing_more(t + 1), here = seeing_more(t) - longer;
+  const int left = rank - total(longer), ends = wave_scan(here);
+  const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(ends <= left)));
+  auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+  const int index = n_tiles - 1 - (longer + left - (ends - here));
+  return {at, of(index), {of(tokens.begin), of(tokens.n)}, of(n_keys)};
+}
+
 // ---------------------------------------------------------------------------
 // The kernel of rows: a workgroup of 4 waves owns 128 rows of one (request, kv head), a wave 32 of them, and walks its share of the
 // 64-key tiles that any of them sees.  K and V tiles go from memory straight into LDS (KvTile), two stages each, K a tile
@@ -76,25 +104,39 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
 
   // ---- which rows, which share of their keys ---------------------------------
-  const RowItem at = row_item(item, src.n_tiles, src.xcd_group, p.n_heads_kv, src.n_shares);
+  const bool ranked = QUANT && src.batch <= 64;
+  RowItem at;
+  if (ranked) {
+    const int i = divide(item, p.by_heads);
+    at = {i, item - i * p.n_heads_kv, 0};
+    if (src.n_shares > 1) {
+      at.place = i / src.n_shares;
+      at.share = i - at.place * src.n_shares;
+    }
+  } else {
+    at = row_item(item, src.n_tiles, src.xcd_group, p.n_heads_kv, src.n_shares);
+  }
   if (at.share < 0) return;
   const int place = __builtin_amdgcn_readfirstlane(at.place), kv_head = __builtin_amdgcn_readfirstlane(at.kv_head);
   const int share = __builtin_amdgcn_readfirstlane(at.share);
-  const RowTile tile = find_row_tile(p, src, place);
+  const RowTile tile = ranked ? find_ranked_tile(p, src, place) : find_row_tile(p, src, place);
   const TokenRange tokens = tile.tokens;
   const int n_rows = tokens.n * p.group;  // (at most n_tokens * group, which the host has checked)
+  auto token_of = [&](int row) { return QUANT ? divide(row, p.by_group) : row / p.group; };
   const int row0 = tile.index * kRowsBM;
   if (tile.index < 0) return;
   const bool prefix = src.cu_groups != nullptr;
   const int n_keys = tile.n_keys, window = prefix ? 0 : p.window, n_starting = p.n_starting;
   // token i of the request is at position n_keys - n + i; every token is past all of a prefix
-  const int first_tok = row0 / p.group, last_tok = (min(row0 + kRowsBM, n_rows) - 1) / p.group;
+  const int first_tok = token_of(row0), last_tok = token_of(min(row0 + kRowsBM, n_rows) - 1);
   const int at0 = prefix ? n_keys - 1 : n_keys - tokens.n, step = prefix ? 0 : 1;
   const KeyGroups groups(window, n_starting, max(at0 + first_tok * step, 0), at0 + last_tok * step);
   const int n_groups = __builtin_amdgcn_readfirstlane(groups.hull_end > 0 ? groups.count() : 0);
   const int tiles_all = (n_groups + 3) / 4, n_shares = min(src.n_shares, max(1, tiles_all / kMinTilesPerShare));
   int t_begin = 0, t_end = 0;
-  if (share < n_shares) {
+  if (QUANT && src.n_shares == 1) {
+    t_end = tiles_all;
+  } else if (share < n_shares) {
     t_begin = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * share / n_shares));
     t_end = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * (share + 1) / n_shares));
   }
@@ -128,7 +170,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     PagedArgs& p = fresh_kernel_args<PagedParams>();
     const int i = (t_begin + rel) * 4 + tid, key = i < 4 * t_end ? group_key(i) : kNoKey;
     if (key == kNoKey) return {key, 0, -1};
-    const int entry = key / p.page_size;
+    const int entry = QUANT ? divide(key / 16, p.by_page) : key / p.page_size;
     return {key, key - entry * p.page_size, src.block_table[tile.b * src.table_stride + entry]};
   };
   auto look_up = [&](int rel, Entry entry) {
@@ -150,7 +192,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   u32x4 q[RT][KS];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = min(row0 + w * 32 + rt * 16 + n, n_rows - 1), tok = r / p.group, head = kv_head * p.group + r % p.group;
+    const int r = min(row0 + w * 32 + rt * 16 + n, n_rows - 1), tok = token_of(r), head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);
     const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (tokens.begin + tok) * p.q_token + head * p.q_head + Tile::element16(g);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + Tile::step16(ks));
@@ -192,6 +234,27 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     return (((unsigned)t < (unsigned)full_first) | ((unsigned)(t - full_begin) < (unsigned)full_count)) & (__builtin_amdgcn_readfirstlane(bad) == 0);
   };
   auto mask = [&](int t, f32x4 (&s)[RT][4]) {
+    if constexpr (QUANT) {
+      // A key's distance to the row's last one is from 0 up to the window, in one unsigned comparison; or it is a first token.
+      const bool first = group_key(t * 4) < n_starting;
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        const int key0 = absent[((t - t_begin) * 4 + kt) % (2 * kTableTiles * 4)] ? kNoKey : group_key(t * 4 + kt);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const int last = max(last_key[rt], -1), to_last = last - key0 - 4 * g;  // (kNoKey: far below 0)
+          if (first) {
+            const int to_first = min(n_starting - 1, last) - key0 - 4 * g;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[rt][kt][e] = ((unsigned)(to_last - e) < (unsigned)reach) | (e <= to_first) ? s[rt][kt][e] : -INFINITY;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[rt][kt][e] = (unsigned)(to_last - e) < (unsigned)reach ? s[rt][kt][e] : -INFINITY;
+          }
+        }
+      }
+      return;
+    }
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
       const bool there = absent[((t - t_begin) * 4 + kt) % (2 * kTableTiles * 4)] == 0;
@@ -343,12 +406,15 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     for (int rt = 0; rt < RT; ++rt) lsum[rt] = 0.0f;
     bool taken = false;  // the tile's maximum
     rescale = false;
-    if (__builtin_expect(!(full & anchored), 0)) {
-      if (!full) mask(t, s_cur);
+    if constexpr (QUANT) {
+      if (__builtin_expect(!full, 0)) mask(t, s_cur);
+    }
+    if (__builtin_expect(!((QUANT || full) & anchored), 0)) {
+      if (!QUANT && !full) mask(t, s_cur);
       raise(s_cur);
       taken = true;
     }
-    // Where every row has a reference and sees the whole tile, its weights are taken against that without looking for its own
+    // Where every row has a reference and sees the whole tile (in 4 bits: or not, the masked weights are 0), its weights are taken against that without looking for its own
     // maximum; the lanes' sums tell afterwards whether that was safe, and if not it is done again.
     __builtin_amdgcn_s_setprio(2);
     constexpr int N = 4 * KS, NL = 2 * LPW;
@@ -440,7 +506,8 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     }
     const int r = row0 + w * 32 + rt * 16 + n;
     if (r >= n_rows) continue;
-    const int64_t token = tokens.begin + r / p.group, head = kv_head * p.group + r % p.group;
+    const int tok = token_of(r);
+    const int64_t token = tokens.begin + tok, head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);
     if (!p.direct) {
       const int64_t at = ((int64_t)(src.first_share + share) * p.n_tokens + token) * p.n_heads_q + head;
       if (g == 0) p.partial_sums[at] = f32x2{m, l};

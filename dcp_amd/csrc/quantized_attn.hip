@@ -479,7 +479,9 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
   };
   int status;
   if (!plan.few)
-    status = launch(DCP_QUANT_KERNEL(quantized_rows_kernel), "quantized_rows_kernel", row_workgroups(p.own.n_tiles, p.own.xcd_group, x.n_heads_kv, plan.n_shares),
+    status = launch(DCP_QUANT_KERNEL(quantized_rows_kernel), "quantized_rows_kernel",
+                    x.batch <= 64 ? (int64_t)p.own.n_tiles * x.n_heads_kv * plan.n_shares
+                                  : row_workgroups(p.own.n_tiles, p.own.xcd_group, x.n_heads_kv, plan.n_shares),
                     kRowsThreads);
   else if (plan.whole && plan.waves == 8)
     status = plan.rows == 16 ? launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 8, true), "quantized_few_kernel", p.n_few, 512)
