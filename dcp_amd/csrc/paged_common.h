@@ -29,7 +29,7 @@ struct PagedSource {
   int table_width, batch;    // of prefixes or requests
   int first_share, n_shares; // see PagedParams::partial_out
   int n_tiles, xcd_group;    // row tiles of a kv head (kernel of rows); as many neighbouring work items are on one XCD
-  int by_few;                // the kernel of few rows takes it and may cut it (own keys)
+  int by_few;                // pieces of rows may be in slots (own keys: where the kernel of few rows takes them, or in 4 bits that of rows cuts them)
 };
 
 struct PagedParams {
@@ -52,7 +52,8 @@ struct PagedParams {
   // the sum of the weights.  The own keys have shares [0, own.n_shares), the prefixes those that follow.
   float* partial_out;
   f32x2* partial_sums;
-  // The kernel of few rows: pieces of the units that are cut between workgroups, and where a row's pieces are (cut_of):
+  // The kernel of few rows (in 4 bits that of rows as well): pieces of the units that are cut between workgroups, and where a row's pieces
+  // are (cut_of):
   // [token][q head]
   int2* cuts;
   float* slot_out;   // [workgroup][2][head of the workgroup][rows][D]

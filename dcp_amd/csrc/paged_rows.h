@@ -36,32 +36,68 @@ __device__ __forceinline__ void load_async_piece(uint32_t lds_at, const uint16_t
                  : "memory");
 }
 
-// The row tile of rank `rank` (negative index: there is none), the ones that see the most keys first, by steps of 64: the last ones to start are
-// the shortest, so that no CU is left with a long one.  A request's tiles that see more than 64 t keys are its last ones, and their number is
-// known from its lengths; t is found by halving.  For up to 64 requests, one a lane.
-__device__ __forceinline__ RowTile find_ranked_tile(PagedArgs& p, SourceArgs& src, int rank) {
+// The row tile of work item `rank` of a kv head (negative index: there is none), and which piece of its keys.  For up to 64 requests, one a lane.
+struct RankedTile {
+  RowTile tile;
+  int share, n_shares;
+};
+constexpr int kMinTilesPerPiece = 3;
+__device__ __forceinline__ RankedTile find_ranked_tile(PagedArgs& p, SourceArgs& src, int rank) {
   const int lane = threadIdx.x & 63, b = min(lane, src.batch - 1);
   const TokenRange tokens = tokens_of(p, src, b);
   const int n_keys = keys_of(p, src, b), n_rows = lane < src.batch ? tokens.n * p.group : 0, at0 = n_keys - tokens.n;
   const int n_tiles = (n_rows + kRowsBM - 1) / kRowsBM;
   const int room = src.table_width * p.page_size / kRowsBN;
   const int most = p.window > 0 ? min((int)(((uint32_t)p.window + (uint32_t)p.n_starting) / kRowsBN), room) + 1 : room + 1;  // what a row can see
+  auto total = [&](int n) { return __builtin_amdgcn_readlane(wave_scan(n), 63); };
+  auto found = [&](int at, int index, int share, int n_shares) {
+    auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
+    return RankedTile{{at, of(index), {of(tokens.begin), of(tokens.n)}, of(n_keys)}, share, n_shares};
+  };
+  const int all = total(n_tiles);
+  // Where there are fewer row tiles than workgroups, those of a request are cut into pieces of about `length` key tiles, the least that leaves
+  // a workgroup for every piece: between an equal share of all key tiles and what that is if every row tile needs one piece more.  One
+  // workgroup a CU where pieces are short: with two, each takes half as many tiles in three quarters of the time, but there is twice as much to be joined.
+  const int places = src.by_few ? divide(p.n_few, p.by_heads) : 0;  // two workgroups a CU
+  if (all < places) {
+    const float tiles = (float)min(min((n_keys + kRowsBN - 1) / kRowsBN, most + 1), 1 << 20);
+    const float sum = (float)total(n_tiles * (int)tiles);  // (less than 2^30)
+    auto pieces = [&](float length) { return n_tiles * max((int)ceilf(tiles * __builtin_amdgcn_rcpf(length)), 1); };
+    auto shortest = [&](int places) {
+      float enough = max(sum / (float)(places - all), 1.0f), least = max(sum / (float)places, 1.0f);
+      for (int i = 0; i < 4; ++i) {
+        const float length = 0.5f * (enough + least);
+        if (total(pieces(length)) <= places) enough = length;
+        else least = length;
+      }
+      return enough;
+    };
+    float length = shortest(places);
+    if (length <= 6.0f && all < places / 2) length = shortest(places / 2);
+    const int n = pieces(max(length, (float)kMinTilesPerPiece)), ends = wave_scan(n);
+    if (rank >= __builtin_amdgcn_readlane(ends, 63)) return {{0, -1, {0, 0}, 0}, 0, 0};
+    const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(ends <= rank)));
+    const int in_request = rank - __builtin_amdgcn_readlane(ends - n, at), of_request = __builtin_amdgcn_readlane(n_tiles, at);
+    const int each = __builtin_amdgcn_readlane(n, at) / of_request, from_last = in_request / each;
+    return found(at, n_tiles - 1 - from_last, in_request - from_last * each, each);
+  }
+  // Otherwise the row tiles that see the most keys come first, by steps of 64: the last ones to start are the shortest, so that no CU is left
+  // with a long one (32 requests of 500 tokens behind up to 2000 keys, lengths spread over a factor of 16: 115 us in the order of the requests, 84
+  // so; 12 prompts of up to 1024 60 and 53).  A request's tiles that see more than 64 t keys are its last ones, and their number is known
+  // from its lengths; t is found by halving.
   auto seeing_more = [&](int t) {  // tiles of the lane's request, all of them for t = 0
     const uint32_t first = kRowsBN * t > at0 ? (uint32_t)(kRowsBN * t) - (uint32_t)at0 : 0;  // the first token that sees more
     const int n = first < (uint32_t)tokens.n ? max(n_tiles - (int)first * p.group / kRowsBM, 0) : 0;
     return t == 0 ? n_tiles : t < most ? n : 0;
   };
-  auto total = [&](int n) { return __builtin_amdgcn_readlane(wave_scan(n), 63); };
-  if (rank >= total(n_tiles)) return {0, -1, {0, 0}, 0};
+  if (rank >= all) return {{0, -1, {0, 0}, 0}, 0, 0};
   int t = 0;
   for (int step = 1 << (31 - __builtin_clz(most)); step > 0; step >>= 1)
     if (t + step < most && total(seeing_more(t + step)) > rank) t += step;
   const int longer = seeing_more(t + 1), here = seeing_more(t) - longer;
   const int left = rank - total(longer), ends = wave_scan(here);
   const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(ends <= left)));
-  auto of = [&](int x) { return __builtin_amdgcn_readlane(x, at); };
-  const int index = n_tiles - 1 - (longer + left - (ends - here));
-  return {at, of(index), {of(tokens.begin), of(tokens.n)}, of(n_keys)};
+  return found(at, n_tiles - 1 - (longer + left - (ends - here)), 0, 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -105,21 +141,23 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 
   // ---- which rows, which share of their keys ---------------------------------
   const bool ranked = QUANT && src.batch <= 64;
-  RowItem at;
+  RowTile tile;
+  int kv_head, share, most_shares = src.n_shares, first_piece = 0;
   if (ranked) {
-    const int i = divide(item, p.by_heads);
-    at = {i, item - i * p.n_heads_kv, 0};
-    if (src.n_shares > 1) {
-      at.place = i / src.n_shares;
-      at.share = i - at.place * src.n_shares;
-    }
+    const int rank = divide(item, p.by_heads);
+    kv_head = item - rank * p.n_heads_kv;
+    const RankedTile at = find_ranked_tile(p, src, rank);
+    tile = at.tile;
+    share = at.share;
+    most_shares = at.n_shares;
+    first_piece = kv_head * divide(p.n_few, p.by_heads) + rank - share;
   } else {
-    at = row_item(item, src.n_tiles, src.xcd_group, p.n_heads_kv, src.n_shares);
+    const RowItem at = row_item(item, src.n_tiles, src.xcd_group, p.n_heads_kv, src.n_shares);
+    if (at.share < 0) return;
+    kv_head = __builtin_amdgcn_readfirstlane(at.kv_head);
+    share = __builtin_amdgcn_readfirstlane(at.share);
+    tile = find_row_tile(p, src, __builtin_amdgcn_readfirstlane(at.place));
   }
-  if (at.share < 0) return;
-  const int place = __builtin_amdgcn_readfirstlane(at.place), kv_head = __builtin_amdgcn_readfirstlane(at.kv_head);
-  const int share = __builtin_amdgcn_readfirstlane(at.share);
-  const RowTile tile = ranked ? find_ranked_tile(p, src, place) : find_row_tile(p, src, place);
   const TokenRange tokens = tile.tokens;
   const int n_rows = tokens.n * p.group;  // (at most n_tokens * group, which the host has checked)
   auto token_of = [&](int row) { return QUANT ? divide(row, p.by_group) : row / p.group; };
@@ -132,9 +170,10 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   const int at0 = prefix ? n_keys - 1 : n_keys - tokens.n, step = prefix ? 0 : 1;
   const KeyGroups groups(window, n_starting, max(at0 + first_tok * step, 0), at0 + last_tok * step);
   const int n_groups = __builtin_amdgcn_readfirstlane(groups.hull_end > 0 ? groups.count() : 0);
-  const int tiles_all = (n_groups + 3) / 4, n_shares = min(src.n_shares, max(1, tiles_all / kMinTilesPerShare));
+  const int tiles_all = (n_groups + 3) / 4, n_shares = min(most_shares, max(1, tiles_all / kMinTilesPerShare));
   int t_begin = 0, t_end = 0;
-  if (QUANT && src.n_shares == 1) {
+  if (ranked & (share >= n_shares)) return;
+  if (QUANT && n_shares == 1) {
     t_end = tiles_all;
   } else if (share < n_shares) {
     t_begin = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * share / n_shares));
@@ -508,7 +547,17 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     if (r >= n_rows) continue;
     const int tok = token_of(r);
     const int64_t token = tokens.begin + tok, head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);
-    if (!p.direct) {
+    if (ranked && src.by_few) {
+      if ((g == 0) & (share == 0)) p.cuts[token * p.n_heads_q + head] = cut_of(first_piece, n_shares, 0, r - row0);
+      if (n_shares > 1) {
+        const int64_t at = (int64_t)(first_piece + share) * 2 * kRowsBM + (r - row0);
+        if (g == 0) p.slot_sums[at] = f32x2{m, l};
+        float* to = p.slot_out + at * D + 4 * g;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4*>(to + 16 * dt) = o[rt][dt];
+        continue;
+      }
+    } else if (!p.direct) {
       const int64_t at = ((int64_t)(src.first_share + share) * p.n_tokens + token) * p.n_heads_q + head;
       if (g == 0) p.partial_sums[at] = f32x2{m, l};
       if (share >= n_shares) continue;  // (nothing is read of a share without weights)

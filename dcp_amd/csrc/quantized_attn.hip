@@ -360,7 +360,9 @@ struct QuantPlan {
   bool few = false;    // the kernel of few rows
   bool whole = false;  // a workgroup takes a unit of it; otherwise an equal share of all tiles
   int waves = 4;       // of a workgroup of it
-  int rows = 16, n_few = 0;
+  bool cut = false;    // units may be cut into pieces, by either kernel
+  int rows = 16, n_few = 0;  // of a unit, and of a piece's slot; workgroups that may have pieces
+  int64_t units = 1;   // as far as the host knows
   int n_shares = 1;    // of a row's keys, by the kernel of rows
   size_t cuts = 0, slots = 0, shares = 0;  // bytes
   size_t bytes() const { return cuts + slots + shares; }
@@ -386,7 +388,7 @@ static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
     // 15.5 and 20, of 4000 25 and 30, of up to 4000 19.6 and 19.5; 64 of 500 9.8 and 12.4, of up to 2000 16.5 and 19.3, of up to 4000 28 and 27,
     // of up to 8192 51 and 40; 128 of up to 300 10.5 and 19.4.  Head size 64: 1 of 1000 7.8 and 10.5, of 2000 10.5 and 10.6; windows of 1016 keys
     // of 32 8.4 and 13.7.  32 rows: 4 of 1000 12.4 and 14.7, of 4000 26 and 18; 24 of up to 1000 12.4 and 14.9, of up to 4000 26 and 22.
-    const int64_t keys = seen_keys(x), units = std::max<int64_t>(x.batch, all_rows / plan.rows) * x.n_heads_kv;
+    const int64_t keys = seen_keys(x), units = plan.units = std::max<int64_t>(x.batch, all_rows / plan.rows) * x.n_heads_kv;
     plan.waves = units <= device_cu_count() ? 8 : 4;
     const double chain_us = keys * (plan.waves == 8 ? 0.0032 : 0.0045) * (x.head_dim == 128 ? 1.0 : 0.6) * (plan.rows == 16 ? 1.0 : 1.6);
     const double bytes_us = (double)units * keys * x.head_dim * 17 / 16 / 7e6;
@@ -395,13 +397,24 @@ static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
     // Two workgroups a CU are enough for the memory, of head size 64 (half of the bytes under way) four.  us, one, two, three and four: four
     // contexts of 131072 keys 93-96, 96, 96-99, 98; 64 of up to 8192 48, 40, 42, 42; at head size 64 40, 29.5, 29, 28.
     plan.n_few = plan.whole ? (int)most_units : (x.head_dim == 128 ? 2 : 4) * device_cu_count();
-    if (!plan.whole) {
-      plan.cuts = ((size_t)x.n_tokens * x.n_heads_q * sizeof(int2) + 15) / 16 * 16;
-      plan.slots = (size_t)plan.n_few * 2 * plan.rows * (x.head_dim + 2) * sizeof(float);
-    }
+    plan.cut = !plan.whole;
+  } else if (x.batch <= 64) {
+    // find_ranked_tile cuts by the lengths that there are.  That they may be is decided by the longest ones: where the time that cutting takes off
+    // them if all are as long is more than what a second kernel and the pieces take, or little less: lengths that differ gain more.  us, whole and cut, 8 kv heads of 128, 13 or 30
+    // tokens a request: 3 of 300 keys 13.8 and 16.5, of 700 21.8 and 17.3; 16 of 1000 30 and 33, of up to 1000 30 and 23; 32 of 1500 43 and 48,
+    // of up to 1500 41 and 27; 48 of 2000 69 and 75, of up to 4000 96 and 63; a prompt of 1024 31 and 41.
+    const int64_t units = plan.units = std::max<int64_t>((all_rows + kRowsBM - 1) / kRowsBM, x.batch) * x.n_heads_kv, places = 2 * device_cu_count();
+    const double tiles = (double)((seen_keys(x) + kRowsBN - 1) / kRowsBN);
+    plan.rows = kRowsBM;
+    plan.n_few = (int)(places / x.n_heads_kv * x.n_heads_kv);
+    plan.cut = units < places && tiles * (1.0 - (double)units / places) > 10.0;
   } else {
     plan.n_shares = row_shares(x, x.batch, seen_keys(x), false).n;
     if (plan.n_shares > 1) plan.shares = (size_t)plan.n_shares * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
+  }
+  if (plan.cut) {
+    plan.cuts = ((size_t)x.n_tokens * x.n_heads_q * sizeof(int2) + 15) / 16 * 16;
+    plan.slots = (size_t)plan.n_few * 2 * plan.rows * (x.head_dim + 2) * sizeof(float);
   }
   return plan;
 }
@@ -456,7 +469,7 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
   p.cu_seqlens_q = x.cu_seqlens_q;
   p.q_token = x.q_token_stride; p.q_head = x.q_head_stride; p.out_token = x.out_token_stride; p.out_head = x.out_head_stride;
   p.page_stride = x.page_stride; p.head_stride = x.head_stride;
-  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_shares, (int)row_tiles(x, x.batch), row_group(x, x.batch), plan.few && !plan.whole};
+  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_shares, (int)row_tiles(x, x.batch), row_group(x, x.batch), plan.cut};
   p.n_pages = x.n_pages; p.page_size = x.page_size;
   p.n_requests = x.batch; p.n_tokens = x.n_tokens;
   p.n_heads_q = x.n_heads_q; p.n_heads_kv = x.n_heads_kv; p.group = x.n_heads_q / x.n_heads_kv;
@@ -480,7 +493,7 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
   int status;
   if (!plan.few)
     status = launch(DCP_QUANT_KERNEL(quantized_rows_kernel), "quantized_rows_kernel",
-                    x.batch <= 64 ? (int64_t)p.own.n_tiles * x.n_heads_kv * plan.n_shares
+                    x.batch <= 64 ? std::max<int64_t>((int64_t)p.own.n_tiles * x.n_heads_kv, plan.cut ? plan.n_few : 0)
                                   : row_workgroups(p.own.n_tiles, p.own.xcd_group, x.n_heads_kv, plan.n_shares),
                     kRowsThreads);
   else if (plan.whole && plan.waves == 8)
@@ -492,10 +505,8 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
   else
     status = plan.rows == 16 ? launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 4, false), "quantized_few_kernel", p.n_few, 256)
                              : launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 4, false), "quantized_few_kernel", p.n_few, 256);
-  if (status == DCP_OK && (p.own.by_few || !p.direct)) {
-    const int64_t units = std::max<int64_t>((int64_t)x.batch * x.n_heads_kv, 1);
-    status = launch_paged_merge(p, x.dtype, x.head_dim, plan.few ? plan.n_few / units + 2 : plan.n_shares, stream);
-  }
+  if (status == DCP_OK && (p.own.by_few || !p.direct))
+    status = launch_paged_merge(p, x.dtype, x.head_dim, plan.cut ? plan.n_few / plan.units + 2 : plan.n_shares, stream);
   return status;
 }
 

@@ -59,6 +59,36 @@ def test_row_tiles_of_many_requests(gpu, requests):
     check(_run(gpu, case), case.truth())
 
 
+RAGGED = {
+    "ragged": dict(keys=[3000, 17, 900, 0, 64, 5, 1500], new=[40, 17, 0, 0, 30, 9, 33]),
+    "five_kv_heads": dict(keys=[2100, 700, 90], new=[30, 60, 90], heads=25, kv_heads=5, head_dim=64),
+    "window": dict(keys=[2500, 100, 1300], new=[70, 100, 200], heads=4, kv_heads=2, window=300, n_starting=70),
+    "fp16": dict(keys=[1800, 250], new=[300, 9], heads=4, kv_heads=4, dtype=F16),
+    "rows_of_many_heads": dict(keys=[1400, 300, 20], new=[9, 300, 3], heads=48, kv_heads=1, head_dim=64),
+    "more_tokens_than_keys": dict(keys=[10, 1100, 0], new=[150, 40, 60], heads=4, kv_heads=2),
+    "alone": dict(keys=[5000], new=[50], heads=8, kv_heads=1, page_size=16),
+}
+
+
+@pytest.mark.parametrize("longest", [1, 200, 1 << 20])
+@pytest.mark.parametrize("name", RAGGED)
+def test_ragged_prompts(gpu, name, longest):
+    """Row tiles taken whole, those that see the most first, and cut into pieces of about one length."""
+    case = Quantized(**RAGGED[name])
+    args = case.to(gpu)
+    wide = torch.full((len(case.keys), 3000), -1, dtype=torch.int32, device=gpu)  # (and of tables with more room than there are keys)
+    wide[:, : args["block_table"].shape[1]] = args["block_table"]
+    truth = case.truth()
+    for table in (args["block_table"], wide):
+        check(_run(gpu, case, sentinel=5.0, max_seqlen_k=longest, block_table=table), truth)
+
+
+@pytest.mark.parametrize("new", [[1] * 64, [33] * 64, [0] * 63 + [200]])
+def test_pieces_of_as_many_requests_as_a_wave_looks_at(gpu, new):
+    case = Quantized([n + (i * 37) % 200 for i, n in enumerate(new)], new=new, heads=2, kv_heads=1, head_dim=64, page_size=16)
+    check(_run(gpu, case, max_seqlen_q=max(max(new), 33), max_seqlen_k=100000), case.truth())
+
+
 def test_a_batch_of_thousands(gpu):
     """Requests past the 64 that a wave looks at together, some of no tokens and no keys among them."""
     n = 1500
