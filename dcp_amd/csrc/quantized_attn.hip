@@ -75,7 +75,7 @@ __device__ __forceinline__ void multiply_v(const QuantGroup<D> (&x)[2], const fl
 // weights are taken against a reference maximum that the tile's own is only looked for where the weights' sum says so.  What is done once a
 // piece is bound by the fetch of its instructions (some 15 ns each the first time they are met), so each step stands once in the
 // code, whichever piece it is of, tiles are not unrolled over their places in LDS, and there is no division by a number known on the host.
-constexpr int kStartTurns = 2;
+constexpr int kStartTurns = 3;
 template <int DTYPE, int D, int RT, int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64, NW == 4 && (RT == 1 || D == 64) ? (RT == 1 && D == 64 ? 4 : 3) : 2) void quantized_few_kernel(const PagedParams) {
   typedef QuantFewLds<D, RT, NW> Lds;
