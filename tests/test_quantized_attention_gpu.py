@@ -174,6 +174,33 @@ def test_tokens_of_no_request_are_left(gpu, keys, new):
     check(_run(gpu, case, sentinel=3.0), case.truth(), untouched=3.0)
 
 
+@pytest.mark.parametrize("group", [16, 32])
+@pytest.mark.parametrize("longest", [64, 100000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, F16])
+def test_rounding_of_a_weight_that_outweighs_the_others_cancels(gpu, dtype, longest, group):
+    """279 keys of weight 1 and value 0, and behind the first of them one of weight w from 2^12.5 to 2^13.5 and value 1: w / (w + 279).  w is
+    rounded by up to eps / 2; were only the product's w, the result would be off by that.  Where the sum's is as well, 279 / (w + 279) < 0.046 of
+    it is left, beside half a step of the result (eps / 4 below 1) and sums in 32 bits."""
+    batch, kv_heads, d, n = 4, 4, 64, 280
+    k, v = (torch.zeros(n, kv_heads, d, dtype=dtype, device=gpu) for _ in range(2))
+    k[270, :, 0], k[270, :, 1], v[270] = 6.0, 0.5, 1.0
+    cache = quantized_cache_pages(18, 16, kv_heads, d, gpu)
+    quantized_cache_write(k, v, torch.arange(n, device=gpu), cache)
+    g = torch.Generator().manual_seed(1)
+    q = torch.zeros(batch, kv_heads * group, d)
+    q[..., 0], q[..., 1] = 11.5625, torch.rand(q.shape[:2], generator=g) * 10
+    q = q.to(dtype)
+    table, lens = torch.arange(18, dtype=torch.int32, device=gpu).expand(batch, 18).contiguous(), torch.full((batch,), n, dtype=torch.int32, device=gpu)
+    cu = torch.arange(batch + 1, dtype=torch.int32, device=gpu)
+    out, lse = quantized_cache_attention(q.to(gpu), cache, table, lens, cu_seqlens_q=cu, max_seqlen_q=1, max_seqlen_k=longest)
+    w = torch.exp((6 * q[..., 0].double() + 0.5 * q[..., 1].double()) * d**-0.5)
+    assert w.log2().min() > 12.5 and w.log2().max() < 13.5
+    off = (out.double().cpu() - (w / (w + n - 1))[..., None]).abs().max()
+    eps = torch.finfo(dtype).eps
+    assert off <= eps / 4 + 0.046 * eps / 2 + 2.0**-16
+    assert (lse.double().cpu().T - (w + n - 1).log()).abs().max() <= 2.0**-18
+
+
 @pytest.mark.parametrize("before", [4, 300])
 @pytest.mark.parametrize("new", [[1, 1], [40, 20]])
 def test_tokens_before_the_first_request_are_left(gpu, before, new):
