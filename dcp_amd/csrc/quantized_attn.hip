@@ -63,18 +63,22 @@ __device__ __forceinline__ void multiply_v(const QuantGroup<D> (&x)[2], const fl
       o[rt][2 * U] = mfma_16x16x32<DTYPE>(even, pb[rt], o[rt][2 * U]);
       o[rt][2 * U + 1] = mfma_16x16x32<DTYPE>(odd, pb[rt], o[rt][2 * U + 1]);
     }
-      multiply_v<DTYPE, D, RT, U + 1>(x, scale, pb, o);
+    multiply_v<DTYPE, D, RT, U + 1>(x, scale, pb, o);
   }
 }
 
 // The kernel of few rows: the waves of a workgroup share no tile.  Each takes tiles of 32 keys of its own and waits for nobody until its
 // share of the keys is done; work is cut as over a cache of 16 bits (FewWalk), or whole units where they are short (WHOLE).
 //
-// What bounds it is the number of instructions: with 4 bits a key the memory would let a SIMD issue 280 of them a tile.  64 conversions
+// What bounds it is the number of instructions: at 7 TB/s the memory would leave a SIMD 335 slots of 4 cycles a tile, and a tile takes 333 with its
+// share of starts and joins (64 contexts of up to 8192 keys, 8 kv heads of 128: 38 us, 5.2 TB/s, a slot taken in 73 % of them).  64 conversions
 // and 32 of their results put in order are what the tile cannot do without; whether it has to be masked is asked once for 32 of them, and
 // weights are taken against a reference maximum that the tile's own is only looked for where the weights' sum says so.  What is done once a
 // piece is bound by the fetch of its instructions (some 15 ns each the first time they are met), so each step stands once in the
 // code, whichever piece it is of, tiles are not unrolled over their places in LDS, and there is no division by a number known on the host.
+//
+// The start of a piece counts as kStartTurns turns of its tiles.  us at 0, 2, 3, 4 and 6: 24 requests of up to 4000 keys and 5 tokens 25.7, 22.3, 20.4,
+// 20.4, 20.9; 64 of up to 8192 43.6, 40.5, 40.0, 40.7, 42.5; 100 of up to 5000, 4 kv heads of 64, 24.3, 21.9, 21.3, 20.7, 21.7.
 constexpr int kStartTurns = 3;
 template <int DTYPE, int D, int RT, int NW, bool WHOLE>
 __global__ __launch_bounds__(NW * 64, NW == 4 && (RT == 1 || D == 64) ? (RT == 1 && D == 64 ? 4 : 3) : 2) void quantized_few_kernel(const PagedParams) {
@@ -354,6 +358,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (RT == 1 || D == 64) ? (RT == 1
   }
 }
 
+// Prompts.  Bound as over a cache of 16 bits by the matrix pipe and the issue of instructions, of which the conversions, once for a workgroup's 128
+// rows, make a slot taken in 89 % of the cycles instead of 83 %: two prompts of 2048 with a window of 4096 256 us (1.09 PFLOP/s; over 16 bits 251-260),
+// one of 8192 from its start 508 (481).
 template <int DTYPE, int D>
 __global__ __launch_bounds__(kRowsThreads, 2) void quantized_rows_kernel(const PagedParams) {
   __shared__ __attribute__((aligned(16))) char lds[RowsLds<D>::BYTES];

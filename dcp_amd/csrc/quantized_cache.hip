@@ -3,7 +3,8 @@
 // Both are bound by HBM where there is enough to do, by a launch and two trips to memory where there is not.  A lane takes 8 elements
 // of a token's row, 16 bytes of the 16-bit side and 4 of the other, for several heads one after the other; the lanes of a wave
 // are 4 tokens (8 at head size 64) with all of their pieces, so that of neighbouring slots both K and V are 256 bytes in a row: lanes of one
-// token and four heads would touch four times that of V.
+// token and four heads touched four times that of V (write and read of 16384 tokens of 8 heads of 128 43.5 us, so 28.9).  By themselves these are
+// 15.0 and 14.4 us, 5.7 and 5.9 TB/s; the read of 131072 tokens takes 127, 5.4 TB/s (a copy of 2 GiB by torch: 4.95).
 #include <algorithm>
 
 #include "quantized_cache.h"
