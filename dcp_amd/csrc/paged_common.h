@@ -148,13 +148,14 @@ struct RowTile {
   TokenRange tokens;
   int n_keys;
 };
+template <int BM = kRowsBM>
 __device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, int place) {
   const int lane = threadIdx.x & 63;
   // Up to 64 requests are counted.  Of more, request b's tiles begin at number floor(first_row / 128) + b: that leaves room for its last,
   // partial one, and needs no sum over the requests before it, but its places without a tile lie among the others, and CUs with two tiles
   // beside CUs with none (24 requests of 128 rows on 1024 keys, nearly half of the places empty: 40 us, counted 35; 64 of 64 rows on 4096 267
   // and 213).
-  auto start = [&](int first, int b) { return (int)((int64_t)first * p.group / kRowsBM) + b; };
+  auto start = [&](int first, int b) { return (int)((int64_t)first * p.group / BM) + b; };
   const bool counted = src.batch <= 64;
   int tile = src.n_tiles - 1 - place, lo = 0, hi = src.batch;  // the last request that begins at or before the tile; 64 candidates a step
   while (hi - lo > 64) {
@@ -167,7 +168,7 @@ __device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, 
   // A lane looks at one request, and at all there is to know of it: another trip to memory for the one that is found is a microsecond.
   const int b = min(lo + lane, hi - 1);
   const TokenRange tokens = tokens_of(p, src, b);
-  const int n_keys = keys_of(p, src, b), n_tiles = (tokens.n * p.group + kRowsBM - 1) / kRowsBM;
+  const int n_keys = keys_of(p, src, b), n_tiles = (tokens.n * p.group + BM - 1) / BM;
   int first_tile = start(tokens.begin, b), passed;
   if (counted) {
     const int ends = wave_scan(lane < hi ? n_tiles : 0);

@@ -42,11 +42,12 @@ struct RankedTile {
   int share, n_shares;
 };
 constexpr int kMinTilesPerPiece = 3;
+template <int BM>
 __device__ __forceinline__ RankedTile find_ranked_tile(PagedArgs& p, SourceArgs& src, int rank) {
   const int lane = threadIdx.x & 63, b = min(lane, src.batch - 1);
   const TokenRange tokens = tokens_of(p, src, b);
   const int n_keys = keys_of(p, src, b), n_rows = lane < src.batch ? tokens.n * p.group : 0, at0 = n_keys - tokens.n;
-  const int n_tiles = (n_rows + kRowsBM - 1) / kRowsBM;
+  const int n_tiles = (n_rows + BM - 1) / BM;
   const int room = src.table_width * p.page_size / kRowsBN;
   const int most = p.window > 0 ? min((int)(((uint32_t)p.window + (uint32_t)p.n_starting) / kRowsBN), room) + 1 : room + 1;  // what a row can see
   auto total = [&](int n) { return __builtin_amdgcn_readlane(wave_scan(n), 63); };
@@ -87,7 +88,7 @@ __device__ __forceinline__ RankedTile find_ranked_tile(PagedArgs& p, SourceArgs&
   // from its lengths; t is found by halving.
   auto seeing_more = [&](int t) {  // tiles of the lane's request, all of them for t = 0
     const uint32_t first = kRowsBN * t > at0 ? (uint32_t)(kRowsBN * t) - (uint32_t)at0 : 0;  // the first token that sees more
-    const int n = first < (uint32_t)tokens.n ? max(n_tiles - (int)first * p.group / kRowsBM, 0) : 0;
+    const int n = first < (uint32_t)tokens.n ? max(n_tiles - (int)first * p.group / BM, 0) : 0;
     return t == 0 ? n_tiles : t < most ? n : 0;
   };
   if (rank >= all) return {{0, -1, {0, 0}, 0}, 0, 0};
@@ -101,8 +102,8 @@ __device__ __forceinline__ RankedTile find_ranked_tile(PagedArgs& p, SourceArgs&
 }
 
 // ---------------------------------------------------------------------------
-// The kernel of rows: a workgroup of 4 waves owns 128 rows of one (request, kv head), a wave 32 of them, and walks its share of the
-// 64-key tiles that any of them sees.  K and V tiles go from memory straight into LDS (KvTile), two stages each, K a tile
+// The kernel of rows: a workgroup of 4 waves owns 64 RT rows of one (request, kv head), 128 over a cache of 16 bits, a wave 16 RT of them, and
+// walks its share of the 64-key tiles that any of them sees.  K and V tiles go from memory straight into LDS (KvTile), two stages each, K a tile
 // ahead of V: S^T of tile t + 1 is multiplied while tile t is exponentiated, MFMA by MFMA in one stream, O^T += V^T P^T
 // of tile t follows as a dense run that the SIMD's other wave fills with its own arithmetic.
 // ---------------------------------------------------------------------------
@@ -130,10 +131,10 @@ struct RowsLds {
 // QUANT: the cache is held in 4 bits.  Wave w brings the tile's 16-key group w through registers: the codes of K of tile t + 3 and of V of
 // tile t + 2 are asked for in iteration t, and those of the tiles before them, there by then, go into LDS as 16 bits, a row's
 // piece between two products.
-template <int DTYPE, int D, bool CORRECTED, bool QUANT = false>
+template <int DTYPE, int D, bool CORRECTED, bool QUANT = false, int RT = 2>
 __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int item, char* lds) {
   typedef KvTile<D> Tile;
-  constexpr int KS = D / 32, DT = D / 16, RT = 2, LPW = Tile::LPW;
+  constexpr int KS = D / 32, DT = D / 16, LPW = Tile::LPW, BM = 64 * RT;
   typedef RowsLds<D> Lds;
   constexpr int TILE_BYTES = Lds::TILE;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4;
@@ -146,7 +147,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   if (ranked) {
     const int rank = divide(item, p.by_heads);
     kv_head = item - rank * p.n_heads_kv;
-    const RankedTile at = find_ranked_tile(p, src, rank);
+    const RankedTile at = find_ranked_tile<BM>(p, src, rank);
     tile = at.tile;
     share = at.share;
     most_shares = at.n_shares;
@@ -156,28 +157,30 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     if (at.share < 0) return;
     kv_head = __builtin_amdgcn_readfirstlane(at.kv_head);
     share = __builtin_amdgcn_readfirstlane(at.share);
-    tile = find_row_tile(p, src, __builtin_amdgcn_readfirstlane(at.place));
+    tile = find_row_tile<BM>(p, src, __builtin_amdgcn_readfirstlane(at.place));
   }
   const TokenRange tokens = tile.tokens;
   const int n_rows = tokens.n * p.group;  // (at most n_tokens * group, which the host has checked)
   auto token_of = [&](int row) { return QUANT ? divide(row, p.by_group) : row / p.group; };
-  const int row0 = tile.index * kRowsBM;
+  const int row0 = tile.index * BM;
   if (tile.index < 0) return;
   const bool prefix = src.cu_groups != nullptr;
   const int n_keys = tile.n_keys, window = prefix ? 0 : p.window, n_starting = p.n_starting;
   // token i of the request is at position n_keys - n + i; every token is past all of a prefix
-  const int first_tok = token_of(row0), last_tok = token_of(min(row0 + kRowsBM, n_rows) - 1);
+  const int first_tok = token_of(row0), last_tok = token_of(min(row0 + BM, n_rows) - 1);
   const int at0 = prefix ? n_keys - 1 : n_keys - tokens.n, step = prefix ? 0 : 1;
   const KeyGroups groups(window, n_starting, max(at0 + first_tok * step, 0), at0 + last_tok * step);
   const int n_groups = __builtin_amdgcn_readfirstlane(groups.hull_end > 0 ? groups.count() : 0);
   const int tiles_all = (n_groups + 3) / 4, n_shares = min(most_shares, max(1, tiles_all / kMinTilesPerShare));
   int t_begin = 0, t_end = 0;
   if (ranked & (share >= n_shares)) return;
-  if (QUANT && n_shares == 1) {
-    t_end = tiles_all;
-  } else if (share < n_shares) {
-    t_begin = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * share / n_shares));
-    t_end = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * (share + 1) / n_shares));
+  if (share < n_shares) {
+    if (QUANT && n_shares == 1) {
+      t_end = tiles_all;
+    } else {
+      t_begin = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * share / n_shares));
+      t_end = __builtin_amdgcn_readfirstlane((int)((int64_t)tiles_all * (share + 1) / n_shares));
+    }
   }
 
   // ---- tiles: lane l brings pieces of rows of the tile's 16-key group l / 16, LPW of K and of V ---------
@@ -231,7 +234,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   u32x4 q[RT][KS];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = min(row0 + w * 32 + rt * 16 + n, n_rows - 1), tok = token_of(r), head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);
+    const int r = min(row0 + w * (16 * RT) + rt * 16 + n, n_rows - 1), tok = token_of(r), head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);
     const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (tokens.begin + tok) * p.q_token + head * p.q_head + Tile::element16(g);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + Tile::step16(ks));
@@ -327,7 +330,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
       without |= m_new == kNoMax;
     }
     anchored = !__any(without);
-    rescale = __any((alpha[0] != 1.0f) | (alpha[1] != 1.0f));
+    rescale = __any((alpha[0] != 1.0f) | (alpha[RT - 1] != 1.0f));
   };
   // Two elements of the lane's 32 weights: pair i is of row tile i / 8, key tile i / 2 % 4.  Weights are rounded to the storage type
   // for the product (half a step each); their sum is of the unrounded ones.
@@ -458,9 +461,8 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     __builtin_amdgcn_s_setprio(2);
     constexpr int N = 4 * KS, NL = 2 * LPW;
     multiply_qk(k_stage(t + 1), s_nxt, [&](int i) {
-      constexpr int PAIRS = 16 / N;
 #pragma unroll
-      for (int x = 0; x < PAIRS; ++x) weigh(s_cur, i * PAIRS + x);
+      for (int x = i * 8 * RT / N; x < (i + 1) * 8 * RT / N; ++x) weigh(s_cur, x);
       if constexpr (QUANT) {
         if (i < KS) put_k(t, i);
         else if (i < KS + 4) put_v(t + 1, i - KS);
@@ -471,10 +473,10 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
         else if (i < NL) load_v(t + 1, off_next, i - LPW);
       }
     });
-    if (__builtin_expect(!taken & __any(!((lsum[0] < kMaxTileSum) & (lsum[1] < kMaxTileSum))), 0)) {
+    if (__builtin_expect(!taken & __any(!((lsum[0] < kMaxTileSum) & (lsum[RT - 1] < kMaxTileSum))), 0)) {
       raise(s_cur);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) weigh(s_cur, i);
+      for (int i = 0; i < 8 * RT; ++i) weigh(s_cur, i);
     }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) l_run[rt] += lsum[rt];
@@ -543,14 +545,14 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[rt][dt][e] *= correction;
     }
-    const int r = row0 + w * 32 + rt * 16 + n;
+    const int r = row0 + w * (16 * RT) + rt * 16 + n;
     if (r >= n_rows) continue;
     const int tok = token_of(r);
     const int64_t token = tokens.begin + tok, head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);
     if (ranked && src.by_few) {
       if ((g == 0) & (share == 0)) p.cuts[token * p.n_heads_q + head] = cut_of(first_piece, n_shares, 0, r - row0);
       if (n_shares > 1) {
-        const int64_t at = (int64_t)(first_piece + share) * 2 * kRowsBM + (r - row0);
+        const int64_t at = (int64_t)(first_piece + share) * 2 * BM + (r - row0);
         if (g == 0) p.slot_sums[at] = f32x2{m, l};
         float* to = p.slot_out + at * D + 4 * g;
 #pragma unroll
@@ -576,14 +578,14 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 // Row tiles of one kv head: every request may have a partial one.  (Of the last one, tile floor(first_row / 128) + batch - 1 + i with
 // i < ceil(rows / 128).)
 template <typename Args>
-int64_t row_tiles(const Args& x, int batch) {
-  return ((int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) - 1) / kRowsBM + batch;
+int64_t row_tiles(const Args& x, int batch, int rows = kRowsBM) {
+  return ((int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) - 1) / rows + batch;
 }
 // Row tiles that go to one XCD together: of one request (or prefix), 16 at most and about equal.  us, single tiles and groups:
 // two prompts of 2048 behind 14336 keys 330 and 265, 16 of 100 behind 900 54 and 43, one of 8192 from its start 520 and 502.
 template <typename Args>
-int row_group(const Args& x, int batch) {
-  const int each = std::max((int)(row_tiles(x, batch) / batch), 1), n = (each + 15) / 16;
+int row_group(const Args& x, int batch, int rows = kRowsBM) {
+  const int each = std::max((int)(row_tiles(x, batch, rows) / batch), 1), n = (each + 15) / 16;
   return (each + n - 1) / n;
 }
 // Shares of a tile's keys: the number that by these figures takes least (us, head size 128, at the longest lengths).  A workgroup begins
@@ -597,10 +599,10 @@ struct RowShares {
   double us;
 };
 template <typename Args>
-RowShares row_shares(const Args& x, int batch, int64_t max_keys, bool joined_anyway) {
+RowShares row_shares(const Args& x, int batch, int64_t max_keys, bool joined_anyway, int tile_rows = kRowsBM) {
   // (about as many tiles as have rows: row_tiles has room for more)
   const int64_t rows = (int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv);
-  const int64_t row_tiles_there = std::max<int64_t>((rows + kRowsBM - 1) / kRowsBM, batch), group = row_group(x, batch);
+  const int64_t row_tiles_there = std::max<int64_t>((rows + tile_rows - 1) / tile_rows, batch), group = row_group(x, batch, tile_rows);
   const int64_t groups = (row_tiles_there + group - 1) / group * x.n_heads_kv;
   const int64_t tiles = (max_keys + kRowsBN - 1) / kRowsBN;
   const int most = (int)std::min<int64_t>(std::max<int64_t>(tiles / kMinTilesPerShare, 1), 64), n_cu = device_cu_count();

@@ -361,11 +361,11 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (RT == 1 || D == 64) ? (RT == 1
 // Prompts.  Bound as over a cache of 16 bits by the matrix pipe and the issue of instructions, of which the conversions, once for a workgroup's 128
 // rows, make a slot taken in 89 % of the cycles instead of 83 %: two prompts of 2048 with a window of 4096 256 us (1.09 PFLOP/s; over 16 bits 251-260),
 // one of 8192 from its start 508 (481).
-template <int DTYPE, int D>
+template <int DTYPE, int D, int RT>
 __global__ __launch_bounds__(kRowsThreads, 2) void quantized_rows_kernel(const PagedParams) {
   __shared__ __attribute__((aligned(16))) char lds[RowsLds<D>::BYTES];
   PagedArgs& p = fresh_kernel_args<PagedParams>();
-  paged_rows<DTYPE, D, false, true>(p, p.own, blockIdx.x, lds);
+  paged_rows<DTYPE, D, false, true, RT>(p, p.own, blockIdx.x, lds);
 }
 
 // ---- host ---------------------------------------------------------------------------
@@ -377,10 +377,17 @@ struct QuantPlan {
   int waves = 4;       // of a workgroup of it
   bool cut = false;    // units may be cut into pieces, by either kernel
   int rows = 16, n_few = 0;  // of a unit, and of a piece's slot; workgroups that may have pieces
-  int64_t units = 1;   // as far as the host knows
+  int64_t parts = 1;   // of a row at most, as far as the host knows
   int n_shares = 1;    // of a row's keys, by the kernel of rows
   size_t cuts = 0, slots = 0, shares = 0;  // bytes
   size_t bytes() const { return cuts + slots + shares; }
+  QuantPlan& with_slots(const dcp_quantized_attn_args& x) {
+    if (cut) {
+      cuts = ((size_t)x.n_tokens * x.n_heads_q * sizeof(int2) + 15) / 16 * 16;
+      slots = (size_t)n_few * 2 * rows * (x.head_dim + 2) * sizeof(float);
+    }
+    return *this;
+  }
 };
 
 // Keys that a request's queries see, of the longest there are.
@@ -403,7 +410,7 @@ static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
     // 15.5 and 20, of 4000 25 and 30, of up to 4000 19.6 and 19.5; 64 of 500 9.8 and 12.4, of up to 2000 16.5 and 19.3, of up to 4000 28 and 27,
     // of up to 8192 51 and 40; 128 of up to 300 10.5 and 19.4.  Head size 64: 1 of 1000 7.8 and 10.5, of 2000 10.5 and 10.6; windows of 1016 keys
     // of 32 8.4 and 13.7.  32 rows: 4 of 1000 12.4 and 14.7, of 4000 26 and 18; 24 of up to 1000 12.4 and 14.9, of up to 4000 26 and 22.
-    const int64_t keys = seen_keys(x), units = plan.units = std::max<int64_t>(x.batch, all_rows / plan.rows) * x.n_heads_kv;
+    const int64_t keys = seen_keys(x), units = std::max<int64_t>(x.batch, all_rows / plan.rows) * x.n_heads_kv;
     plan.waves = units <= device_cu_count() ? 8 : 4;
     const double chain_us = keys * (plan.waves == 8 ? 0.0032 : 0.0045) * (x.head_dim == 128 ? 1.0 : 0.6) * (plan.rows == 16 ? 1.0 : 1.6);
     const double bytes_us = (double)units * keys * x.head_dim * 17 / 16 / 7e6;
@@ -413,25 +420,31 @@ static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
     // contexts of 131072 keys 93-96, 96, 96-99, 98; 64 of up to 8192 48, 40, 42, 42; at head size 64 40, 29.5, 29, 28.
     plan.n_few = plan.whole ? (int)most_units : (x.head_dim == 128 ? 2 : 4) * device_cu_count();
     plan.cut = !plan.whole;
-  } else if (x.batch <= 64) {
+    plan.parts = plan.n_few / units + 2;
+    return plan.with_slots(x);
+  }
+  // The kernel of rows, with tiles of 64 rows where no request has more.  us, of 128 and of 64: 16 requests of 16 tokens behind 4000 keys, 8 kv heads
+  // of 128, 46.5 and 39.7, 3 of 300 13.8 and 11.8; 22 of 8 tokens of 40 heads behind up to 9178, head size 64, 39.0 and 31.7.
+  plan.rows = own_rows <= 64 ? 64 : kRowsBM;
+  const double tiles = (double)((seen_keys(x) + kRowsBN - 1) / kRowsBN);
+  if (x.batch <= 64) {
     // find_ranked_tile cuts by the lengths that there are.  That they may be is decided by the longest ones: where the time that cutting takes off
-    // them if all are as long is more than what a second kernel and the pieces take, or little less: lengths that differ gain more.  us, whole and cut, 8 kv heads of 128, 13 or 30
-    // tokens a request: 3 of 300 keys 13.8 and 16.5, of 700 21.8 and 17.3; 16 of 1000 30 and 33, of up to 1000 30 and 23; 32 of 1500 43 and 48,
-    // of up to 1500 41 and 27; 48 of 2000 69 and 75, of up to 4000 96 and 63; a prompt of 1024 31 and 41.
-    const int64_t units = plan.units = std::max<int64_t>((all_rows + kRowsBM - 1) / kRowsBM, x.batch) * x.n_heads_kv, places = 2 * device_cu_count();
-    const double tiles = (double)((seen_keys(x) + kRowsBN - 1) / kRowsBN);
-    plan.rows = kRowsBM;
+    // them if all are as long is more than what a second kernel and the pieces take, or little less: lengths that differ gain more.  us, whole
+    // and cut, 8 kv heads of 128 in tiles of 128 rows, 13 or 30 tokens a request: 3 of 300 keys 13.8 and 16.5, of 700 21.8 and 17.3; 16 of 1000 30
+    // and 33, of up to 1000 30 and 23; 32 of 1500 43 and 48, of up to 1500 41 and 27; 48 of 2000 69 and 75, of up to 4000 96 and 63; a prompt of
+    // 1024 31 and 41.  (Tiles of 64 rows of size 64 are done faster by four workgroups a CU than by two: 64 requests of 12 tokens behind up to
+    // 2000 keys 24.7 and 32.9, 8 of 9 behind up to 26124 32.7 and 35.5.)
+    const int64_t units = std::max<int64_t>((all_rows + plan.rows - 1) / plan.rows, x.batch) * x.n_heads_kv;
+    const int64_t places = (plan.rows == 64 && x.head_dim == 64 ? 4 : 2) * device_cu_count();
     plan.n_few = (int)(places / x.n_heads_kv * x.n_heads_kv);
     plan.cut = units < places && tiles * (1.0 - (double)units / places) > 10.0;
+    plan.parts = std::min<int64_t>(plan.n_few / units + 2, (int64_t)tiles / kMinTilesPerPiece + 1);
   } else {
-    plan.n_shares = row_shares(x, x.batch, seen_keys(x), false).n;
+    plan.n_shares = row_shares(x, x.batch, seen_keys(x), false, plan.rows).n;
+    plan.parts = plan.n_shares;
     if (plan.n_shares > 1) plan.shares = (size_t)plan.n_shares * x.n_tokens * x.n_heads_q * (x.head_dim + 2) * sizeof(float);
   }
-  if (plan.cut) {
-    plan.cuts = ((size_t)x.n_tokens * x.n_heads_q * sizeof(int2) + 15) / 16 * 16;
-    plan.slots = (size_t)plan.n_few * 2 * plan.rows * (x.head_dim + 2) * sizeof(float);
-  }
-  return plan;
+  return plan.with_slots(x);
 }
 
 namespace {
@@ -467,7 +480,7 @@ int check_quantized(const dcp_quantized_attn_args& x) {
   DCP_REQUIRE(x.q && x.out && x.lse && x.block_table && x.seq_lens && (x.n_pages == 0 || x.cache), "quantized_attn: null argument");
   DCP_REQUIRE(x.max_seqlen_q > 0 && x.max_seqlen_k > 0, "quantized_attn: the longest lengths must be positive");
   // (every kernel's work items: at most 64 shares of a row tile)
-  DCP_REQUIRE(row_tiles(x, x.batch) * x.n_heads_kv < ((int64_t)1 << 31) - (1 << 20), "quantized_attn: too many rows");
+  DCP_REQUIRE(row_tiles(x, x.batch, 64) * x.n_heads_kv < ((int64_t)1 << 31) - (1 << 20), "quantized_attn: too many rows");
   return DCP_OK;
 }
 
@@ -484,7 +497,7 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
   p.cu_seqlens_q = x.cu_seqlens_q;
   p.q_token = x.q_token_stride; p.q_head = x.q_head_stride; p.out_token = x.out_token_stride; p.out_head = x.out_head_stride;
   p.page_stride = x.page_stride; p.head_stride = x.head_stride;
-  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_shares, (int)row_tiles(x, x.batch), row_group(x, x.batch), plan.cut};
+  p.own = {x.block_table, x.seq_lens, nullptr, x.table_stride, x.table_width, x.batch, 0, plan.n_shares, plan.few ? 0 : (int)row_tiles(x, x.batch, plan.rows), plan.few ? 1 : row_group(x, x.batch, plan.rows), plan.cut};
   p.n_pages = x.n_pages; p.page_size = x.page_size;
   p.n_requests = x.batch; p.n_tokens = x.n_tokens;
   p.n_heads_q = x.n_heads_q; p.n_heads_kv = x.n_heads_kv; p.group = x.n_heads_q / x.n_heads_kv;
@@ -506,12 +519,12 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
     return check_launch(name);
   };
   int status;
-  if (!plan.few)
-    status = launch(DCP_QUANT_KERNEL(quantized_rows_kernel), "quantized_rows_kernel",
-                    x.batch <= 64 ? std::max<int64_t>((int64_t)p.own.n_tiles * x.n_heads_kv, plan.cut ? plan.n_few : 0)
-                                  : row_workgroups(p.own.n_tiles, p.own.xcd_group, x.n_heads_kv, plan.n_shares),
-                    kRowsThreads);
-  else if (plan.whole && plan.waves == 8)
+  if (!plan.few) {
+    const int64_t n_wg = x.batch <= 64 ? std::max<int64_t>((int64_t)p.own.n_tiles * x.n_heads_kv, plan.cut ? plan.n_few : 0)
+                                       : row_workgroups(p.own.n_tiles, p.own.xcd_group, x.n_heads_kv, plan.n_shares);
+    status = plan.rows == 64 ? launch(DCP_QUANT_KERNEL(quantized_rows_kernel, 1), "quantized_rows_kernel", n_wg, kRowsThreads)
+                             : launch(DCP_QUANT_KERNEL(quantized_rows_kernel, 2), "quantized_rows_kernel", n_wg, kRowsThreads);
+  } else if (plan.whole && plan.waves == 8)
     status = plan.rows == 16 ? launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 8, true), "quantized_few_kernel", p.n_few, 512)
                              : launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 8, true), "quantized_few_kernel", p.n_few, 512);
   else if (plan.whole)
@@ -521,7 +534,7 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
     status = plan.rows == 16 ? launch(DCP_QUANT_KERNEL(quantized_few_kernel, 1, 4, false), "quantized_few_kernel", p.n_few, 256)
                              : launch(DCP_QUANT_KERNEL(quantized_few_kernel, 2, 4, false), "quantized_few_kernel", p.n_few, 256);
   if (status == DCP_OK && (p.own.by_few || !p.direct))
-    status = launch_paged_merge(p, x.dtype, x.head_dim, plan.cut ? plan.n_few / plan.units + 2 : plan.n_shares, stream);
+    status = launch_paged_merge(p, x.dtype, x.head_dim, plan.parts, stream);
   return status;
 }
 

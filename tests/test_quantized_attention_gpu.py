@@ -67,6 +67,9 @@ RAGGED = {
     "rows_of_many_heads": dict(keys=[1400, 300, 20], new=[9, 300, 3], heads=48, kv_heads=1, head_dim=64),
     "more_tokens_than_keys": dict(keys=[10, 1100, 0], new=[150, 40, 60], heads=4, kv_heads=2),
     "alone": dict(keys=[5000], new=[50], heads=8, kv_heads=1, page_size=16),
+    "at_most_64_rows": dict(keys=[3000, 17, 900, 0, 64, 1500], new=[16, 9, 0, 3, 16, 1]),
+    "at_most_64_rows_fp16_d64": dict(keys=[2500, 40, 1300], new=[13, 13, 12], heads=25, kv_heads=5, head_dim=64, dtype=F16),
+    "at_most_64_rows_window": dict(keys=[2500, 100, 1300], new=[33, 30, 64], heads=3, kv_heads=3, head_dim=64, window=300, n_starting=70),
 }
 
 
@@ -81,6 +84,16 @@ def test_ragged_prompts(gpu, name, longest):
     truth = case.truth()
     for table in (args["block_table"], wide):
         check(_run(gpu, case, sentinel=5.0, max_seqlen_k=longest, block_table=table), truth)
+
+
+@pytest.mark.parametrize("longest_q", [9, 16, 100])
+@pytest.mark.parametrize("requests", [5, 70])
+def test_tiles_of_rows_the_host_does_not_know(gpu, requests, longest_q):
+    """36 rows are taken by tiles of 64, 400 by tiles of 128, whatever the requests have."""
+    new = [(0, 3, 17, 40, 9)[i % 5] for i in range(requests)]
+    case = Quantized([n + (i * 37) % 200 for i, n in enumerate(new)], new=new, heads=4, kv_heads=1, head_dim=64, page_size=16)
+    for longest in (64, 100000):
+        check(_run(gpu, case, max_seqlen_q=longest_q, max_seqlen_k=longest), case.truth())
 
 
 @pytest.mark.parametrize("new", [[1] * 64, [33] * 64, [0] * 63 + [200]])
