@@ -41,6 +41,7 @@ struct RankedTile {
   RowTile tile;
   int share, n_shares;
 };
+// Tiles of the shortest piece.  us at 2, 3 and 4: 3 requests of 13 tokens of 1000 keys 17.7, 18.1, 18.8; 2 of 100 tokens of 1000 25.9, 23.8, 23.5.
 constexpr int kMinTilesPerPiece = 3;
 template <int BM>
 __device__ __forceinline__ RankedTile find_ranked_tile(PagedArgs& p, SourceArgs& src, int rank) {
@@ -57,9 +58,11 @@ __device__ __forceinline__ RankedTile find_ranked_tile(PagedArgs& p, SourceArgs&
   };
   const int all = total(n_tiles);
   // Where there are fewer row tiles than workgroups, those of a request are cut into pieces of about `length` key tiles, the least that leaves
-  // a workgroup for every piece: between an equal share of all key tiles and what that is if every row tile needs one piece more.  One
-  // workgroup a CU where pieces are short: with two, each takes half as many tiles in three quarters of the time, but there is twice as much to be joined.
-  const int places = src.by_few ? divide(p.n_few, p.by_heads) : 0;  // two workgroups a CU
+  // a workgroup for every piece: between an equal share of all key tiles and what that is if every row tile needs one piece more.  Half as many
+  // workgroups where pieces are short: there is less to be joined then, and a workgroup that has a CU to itself takes three quarters of the time a
+  // tile (us, all and half: 10 requests of 40 tokens of 2000 keys, 2 kv heads, 31.4 and 27.1; where pieces are longer than 6 tiles all are better, 24
+  // of 40 tokens of up to 4000 44 and 84).
+  const int places = src.by_few ? divide(p.n_few, p.by_heads) : 0;
   if (all < places) {
     const float tiles = (float)min(min((n_keys + kRowsBN - 1) / kRowsBN, most + 1), 1 << 20);
     const float sum = (float)total(n_tiles * (int)tiles);  // (less than 2^30)
