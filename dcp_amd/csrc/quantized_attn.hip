@@ -416,9 +416,11 @@ static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
     const double bytes_us = (double)units * keys * x.head_dim * 17 / 16 / 7e6;
     plan.whole = chain_us < (plan.rows == 16 ? 4.5 : 6.5) + std::min(0.45 * bytes_us, 12.0);
     if (!plan.whole) plan.waves = 4;
-    // Two workgroups a CU are enough for the memory, of head size 64 (half of the bytes under way) four.  us, one, two, three and four: four
-    // contexts of 131072 keys 93-96, 96, 96-99, 98; 64 of up to 8192 48, 40, 42, 42; at head size 64 40, 29.5, 29, 28.
-    plan.n_few = plan.whole ? (int)most_units : (x.head_dim == 128 ? 2 : 4) * device_cu_count();
+    // Two workgroups a CU are enough for the memory, of head size 64 (half of the bytes under way) four, of 32 rows three, as many as there are
+    // registers for.  us, one, two, three and four: four contexts of 131072 keys 93-96, 96, 96-99, 98; 64 of up to 8192 48, 40, 42, 42; at head
+    // size 64 40, 29.5, 29, 28.  32 rows of size 64, two, three and four: 40 requests of up to 9000 keys and 4 tokens of 40 heads 31.4, 29.8, 33.6, 100
+    // 64, 59, 64.
+    plan.n_few = plan.whole ? (int)most_units : (x.head_dim == 128 ? 2 : plan.rows == 32 ? 3 : 4) * device_cu_count();
     plan.cut = !plan.whole;
     plan.parts = plan.n_few / units + 2;
     return plan.with_slots(x);
