@@ -167,6 +167,10 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   auto token_of = [&](int row) { return QUANT ? divide(row, p.by_group) : row / p.group; };
   const int row0 = tile.index * BM;
   if (tile.index < 0) return;
+  // In 4 bits a wave without rows brings its part of the tiles and does no more, and a CU's second workgroup has its first rows on other SIMDs: one
+  // prompt of 500 tokens beside 31 single tokens behind up to 8000 keys 94 us -> 80.
+  const int w_rows = QUANT ? w ^ (item >> 8 & 1) << 1 : w;
+  const bool idle = QUANT && row0 + w_rows * (16 * RT) >= n_rows;
   const bool prefix = src.cu_groups != nullptr;
   const int n_keys = tile.n_keys, window = prefix ? 0 : p.window, n_starting = p.n_starting;
   // token i of the request is at position n_keys - n + i; every token is past all of a prefix
@@ -237,7 +241,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   u32x4 q[RT][KS];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int r = min(row0 + w * (16 * RT) + rt * 16 + n, n_rows - 1), tok = token_of(r), head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);
+    const int r = min(row0 + w_rows * (16 * RT) + rt * 16 + n, n_rows - 1), tok = token_of(r), head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);
     const uint16_t* from = reinterpret_cast<const uint16_t*>(p.q) + (tokens.begin + tok) * p.q_token + head * p.q_head + Tile::element16(g);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[rt][ks] = *reinterpret_cast<const u32x4*>(from + Tile::step16(ks));
@@ -447,6 +451,15 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
       k_from = quant_at(t + 3);
       v_from = quant_at(t + 2);
     }
+    if (QUANT && idle) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i) put_k(t, i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) put_v(t + 1, j);
+      codes.load_k(k_from, lane_here());
+      codes.load_v(v_from, lane_here());
+      return;
+    }
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) lsum[rt] = 0.0f;
     bool taken = false;  // the tile's maximum
@@ -548,7 +561,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[rt][dt][e] *= correction;
     }
-    const int r = row0 + w * (16 * RT) + rt * 16 + n;
+    const int r = row0 + w_rows * (16 * RT) + rt * 16 + n;
     if (r >= n_rows) continue;
     const int tok = token_of(r);
     const int64_t token = tokens.begin + tok, head = kv_head * p.group + (QUANT ? r - tok * p.group : r % p.group);

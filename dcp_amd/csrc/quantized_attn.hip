@@ -360,7 +360,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (RT == 1 || D == 64) ? (RT == 1
 
 // Prompts.  Bound as over a cache of 16 bits by the matrix pipe and the issue of instructions, of which the conversions, once for a workgroup's 128
 // rows, make a slot taken in 89 % of the cycles instead of 83 %: two prompts of 2048 with a window of 4096 256 us (1.09 PFLOP/s; over 16 bits 251-263),
-// one of 8192 from its start 508 (481).
+// one of 8192 from its start 498 (481).
 template <int DTYPE, int D, int RT>
 __global__ __launch_bounds__(kRowsThreads, 2) void quantized_rows_kernel(const PagedParams) {
   __shared__ __attribute__((aligned(16))) char lds[RowsLds<D>::BYTES];
