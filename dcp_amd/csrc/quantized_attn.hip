@@ -120,7 +120,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (RT == 1 || D == 64) ? (RT == 1
   auto told = [&]() {
     PagedArgs& p = fresh_kernel_args<PagedParams>();
     const bool there = (unsigned)lane_page < (unsigned)p.n_pages;
-    lane_off = there ? lane_page * p.page_stride + lane_tile * Tile::BYTES : 0;
+    lane_off = there ? lane_page * p.page_stride + (int64_t)lane_tile * Tile::BYTES : 0;
     const int key = lane_key_ahead = there ? lane_key_ahead : kNoKey;
     full_ahead = __ballot((key + 15 <= all_last) & ((key >= all_first) | (key + 15 < p.n_starting)));
   };
