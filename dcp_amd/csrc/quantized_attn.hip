@@ -398,11 +398,11 @@ static int64_t seen_keys(const dcp_quantized_attn_args& x) {
 static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
   QuantPlan plan;
   const int group = x.n_heads_q / x.n_heads_kv;
-  // The kernel of few rows: of requests with up to 32.  Its sums of tiles have to fit 32 bits whatever the lengths are.
+  // The kernel of few rows: of requests with up to 32.  Its sums of tiles, the starts of units among them, have to fit 32 bits whatever the lengths are.
   const int64_t own_rows = (int64_t)x.max_seqlen_q * group, all_rows = (int64_t)x.n_tokens * group;
   plan.rows = own_rows <= 16 ? 16 : 32;
   const int64_t most_units = (all_rows + (int64_t)x.batch * (plan.rows - 1)) / plan.rows * x.n_heads_kv;
-  plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2) < 2e9;
+  plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2 + kStartTurns) < 2e9;
   if (plan.few) {
     // Whole units where they are short: a unit's chain of tiles, by eight waves where every unit has a CU to itself, against what cutting costs,
     // a second kernel and more starts, which grows with the bytes there are (at 7 TB/s, if all were as long as the longest).  us, whole and cut,
@@ -515,7 +515,7 @@ int quantized_attn(const dcp_quantized_attn_args& x, void* workspace, size_t wor
   p.by_page = Divider::of(x.page_size / kQuantTokens); p.by_group = Divider::of(p.group); p.by_heads = Divider::of(x.n_heads_kv);
   p.few_rows = plan.rows; p.few_whole = plan.whole; p.n_few = plan.n_few;
   const auto launch = [&](auto kernel, const char* name, int64_t n_wg, int threads) {
-    if (n_wg >= (int64_t)1 << 31) return fail(DCP_ERR_ARG, "quantized_attn: too many work items");
+    if (n_wg * threads >= (int64_t)1 << 32) return fail(DCP_ERR_ARG, "quantized_attn: too many work items");  // (what a launch can have)
     KernelTimer timer(name, stream);
     hipLaunchKernelGGL(kernel, dim3((unsigned)n_wg), dim3(threads), 0, (hipStream_t)stream, p);
     return check_launch(name);
