@@ -130,6 +130,9 @@ struct RowsLds {
 // request 0.0023 -> 0.0019, 64 tokens each 0.0023 -> 0.0020.  Beside a prefix's chain of tiles the second sum costs nothing (64 requests of
 // one token on a prefix of 32768 74.3 and 74.6 us), where products bound it 3-4 % (32 requests of 256 tokens on one of 4096 663 and 690, 4
 // of 2048 on 16384 2105 and 2178).  Own keys have it not: a prompt of 8192 481 and 521 us, for an error of 0.0023 and 0.0022.
+// In 4 bits requests of up to kQuantFewRows rows have it: those that the kernel of few rows takes where none longer is beside them, so that a token's
+// rounding is that of the token alone.  31 single tokens of up to 8000 keys and a prompt of 500 80 us and 83, prompts without such as before
+// (one of 8192 492; were they corrected as well 504, at head size 64 351 and 380).
 //
 // QUANT: the cache is held in 4 bits.  Wave w brings the tile's 16-key group w through registers: the codes of K of tile t + 3 and of V of
 // tile t + 2 are asked for in iteration t, and those of the tiles before them, there by then, go into LDS as 16 bits, a row's
@@ -171,6 +174,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
   // prompt of 500 tokens beside 31 single tokens behind up to 8000 keys 94 us -> 80.
   const int w_rows = QUANT ? w ^ (item >> 8 & 1) << 1 : w;
   const bool idle = QUANT && row0 + w_rows * (16 * RT) >= n_rows;
+  const bool corrected = CORRECTED || (QUANT && n_rows <= kQuantFewRows);
   const bool prefix = src.cu_groups != nullptr;
   const int n_keys = tile.n_keys, window = prefix ? 0 : p.window, n_starting = p.n_starting;
   // token i of the request is at position n_keys - n + i; every token is past all of a prefix
@@ -387,6 +391,12 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     }
 #pragma unroll
     for (int rt = 0; CORRECTED && rt < RT; ++rt) l_rounded[rt] += rounded[rt];
+    if (QUANT && corrected) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int x = 0; x < 8; ++x) l_rounded[rt] = add_pair<DTYPE>(pb[rt][x / 4][x % 4], l_rounded[rt]);
+    }
   };
 
   // ---- key loop ------------------------------------------------------------------------
@@ -499,7 +509,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
     if (__builtin_expect(rescale, 0)) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        if (CORRECTED) l_rounded[rt] *= alpha[rt];
+        if (CORRECTED || QUANT) l_rounded[rt] *= alpha[rt];
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -554,7 +564,7 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const float l = rows_sum(l_run[rt]), m = l == 0.0f ? -INFINITY : m_run[rt];
-    if constexpr (CORRECTED) {
+    if (corrected) {
       const float rounded = rows_sum(l_rounded[rt]), correction = rounded == 0.0f ? 1.0f : l / rounded;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)

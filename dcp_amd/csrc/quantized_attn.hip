@@ -398,11 +398,11 @@ static int64_t seen_keys(const dcp_quantized_attn_args& x) {
 static QuantPlan plan_quantized(const dcp_quantized_attn_args& x) {
   QuantPlan plan;
   const int group = x.n_heads_q / x.n_heads_kv;
-  // The kernel of few rows: of requests with up to 32.  Its sums of tiles, the starts of units among them, have to fit 32 bits whatever the lengths are.
+  // The kernel of few rows: of requests with up to kQuantFewRows.  Its sums of tiles, the starts of units among them, have to fit 32 bits whatever the lengths are.
   const int64_t own_rows = (int64_t)x.max_seqlen_q * group, all_rows = (int64_t)x.n_tokens * group;
   plan.rows = own_rows <= 16 ? 16 : 32;
   const int64_t most_units = (all_rows + (int64_t)x.batch * (plan.rows - 1)) / plan.rows * x.n_heads_kv;
-  plan.few = own_rows <= 32 && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2 + kStartTurns) < 2e9;
+  plan.few = own_rows <= kQuantFewRows && x.batch <= kFewMaxBatch && (double)most_units * ((double)x.table_width * x.page_size / kFewBN + 2 + kStartTurns) < 2e9;
   if (plan.few) {
     // Whole units where they are short: a unit's chain of tiles, by eight waves where every unit has a CU to itself, against what cutting costs,
     // a second kernel and more starts, which grows with the bytes there are (at 7 TB/s, if all were as long as the longest).  us, whole and cut,

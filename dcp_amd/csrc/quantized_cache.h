@@ -22,6 +22,7 @@
 namespace dcp {
 
 constexpr int kQuantTokens = 16, kQuantBlock = 32;
+constexpr int kQuantFewRows = 32;  // rows of a kv head of a request that the attention's kernel of few rows takes
 
 template <int D>
 struct QuantTile {
