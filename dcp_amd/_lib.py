@@ -60,6 +60,8 @@ SIGNATURES = {
     "dcp_paged_attn": [_P, _P, c_size_t, _P],
     "dcp_quantized_cache_write": [_P] * 4 + [_I] * 4 + [_L] * 3 + [_I, _L, _L, _P],
     "dcp_quantized_cache_read": [_P] * 4 + [_I] * 4 + [_L] * 3 + [_I, _L, _L, _P],
+    "dcp_quantized_cache_write_strided": [_P] * 4 + [_I] * 4 + [_L] * 5 + [_I, _L, _L, _P],
+    "dcp_quantized_cache_read_strided": [_P] * 4 + [_I] * 4 + [_L] * 5 + [_I, _L, _L, _P],
     "dcp_quantized_attn_workspace_bytes": [_P],
     "dcp_quantized_attn": [_P, _P, c_size_t, _P],
     "dcp_greedy_stage_selection": [_I, _P, _I, _P, _P, _I, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _L, _P, _P, _P],

@@ -17,8 +17,8 @@ struct QuantRowsParams {
   char* v;
   const int64_t* slots;
   char* cache;
-  int64_t token, head;             // strides of the rows in bytes
-  int64_t page_stride, head_stride;  // of the cache in bytes
+  int64_t k_token, k_head, v_token, v_head;  // strides of the rows in bytes
+  int64_t page_stride, head_stride;          // of the cache in bytes
   int64_t n_slots;
   int n_tokens, page_size, n_heads;
   int head_groups;  // of kQuantHeads heads
@@ -84,13 +84,15 @@ __global__ __launch_bounds__(kQuantThreads) void quantized_write_kernel(const Qu
   typedef QuantTile<D> Tile;
   const QuantRows<D> rows(p);
   if (rows.token >= p.n_tokens) return;  // (a block's four lanes are of one token)
-  const int64_t slot = p.slots[rows.token], from = rows.token * p.token + rows.piece * 16;
+  const int64_t slot = p.slots[rows.token];
+  const char* k_from = p.k + (rows.token * p.k_token + rows.piece * 16);
+  const char* v_from = p.v + (rows.token * p.v_token + rows.piece * 16);
   u32x4 x[kQuantHeads][2];
 #pragma unroll
   for (int h = 0; h < kQuantHeads; ++h) {
     if (rows.head + h >= rows.head_end) break;
-    x[h][0] = *reinterpret_cast<const u32x4*>(p.k + from + (rows.head + h) * p.head);
-    x[h][1] = *reinterpret_cast<const u32x4*>(p.v + from + (rows.head + h) * p.head);
+    x[h][0] = *reinterpret_cast<const u32x4*>(k_from + (rows.head + h) * p.k_head);
+    x[h][1] = *reinterpret_cast<const u32x4*>(v_from + (rows.head + h) * p.v_head);
   }
   if ((slot < 0) | (slot >= p.n_slots)) return;
   int j;
@@ -120,7 +122,9 @@ __global__ __launch_bounds__(kQuantThreads) void quantized_read_kernel(const Qua
   typedef QuantTile<D> Tile;
   const QuantRows<D> rows(p);
   if (rows.token >= p.n_tokens) return;
-  const int64_t slot = p.slots[rows.token], to = rows.token * p.token + rows.piece * 16;
+  const int64_t slot = p.slots[rows.token];
+  char* k_to = p.k + (rows.token * p.k_token + rows.piece * 16);
+  char* v_to = p.v + (rows.token * p.v_token + rows.piece * 16);
   const bool there = (slot >= 0) & (slot < p.n_slots);
   uint32_t codes[kQuantHeads][2], exps[kQuantHeads][2];
   if (there) {
@@ -144,7 +148,7 @@ __global__ __launch_bounds__(kQuantThreads) void quantized_read_kernel(const Qua
     for (int of = 0; of < 2; ++of) {
       u32x4 x = {0, 0, 0, 0};
       if (there) x = eight_of_codes<DTYPE>(codes[h][of], exponent_scale(exps[h][of], 0));
-      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>((of ? p.v : p.k) + to + (rows.head + h) * p.head));
+      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(of ? v_to + (rows.head + h) * p.v_head : k_to + (rows.head + h) * p.k_head));
     }
   }
 }
@@ -156,16 +160,24 @@ int64_t row_workgroups(const QuantRowsParams& p, int head_dim) {
   return (p.n_tokens + tokens - 1) / tokens * p.head_groups;
 }
 
-// What the two calls have in common: their arguments, checked, as the kernels take them.
+// Strides of an axis, in elements; of an axis of one they say nothing.
+struct RowStrides {
+  int64_t token, head;
+  RowStrides of(int n_tokens, int n_heads) const { return {n_tokens == 1 ? 0 : token, n_heads == 1 ? 0 : head}; }
+  bool good() const { return token >= 0 && head >= 0 && token % 8 == 0 && head % 8 == 0; }
+};
+
+// What the calls have in common: their arguments, checked, as the kernels take them.
 int quantized_rows(const char* what, QuantRowsParams& p, const void* k, const void* v, const int64_t* slot_mapping, const void* cache, int n_tokens,
-                   int n_heads_kv, int head_dim, int dtype, int64_t token_stride, int64_t head_stride, int64_t n_pages, int page_size,
+                   int n_heads_kv, int head_dim, int dtype, RowStrides k_strides, RowStrides v_strides, int64_t n_pages, int page_size,
                    int64_t cache_page_stride, int64_t cache_head_stride) {
   if (dtype != DCP_DTYPE_BF16 && dtype != DCP_DTYPE_FP16) return fail(DCP_ERR_UNSUPPORTED, "%s: dtype %d unsupported (bf16 and fp16 only)", what, dtype);
   if (head_dim != 64 && head_dim != 128) return fail(DCP_ERR_UNSUPPORTED, "%s: head_dim %d unsupported (64 or 128)", what, head_dim);
   DCP_REQUIRE(n_tokens >= 0 && n_pages >= 0 && n_heads_kv > 0, "%s: sizes must be positive", what);
   DCP_REQUIRE(page_size > 0 && page_size % kQuantTokens == 0, "%s: page_size %d must be a positive multiple of 16", what, page_size);
-  DCP_REQUIRE(token_stride >= 0 && head_stride >= 0 && token_stride % 8 == 0 && head_stride % 8 == 0,
-              "%s: strides of k and v must be multiples of 8 elements, not negative", what);
+  k_strides = k_strides.of(n_tokens, n_heads_kv);
+  v_strides = v_strides.of(n_tokens, n_heads_kv);
+  DCP_REQUIRE(k_strides.good() && v_strides.good(), "%s: strides of k and v must be multiples of 8 elements, not negative", what);
   DCP_REQUIRE(cache_page_stride >= 0 && cache_head_stride >= 0 && cache_page_stride % 16 == 0 && cache_head_stride % 16 == 0,
               "%s: strides of the cache must be multiples of 16 bytes, not negative", what);
   DCP_REQUIRE(n_heads_kv <= 1 << 20, "%s: too many heads", what);
@@ -173,8 +185,8 @@ int quantized_rows(const char* what, QuantRowsParams& p, const void* k, const vo
   if (n_tokens == 0) return DCP_OK;
   DCP_REQUIRE(k && v && slot_mapping && (n_pages == 0 || cache), "%s: null argument", what);
   DCP_REQUIRE((((uintptr_t)k | (uintptr_t)v | (uintptr_t)cache) & 15) == 0, "%s: k, v and the cache must be 16-byte aligned", what);
-  p = {(char*)k, (char*)v, slot_mapping, (char*)cache, token_stride * 2, head_stride * 2, cache_page_stride, cache_head_stride, n_pages * page_size,
-       n_tokens, page_size, n_heads_kv, (n_heads_kv + kQuantHeads - 1) / kQuantHeads};
+  p = {(char*)k, (char*)v, slot_mapping, (char*)cache, k_strides.token * 2, k_strides.head * 2, v_strides.token * 2, v_strides.head * 2,
+       cache_page_stride, cache_head_stride, n_pages * page_size, n_tokens, page_size, n_heads_kv, (n_heads_kv + kQuantHeads - 1) / kQuantHeads};
   DCP_REQUIRE(row_workgroups(p, head_dim) < (int64_t)1 << 31, "%s: too many rows", what);
   return DCP_OK;
 }
@@ -195,28 +207,46 @@ using namespace dcp;
   (dtype == DCP_DTYPE_BF16 ? (head_dim == 128 ? kernel<DCP_DTYPE_BF16, 128> : kernel<DCP_DTYPE_BF16, 64>) \
                            : (head_dim == 128 ? kernel<DCP_DTYPE_FP16, 128> : kernel<DCP_DTYPE_FP16, 64>))
 
-extern "C" int dcp_quantized_cache_write(const void* k, const void* v, const int64_t* slot_mapping, void* cache, int n_tokens, int n_heads_kv,
-                                         int head_dim, int dtype, int64_t token_stride, int64_t head_stride, int64_t n_pages, int page_size,
-                                         int64_t cache_page_stride, int64_t cache_head_stride, void* stream) {
-  DCP_RECORDED(dcp_quantized_cache_write(k, v, slot_mapping, cache, n_tokens, n_heads_kv, head_dim, dtype, token_stride, head_stride, n_pages,
-      page_size, cache_page_stride, cache_head_stride, stream));
+extern "C" int dcp_quantized_cache_write_strided(const void* k, const void* v, const int64_t* slot_mapping, void* cache, int n_tokens, int n_heads_kv,
+                                                 int head_dim, int dtype, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                                                 int64_t v_head_stride, int64_t n_pages, int page_size, int64_t cache_page_stride,
+                                                 int64_t cache_head_stride, void* stream) {
+  DCP_RECORDED(dcp_quantized_cache_write_strided(k, v, slot_mapping, cache, n_tokens, n_heads_kv, head_dim, dtype, k_token_stride, k_head_stride,
+      v_token_stride, v_head_stride, n_pages, page_size, cache_page_stride, cache_head_stride, stream));
   QuantRowsParams p;
-  if (const int status = quantized_rows("quantized_cache_write", p, k, v, slot_mapping, cache, n_tokens, n_heads_kv, head_dim, dtype, token_stride,
-                                        head_stride, n_pages, page_size, cache_page_stride, cache_head_stride))
+  if (const int status = quantized_rows("quantized_cache_write", p, k, v, slot_mapping, cache, n_tokens, n_heads_kv, head_dim, dtype,
+                                        {k_token_stride, k_head_stride}, {v_token_stride, v_head_stride}, n_pages, page_size, cache_page_stride,
+                                        cache_head_stride))
     return status;
   if (n_tokens == 0 || n_pages == 0) return DCP_OK;
   return launch_rows(DCP_QUANT_KERNEL(quantized_write_kernel), "quantized_write_kernel", p, head_dim, stream);
 }
 
-extern "C" int dcp_quantized_cache_read(const void* cache, const int64_t* slot_mapping, void* k, void* v, int n_tokens, int n_heads_kv, int head_dim,
-                                        int dtype, int64_t token_stride, int64_t head_stride, int64_t n_pages, int page_size,
-                                        int64_t cache_page_stride, int64_t cache_head_stride, void* stream) {
-  DCP_RECORDED(dcp_quantized_cache_read(cache, slot_mapping, k, v, n_tokens, n_heads_kv, head_dim, dtype, token_stride, head_stride, n_pages,
-      page_size, cache_page_stride, cache_head_stride, stream));
+extern "C" int dcp_quantized_cache_write(const void* k, const void* v, const int64_t* slot_mapping, void* cache, int n_tokens, int n_heads_kv,
+                                         int head_dim, int dtype, int64_t token_stride, int64_t head_stride, int64_t n_pages, int page_size,
+                                         int64_t cache_page_stride, int64_t cache_head_stride, void* stream) {
+  return dcp_quantized_cache_write_strided(k, v, slot_mapping, cache, n_tokens, n_heads_kv, head_dim, dtype, token_stride, head_stride, token_stride,
+                                           head_stride, n_pages, page_size, cache_page_stride, cache_head_stride, stream);
+}
+
+extern "C" int dcp_quantized_cache_read_strided(const void* cache, const int64_t* slot_mapping, void* k, void* v, int n_tokens, int n_heads_kv,
+                                                int head_dim, int dtype, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                                                int64_t v_head_stride, int64_t n_pages, int page_size, int64_t cache_page_stride,
+                                                int64_t cache_head_stride, void* stream) {
+  DCP_RECORDED(dcp_quantized_cache_read_strided(cache, slot_mapping, k, v, n_tokens, n_heads_kv, head_dim, dtype, k_token_stride, k_head_stride,
+      v_token_stride, v_head_stride, n_pages, page_size, cache_page_stride, cache_head_stride, stream));
   QuantRowsParams p;
-  if (const int status = quantized_rows("quantized_cache_read", p, k, v, slot_mapping, cache, n_tokens, n_heads_kv, head_dim, dtype, token_stride,
-                                        head_stride, n_pages, page_size, cache_page_stride, cache_head_stride))
+  if (const int status = quantized_rows("quantized_cache_read", p, k, v, slot_mapping, cache, n_tokens, n_heads_kv, head_dim, dtype,
+                                        {k_token_stride, k_head_stride}, {v_token_stride, v_head_stride}, n_pages, page_size, cache_page_stride,
+                                        cache_head_stride))
     return status;
   if (n_tokens == 0) return DCP_OK;
   return launch_rows(DCP_QUANT_KERNEL(quantized_read_kernel), "quantized_read_kernel", p, head_dim, stream);
+}
+
+extern "C" int dcp_quantized_cache_read(const void* cache, const int64_t* slot_mapping, void* k, void* v, int n_tokens, int n_heads_kv, int head_dim,
+                                        int dtype, int64_t token_stride, int64_t head_stride, int64_t n_pages, int page_size,
+                                        int64_t cache_page_stride, int64_t cache_head_stride, void* stream) {
+  return dcp_quantized_cache_read_strided(cache, slot_mapping, k, v, n_tokens, n_heads_kv, head_dim, dtype, token_stride, head_stride, token_stride,
+                                          head_stride, n_pages, page_size, cache_page_stride, cache_head_stride, stream);
 }

@@ -49,26 +49,29 @@ def _cache_args(cache: torch.Tensor, here: int) -> tuple:
 
 
 def _rows(k, v, slot_mapping, heads: int, head_dim: int, here: int) -> tuple:
-    """``(k, v, slots, n_tokens, dtype, token stride, head stride)`` of rows that belong into a cache of these sizes."""
+    """``(k, v, slots, n_tokens, dtype, strides)`` of rows that belong into a cache of these sizes; strides of tokens and heads, of both or, where
+    they differ, of k and of v."""
     try:
         dtype, shape, strides = k.dtype, k.shape, k.stride()
         good = (len(shape) == 3 and shape[1] == heads and shape[2] == head_dim and strides[2] == 1 and shape == v.shape and strides == v.stride() and
-                v.dtype is dtype and k.get_device() == here and v.get_device() == here)
-        slots_good = (slot_mapping.dtype is torch.int64 and slot_mapping.dim() == 1 and slot_mapping.get_device() == here and
-                      slot_mapping.is_contiguous())
+                v.dtype is dtype and k.get_device() == here and v.get_device() == here and
+                slot_mapping.dtype is torch.int64 and slot_mapping.dim() == 1 and slot_mapping.get_device() == here and
+                slot_mapping.is_contiguous() and slot_mapping.shape[0] == shape[0])
     except AttributeError:
         good, dtype = False, getattr(k, "dtype", torch.bfloat16)
-    if not good:
+    if good:
+        strides = strides[:2]
+    else:
         _check(k, dtype, "k", here, dense=False), _check(v, dtype, "v", here, dense=False)
-        if isinstance(slot_mapping, torch.Tensor):
-            raise ValueError(f"k and v must be [n_tokens, {heads}, {head_dim}] with the same strides and dense rows")
-    if not good or not slots_good or slot_mapping.shape[0] != shape[0]:
-        _check(slot_mapping, torch.int64, "slot_mapping", here, (shape[0],))
-    return k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), shape[0], dtype_code(dtype), strides[0], strides[1]
+        if k.dim() != 3 or tuple(k.shape[1:]) != (heads, head_dim) or k.shape != v.shape or k.stride(2) != 1 or v.stride(2) != 1:
+            raise ValueError(f"k and v must be [n_tokens, {heads}, {head_dim}] with dense rows, got {list(k.shape)} and {list(v.shape)}")
+        _check(slot_mapping, torch.int64, "slot_mapping", here, (k.shape[0],))
+        strides = k.stride()[:2] + v.stride()[:2]
+    return k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), shape[0], dtype_code(dtype), strides
 
 
 def quantized_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, cache: torch.Tensor) -> None:
-    """Writes ``k`` and ``v`` (bf16 or fp16 ``[n_tokens, n_heads_kv, D]``, any strides that are multiples of 8) into ``cache``
+    """Writes ``k`` and ``v`` (bf16 or fp16 ``[n_tokens, n_heads_kv, D]``, each at any strides that are multiples of 8) into ``cache``
     (``quantized_cache_pages``) at ``slot_mapping`` (int64 ``[n_tokens]``: ``page * page_size + offset``).
 
     A block of 32 elements takes the smallest power of two 2^e of which none of them is more than 7 times as large, an element the
@@ -78,11 +81,11 @@ def quantized_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.
     have to differ from each other, and ``k`` and ``v`` may not lie in the cache."""
     here = torch._C._cuda_getDevice()
     cache_at, heads, head_dim, n_pages, page_size, page, head = _cache_args(cache, here)
-    k_at, v_at, slots, n_tokens, dtype, token_stride, head_stride = _rows(k, v, slot_mapping, heads, head_dim, here)
+    k_at, v_at, slots, n_tokens, dtype, strides = _rows(k, v, slot_mapping, heads, head_dim, here)
     if (n_tokens | page_size | heads) >> 31:
         _in_32_bits(n_tokens=n_tokens, page_size=page_size, n_heads_kv=heads)
-    _lib.call("dcp_quantized_cache_write", k_at, v_at, slots, cache_at, n_tokens, heads, head_dim, dtype, token_stride, head_stride, n_pages,
-              page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
+    _lib.call("dcp_quantized_cache_write" if len(strides) == 2 else "dcp_quantized_cache_write_strided", k_at, v_at, slots, cache_at, n_tokens,
+              heads, head_dim, dtype, *strides, n_pages, page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
 
 
 def quantized_cache_read(cache: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
@@ -90,7 +93,7 @@ def quantized_cache_read(cache: torch.Tensor, slot_mapping: torch.Tensor, dtype:
     """The rows at ``slot_mapping`` (int64 ``[n_tokens]``) as ``(k, v)``, ``[n_tokens, n_heads_kv, D]`` of ``dtype`` (bf16 or fp16):
     what ``quantized_cache_attention`` sees of them.  Rows written from this type are exact; what the type does not hold is rounded.
     Rows of slots outside of the cache are zeros.  ``out``: two tensors to write to, not in the cache (``dtype`` is then theirs);
-    any strides that are multiples of 8 and put no two rows at the same place."""
+    each at any strides that are multiples of 8 and put no two rows at the same place."""
     here = torch._C._cuda_getDevice()
     cache_at, heads, head_dim, n_pages, page_size, page, head = _cache_args(cache, here)
     if out is None:
@@ -100,12 +103,12 @@ def quantized_cache_read(cache: torch.Tensor, slot_mapping: torch.Tensor, dtype:
         n_tokens, code = slot_mapping.shape[0], dtype_code(dtype)
         k = cache.new_empty((n_tokens, heads, head_dim), dtype=dtype)
         v = torch.empty_like(k)
-        k_at, v_at, slots, token_stride, head_stride = k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), heads * head_dim, head_dim
+        k_at, v_at, slots, strides = k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), (heads * head_dim, head_dim)
     else:
         k, v = out
-        k_at, v_at, slots, n_tokens, code, token_stride, head_stride = _rows(k, v, slot_mapping, heads, head_dim, here)
+        k_at, v_at, slots, n_tokens, code, strides = _rows(k, v, slot_mapping, heads, head_dim, here)
     if (n_tokens | page_size | heads) >> 31:
         _in_32_bits(n_tokens=n_tokens, page_size=page_size, n_heads_kv=heads)
-    _lib.call("dcp_quantized_cache_read", cache_at, slots, k_at, v_at, n_tokens, heads, head_dim, code, token_stride, head_stride, n_pages,
-              page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
+    _lib.call("dcp_quantized_cache_read" if len(strides) == 2 else "dcp_quantized_cache_read_strided", cache_at, slots, k_at, v_at, n_tokens,
+              heads, head_dim, code, *strides, n_pages, page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
     return k, v

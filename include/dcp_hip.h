@@ -764,7 +764,9 @@ int dcp_paged_attn(const dcp_paged_attn_args* args, void* workspace,
  * What was written from the same type is exact, what the type does not hold is
  * rounded.  Rows of slots outside of the cache are zeros.
  *  - Supported: bf16 and fp16, head_dim 64 or 128, page_size a multiple of 16;
- *    16-byte aligned rows (strides multiples of 8 elements).
+ *    16-byte aligned rows (strides multiples of 8 elements; those of an axis of
+ *    one are not looked at).
+ *  - _strided: K and V at strides of their own, otherwise the same.
  */
 int dcp_quantized_cache_write(const void* k, const void* v,
                               const int64_t* slot_mapping, void* cache,
@@ -779,6 +781,18 @@ int dcp_quantized_cache_read(const void* cache, const int64_t* slot_mapping,
                              int64_t head_stride, int64_t n_pages,
                              int page_size, int64_t cache_page_stride,
                              int64_t cache_head_stride, void* stream);
+int dcp_quantized_cache_write_strided(
+    const void* k, const void* v, const int64_t* slot_mapping, void* cache,
+    int n_tokens, int n_heads_kv, int head_dim, int dtype,
+    int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+    int64_t v_head_stride, int64_t n_pages, int page_size,
+    int64_t cache_page_stride, int64_t cache_head_stride, void* stream);
+int dcp_quantized_cache_read_strided(
+    const void* cache, const int64_t* slot_mapping, void* k, void* v,
+    int n_tokens, int n_heads_kv, int head_dim, int dtype,
+    int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+    int64_t v_head_stride, int64_t n_pages, int page_size,
+    int64_t cache_page_stride, int64_t cache_head_stride, void* stream);
 
 /*
  * Attention over a cache held in 4 bits: dcp_paged_attn's own keys, with its
