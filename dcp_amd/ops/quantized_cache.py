@@ -49,8 +49,8 @@ def _cache_args(cache: torch.Tensor, here: int) -> tuple:
 
 
 def _rows(k, v, slot_mapping, heads: int, head_dim: int, here: int) -> tuple:
-    """``(k, v, slots, n_tokens, dtype, strides)`` of rows that belong into a cache of these sizes; strides of tokens and heads, of both or, where
-    they differ, of k and of v."""
+    """``(k, v, slots, n_tokens, dtype, token stride, head stride, v's two)`` of rows that belong into a cache of these sizes; the last is None
+    where v has the strides of k."""
     try:
         dtype, shape, strides = k.dtype, k.shape, k.stride()
         good = (len(shape) == 3 and shape[1] == heads and shape[2] == head_dim and strides[2] == 1 and shape == v.shape and strides == v.stride() and
@@ -59,15 +59,14 @@ def _rows(k, v, slot_mapping, heads: int, head_dim: int, here: int) -> tuple:
                 slot_mapping.is_contiguous() and slot_mapping.shape[0] == shape[0])
     except AttributeError:
         good, dtype = False, getattr(k, "dtype", torch.bfloat16)
-    if good:
-        strides = strides[:2]
-    else:
+    v_strides = None
+    if not good:
         _check(k, dtype, "k", here, dense=False), _check(v, dtype, "v", here, dense=False)
         if k.dim() != 3 or tuple(k.shape[1:]) != (heads, head_dim) or k.shape != v.shape or k.stride(2) != 1 or v.stride(2) != 1:
             raise ValueError(f"k and v must be [n_tokens, {heads}, {head_dim}] with dense rows, got {list(k.shape)} and {list(v.shape)}")
         _check(slot_mapping, torch.int64, "slot_mapping", here, (k.shape[0],))
-        strides = k.stride()[:2] + v.stride()[:2]
-    return k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), shape[0], dtype_code(dtype), strides
+        v_strides = v.stride()[:2]
+    return k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), shape[0], dtype_code(dtype), strides[0], strides[1], v_strides
 
 
 def quantized_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, cache: torch.Tensor) -> None:
@@ -81,11 +80,15 @@ def quantized_cache_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.
     have to differ from each other, and ``k`` and ``v`` may not lie in the cache."""
     here = torch._C._cuda_getDevice()
     cache_at, heads, head_dim, n_pages, page_size, page, head = _cache_args(cache, here)
-    k_at, v_at, slots, n_tokens, dtype, strides = _rows(k, v, slot_mapping, heads, head_dim, here)
+    k_at, v_at, slots, n_tokens, dtype, token_stride, head_stride, v_strides = _rows(k, v, slot_mapping, heads, head_dim, here)
     if (n_tokens | page_size | heads) >> 31:
         _in_32_bits(n_tokens=n_tokens, page_size=page_size, n_heads_kv=heads)
-    _lib.call("dcp_quantized_cache_write" if len(strides) == 2 else "dcp_quantized_cache_write_strided", k_at, v_at, slots, cache_at, n_tokens,
-              heads, head_dim, dtype, *strides, n_pages, page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
+    if v_strides is None:
+        _lib.call("dcp_quantized_cache_write", k_at, v_at, slots, cache_at, n_tokens, heads, head_dim, dtype, token_stride, head_stride, n_pages,
+                  page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
+    else:
+        _lib.call("dcp_quantized_cache_write_strided", k_at, v_at, slots, cache_at, n_tokens, heads, head_dim, dtype, token_stride, head_stride,
+                  *v_strides, n_pages, page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
 
 
 def quantized_cache_read(cache: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
@@ -103,12 +106,17 @@ def quantized_cache_read(cache: torch.Tensor, slot_mapping: torch.Tensor, dtype:
         n_tokens, code = slot_mapping.shape[0], dtype_code(dtype)
         k = cache.new_empty((n_tokens, heads, head_dim), dtype=dtype)
         v = torch.empty_like(k)
-        k_at, v_at, slots, strides = k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), (heads * head_dim, head_dim)
+        k_at, v_at, slots, token_stride, head_stride = k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), heads * head_dim, head_dim
+        v_strides = None
     else:
         k, v = out
-        k_at, v_at, slots, n_tokens, code, strides = _rows(k, v, slot_mapping, heads, head_dim, here)
+        k_at, v_at, slots, n_tokens, code, token_stride, head_stride, v_strides = _rows(k, v, slot_mapping, heads, head_dim, here)
     if (n_tokens | page_size | heads) >> 31:
         _in_32_bits(n_tokens=n_tokens, page_size=page_size, n_heads_kv=heads)
-    _lib.call("dcp_quantized_cache_read" if len(strides) == 2 else "dcp_quantized_cache_read_strided", cache_at, slots, k_at, v_at, n_tokens,
-              heads, head_dim, code, *strides, n_pages, page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
+    if v_strides is None:
+        _lib.call("dcp_quantized_cache_read", cache_at, slots, k_at, v_at, n_tokens, heads, head_dim, code, token_stride, head_stride, n_pages,
+                  page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
+    else:
+        _lib.call("dcp_quantized_cache_read_strided", cache_at, slots, k_at, v_at, n_tokens, heads, head_dim, code, token_stride, head_stride,
+                  *v_strides, n_pages, page_size, page, head, torch._C._cuda_getCurrentRawStream(here))
     return k, v
