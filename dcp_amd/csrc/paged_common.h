@@ -53,16 +53,15 @@ struct PagedParams {
   float* partial_out;
   f32x2* partial_sums;
   // The kernel of few rows (in 4 bits that of rows as well): pieces of the units that are cut between workgroups, and where a row's pieces
-  // are (cut_of):
-  // [token][q head]
-  int2* cuts;
+  // are (cut_of).
+  int2* cuts;        // [token][q head]
   float* slot_out;   // [workgroup][2][head of the workgroup][rows][D]
   f32x2* slot_sums;  // [workgroup][2][head of the workgroup][rows]
   int few_rows, few_heads_log2;  // rows of a unit; kv heads a workgroup takes at once: 1, 2 or 4
   int few_whole;                 // a workgroup takes a unit
   int n_few, few_first;     // workgroups; of paged_both_kernel those before the ones of rows
   int merge_sets;           // of lanes that share a row in the merge, a power of two
-  Divider by_page, by_group, by_heads;  // page_size / 16, group, n_heads_kv (quantized_few_kernel)
+  Divider by_page, by_group, by_heads;  // page_size / 16, group, n_heads_kv (in 4 bits)
 };
 typedef KernArgs<PagedParams> PagedArgs;
 typedef KernArgs<PagedSource> SourceArgs;
@@ -151,7 +150,7 @@ struct RowTile {
 template <int BM = kRowsBM>
 __device__ __forceinline__ RowTile find_row_tile(PagedArgs& p, SourceArgs& src, int place) {
   const int lane = threadIdx.x & 63;
-  // Up to 64 requests are counted.  Of more, request b's tiles begin at number floor(first_row / 128) + b: that leaves room for its last,
+  // Up to 64 requests are counted.  Of more, request b's tiles begin at number floor(first_row / BM) + b: that leaves room for its last,
   // partial one, and needs no sum over the requests before it, but its places without a tile lie among the others, and CUs with two tiles
   // beside CUs with none (24 requests of 128 rows on 1024 keys, nearly half of the places empty: 40 us, counted 35; 64 of 64 rows on 4096 267
   // and 213).

@@ -601,8 +601,8 @@ __device__ __forceinline__ void paged_rows(PagedArgs& p, SourceArgs& src, int it
 
 // ---- host ---------------------------------------------------------------------------
 
-// Row tiles of one kv head: every request may have a partial one.  (Of the last one, tile floor(first_row / 128) + batch - 1 + i with
-// i < ceil(rows / 128).)
+// Tiles of `rows` rows of one kv head: every request may have a partial one.  (Of the last one, tile floor(first_row / rows) + batch - 1 + i with
+// i < ceil(its rows / rows).)
 template <typename Args>
 int64_t row_tiles(const Args& x, int batch, int rows = kRowsBM) {
   return ((int64_t)x.n_tokens * (x.n_heads_q / x.n_heads_kv) - 1) / rows + batch;
