@@ -71,7 +71,7 @@ __device__ __forceinline__ void multiply_v(const QuantGroup<D> (&x)[2], const fl
 // share of the keys is done; work is cut as over a cache of 16 bits (FewWalk), or whole units where they are short (WHOLE).
 //
 // What bounds it is the number of instructions: at 7 TB/s the memory would leave a SIMD 335 slots of 4 cycles a tile, and a tile takes 333 with its
-// share of starts and joins (64 contexts of up to 8192 keys, 8 kv heads of 128: 38 us, 5.2 TB/s, a slot taken in 74 % of them).  64 conversions
+// share of starts and joins (64 contexts of up to 8192 keys, 8 kv heads of 128: 38 us, 5.2 TB/s, a slot taken in 73 % of them).  64 conversions
 // and 32 of their results put in order are what the tile cannot do without; whether it has to be masked is asked once for 32 of them, and
 // weights are taken against a reference maximum that the tile's own is only looked for where the weights' sum says so.  What is done once a
 // piece is bound by the fetch of its instructions (some 15 ns each the first time they are met), so each step stands once in the
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 && (RT == 1 || D == 64) ? (RT == 1
 }
 
 // Prompts.  Bound as over a cache of 16 bits by the matrix pipe and the issue of instructions, of which the conversions, once for a workgroup's 128
-// rows, make a slot taken in 89 % of the cycles instead of 83 %: two prompts of 2048 with a window of 4096 256 us (1.09 PFLOP/s; over 16 bits 251-263),
+// rows, make a slot taken in 90 % of the cycles instead of 83 %: two prompts of 2048 with a window of 4096 256 us (1.09 PFLOP/s; over 16 bits 251-263),
 // one of 8192 from its start 492 (481).
 template <int DTYPE, int D, int RT>
 __global__ __launch_bounds__(kRowsThreads, 2) void quantized_rows_kernel(const PagedParams) {
